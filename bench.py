@@ -60,7 +60,7 @@ TRAFFIC_MEASURED_AGAINST = {
     "gemm_tile_bf16.hip": "d2866de7d66d",
 }
 _PREFILL_SOURCES, _DECODE_SOURCES = ("attn_common.h", "attn_prefill.hip"), ("attn_common.h", "attn_decode.hip", "quant_q8.h")
-_ROPE_SOURCES, _NORM_SOURCES = ("attn_common.h", "rope.hip", "quant_q8.h"), ("attn_common.h", "rmsnorm.hip")
+_ROPE_SOURCES, _NORM_SOURCES = ("attn_common.h", "attn_paged.h", "rope.hip", "quant_q8.h"), ("attn_common.h", "rmsnorm.hip")
 _GEMM_SOURCES = ("attn_common.h", "gemm.hip", "gemm_common.h", "gemm_plan.h", "quant_q8.h")
 _TILE_SOURCES = _GEMM_SOURCES + ("gemm_tile.h", "gemm_tile_f16.hip", "gemm_tile_bf16.hip")
 TRAFFIC_ROW_SOURCES = {

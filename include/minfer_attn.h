@@ -180,6 +180,74 @@ int minfer_rope_kv_append_norm(int dtype, int style, int cache_type, void* q, co
                                int64_t cache_stride_b, int64_t cache_stride_h, int64_t cache_stride_row,
                                int64_t rotary_dim, double freq_base, void* stream);
 
+/* Type of a paged cache's pages besides the activations' own: e4m3 codes with a power of two as the scale of each page, KV head and
+ * tensor. */
+#define MINFER_FP8_E4M3 256
+
+/*
+ * A paged KV cache: pools of pages [n_pages, Hkv, page_size, D] for k and for v and a table of pages per sequence.  Row r of
+ * sequence s lies in page block_table[s * table_stride + r / page_size], at row r % page_size.  block_table is int32 on the device and
+ * is not trusted: an entry outside 0..n_pages-1 means that the page is not there (not mapped yet, or given back); its rows are neither
+ * attended nor written, and the other entries keep their places.  page_size is a power of two in 16..1024.  Strides are those of dims
+ * 0..2, shared by k and v, in elements (multiples of 8) or, for 8-bit pages, bytes (multiples of 16); dim 3 is dense; page_size *
+ * stride_row stays below 2^30.  Pools are 16-byte aligned.  k_scales and v_scales (8-bit pages only) are bytes [n_pages, Hkv], dense:
+ * byte b stands for 2^(b - 127) (E8M0; 255 is NaN).  No counterpart in the reference, whose cache is one slab
+ * (src/minfer/core.py:105-127).
+ */
+typedef struct minfer_kv_pages {
+    void* k;
+    void* v;
+    void* k_scales;
+    void* v_scales;
+    int64_t n_pages, page_size;
+    int64_t stride_page, stride_head, stride_row;
+    const int32_t* block_table;
+    int64_t table_stride, pages_per_seq;
+} minfer_kv_pages;
+
+/*
+ * minfer_rope_kv_append into a paged cache, for packed tokens: q [T,Hq,D] is rotated in place; token cu_seqlens[s] + i stands at
+ * position positions[s] + i of sequence s, and its rotated k and its v [T,Hkv,D] go to that row of the sequence's pages.  cu_seqlens
+ * int32 [n_seqs + 1] and positions int32 [n_seqs] are on the device; sequences are cut to their part inside [0, T), tokens that
+ * belong to none are left alone, and rows whose position is negative or whose page is not there are not written (q is still rotated).
+ * page_type is the activations' dtype, and the rows are those that minfer_rope_kv_append would write, or MINFER_FP8_E4M3.
+ *
+ * 8-bit pages: what a 16-bit cache would have held is rounded to e4m3 (to nearest, ties to even) after division by the scale of
+ * its page and head.  The scale that rows need is the smallest power of two 2^e with their largest finite magnitude <= 448 * 2^e, -100 <= e
+ * <= 7 (fp16) or 119 (bf16), -100 where all are zero; magnitudes beyond 448 * 2^e are cut to it, and what is infinite or NaN becomes NaN.  A page whose row 0
+ * is among the new rows gets the scale that its new rows need; another page keeps the larger of its scale and that, and where its scale grows the codes of
+ * its rows in front of the new ones move to it (rounded again only where they leave e4m3's normal numbers; NaN stays NaN).  Rows behind the new ones keep their bytes.
+ * The result does not depend on the order in which anything runs.  A page that a call writes to must belong to one sequence of that call.
+ *
+ * All pointers 16-byte aligned; D is 64 or 128; rotary_dim a multiple of 8 (interleaved) or 16 (NeoX).
+ */
+int minfer_rope_kv_append_paged(int dtype, int style, int page_type, void* q, const void* k, const void* v,
+                                const int32_t* cu_seqlens, const int32_t* positions, const minfer_kv_pages* pages,
+                                int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t rotary_dim, double freq_base, void* stream);
+
+/* Bytes of workspace for minfer_flash_attn_paged (partial results of a sequence's rows that are split); max_context is
+ * pages_per_seq * page_size. */
+size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                               int64_t max_context, int64_t max_q_len);
+
+/*
+ * Attention of packed tokens over a paged cache that already holds their own rows: q,out [1,Hq,T,D] (strides->q1, q2, o1, o2; the others
+ * are ignored); tokens cu_seqlens[s] .. cu_seqlens[s+1]-1 are the last ones of sequence s, which has ctx_lens[s] rows in the
+ * cache: of n of them, token i stands at position ctx_lens[s] - n + i and attends rows 0 .. that position whose pages are there.  One
+ * token a sequence is a decode step, a few are drafts, many a chunk of a prompt or all of it; sequences of a call may differ.  A token without rows
+ * (a negative position, no page there) yields zeros.  max_q_len: an upper bound of the sequences' numbers of tokens (0 = not known); it
+ * sizes the launch, and tokens of a sequence past it are not computed.  cu_seqlens int32 [n_seqs + 1] and ctx_lens int32 [n_seqs] are
+ * read on the device only and not trusted: sequences are cut to their part inside [0, T), contexts to 0 .. pages_per_seq * page_size.
+ * out is written for the tokens of the sequences only.  The order of the sums depends on the sizes given here and the device data, not on timing: a call
+ * repeated on the same stream gives the same bits.  Rows that nothing was written to may hold anything.
+ * Over 8-bit pages the result is that over the 16-bit rows code * scale, as far as dtype holds them.
+ */
+int minfer_flash_attn_paged(int dtype, int page_type, const void* q, const minfer_kv_pages* pages,
+                            const int32_t* cu_seqlens, const int32_t* ctx_lens, void* out,
+                            int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len,
+                            const minfer_attn_strides* strides, void* workspace, size_t workspace_bytes, void* stream);
+
 /*
  * RMS normalisation: in, out are n_vectors contiguous vectors of length dim; w has dim elements;
  *   out[v, i] = in[v, i] * w[i] / sqrt(mean_i(in[v, :]^2) + eps)      (fp32 arithmetic, one rounding)

@@ -1,0 +1,105 @@
+// What the operators over a paged KV cache share: the cache as the kernels see it, and the checks of its description.
+//
+// A cache is a pool of pages, [n_pages, Hkv, page_size, D] for k and for v, and a table of pages per sequence: row r of sequence s
+// lies in page block_table[s, r / page_size] at row r % page_size.  The table is device data that nobody has checked: an entry
+// outside [0, n_pages) means that the page is not there (never mapped, or given back by a window that moved on); its rows are
+// not attended and not written, and no address is made from it.  Pages are whole in memory, so any row of one may be read,
+// but rows that nothing was written to may hold anything, NaN included.
+//
+// 8-bit pages hold e4m3 codes (four significant bits, exponents from 2^-6 to 2^8, 448 the largest) and one scale for each page, KV head
+// and tensor, a power of two kept as its biased exponent (E8M0).  A power of two, because a page fills token by token: when a
+// later token needs a larger scale the codes that are there move to it by a change of their exponents, exact unless they
+// fall below the smallest normal code, where any other factor would round each of them once more.  And it makes code * scale a
+// number of the 16-bit types, so that attention over 8-bit pages is attention over 16-bit rows, nothing rounded in between.
+#pragma once
+
+#include "attn_common.h"
+#include "attn_host.h"
+
+namespace minfer_attn {
+
+struct PagedCache {
+    void* k; void* v;
+    uint8_t* k_scales; uint8_t* v_scales;   // 8-bit pages: [n_pages][Hkv]
+    const int32_t* table;
+    int64_t page_stride, head_stride, row_stride, table_stride;   // elements (bytes where the pages are 8-bit)
+    int n_pages, page_log2, width;          // pages in the pool, log2 of a page's rows, table entries per sequence
+};
+
+// Input that no kernel of the launch writes, as constant memory: a load at a wave-uniform address is then a scalar one, and waiting
+// for it does not wait for the vector loads in flight.
+template <class V> MA_DEV V const_load(const V* p) {
+    typedef const __attribute__((address_space(4))) V* const_ptr;
+    return *(const_ptr)(uintptr_t)p;
+}
+
+// The same of a byte, through the aligned word that holds it (scalar loads are of words; a word never lies in two memory pages, so that
+// one which holds a byte of a tensor may be read).
+MA_DEV uint32_t const_byte(const uint8_t* p) {
+    const uintptr_t at = (uintptr_t)p;
+    return (const_load((const uint32_t*)(at & ~(uintptr_t)3)) >> (8 * (at & 3))) & 255u;
+}
+
+// The two numbers that say where a sequence's tokens of this call are, whatever cu_seqlens holds: a start in [0, T] and a length that
+// stays inside.
+struct TokenRange { int lo, len; };
+MA_DEV TokenRange token_range(int lo, int hi, int T) {
+    lo = min(max(lo, 0), T);
+    return TokenRange{lo, min(max(hi, lo), T) - lo};
+}
+
+// 2^(bits - 127) for a scale's byte; 255 is no number.  (2^-127 is a subnormal fp32.)
+MA_DEV float scale_value(uint32_t bits) {
+    return __builtin_bit_cast(float, bits == 0u ? 0x00400000u : bits == 255u ? 0x7fc00000u : bits << 23);
+}
+
+// Two e4m3 codes (the word's upper two with HI) times a scale as a pair of 16-bit values, one instruction: rounded once where the type cannot
+// hold the product, which it can unless that is beyond its range; 2^-127 and NaN are scales like any other (checked for
+// every code and scale).
+template <class T, bool HI> MA_DEV uint32_t widen2(uint32_t codes, float scale) {
+    if constexpr (std::is_same_v<T, F16>) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HI));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HI));
+}
+MA_DEV void lds_write_b128(uint32_t addr, int imm, s16x8 x) {
+    typedef __attribute__((address_space(3))) s16x8 lds_s16x8;
+    *(lds_s16x8*)(uintptr_t)(addr + imm) = x;
+}
+
+// Checks of a cache's description, for an operator called `op`; fills `c`.
+inline int check_pages(const char* op, int dtype, int page_type, const minfer_kv_pages* pages, int64_t n_seqs, int64_t Hkv, int64_t D, PagedCache& c) {
+    char msg[256];
+    auto bad = [&](const char* what) { snprintf(msg, sizeof msg, "%s: %s", op, what); return fail(MINFER_ATTN_EINVAL, msg); };
+    const bool eight = page_type == MINFER_FP8_E4M3;
+    if (dtype != MINFER_ATTN_F16 && dtype != MINFER_ATTN_BF16) return bad("dtype must be MINFER_ATTN_F16 or MINFER_ATTN_BF16");
+    if (!eight && page_type != dtype) return bad("page_type must be the activations' dtype or MINFER_FP8_E4M3");
+    if (D != 64 && D != 128) return bad("head_dim must be 64 or 128");
+    if (Hkv <= 0 || Hkv > 65535) return bad("n_kv_heads must be in 1..65535");
+    if (!pages) return bad("pages is null");
+    if (pages->page_size < 16 || pages->page_size > 1024 || (pages->page_size & (pages->page_size - 1)) != 0)
+        return bad("page_size must be a power of two in 16..1024");
+    if (pages->n_pages < 0 || pages->n_pages > 0x7fffffffLL || pages->pages_per_seq < 0) return bad("bad number of pages");
+    if (pages->pages_per_seq * pages->page_size > (int64_t)1 << 30) return bad("pages_per_seq * page_size > 2^30 unsupported");
+    if (pages->table_stride < 0) return bad("table_stride must be non-negative");
+    if (n_seqs > 0 && pages->pages_per_seq > 0 && !pages->block_table) return bad("block_table is null");
+    if (pages->n_pages > 0) {
+        if (!pages->k || !pages->v) return bad("k and v pages must be non-null");
+        if (!aligned16(pages->k) || !aligned16(pages->v)) return bad("pages must be 16-byte aligned");
+        if (eight && (!pages->k_scales || !pages->v_scales)) return bad("8-bit pages need k_scales and v_scales");
+    }
+    const int64_t unit = eight ? 16 : 8, s[3] = {pages->stride_page, pages->stride_head, pages->stride_row};
+    for (int i = 0; i < 3; ++i)
+        if (s[i] < 0 || s[i] % unit != 0) return bad(eight ? "page strides must be non-negative multiples of 16 bytes" : "page strides must be non-negative multiples of 8 elements");
+    // (a lane's offset from a page's first row is 32 bits)
+    if (pages->page_size * pages->stride_row >= (int64_t)1 << 30) return bad("page_size * stride_row >= 2^30 unsupported");
+    c.k = pages->k; c.v = pages->v;
+    c.k_scales = (uint8_t*)pages->k_scales; c.v_scales = (uint8_t*)pages->v_scales;
+    c.table = pages->block_table;
+    c.page_stride = pages->stride_page; c.head_stride = pages->stride_head; c.row_stride = pages->stride_row;
+    c.table_stride = pages->table_stride;
+    c.n_pages = (int)pages->n_pages;
+    c.page_log2 = __builtin_ctzll((unsigned long long)pages->page_size);
+    c.width = (int)(pages->n_pages > 0 ? pages->pages_per_seq : 0);   // a pool without pages: nothing to attend or write, no table to read
+    return MINFER_ATTN_OK;
+}
+
+}  // namespace minfer_attn

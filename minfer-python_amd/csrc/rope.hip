@@ -19,10 +19,14 @@
 // written back, the cache row is written once.  With Q8_0 caches (Q8 = true; rows of D/32 blocks of 34 bytes,
 // strides in bytes) the rotated k and the v values are quantised on the way, from the values an fp16/bf16 cache
 // would have held: the four lanes that hold a block's 32 values agree on its scale through two lane exchanges.
+//
+// Paged caches (PAGED = true; csrc/attn_paged.h): packed tokens, each of which looks its sequence up in cu_seqlens and its cache row in the
+// sequence's table of pages, while its chunks are on their way.  8-bit pages have a kernel of their own (append8_kernel).
 #include <algorithm>
 
 #include "attn_common.h"
 #include "attn_host.h"
+#include "attn_paged.h"
 #include "quant_q8.h"
 
 namespace minfer_attn {
@@ -42,6 +46,9 @@ struct RopeParams {
     int64_t c0, c1, c2;
     int B, L, H, Hkv, D, rd, Lmax;
     int start_pos;            // not fused: position of token l is start_pos + l
+    int n_seqs;               // paged: B = 1, L = the packed tokens; positions [n_seqs]
+    const int32_t* cu;        // paged: [n_seqs + 1]
+    PagedCache pages;         // paged: the cache, in place of the fields above
     double inv_freq[kMaxPairs];
 };
 
@@ -76,6 +83,27 @@ MA_DEV f32x2 table_entry(double inv_freq, int pos) {
     return f32x2{c, s};
 }
 
+// The sequence that packed token `tok` belongs to and its first token, or seq = -1; the same for all lanes of the wave.  The last start that
+// is not behind the token, 64 candidates at a time (up to 64 sequences one load, up to 4096 two); whatever cu_seqlens holds, the result is a
+// sequence that contains the token or none.
+struct TokenOwner { int seq, first; };
+MA_DEV TokenOwner owner_of(const int32_t* cu, int n_seqs, int tok) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = n_seqs;
+    while (n > 0) {
+        const int step = (n + 63) >> 6, i = lane * step;
+        const uint64_t hit = __ballot(i < n && cu[lo + min(i, n - 1)] <= tok);
+        if (hit == 0) return TokenOwner{-1, 0};
+        const int at = __builtin_amdgcn_readfirstlane(63 - __clzll((long long)hit)) * step;
+        lo += at;
+        if (step == 1) break;
+        n = min(step, n - at);
+    }
+    if (n_seqs <= 0) return TokenOwner{-1, 0};
+    const int first = const_load(cu + lo), end = const_load(cu + lo + 1);
+    return first <= tok && tok < end && first >= 0 ? TokenOwner{lo, first} : TokenOwner{-1, 0};
+}
+
 // Per token: every thread requests the 16-byte chunks it owns (a few in flight), the first rd/2 threads
 // meanwhile fill the token's cos/sin table, one barrier, then rotate and store.  The producer into Q8_0 caches
 // requests the first chunks of its next token before it works on the current one.
@@ -84,9 +112,9 @@ MA_DEV f32x2 table_entry(double inv_freq, int pos) {
 // head hd covers elements 8c..8c+7 (pairs 4c..4c+3), rd/8 chunks per head; NeoX style, chunk c covers
 // elements 8c..8c+7 and their partners rd/2 + 8c.., rd/16 chunks per head.  Sections, in order: q rotary,
 // then (fused only) k rotary, k tail (elements rd..D-1, copied), v (copied).
-template <class T, int STYLE, bool FUSED, bool Q8, bool STREAM>
+template <class T, int STYLE, bool FUSED, bool Q8, bool STREAM, bool PAGED = false>
 __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const RopeParams p) {
-    static_assert(FUSED || !Q8, "only the fused producer writes a cache");
+    static_assert(FUSED || (!Q8 && !PAGED), "only the fused producer writes a cache");
     __shared__ f32x2 tab[2][kMaxPairs];
     __shared__ double freq[kMaxPairs];   // the kernel argument array, where a thread can index it cheaply
     const int tid = threadIdx.x;
@@ -116,9 +144,32 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
         short* xq; const short* xk; const short* xv;
         short* ck; short* cv;      // the token's cache row of head 0: element pointers ...
         char* qk; char* qv;        // ... or byte pointers (Q8_0)
+        bool owned;                // paged: the token belongs to a sequence
+    };
+    const int64_t head_stride = PAGED ? p.pages.head_stride : p.c1;
+    // (paged: the token's sequence, position and cache row; after its chunks have been requested)
+    auto locate = [&](Token& k, int tok) __attribute__((always_inline)) {
+        const TokenOwner o = owner_of(p.cu, p.n_seqs, tok);
+        k.owned = o.seq >= 0;
+        const int s = max(o.seq, 0);
+        k.pos = (int)((uint32_t)const_load(p.positions + s) + (uint32_t)(tok - o.first));
+        const int at = k.pos >> p.pages.page_log2;
+        int id = -1;
+        if (k.owned && k.pos >= 0 && at < p.pages.width) id = const_load(p.pages.table + (int64_t)s * p.pages.table_stride + at);
+        k.row_ok = (unsigned)id < (unsigned)p.pages.n_pages;
+        const int64_t row = (int64_t)id * p.pages.page_stride + (int64_t)(k.pos & ((1 << p.pages.page_log2) - 1)) * p.pages.row_stride;
+        k.ck = (short*)p.pages.k + row;
+        k.cv = (short*)p.pages.v + row;
     };
     auto token_at = [&](int tok) __attribute__((always_inline)) {
         Token k;
+        if (PAGED) {
+            k.xq = (short*)p.x + (int64_t)tok * p.H * p.D;
+            k.xk = (const short*)p.k + (int64_t)tok * p.Hkv * p.D;
+            k.xv = (const short*)p.v + (int64_t)tok * p.Hkv * p.D;
+            k.qk = k.qv = nullptr;
+            return k;
+        }
         const int b = __builtin_amdgcn_readfirstlane(tok / p.L), l = tok - b * p.L;
         // positions is an input nothing writes: read as constant memory the load is a scalar one, and waiting for it
         // does not wait for the chunk loads and stores in flight
@@ -156,7 +207,7 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
         return Slot{sect, i < n ? (uint32_t)hd << 16 | (uint32_t)(elem0 + 8 * (i - hd * per)) : ~0u};
     };
     auto live = [&](const Token& k, const Slot& s) __attribute__((always_inline)) {
-        return s.valid() && (s.sect == Q_ROT || k.row_ok);
+        return s.valid() && (s.sect == Q_ROT ? !PAGED || k.owned : k.row_ok);
     };
     // chunks in flight per thread and buffer: a NeoX rotary chunk is two 16-byte pieces, so half as many
     constexpr int UN = STYLE == ROPE_IL ? 4 : 2;
@@ -174,9 +225,10 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
             const Slot s = slots.s[u];
             const short* src = (s.sect == Q_ROT ? k.xq : s.sect == V_COPY ? k.xv : k.xk) + (s.hd() * p.D + s.elem());
             buf.lo[u] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (live(k, s)) buf.lo[u] = load_once<STREAM>(reinterpret_cast<const s16x8*>(src));
+            const bool wanted = PAGED ? s.valid() : live(k, s);   // (a packed token's row is there to be read, whoever it belongs to)
+            if (wanted) buf.lo[u] = load_once<STREAM>(reinterpret_cast<const s16x8*>(src));
             buf.hi[u] = buf.lo[u];
-            if (STYLE == ROPE_NEOX && live(k, s) && s.sect <= K_ROT) buf.hi[u] = load_once<STREAM>(reinterpret_cast<const s16x8*>(src + half_rd));
+            if (STYLE == ROPE_NEOX && wanted && s.sect <= K_ROT) buf.hi[u] = load_once<STREAM>(reinterpret_cast<const s16x8*>(src + half_rd));
         }
     };
     // 8 values to their place: as they are, or (Q8_0 cache) quantised with the block's three other lanes
@@ -201,7 +253,7 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
             const int elem = s.elem(), chunk = elem >> 3;
             if (s.sect == Q_ROT) dst = k.xq + (s.hd() * p.D + elem);
             else if (Q8) crow = (s.sect == V_COPY ? k.qv : k.qk) + s.hd() * p.c1;
-            else dst = (s.sect == V_COPY ? k.cv : k.ck) + (s.hd() * p.c1 + elem);
+            else dst = (s.sect == V_COPY ? k.cv : k.ck) + (s.hd() * head_stride + elem);
             s16x8 a = buf.lo[u];
             if (s.sect <= K_ROT) {
                 if (STYLE == ROPE_IL) {
@@ -252,8 +304,9 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
         Buffer buf;
         int parity = 0;
         for (; tok < tokens; tok += stride, parity ^= 1) {
-            const Token k = token_at(tok);
+            Token k = token_at(tok);
             request(k, first, buf);
+            if (PAGED) locate(k, tok);
             one_token(k, buf, parity);
         }
         return;
@@ -475,6 +528,242 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_append_kernel(const No
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// The producer into 8-bit pages (csrc/attn_paged.h).  A page's scale needs the largest of all its new rows, so a workgroup takes one page that
+// the call writes to, for HPW KV heads: D/8 lanes hold one row of one (head, tensor), 16 rows one after the other in registers, and
+// the groups of lanes that the heads leave over share the rows out (`parts`).  k is rotated as it is loaded; then the largest
+// magnitude, the scale, the codes.  Pages with more rows than parts * 16 go through their rows twice.  One workgroup reads, moves and writes
+// all of a (page, head)'s rows and its scale, so nothing depends on an order.  The launch's further workgroups rotate q, a token each.
+// ------------------------------------------------------------------------------------------------
+constexpr int kAppendRows = 16;   // rows a group of lanes holds
+
+struct Append8Params {
+    RopeParams r;
+    int hpw_log2, n_hg;    // KV heads per workgroup = 1 << hpw_log2, workgroups per page
+    int items;             // bound of the pages that the call writes to
+    int max_e;             // largest scale exponent: 448 * 2^max_e is a finite number of the activations' type
+};
+
+// Exponent of the scale that rows of largest finite magnitude amax need: the least e with amax <= 448 * 2^e = 1.75 * 2^(8 + e).
+MA_DEV int scale_exponent(float amax, int max_e) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, amax);
+    const int e = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
+    return min(max(amax > 0.f ? e : -100, -100), max_e);
+}
+MA_DEV float power_of_two(int e) { return __builtin_ldexpf(1.f, e); }
+// Eight values over 2^e (down = 2^-e) as e4m3 codes, cut to the largest; what is not finite becomes NaN.
+MA_DEV uint2 narrow8(const float (&f)[8], float down) {
+    float c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        c[i] = __builtin_fabsf(f[i]) < INFINITY ? __builtin_amdgcn_fmed3f(f[i] * down, -448.f, 448.f) : __builtin_nanf("");
+    uint2 r;
+    r.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false), true);
+    r.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[6], c[7], __builtin_amdgcn_cvt_pk_fp8_f32(c[4], c[5], 0, false), true);
+    return r;
+}
+// Four codes times a factor, a power of two below 1, as codes: exact unless they leave the normal numbers, where they are rounded.
+MA_DEV uint32_t move4(uint32_t codes, float factor) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[0] * factor, b[1] * factor, __builtin_amdgcn_cvt_pk_fp8_f32(a[0] * factor, a[1] * factor, 0, false), true);
+}
+
+template <class T, int STYLE, int D>
+__global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Params ap) {
+    const RopeParams& p = ap.r;
+    const PagedCache& pc = p.pages;
+    constexpr int GL = D / 8, NG = kRopeThreads / GL;   // lanes per row, groups of lanes
+    extern __shared__ f32x2 tab[];                       // [rows of a round][rd/2]: cosine and sine
+    __shared__ float most[NG];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int half_rd = p.rd >> 1;
+    const int S_log2 = pc.page_log2, S = 1 << S_log2;
+
+    if ((int)blockIdx.x >= ap.items * ap.n_hg) {   // ---- q: one token per workgroup and trip ----
+        const int cph = STYLE == ROPE_IL ? p.rd >> 3 : p.rd >> 4, n = p.H * cph;
+        const int q_wgs = (int)gridDim.x - ap.items * ap.n_hg;
+        for (int tok = (int)blockIdx.x - ap.items * ap.n_hg; tok < p.L; tok += q_wgs) {
+            const TokenOwner o = owner_of(p.cu, p.n_seqs, tok);
+            if (o.seq >= 0) {
+                const int pos = (int)((uint32_t)const_load(p.positions + o.seq) + (uint32_t)(tok - o.first));
+                if (tid < half_rd) tab[tid] = table_entry(p.inv_freq[tid], pos);
+            }
+            __syncthreads();
+            if (o.seq >= 0) {
+                short* xq = (short*)p.x + (int64_t)tok * p.H * D;
+                for (int i = tid; i < n; i += kRopeThreads) {
+                    const int hd = i / cph, chunk = i - hd * cph;
+                    short* at = xq + hd * D + 8 * chunk;
+                    s16x8 a = *reinterpret_cast<const s16x8*>(at);
+                    if (STYLE == ROPE_IL) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const f32x2 cs = tab[4 * chunk + j];
+                            const uint32_t pk = rotate_pair<T>(cs[0], cs[1], a[2 * j], a[2 * j + 1]);
+                            a[2 * j] = (short)(pk & 0xffffu);
+                            a[2 * j + 1] = (short)(pk >> 16);
+                        }
+                    } else {
+                        s16x8 b = *reinterpret_cast<const s16x8*>(at + half_rd);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const f32x2 cs = tab[8 * chunk + j];
+                            const uint32_t pk = rotate_pair<T>(cs[0], cs[1], a[j], b[j]);
+                            a[j] = (short)(pk & 0xffffu);
+                            b[j] = (short)(pk >> 16);
+                        }
+                        *reinterpret_cast<s16x8*>(at + half_rd) = b;
+                    }
+                    *reinterpret_cast<s16x8*>(at) = a;
+                }
+            }
+            __syncthreads();   // the table is written again
+        }
+        return;
+    }
+
+    // ---- a page: the x-th that the call writes to, counted sequence by sequence ----
+    int x = (int)blockIdx.x / ap.n_hg;
+    const int hg = (int)blockIdx.x - x * ap.n_hg;
+    int seq = -1, first_tok = 0, pos0 = 0, a = 0, b = 0;
+    for (int base = 0; base < p.n_seqs; base += 64) {
+        const int s = base + lane;
+        TokenRange r{0, 0};
+        int at = 0, lo = 0, hi = 0;
+        if (s < p.n_seqs) {
+            r = token_range(p.cu[s], p.cu[s + 1], p.L);
+            at = p.positions[s];
+            lo = max(at, 0);                                                        // rows lo .. hi - 1 of the sequence are written
+            hi = (int)min((int64_t)at + r.len, (int64_t)pc.width << S_log2);
+        }
+        const int n = hi > lo ? ((hi - 1) >> S_log2) - (lo >> S_log2) + 1 : 0;
+        const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
+        if (x < total) {
+            const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
+            seq = base + src;
+            x -= lane_value(incl - n, src);
+            first_tok = lane_value(r.lo, src);
+            pos0 = lane_value(at, src);
+            a = lane_value(lo, src);
+            b = lane_value(hi, src);
+            break;
+        }
+        x -= total;
+    }
+    if (seq < 0) return;
+    const int page = (a >> S_log2) + x;
+    const int id = const_load(pc.table + (int64_t)seq * pc.table_stride + page);
+    if ((unsigned)id >= (unsigned)pc.n_pages) return;
+    const int row_lo = max(a, page << S_log2), row_hi = min(b, (page + 1) << S_log2), n_rows = row_hi - row_lo;
+    const int n_old = row_lo - (page << S_log2);   // rows that the page holds already
+
+    const int c = tid & (GL - 1), gi = tid / GL;   // chunk of the row: elements 8c .. 8c + 7; group of lanes
+    const int units = 2 << ap.hpw_log2, parts = NG / units;
+    const int unit = gi & (units - 1), part = gi / units;
+    const bool is_v = (unit >> ap.hpw_log2) != 0;
+    const int head = (hg << ap.hpw_log2) + (unit & ((1 << ap.hpw_log2) - 1));
+    const bool on = head < p.Hkv;
+    const int rot_chunks = STYLE == ROPE_IL ? p.rd >> 3 : p.rd >> 4;
+    const bool hi_half = STYLE == ROPE_NEOX && c >= rot_chunks;              // holds the second elements of its pairs
+    const bool rotates = !is_v && (STYLE == ROPE_IL ? c < rot_chunks : c < 2 * rot_chunks);
+    const int pair0 = STYLE == ROPE_IL ? 4 * c : 8 * (hi_half ? c - rot_chunks : c);
+    const int partner = hi_half ? -half_rd : half_rd;                        // NeoX: where the other elements of the pairs are
+    const int64_t tok0 = first_tok + (row_lo - pos0);
+    const short* src = (const short*)(is_v ? p.v : p.k) + (tok0 * p.Hkv + (on ? head : 0)) * D + 8 * c;
+    char* rows = (char*)(is_v ? pc.v : pc.k) + (int64_t)id * pc.page_stride + (int64_t)(on ? head : 0) * pc.head_stride + 8 * c;
+    uint8_t* scale_at = (is_v ? pc.v_scales : pc.k_scales) + (int64_t)id * p.Hkv + (on ? head : 0);
+    const int e_held = n_old > 0 ? (int)*scale_at - 127 : -128;              // a page's first rows ask nobody
+
+    const int per_round = kAppendRows * parts, rounds = (n_rows + per_round - 1) / per_round;
+    s16x8 xs[kAppendRows];
+    // rows part, part + parts, .. of a round, rotated; those past the last row are zero
+    auto load_round = [&](int round) __attribute__((always_inline)) {
+        const int r0 = round * per_round;
+        __syncthreads();   // the table of the round before has been read
+        for (int i = tid; i < min(per_round, n_rows - r0) * half_rd; i += kRopeThreads) {
+            const int row = i / half_rd, pair = i - row * half_rd;
+            tab[i] = table_entry(p.inv_freq[pair], row_lo + r0 + row);
+        }
+#pragma unroll
+        for (int i = 0; i < kAppendRows; ++i) {
+            const int row = r0 + part + i * parts;
+            xs[i] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (on && row < n_rows) xs[i] = *reinterpret_cast<const s16x8*>(src + (int64_t)row * p.Hkv * D);
+        }
+        __syncthreads();
+        if (on && rotates) {
+#pragma unroll
+            for (int i = 0; i < kAppendRows; ++i) {
+                const int row = part + i * parts;
+                if (r0 + row >= n_rows) continue;
+                const f32x2* cs = tab + row * half_rd + pair0;
+                uint32_t r[4];
+                if (STYLE == ROPE_IL) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r[j] = rotate_pair<T>(cs[j][0], cs[j][1], xs[i][2 * j], xs[i][2 * j + 1]);
+                } else {
+                    const s16x8 o = *reinterpret_cast<const s16x8*>(src + (int64_t)(r0 + row) * p.Hkv * D + partner);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float s0 = cs[2 * j][1], s1 = cs[2 * j + 1][1];
+                        r[j] = T::pack2(rotate_one<T>(cs[2 * j][0], hi_half ? s0 : -s0, xs[i][2 * j], o[2 * j]),
+                                        rotate_one<T>(cs[2 * j + 1][0], hi_half ? s1 : -s1, xs[i][2 * j + 1], o[2 * j + 1]));
+                    }
+                }
+                xs[i] = __builtin_bit_cast(s16x8, u32x4{r[0], r[1], r[2], r[3]});
+            }
+        }
+    };
+    float amax = 0.f;
+    for (int round = 0; round < rounds; ++round) {
+        load_round(round);
+#pragma unroll
+        for (int i = 0; i < kAppendRows; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float f = __builtin_fabsf(T::to_float(xs[i][j]));
+                amax = f < INFINITY ? fmaxf(amax, f) : amax;
+            }
+    }
+    // over the lanes of the row, then over the parts
+    amax = fmaxf(amax, row_exchange<0xb1>(amax));
+    amax = fmaxf(amax, row_exchange<0x4e>(amax));
+    amax = fmaxf(amax, row_exchange<0x141>(amax));
+    if (GL > 8) amax = fmaxf(amax, row_exchange<0x140>(amax));
+    if (c == 0) most[gi] = amax;
+    __syncthreads();
+    for (int i = 0; i < parts; ++i) amax = fmaxf(amax, most[i * units + unit]);
+    const int e = max(e_held, scale_exponent(amax, ap.max_e));
+    if (on && part == 0 && c == 0) *scale_at = (uint8_t)(e + 127);
+    if (on && n_old > 0 && e > e_held) {
+        const float factor = power_of_two(e_held - e);
+        for (int row = part; row < n_old; row += parts) {
+            uint2* at = reinterpret_cast<uint2*>(rows + row * (int)pc.row_stride);
+            uint2 codes = *at;
+            codes.x = move4(codes.x, factor);
+            codes.y = move4(codes.y, factor);
+            *at = codes;
+        }
+    }
+    const float down = e == 128 ? __builtin_nanf("") : power_of_two(-e);
+    auto store_round = [&](int round) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kAppendRows; ++i) {
+            const int row = round * per_round + part + i * parts;
+            if (!on || row >= n_rows) continue;
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = T::to_float(xs[i][j]);
+            *reinterpret_cast<uint2*>(rows + (n_old + row) * (int)pc.row_stride) = narrow8(f, down);
+        }
+    };
+    store_round(rounds - 1);   // the last round's rows are still there
+    for (int round = 0; round + 1 < rounds; ++round) {
+        load_round(round);
+        store_round(round);
+    }
+}
+
 // freq_base^(-2 i / rotary_dim) in fp64.  The powers are 64 of them at head_dim 128, 0.7 of the 6.7 us that issuing the append takes with
 // them, and the same for every layer and token of a model: a thread keeps the last table it made.
 static void inverse_frequencies(double* out, int64_t rotary_dim, double freq_base) {
@@ -513,26 +802,26 @@ static bool vector_ok(int style, int64_t D, int64_t rd) {
     return D % 8 == 0 && rd % (style == ROPE_IL ? 8 : 16) == 0;
 }
 
-template <bool FUSED, bool Q8, bool STREAM>
+template <bool FUSED, bool Q8, bool STREAM, bool PAGED>
 static void launch_rope_as(int dtype, int style, const RopeParams& p, int grid, hipStream_t stream) {
     if (dtype == MINFER_ATTN_F16) {
-        if (style == ROPE_IL) hipLaunchKernelGGL((rope_kernel<F16, ROPE_IL, FUSED, Q8, STREAM>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
-        else hipLaunchKernelGGL((rope_kernel<F16, ROPE_NEOX, FUSED, Q8, STREAM>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
+        if (style == ROPE_IL) hipLaunchKernelGGL((rope_kernel<F16, ROPE_IL, FUSED, Q8, STREAM, PAGED>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
+        else hipLaunchKernelGGL((rope_kernel<F16, ROPE_NEOX, FUSED, Q8, STREAM, PAGED>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
     } else {
-        if (style == ROPE_IL) hipLaunchKernelGGL((rope_kernel<BF16, ROPE_IL, FUSED, Q8, STREAM>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
-        else hipLaunchKernelGGL((rope_kernel<BF16, ROPE_NEOX, FUSED, Q8, STREAM>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
+        if (style == ROPE_IL) hipLaunchKernelGGL((rope_kernel<BF16, ROPE_IL, FUSED, Q8, STREAM, PAGED>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
+        else hipLaunchKernelGGL((rope_kernel<BF16, ROPE_NEOX, FUSED, Q8, STREAM, PAGED>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
     }
 }
 
-template <bool FUSED, bool Q8 = false>
+template <bool FUSED, bool Q8 = false, bool PAGED = false>
 static int launch_rope(int dtype, int style, const RopeParams& p, hipStream_t stream) {
     const int tokens = p.B * p.L;
     const int grid = std::min(tokens, 256 * 16);
     // distinct bytes the launch touches: q's rotary part (in place), and for the producer k, v and their cache rows
     int64_t touched = (int64_t)tokens * p.H * p.rd * 2;
     if (FUSED) touched += (int64_t)tokens * p.Hkv * p.D * 2 * (Q8 ? 3 : 4);
-    if (touched > kStreamBytes) launch_rope_as<FUSED, Q8, true>(dtype, style, p, grid, stream);
-    else launch_rope_as<FUSED, Q8, false>(dtype, style, p, grid, stream);
+    if (touched > kStreamBytes) launch_rope_as<FUSED, Q8, true, PAGED>(dtype, style, p, grid, stream);
+    else launch_rope_as<FUSED, Q8, false, PAGED>(dtype, style, p, grid, stream);
     return check_launch("rope_kernel");
 }
 
@@ -670,4 +959,55 @@ MINFER_ATTN_EXPORT int minfer_rope_kv_append_norm(int dtype, int style, int cach
         else { if (q8) launch_norm_append_as<BF16, ROPE_NEOX, true>(np, (int)D, hint, grid, stream); else launch_norm_append_as<BF16, ROPE_NEOX, false>(np, (int)D, hint, grid, stream); }
     }
     return check_launch("rope_norm_append_kernel");
+}
+
+MINFER_ATTN_EXPORT int minfer_rope_kv_append_paged(int dtype, int style, int page_type, void* q, const void* k, const void* v,
+                                                   const int32_t* cu_seqlens, const int32_t* positions, const minfer_kv_pages* pages,
+                                                   int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rotary_dim,
+                                                   double freq_base, void* stream_v) {
+    clear_error();
+    Append8Params ap{};
+    RopeParams& p = ap.r;
+    if (int rc = fill_rope(p, dtype, style, 1, T, Hq, D, rotary_dim, freq_base, "rope_kv_append_paged")) return rc;
+    if (int rc = check_pages("rope_kv_append_paged", dtype, page_type, pages, n_seqs, Hkv, D, p.pages)) return rc;
+    const bool eight = page_type == MINFER_FP8_E4M3;
+    auto bad = [&](const char* what) { return fail(MINFER_ATTN_EINVAL, what); };
+    if (n_seqs < 0 || n_seqs > (1 << 24) || T > (1 << 30)) return bad("rope_kv_append_paged: bad number of sequences or tokens");
+    // (what is written may not lie on itself; readers take any strides)
+    if (pages->n_pages > 0 && (pages->stride_row < D || (Hkv > 1 && pages->stride_head <= 0) || (pages->n_pages > 1 && pages->stride_page <= 0)))
+        return bad("rope_kv_append_paged: pages must not overlap");
+    if (!vector_ok(style, D, rotary_dim)) return bad("rope_kv_append_paged: rotary_dim must be a multiple of 8 (interleaved) or 16 (NeoX)");
+    if (n_seqs == 0 || T == 0) return MINFER_ATTN_OK;
+    if (!q || !k || !v || !cu_seqlens || !positions) return bad("rope_kv_append_paged: null pointer");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return bad("rope_kv_append_paged: q, k and v must be 16-byte aligned");
+    p.x = q; p.k = k; p.v = v; p.positions = positions; p.cu = cu_seqlens; p.n_seqs = (int)n_seqs; p.Hkv = (int)Hkv;
+    hipStream_t stream = (hipStream_t)stream_v;
+    if (!eight) return launch_rope<true, false, true>(dtype, style, p, stream);
+
+    const int64_t S = pages->page_size;
+    const int64_t items = p.pages.width > 0 ? std::min(T, T / S + 2 * n_seqs) : 0;
+    // KV heads per workgroup: all the groups of lanes have a row where pages get few rows; where they get many, fewer heads and more rows
+    // at a time (two heads at least: a round's table of angles is then 32 KiB at most)
+    const int64_t rows = std::min(S, T / n_seqs + 1);
+    const int groups = kRopeThreads / ((int)D / 8);
+    int hpw_log2 = 3;
+    while (hpw_log2 > 1 && ((1 << hpw_log2) >= 2 * Hkv || rows > kAppendRows * groups / (2 << hpw_log2))) --hpw_log2;
+    ap.hpw_log2 = hpw_log2;
+    ap.n_hg = (int)((Hkv + (1 << hpw_log2) - 1) >> hpw_log2);
+    ap.items = (int)items;
+    ap.max_e = dtype == MINFER_ATTN_F16 ? 7 : 119;
+    const int64_t q_wgs = std::min<int64_t>(T, 256 * 16), grid = items * ap.n_hg + q_wgs;
+    if (grid > 0x7fffffffLL) return bad("rope_kv_append_paged: problem too large for one launch");
+    const int parts = groups / (2 << hpw_log2);
+    const size_t lds = (size_t)std::max<int64_t>(1, std::min<int64_t>(kAppendRows * parts, S)) * (rotary_dim / 2) * sizeof(f32x2) + sizeof(f32x2);
+#define MINFER_APPEND8(T_, STYLE_) \
+    if (D == 128) hipLaunchKernelGGL((append8_kernel<T_, STYLE_, 128>), dim3((unsigned)grid), dim3(kRopeThreads), lds, stream, ap); \
+    else hipLaunchKernelGGL((append8_kernel<T_, STYLE_, 64>), dim3((unsigned)grid), dim3(kRopeThreads), lds, stream, ap)
+    if (dtype == MINFER_ATTN_F16) {
+        if (style == ROPE_IL) { MINFER_APPEND8(F16, ROPE_IL); } else { MINFER_APPEND8(F16, ROPE_NEOX); }
+    } else {
+        if (style == ROPE_IL) { MINFER_APPEND8(BF16, ROPE_IL); } else { MINFER_APPEND8(BF16, ROPE_NEOX); }
+    }
+#undef MINFER_APPEND8
+    return check_launch("append8_kernel");
 }

@@ -48,7 +48,8 @@ void* current_stream() {
 // as ScalarType and Device they go through the translation of an argument (25 and 16 ns; of the 6 to 7 us that issuing an operator takes
 // 0.1 to 0.3).
 const int32_t kHalf = aoti_torch_dtype_float16(), kBFloat16 = aoti_torch_dtype_bfloat16(), kFloat = aoti_torch_dtype_float32(),
-              kByte = aoti_torch_dtype_uint8(), kInt = aoti_torch_dtype_int32(), kBool = aoti_torch_dtype_bool();
+              kByte = aoti_torch_dtype_uint8(), kInt = aoti_torch_dtype_int32(), kBool = aoti_torch_dtype_bool(),
+              kE4m3 = aoti_torch_dtype_float8_e4m3fn(), kE8m0 = (int32_t)ScalarType::Float8_e8m0fnu;   // (the ABI has no name for the last)
 
 // The types that these operators take; Undefined for any other.
 ScalarType type_of(const Tensor& t) {
@@ -59,6 +60,8 @@ ScalarType type_of(const Tensor& t) {
     if (d == kByte) return ScalarType::Byte;
     if (d == kInt) return ScalarType::Int;
     if (d == kBool) return ScalarType::Bool;
+    if (d == kE4m3) return ScalarType::Float8_e4m3fn;
+    if (d == kE8m0) return ScalarType::Float8_e8m0fnu;
     return d == kFloat ? ScalarType::Float : ScalarType::Undefined;
 }
 
@@ -438,6 +441,150 @@ void rope_kv_append_norm_hip(int64_t style, int64_t rotary_dim, double freq_base
              "rope_kv_append_norm");
 }
 
+// ---- operators over a paged cache --------------------------------------------------------------------------------
+// The pools are [n_pages, n_kv_heads, page_size, head_dim] and the table [n_seqs, pages per sequence] int32; 8-bit pools are float8_e4m3fn with
+// float8_e8m0fnu scales [n_pages, n_kv_heads].  No counterpart in the reference.
+namespace {
+// The tensors' device as the current one, for the launch and its stream, where it is not already.
+class OnDeviceOf {
+public:
+    explicit OnDeviceOf(const Tensor& t) {
+        if (t.get_device_index() != torch::stable::accelerator::getCurrentDeviceIndex()) guard_.emplace(t.get_device_index());
+    }
+
+private:
+    std::optional<torch::stable::accelerator::DeviceGuard> guard_;
+};
+
+struct ScalePair { const Tensor* k; const Tensor* v; };   // null: 16-bit pages
+
+int activation_code(const Tensor& q, const char* op) {
+    const ScalarType t = type_of(q);
+    STD_TORCH_CHECK(t == ScalarType::Half || t == ScalarType::BFloat16, op, ": q must be float16 or bfloat16");
+    return t == ScalarType::Half ? MINFER_ATTN_F16 : MINFER_ATTN_BF16;
+}
+
+void check_index(const Tensor& t, int64_t n, const Tensor& q, const char* op, const char* name) {
+    STD_TORCH_CHECK(t.is_cuda() && t.get_device_index() == q.get_device_index(), op, ": ", name, " must be on q's device");
+    STD_TORCH_CHECK(type_of(t) == ScalarType::Int && t.dim() == 1 && t.is_contiguous() && t.size(0) == n, op, ": ", name,
+                    " must be contiguous int32 with ", n, " entries");
+}
+
+minfer_kv_pages pages_of(const Tensor& q, int64_t n_seqs, int64_t D, const Tensor& block_table, const Tensor& k_pages, const Tensor& v_pages,
+                         ScalePair scales, const char* op) {
+    STD_TORCH_CHECK(k_pages.is_cuda() && v_pages.is_cuda() && block_table.is_cuda() && k_pages.get_device_index() == q.get_device_index() &&
+                    v_pages.get_device_index() == q.get_device_index() && block_table.get_device_index() == q.get_device_index(),
+                    op, ": the pages and block_table must be on q's device");
+    STD_TORCH_CHECK(type_of(k_pages) == (scales.k ? ScalarType::Float8_e4m3fn : type_of(q)) && type_of(v_pages) == type_of(k_pages), op,
+                    scales.k ? ": k_pages and v_pages must be float8_e4m3fn" : ": k_pages and v_pages must have q's dtype");
+    STD_TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 4 && k_pages.sizes().equals(v_pages.sizes()) && k_pages.size(3) == D, op,
+                    ": expected k_pages and v_pages [n_pages, n_kv_heads, page_size, head_dim]");
+    STD_TORCH_CHECK(k_pages.stride(3) == 1 && v_pages.stride(3) == 1 && k_pages.stride(0) == v_pages.stride(0) &&
+                    k_pages.stride(1) == v_pages.stride(1) && k_pages.stride(2) == v_pages.stride(2), op,
+                    ": the pages must be contiguous in head_dim and share strides");
+    STD_TORCH_CHECK(type_of(block_table) == ScalarType::Int && block_table.dim() == 2 && block_table.size(0) == n_seqs &&
+                    (block_table.size(1) <= 1 || block_table.stride(1) == 1), op,
+                    ": block_table must be int32 [n_seqs, pages per sequence], contiguous in its last dimension");
+    minfer_kv_pages r{};
+    r.k = const_cast<void*>(k_pages.const_data_ptr());
+    r.v = const_cast<void*>(v_pages.const_data_ptr());
+    if (scales.k) {
+        for (const Tensor* t : {scales.k, scales.v})
+            STD_TORCH_CHECK(t->is_cuda() && t->get_device_index() == q.get_device_index() && type_of(*t) == ScalarType::Float8_e8m0fnu &&
+                            t->dim() == 2 && t->is_contiguous() && t->size(0) == k_pages.size(0) && t->size(1) == k_pages.size(1), op,
+                            ": k_scales and v_scales must be contiguous float8_e8m0fnu [n_pages, n_kv_heads] on q's device");
+        r.k_scales = const_cast<void*>(scales.k->const_data_ptr());
+        r.v_scales = const_cast<void*>(scales.v->const_data_ptr());
+    }
+    r.n_pages = k_pages.size(0);
+    r.page_size = k_pages.size(2);
+    r.stride_page = k_pages.stride(0); r.stride_head = k_pages.stride(1); r.stride_row = k_pages.stride(2);
+    r.block_table = static_cast<const int32_t*>(block_table.const_data_ptr());
+    r.table_stride = block_table.stride(0);
+    r.pages_per_seq = block_table.size(1);
+    return r;
+}
+
+void append_paged(const char* op, int64_t style, int64_t rotary_dim, double freq_base, Tensor& q, const Tensor& k, const Tensor& v,
+                  const Tensor& cu_seqlens, const Tensor& positions, const Tensor& block_table, Tensor& k_pages, Tensor& v_pages, ScalePair scales) {
+    STD_TORCH_CHECK(on_gpu(q) && on_gpu(k) && on_gpu(v) && k.get_device_index() == q.get_device_index() && v.get_device_index() == q.get_device_index(),
+                    op, ": all tensors must be on one GPU");
+    const int dtype = activation_code(q, op);
+    STD_TORCH_CHECK(type_of(k) == type_of(q) && type_of(v) == type_of(q), op, ": q, k and v must share one dtype");
+    STD_TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && q.is_contiguous() && k.is_contiguous() && v.is_contiguous(), op,
+                    ": q, k and v must be 4-D and contiguous");
+    STD_TORCH_CHECK(q.size(0) == 1 && k.size(0) == 1 && k.sizes().equals(v.sizes()) && q.size(1) == k.size(1) && q.size(3) == k.size(3), op,
+                    ": expected q [1,T,Hq,D], k/v [1,T,Hkv,D]");
+    STD_TORCH_CHECK(style == MINFER_ROPE_INTERLEAVED || style == MINFER_ROPE_NEOX, op, ": style must be 0 (interleaved) or 1 (NeoX)");
+    STD_TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) >= 1, op, ": cu_seqlens must be 1-D with at least one entry");
+    const int64_t n_seqs = cu_seqlens.size(0) - 1, T = q.size(1), D = q.size(3);
+    check_index(cu_seqlens, n_seqs + 1, q, op, "cu_seqlens");
+    check_index(positions, n_seqs, q, op, "positions");
+    const minfer_kv_pages pages = pages_of(q, n_seqs, D, block_table, k_pages, v_pages, scales, op);
+    STD_TORCH_CHECK(k_pages.size(1) == k.size(2), op, ": the pages' number of heads is not k's");
+    STD_TORCH_CHECK(rotary_dim <= D, op, ": rotary_dim exceeds head_dim");
+    if (T == 0 || n_seqs == 0) return;
+    const OnDeviceOf on(q);
+    check_rc(minfer_rope_kv_append_paged(dtype, (int)style, scales.k ? MINFER_FP8_E4M3 : dtype, q.mutable_data_ptr(), k.const_data_ptr(),
+                                         v.const_data_ptr(), static_cast<const int32_t*>(cu_seqlens.const_data_ptr()),
+                                         static_cast<const int32_t*>(positions.const_data_ptr()), &pages, n_seqs, T, q.size(2), k.size(2), D,
+                                         rotary_dim, freq_base, current_stream()),
+             op);
+}
+
+void attend_paged(const char* op, int64_t qtype_int, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, ScalePair scales,
+                  const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& ctx_lens, int64_t max_q_len, Tensor& out) {
+    STD_TORCH_CHECK(on_gpu(q) && on_gpu(out) && out.get_device_index() == q.get_device_index(), op, ": all tensors must be on one GPU");
+    STD_TORCH_CHECK(qtype_int != MINFER_Q8_0, op, ": pages of Q8_0 blocks are not built; 8-bit pages are float8_e4m3fn (flash_attn_paged_fp8)");
+    const int dtype = activation_code(q, op);
+    STD_TORCH_CHECK(type_of(out) == type_of(q), op, ": q and out must share one dtype");
+    STD_TORCH_CHECK(q.dim() == 4 && out.dim() == 4 && q.sizes().equals(out.sizes()) && q.size(0) == 1, op, ": expected q and out [1,Hq,T,D]");
+    STD_TORCH_CHECK(q.stride(3) == 1 && out.stride(3) == 1, op, ": q and out must be contiguous in head_dim");
+    STD_TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) >= 1, op, ": cu_seqlens must be 1-D with at least one entry");
+    STD_TORCH_CHECK(max_q_len >= 0, op, ": max_q_len must not be negative");
+    const int64_t n_seqs = cu_seqlens.size(0) - 1, Hq = q.size(1), T = q.size(2), D = q.size(3);
+    check_index(cu_seqlens, n_seqs + 1, q, op, "cu_seqlens");
+    check_index(ctx_lens, n_seqs, q, op, "ctx_lens");
+    const minfer_kv_pages pages = pages_of(q, n_seqs, D, block_table, k_pages, v_pages, scales, op);
+    const int64_t Hkv = k_pages.size(1);
+    STD_TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0, op, ": n_heads must be a multiple of n_kv_heads");
+    if (T == 0 || n_seqs == 0) return;
+    const OnDeviceOf on(q);
+    const minfer_attn_strides st{0, q.stride(1), q.stride(2), 0, 0, 0, 0, out.stride(1), out.stride(2)};
+    const size_t ws_bytes = minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, pages.n_pages > 0 ? pages.pages_per_seq * pages.page_size : 0, max_q_len);
+    const Workspace ws(q, ws_bytes);
+    check_rc(minfer_flash_attn_paged(dtype, scales.k ? MINFER_FP8_E4M3 : dtype, q.const_data_ptr(), &pages,
+                                     static_cast<const int32_t*>(cu_seqlens.const_data_ptr()), static_cast<const int32_t*>(ctx_lens.const_data_ptr()),
+                                     out.mutable_data_ptr(), n_seqs, T, Hq, Hkv, D, max_q_len, &st, ws.ptr(), ws_bytes, current_stream()),
+             op);
+}
+}  // namespace
+
+// rope(q) in place, rope(k) and v into the pages, for packed tokens (q [1, T, n_heads, head_dim], k and v [1, T, n_kv_heads, head_dim];
+// cu_seqlens [n_seqs + 1]; positions [n_seqs]: rows that each sequence already holds).
+void rope_kv_append_paged_hip(int64_t style, int64_t rotary_dim, double freq_base, Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_seqlens,
+                              const Tensor& positions, const Tensor& block_table, Tensor& k_pages, Tensor& v_pages) {
+    append_paged("rope_kv_append_paged", style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions, block_table, k_pages, v_pages, ScalePair{nullptr, nullptr});
+}
+void rope_kv_append_paged_fp8_hip(int64_t style, int64_t rotary_dim, double freq_base, Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_seqlens,
+                                  const Tensor& positions, const Tensor& block_table, Tensor& k_pages, Tensor& v_pages, Tensor& k_scales, Tensor& v_scales) {
+    append_paged("rope_kv_append_paged_fp8", style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions, block_table, k_pages, v_pages, ScalePair{&k_scales, &v_scales});
+}
+
+// Attention of packed tokens over the pages, their own rows among them (q and out [1, n_heads, T, head_dim]; ctx_lens [n_seqs]: rows that each
+// sequence holds with its new ones).
+void flash_attn_paged_hip(int64_t qtype_int, int64_t qblock_size, int64_t qtype_size, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                          const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& ctx_lens, int64_t max_q_len, Tensor& out) {
+    (void)qblock_size; (void)qtype_size;
+    attend_paged("flash_attn_paged", qtype_int, q, k_pages, v_pages, ScalePair{nullptr, nullptr}, block_table, cu_seqlens, ctx_lens, max_q_len, out);
+}
+void flash_attn_paged_fp8_hip(int64_t qtype_int, int64_t qblock_size, int64_t qtype_size, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                              const Tensor& k_scales, const Tensor& v_scales, const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& ctx_lens,
+                              int64_t max_q_len, Tensor& out) {
+    (void)qblock_size; (void)qtype_size;
+    attend_paged("flash_attn_paged_fp8", qtype_int, q, k_pages, v_pages, ScalePair{&k_scales, &v_scales}, block_table, cu_seqlens, ctx_lens, max_q_len, out);
+}
+
 // Same signature, argument meaning and checks as the reference's rmsnorm_cuda
 // (reference: src/minfer/kernels/torch_ext/csrc/cuda/rmsnorm/op.cuh:20-70); bfloat16 is admitted as well.
 void rmsnorm_hip(double eps,
@@ -665,6 +812,10 @@ STABLE_TORCH_LIBRARY(minfer, m) {
     m.def("flash_attn_varlen(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, Tensor(a!) out) -> ()");
     m.def("rope_kv_append(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor positions, Tensor(b!) k_cache, Tensor(c!) v_cache) -> ()");
     m.def("rope_kv_append_norm(int style, int rotary_dim, float freq_base, float eps, Tensor(a!) q, Tensor k, Tensor v, Tensor wq_norm, Tensor wk_norm, Tensor positions, Tensor(b!) k_cache, Tensor(c!) v_cache) -> ()");
+    m.def("rope_kv_append_paged(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor positions, Tensor block_table, Tensor(b!) k_pages, Tensor(c!) v_pages) -> ()");
+    m.def("rope_kv_append_paged_fp8(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor positions, Tensor block_table, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor(d!) k_scales, Tensor(e!) v_scales) -> ()");
+    m.def("flash_attn_paged(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cu_seqlens, Tensor ctx_lens, int max_q_len, Tensor(a!) out) -> ()");
+    m.def("flash_attn_paged_fp8(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor cu_seqlens, Tensor ctx_lens, int max_q_len, Tensor(a!) out) -> ()");
 }
 
 STABLE_TORCH_LIBRARY_IMPL(minfer, CUDA, m) {  // "CUDA" is PyTorch's dispatch-key name for ROCm devices too
@@ -680,6 +831,10 @@ STABLE_TORCH_LIBRARY_IMPL(minfer, CUDA, m) {  // "CUDA" is PyTorch's dispatch-ke
     m.impl("neox_rope", TORCH_BOX(&neox_rope_hip));
     m.impl("rope_kv_append", TORCH_BOX(&rope_kv_append_hip));
     m.impl("rope_kv_append_norm", TORCH_BOX(&rope_kv_append_norm_hip));
+    m.impl("rope_kv_append_paged", TORCH_BOX(&rope_kv_append_paged_hip));
+    m.impl("rope_kv_append_paged_fp8", TORCH_BOX(&rope_kv_append_paged_fp8_hip));
+    m.impl("flash_attn_paged", TORCH_BOX(&flash_attn_paged_hip));
+    m.impl("flash_attn_paged_fp8", TORCH_BOX(&flash_attn_paged_fp8_hip));
 }
 
 }  // namespace minfer

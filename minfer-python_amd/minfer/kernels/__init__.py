@@ -6,8 +6,9 @@ projection and rotary-embedding steps that feed it, and the Q8_0 quantisers of i
 class KernelBackend:
     def __init__(self, backend: str):
         if backend == "torch_ext":
-            from .torch_ext import (_dequant, _quant, flash_attn, flash_attn_decode, flash_attn_varlen, gemm, il_rope,
-                                    neox_rope, qkv, rmsnorm, rope_kv_append, rope_kv_append_norm)
+            from .torch_ext import (_dequant, _quant, flash_attn, flash_attn_decode, flash_attn_paged, flash_attn_paged_fp8,
+                                    flash_attn_varlen, gemm, il_rope, neox_rope, qkv, rmsnorm, rope_kv_append,
+                                    rope_kv_append_norm, rope_kv_append_paged, rope_kv_append_paged_fp8)
             self._dequant = _dequant
             self._quant = _quant
             self.rmsnorm = rmsnorm
@@ -20,5 +21,9 @@ class KernelBackend:
             self.flash_attn = flash_attn
             self.flash_attn_decode = flash_attn_decode
             self.flash_attn_varlen = flash_attn_varlen
+            self.rope_kv_append_paged = rope_kv_append_paged
+            self.rope_kv_append_paged_fp8 = rope_kv_append_paged_fp8
+            self.flash_attn_paged = flash_attn_paged
+            self.flash_attn_paged_fp8 = flash_attn_paged_fp8
         else:
             raise ValueError(f"KernelBackend init: unsupported backend {backend}")

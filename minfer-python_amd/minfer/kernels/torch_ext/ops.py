@@ -206,6 +206,133 @@ def _(style, rotary_dim, freq_base, eps, q, k, v, wq_norm, wk_norm, positions, k
     torch._check(rotary_dim <= q.size(3))
 
 
+def _check_pages(q, k_pages, v_pages, scales, block_table, cu_seqlens, lens):
+    page_dtype = q.dtype if scales is None else torch.float8_e4m3fn
+    torch._check(q.dtype in _ACT_DTYPES)
+    torch._check(k_pages.dtype == page_dtype and v_pages.dtype == page_dtype)
+    torch._check(all(t.dtype == torch.int32 for t in (block_table, cu_seqlens, lens)))
+    torch._check(all(t.device == q.device for t in (k_pages, v_pages, block_table, cu_seqlens, lens)))
+    torch._check(q.device.type == "cuda")
+    torch._check(q.dim() == 4 and k_pages.dim() == 4 and v_pages.dim() == 4 and block_table.dim() == 2)
+    torch._check(cu_seqlens.dim() == 1 and lens.dim() == 1)
+    if scales is not None:
+        torch._check(all(t.dtype == torch.float8_e8m0fnu and t.dim() == 2 and t.device == q.device for t in scales))
+
+
+def rope_kv_append_paged(
+    style: int,
+    rotary_dim: int,
+    freq_base: float,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    positions: torch.Tensor,
+    block_table: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+):
+    """rope_kv_append into a paged cache, for packed tokens: rotates q [1,T,n_heads,D] in place and writes the rotated
+    k [1,T,n_kv_heads,D] and v into k_pages/v_pages [n_pages,n_kv_heads,page_size,D].  Tokens cu_seqlens[s] ..
+    cu_seqlens[s+1]-1 are sequence s's rows positions[s], positions[s]+1, ..; row r lies in page block_table[s, r // page_size]
+    at row r % page_size.  All index tensors int32 (cu_seqlens [n_seqs+1], positions [n_seqs], block_table [n_seqs, pages]).
+    A table entry outside the pool (-1) means no page: its rows are not written.  page_size is a power of two in 16..1024."""
+    return torch.ops.minfer.rope_kv_append_paged.default(style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions,
+                                                         block_table, k_pages, v_pages)
+
+
+@torch.library.register_fake("minfer::rope_kv_append_paged")
+def _(style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions, block_table, k_pages, v_pages):
+    _check_pages(q, k_pages, v_pages, None, block_table, cu_seqlens, positions)
+    torch._check(k.dtype == q.dtype and v.dtype == q.dtype and k.dim() == 4 and v.dim() == 4)
+    torch._check(rotary_dim <= q.size(3))
+
+
+def rope_kv_append_paged_fp8(
+    style: int,
+    rotary_dim: int,
+    freq_base: float,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    positions: torch.Tensor,
+    block_table: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+):
+    """rope_kv_append_paged into 8-bit pages: float8_e4m3fn codes with a power of two as the scale of each page and head
+    (float8_e8m0fnu [n_pages,n_kv_heads]), the smallest with which the page's rows fit.  A page that gets its row 0 starts
+    with the scale its new rows need; in a page that goes on, the scale grows if they need it, and the codes that are there
+    move to it.  A page that a call writes to belongs to one sequence of that call."""
+    return torch.ops.minfer.rope_kv_append_paged_fp8.default(style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions,
+                                                             block_table, k_pages, v_pages, k_scales, v_scales)
+
+
+@torch.library.register_fake("minfer::rope_kv_append_paged_fp8")
+def _(style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions, block_table, k_pages, v_pages, k_scales, v_scales):
+    _check_pages(q, k_pages, v_pages, (k_scales, v_scales), block_table, cu_seqlens, positions)
+    torch._check(k.dtype == q.dtype and v.dtype == q.dtype and k.dim() == 4 and v.dim() == 4)
+    torch._check(rotary_dim <= q.size(3))
+
+
+def flash_attn_paged(
+    qtype_int: int,
+    qblock_size: int,
+    qtype_size: int,
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    max_q_len: int,
+    out: torch.Tensor,
+):
+    """Attention of packed tokens over a paged cache that holds their own rows already (rope_kv_append_paged): q/out
+    [1,n_heads,T,D]; tokens cu_seqlens[s] .. cu_seqlens[s+1]-1 are the last ones of sequence s, which has ctx_lens[s] rows, and
+    each attends the rows up to its own.  One token per sequence is a decode step, a few are drafts, many a chunk of a
+    prompt; a call may mix them.  Rows of pages that are not there (table entry -1) are not attended; a token without any
+    row yields zeros.  max_q_len bounds the tokens of a sequence (0 = not known); tokens past it are not computed."""
+    return torch.ops.minfer.flash_attn_paged.default(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, block_table,
+                                                     cu_seqlens, ctx_lens, max_q_len, out)
+
+
+@torch.library.register_fake("minfer::flash_attn_paged")
+def _(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, block_table, cu_seqlens, ctx_lens, max_q_len, out):
+    _check_pages(q, k_pages, v_pages, None, block_table, cu_seqlens, ctx_lens)
+    torch._check(out.dtype == q.dtype and out.shape == q.shape)
+
+
+def flash_attn_paged_fp8(
+    qtype_int: int,
+    qblock_size: int,
+    qtype_size: int,
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    max_q_len: int,
+    out: torch.Tensor,
+):
+    """flash_attn_paged over 8-bit pages (rope_kv_append_paged_fp8): a row is its float8_e4m3fn codes times the page's and
+    head's scale (float8_e8m0fnu [n_pages,n_kv_heads]), a number that q's dtype holds."""
+    return torch.ops.minfer.flash_attn_paged_fp8.default(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, k_scales,
+                                                         v_scales, block_table, cu_seqlens, ctx_lens, max_q_len, out)
+
+
+@torch.library.register_fake("minfer::flash_attn_paged_fp8")
+def _(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, ctx_lens, max_q_len, out):
+    _check_pages(q, k_pages, v_pages, (k_scales, v_scales), block_table, cu_seqlens, ctx_lens)
+    torch._check(out.dtype == q.dtype and out.shape == q.shape)
+
+
 def rmsnorm(eps: float, input: torch.Tensor, w: torch.Tensor, out: torch.Tensor):
     """RMS normalisation over vectors of length len(w) (the whole hidden dimension, or per head)."""
     return torch.ops.minfer.rmsnorm.default(eps, input, w, out)
