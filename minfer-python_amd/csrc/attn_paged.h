@@ -102,4 +102,23 @@ inline int check_pages(const char* op, int dtype, int page_type, const minfer_kv
     return MINFER_ATTN_OK;
 }
 
+// One call of the attention over a paged cache, as its kernels see it.
+struct PagedParams {
+    PagedCache c;
+    const void* q; void* out;
+    const int32_t* cu; const int32_t* ctx;
+    float* part_o;     // partial results, un-normalised, [row][slot][D] ...
+    float* part_ml;    // ... with their reference (log2 units) and sum, [row][slot][2]
+    int64_t q1, q2, o1, o2;
+    int n_seqs, T, Hq, Hkv, n_rep;
+    int max_q;         // tokens of a sequence past this many are not computed
+    int slots;         // partial results a row can have
+    float scale_log2, inv_scale_log2;  // softmax scale * log2(e), and one over it
+};
+
+// Few query rows per KV head (csrc/attn_paged_decode.hip): whether a call with these sizes is one, its workspace, its launch.
+bool paged_decode_takes(int64_t Hq, int64_t Hkv, int64_t max_q);
+size_t paged_decode_workspace_bytes(int64_t n_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q);
+int launch_paged_decode(PagedParams p, int dtype, int64_t D, bool eight, int64_t max_context, void* workspace, hipStream_t stream);
+
 }  // namespace minfer_attn

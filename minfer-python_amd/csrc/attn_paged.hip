@@ -19,19 +19,6 @@
 
 namespace minfer_attn {
 
-struct PagedParams {
-    PagedCache c;
-    const void* q; void* out;
-    const int32_t* cu; const int32_t* ctx;
-    float* part_o;     // [T * Hq][n_split][D]
-    float* part_ml;    // [T * Hq][n_split][2]: reference (log2 units), sum
-    int64_t q1, q2, o1, o2;
-    int n_seqs, T, Hq, Hkv, n_rep;
-    int max_q;         // tokens of a sequence past this many are not computed
-    int n_split;       // ranges that the tiles of a block of rows are cut into
-    float scale_log2, inv_scale_log2;  // softmax scale * log2(e), and one over it
-};
-
 template <int D, int NW> struct PagedGeom {
     static constexpr int RB = D * 2;                 // bytes per 16-bit row
     static constexpr int G = RB / 16;                // 16-byte granules per row
@@ -82,8 +69,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
         g = (int)blockIdx.x % p.Hkv;
         rank = (int)blockIdx.x / p.Hkv;
     }
-    const int split = rank % p.n_split;
-    int x = rank / p.n_split, seq = -1, seq_lo = 0, seq_len = 0, blocks = 0;
+    const int split = rank % p.slots;
+    int x = rank / p.slots, seq = -1, seq_lo = 0, seq_len = 0, blocks = 0;
     for (int base = 0; base < p.n_seqs; base += 64) {
         const int s = base + lane;
         TokenRange r{0, 0};
@@ -109,7 +96,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     const int row0 = block * BR + w * 32;                                // the wave's first row
     const bool wave_on = row0 < rows;
     const int keys = max(pos0 + min(block * BR + BR - 1, last_row) / p.n_rep + 1, 0);   // of the workgroup's last row
-    const int n_tiles = (keys + 63) >> 6, per = (n_tiles + p.n_split - 1) / p.n_split;
+    const int n_tiles = (keys + 63) >> 6, per = (n_tiles + p.slots - 1) / p.slots;
     const int t_lo = min(split * per, n_tiles), n_own = min(t_lo + per, n_tiles) - t_lo;
     const int wave_first = pos0 + min(row0, last_row) / p.n_rep, wave_last = pos0 + min(row0 + 31, last_row) / p.n_rep;
 
@@ -412,12 +399,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     float l_all[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) l_all[qb] = sum_across_quads(l_sum[qb]);
-    if (p.n_split > 1) {
+    if (p.slots > 1) {
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
             const int r = row0 + 16 * qb + l16, t = r / p.n_rep;
             if (r > last_row) continue;
-            const int64_t slot = ((int64_t)(seq_lo + t) * p.Hq + g * p.n_rep + r - t * p.n_rep) * p.n_split + split;
+            const int64_t slot = ((int64_t)(seq_lo + t) * p.Hq + g * p.n_rep + r - t * p.n_rep) * p.slots + split;
             float* dst = p.part_o + slot * D + 4 * quad;
 #pragma unroll
             for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = o_acc[db][qb];
@@ -465,16 +452,16 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p,
     const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
     if (row >= min(r.len, p.max_q) * p.Hq) return;
     const int t = row / p.Hq, head = row - t * p.Hq;
-    const int64_t slot0 = ((int64_t)(r.lo + t) * p.Hq + head) * p.n_split;
+    const int64_t slot0 = ((int64_t)(r.lo + t) * p.Hq + head) * p.slots;
     float m = -INFINITY, l = 0.f;
-    if (lane < p.n_split) { m = p.part_ml[(slot0 + lane) * 2]; l = p.part_ml[(slot0 + lane) * 2 + 1]; }
+    if (lane < p.slots) { m = p.part_ml[(slot0 + lane) * 2]; l = p.part_ml[(slot0 + lane) * 2 + 1]; }
     const float top = wave_max(m);
     const float wgt = m > -INFINITY ? fast_exp2(m - top) : 0.f;
     const float total = lane_sum<64>(l * wgt);
     float acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-    for (int i = 0; i < p.n_split; ++i) {
+    for (int i = 0; i < p.slots; ++i) {
         if (lane_value(l, i) == 0.f) continue;
         const float wi = lane_value(wgt, i);
         const float* src = p.part_o + (slot0 + i) * D + EPL * lane;
@@ -487,18 +474,18 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p,
     else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
 }
 
+static int64_t bounded_tokens(int64_t T, int64_t max_q_len) { return max_q_len > 0 && max_q_len < T ? max_q_len : T; }
+
 // How a call is laid out, from its sizes alone (contexts and lengths are on the device).
 struct PagedPlan {
-    int64_t max_q;     // bound of a sequence's tokens
     int64_t blocks;    // bound of the blocks of rows of all sequences
     int64_t n_split;
     size_t o_bytes, ml_bytes;
 };
-static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q_len, int rows_per_wg) {
+static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q, int rows_per_wg) {
     PagedPlan r{};
     const int64_t n_rep = Hq / Hkv;
-    r.max_q = max_q_len > 0 && max_q_len < T ? max_q_len : T;
-    r.blocks = std::min(n_seqs * ((r.max_q * n_rep + rows_per_wg - 1) / rows_per_wg), T * n_rep / rows_per_wg + n_seqs);
+    r.blocks = std::min(n_seqs * ((max_q * n_rep + rows_per_wg - 1) / rows_per_wg), T * n_rep / rows_per_wg + n_seqs);
     const int64_t wgs = r.blocks * Hkv, most = std::min<int64_t>(64, max_context / 256);
     r.n_split = std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(wgs, 1)));
     if (r.n_split > 1) {
@@ -515,7 +502,7 @@ static int launch_paged(const PagedParams& p, const PagedPlan& plan, hipStream_t
     hipLaunchKernelGGL((paged_tile_kernel<T, D, FP8, kPagedWaves>), dim3((unsigned)(plan.blocks * p.Hkv * plan.n_split)), dim3(kPagedWaves * 64), 0, stream, p);
     if (int rc = check_launch("paged_tile_kernel")) return rc;
     if (plan.n_split == 1) return MINFER_ATTN_OK;
-    const int64_t per = (plan.max_q * p.Hq + 3) / 4;
+    const int64_t per = ((int64_t)p.max_q * p.Hq + 3) / 4;
     hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3((unsigned)(per * p.n_seqs)), dim3(256), 0, stream, p, (int)per);
     return check_launch("paged_combine_kernel");
 }
@@ -530,8 +517,10 @@ using namespace minfer_attn;
 
 MINFER_ATTN_EXPORT size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context,
                                                                   int64_t max_q_len) {
-    if (n_seqs <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_context <= 0 || Hq % Hkv != 0) return 0;
-    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_context, max_q_len, kPagedWaves * 32);
+    if (n_seqs <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_context < 0 || Hq % Hkv != 0) return 0;
+    const int64_t max_q = bounded_tokens(T, max_q_len);
+    if (paged_decode_takes(Hq, Hkv, max_q)) return paged_decode_workspace_bytes(n_seqs, Hq, Hkv, D, max_context, max_q);
+    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_context, max_q, kPagedWaves * 32);
     return r.o_bytes + r.ml_bytes;
 }
 
@@ -554,22 +543,29 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
     for (int i = 0; i < 4; ++i)
         if (s[i] < 0 || s[i] % 8 != 0) return bad("flash_attn_paged: strides of q and out must be non-negative multiples of 8 elements");
     const int64_t max_context = (int64_t)p.c.width << p.c.page_log2;
-    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_context, max_q_len, kPagedWaves * 32);
-    // (rows of a sequence, workgroups and their ids are 32-bit numbers; so are the seqs' first rows on the line of blocks)
-    if (T > (1 << 30) || T * Hq > 0x7fffffffLL || n_seqs > (1 << 24) || plan.blocks * Hkv * plan.n_split > 0x7fffffffLL ||
-        (plan.max_q * Hq + 3) / 4 * n_seqs > 0x7fffffffLL)
-        return bad("flash_attn_paged: problem too large for one launch");
-    if (plan.n_split > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes))
-        return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
     p.q = q; p.out = out; p.cu = cu_seqlens; p.ctx = ctx_lens;
     p.q1 = st->q1; p.q2 = st->q2; p.o1 = st->o1; p.o2 = st->o2;
     p.n_seqs = (int)n_seqs; p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.n_rep = (int)(Hq / Hkv);
-    p.max_q = (int)plan.max_q;
-    p.n_split = (int)plan.n_split;
-    p.part_o = (float*)workspace;
-    p.part_ml = (float*)((char*)workspace + plan.o_bytes);
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
     p.inv_scale_log2 = (float)(sqrt((double)D) / 1.4426950408889634);
     const bool eight = page_type == MINFER_FP8_E4M3;
+    const int64_t max_q = bounded_tokens(T, max_q_len);
+    if (T > (1 << 30) || T * Hq > 0x7fffffffLL || n_seqs > (1 << 24)) return bad("flash_attn_paged: problem too large for one launch");
+    p.max_q = (int)max_q;
+    if (paged_decode_takes(Hq, Hkv, max_q)) {
+        const size_t need = paged_decode_workspace_bytes(n_seqs, Hq, Hkv, D, max_context, max_q);
+        if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+            return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
+        return launch_paged_decode(p, dtype, D, eight, max_context, workspace, (hipStream_t)stream_v);
+    }
+    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_context, max_q, kPagedWaves * 32);
+    // (workgroups and their ids are 32-bit numbers)
+    if (plan.blocks * Hkv * plan.n_split > 0x7fffffffLL || (max_q * Hq + 3) / 4 * n_seqs > 0x7fffffffLL)
+        return bad("flash_attn_paged: problem too large for one launch");
+    if (plan.n_split > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes))
+        return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
+    p.slots = (int)plan.n_split;
+    p.part_o = (float*)workspace;
+    p.part_ml = (float*)((char*)workspace + plan.o_bytes);
     return dtype == MINFER_ATTN_F16 ? launch_paged_as<F16>(p, plan, D, eight, (hipStream_t)stream_v) : launch_paged_as<BF16>(p, plan, D, eight, (hipStream_t)stream_v);
 }

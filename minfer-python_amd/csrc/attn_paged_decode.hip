@@ -1,0 +1,476 @@
+// Attention of few query rows per KV head over a paged cache for gfx950: single tokens of many sequences, drafts of a few tokens.
+//
+// HBM-bound: each cached row is used by at most 16 columns (a token and head each) at a time, so what counts is bytes in flight.  The columns of a
+// KV head are its group's query heads for every new token of the sequence, token by token; up to 16 of them are the columns of one
+// 16-wide matrix product, each with a limit of its own (the row of its token), so a few drafts read the cache once.
+//
+// A wave streams rows of one (sequence, KV head) on its own, with a ring of groups of rows in registers: 16 rows of 16-bit values,
+// loaded as whole rows and turned into matrix operands in the wave's LDS; or 32 rows of e4m3 codes, K loaded straight in the
+// operand's layout (the order of the contraction is free as long as q is loaded in the same), V as whole rows, both widened on the way.
+// A page holds at least 16 rows, so a group (or half of one) lies in one page, whose table entry is read as a scalar a group ahead.
+// S^T[keys x 16 columns] = K Q^T, softmax per column with a lazy reference, O^T += V^T P^T.
+//
+// Two ways to share the work out:
+// * the line: all rows to be read, sequence by sequence, KV head by KV head, cut into as many equal shares as the launch has waves; a
+//   wave's share covers parts of a few (sequence, KV head) pairs, each of which leaves a partial result that
+//   paged_merge_kernel puts together.  Whatever the mix of contexts, all waves end together.
+// * chunks, for few pairs: eight waves of a workgroup share one chunk of a pair and merge in LDS, and the last workgroup of a pair merges its
+//   chunks (on the null stream; elsewhere paged_chunk_merge_kernel does).  A sequence is cut by its own context, which the host does not know.
+#include <algorithm>
+#include <atomic>
+
+#include "attn_paged.h"
+
+namespace minfer_attn {
+
+constexpr int kLineWaves = 4;          // waves per workgroup of the line
+constexpr int kLineWgPerCu = 2;
+constexpr int kChunkWaves = 8;
+constexpr int kMaxSlots = 64;          // partial results a row can have: a wave merges them, one to a lane
+
+struct DecodeWork {
+    PagedParams p;
+    int32_t* seq_off;   // line: [n_seqs + 2] start of every sequence on the line, its length, the quota; written by workgroup 0
+    int n_col;          // columns per KV head: max_q * n_rep
+    int n_hg;           // groups of <= 16 columns per KV head
+    int n_wg;           // line: workgroups
+    uint32_t* done;     // chunks: zeroed counters, one per pair, left zero; or null
+};
+
+template <bool FP8> constexpr int kRows = FP8 ? 32 : 16;   // rows of a group
+
+// What a wave has to know about a sequence.
+struct SeqInfo { int lo, len, ctx; };   // first token, tokens that are computed against .. and the rows they have
+MA_DEV SeqInfo seq_info(const PagedParams& p, int s) {
+    const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
+    return SeqInfo{r.lo, r.len, min(max(const_load(p.ctx + s), 0), p.c.width << p.c.page_log2)};
+}
+
+template <int D> struct ColumnAcc {
+    f32x4 o[D / 16];   // lane (l16, quad): column l16, O at d = 16db + 4 quad + 0..3, un-normalised
+    float m, l;        // the column's reference (log2 units) and sum
+};
+
+template <int D> struct DecodeGeom {
+    static constexpr int RB = D * 2;
+    static constexpr int G = RB / 16;
+    static constexpr int RPI = 1024 / RB;              // 16-bit rows that one wave-wide load covers
+    static constexpr int NI = 16 / RPI;                // such loads per 16 rows
+    static constexpr int RPI8 = 1024 / D;              // the same for rows of codes
+    static constexpr int NI8 = 16 / RPI8;
+    static MA_DEV int swz_v(int row) { return D == 128 ? ((row & 7) << 1) : (((row >> 1) & 3) << 1); }
+    static MA_DEV int swz_k(int row) { return D == 128 ? (row & 15) : ((row >> 1) & 7); }
+};
+template <int D, bool FP8> constexpr int kWaveLds = FP8 ? 32 * D * 2 : 2 * 16 * D * 2;   // V of 32 rows; or K and V of 16
+
+// The columns of a group: what lane l16 needs of its own.
+struct Column { const short* q; int limit; };   // its query row (null: no column), and the rows that it attends: 0 .. limit - 1
+MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg) {
+    const PagedParams& p = w.p;
+    const int col = hg * 16 + ((int)threadIdx.x & 15), tok = p.n_rep > 16 || p.max_q == 1 ? 0 : col / p.n_rep;
+    Column c{nullptr, 0};
+    if (col < w.n_col && tok < info.len) {
+        c.q = (const short*)p.q + (int64_t)(info.lo + tok) * p.q2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.q1;
+        c.limit = info.ctx - info.len + tok + 1;
+    }
+    return c;
+}
+
+// Streams groups g0 .. g1 - 1 (at least one) of (sequence s, KV head g) for the columns of group hg; `area` is the wave's own LDS.
+template <class T, int D, bool FP8>
+MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, int g1, char* area, ColumnAcc<D>& acc) {
+    const PagedParams& p = work.p;
+    using GEO = DecodeGeom<D>;
+    constexpr int RB = GEO::RB, G = GEO::G, RPI = GEO::RPI, NI = GEO::NI, RPI8 = GEO::RPI8, NI8 = GEO::NI8;
+    constexpr int KC = D / 32, DB = D / 16, GR = kRows<FP8>, NH = GR / 16;   // halves of 16 rows in a group
+    constexpr int NS = 3;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const int ctx = info.ctx, page_mask = (1 << p.c.page_log2) - 1;
+    const int32_t* const table = p.c.table + (int64_t)s * p.c.table_stride;
+    const Column col = column_of(work, info, g, hg);
+
+    // Q^T fragments (B operand): column l16; contraction step c takes d = 32c + 8 quad + 0..7, or for codes, whose 16-byte pieces hold
+    // two steps, d = 64 (c / 2) + 16 quad + 8 (c % 2) + 0..7
+    s16x8 qf[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+        const int d = FP8 ? 64 * (c / 2) + 16 * quad + 8 * (c % 2) : 32 * c + 8 * quad;
+        qf[c] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (col.q) qf[c] = *reinterpret_cast<const s16x8*>(col.q + d);
+    }
+
+    // ---- pages ----
+    struct Ids { int id[NH]; };
+    auto ids_of = [&](int t) __attribute__((always_inline)) {
+        Ids r;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) r.id[h] = const_load(table + min((min(t, g1 - 1) * GR + 16 * h) >> p.c.page_log2, p.c.width - 1));
+        return r;
+    };
+    auto is_there = [&](int id) __attribute__((always_inline)) { return (unsigned)id < (unsigned)p.c.n_pages; };
+    const int64_t head_at = (int64_t)g * p.c.head_stride;
+    auto half_at = [&](int id, int row) __attribute__((always_inline)) -> int64_t {
+        return (int64_t)(is_there(id) ? id : 0) * p.c.page_stride + head_at + (int64_t)(row & page_mask) * p.c.row_stride;
+    };
+
+    // ---- a ring of groups on their way ----
+    constexpr int NK = FP8 ? NH * D / 64 : NI, NV = FP8 ? NH * NI8 : NI;
+    struct Stage { u32x4 k[NK], v[NV]; float ks[NH], vs[NH]; int there; } ring[NS];
+    // a lane's place inside the 16 rows: its row and chunk of load j, and its key's pieces of K's codes
+    const int stride = (int)p.c.row_stride;
+    constexpr int VPI = FP8 ? RPI8 : RPI, CPR = 64 / VPI;   // rows a load covers, 16-byte pieces per row
+    const int v_row = lane / CPR, v_piece = (FP8 ? 16 : 8) * (lane % CPR), k_piece = 16 * quad;
+    auto load_group = [&](int t, const Ids& ids, Stage& st) __attribute__((always_inline)) {
+        // slots past the last group have every row of theirs be one row of that group, which costs a few cache lines
+        const bool real = t < g1;
+        const int step = real ? stride : 0, t_row = min(t, g1 - 1) * GR;
+        st.there = 0;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            const int row0 = t_row + 16 * h, id = ids.id[h];
+            st.there |= (is_there(id) && row0 < ctx) ? 1 << h : 0;
+            const int64_t at = half_at(id, row0);
+            if constexpr (FP8) {
+                const char* kb = (const char*)p.c.k + at;
+                const char* vb = (const char*)p.c.v + at;
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) st.k[h * (D / 64) + j] = stream_load(reinterpret_cast<const u32x4*>(kb + (uint32_t)(l16 * step + k_piece + 64 * j)));
+#pragma unroll
+                for (int j = 0; j < NI8; ++j) st.v[h * NI8 + j] = stream_load(reinterpret_cast<const u32x4*>(vb + (uint32_t)((j * RPI8 + v_row) * step + v_piece)));
+                const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
+                st.ks[h] = scale_value(const_byte(p.c.k_scales + sc));
+                st.vs[h] = scale_value(const_byte(p.c.v_scales + sc));
+            } else {
+                const short* kb = (const short*)p.c.k + at;
+                const short* vb = (const short*)p.c.v + at;
+#pragma unroll
+                for (int j = 0; j < NI; ++j) st.k[j] = stream_load(reinterpret_cast<const u32x4*>(kb + (uint32_t)((j * RPI + v_row) * step + v_piece)));
+#pragma unroll
+                for (int j = 0; j < NI; ++j) st.v[j] = stream_load(reinterpret_cast<const u32x4*>(vb + (uint32_t)((j * RPI + v_row) * step + v_piece)));
+            }
+        }
+    };
+
+    f32x4 (&o_acc)[DB] = acc.o;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o_acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_ref = -INFINITY, l_sum = 0.f;
+    const float c2 = p.scale_log2;
+    constexpr float kLazyLog2 = 6.f;
+    char* const my_v = area;
+    char* const my_k = area + 16 * RB;   // 16-bit rows only
+
+    auto consume = [&](int t, Stage& st) __attribute__((always_inline)) {
+        f32x4 sc[NH];
+        // V rows behind the context may hold anything, NaN too, and their weight of zero would not take it out of the sums (of K only the
+        // row's own scores are made, which are replaced)
+        const int past = ctx - t * GR;
+        if (past < GR) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) st.v[j] = j * VPI + v_row < past ? st.v[j] : u32x4{0u, 0u, 0u, 0u};
+        }
+        if constexpr (FP8) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const u32x4 x = st.k[h * (D / 64) + c / 2];
+                    const uint32_t lo = x[2 * (c % 2)], hi = x[2 * (c % 2) + 1];
+                    const u32x4 a = {widen2<T, false>(lo, st.ks[h]), widen2<T, true>(lo, st.ks[h]), widen2<T, false>(hi, st.ks[h]), widen2<T, true>(hi, st.ks[h])};
+                    sc[h] = T::mfma16(__builtin_bit_cast(s16x8, a), qf[c], sc[h]);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                const bool on = (st.there >> h & 1) != 0;   // (a page that is not there: what was loaded in its place is not multiplied)
+                const float vs = on ? st.vs[h] : 1.f;
+#pragma unroll
+                for (int j = 0; j < NI8; ++j) {
+                    const int row = 16 * h + j * RPI8 + lane / (D / 16), gr = 2 * (lane % (D / 16));
+                    const u32x4 x = on ? st.v[h * NI8 + j] : u32x4{0u, 0u, 0u, 0u};
+                    char* rowp = my_v + row * RB;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const u32x4 a = {widen2<T, false>(x[2 * i], vs), widen2<T, true>(x[2 * i], vs), widen2<T, false>(x[2 * i + 1], vs), widen2<T, true>(x[2 * i + 1], vs)};
+                        *reinterpret_cast<u32x4*>(rowp + 16 * ((gr + i) ^ GEO::swz_v(row))) = a;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int row = j * RPI + lane / G;
+                *reinterpret_cast<u32x4*>(my_k + row * RB + 16 * ((lane % G) ^ GEO::swz_k(row))) = st.k[j];
+            }
+            const char* rowp = my_k + l16 * RB;
+            const int sw = GEO::swz_k(l16);
+            sc[0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) sc[0] = T::mfma16(*reinterpret_cast<const s16x8*>(rowp + 16 * ((4 * c + quad) ^ sw)), qf[c], sc[0]);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int row = j * RPI + lane / G;
+                *reinterpret_cast<u32x4*>(my_v + row * RB + 16 * ((lane % G) ^ GEO::swz_v(row))) = st.v[j];
+            }
+        }
+        // rows that the column does not attend
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            const int left = (NH == 1 || (st.there >> h & 1)) ? col.limit - (t * GR + 16 * h + 4 * quad) : 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[h][r] = r < left ? sc[h][r] : -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+        if (NH == 2) mx = fmaxf(mx, fmaxf(fmaxf(sc[NH - 1][0], sc[NH - 1][1]), fmaxf(sc[NH - 1][2], sc[NH - 1][3])));
+        auto grows = [&](float x) { return (x * c2 - m_ref) > kLazyLog2 || (m_ref == -INFINITY && x > -INFINITY); };
+        if (__any(grows(mx))) {   // (one of the column's four lanes holds its largest score)
+            mx = max_across_quads(mx);
+            const float m_new = grows(mx) ? mx * c2 : m_ref;
+            const float alpha = (m_ref == -INFINITY) ? 0.f : fast_exp2(m_ref - m_new);
+            m_ref = m_new;
+            l_sum *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o_acc[db] *= alpha;
+        }
+        const float mc = (m_ref == -INFINITY) ? 0.f : m_ref;
+        uint32_t pk[2 * NH];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            pk[2 * h] = T::pack2(fast_exp2(fmaf(sc[h][0], c2, -mc)), fast_exp2(fmaf(sc[h][1], c2, -mc)));
+            pk[2 * h + 1] = T::pack2(fast_exp2(fmaf(sc[h][2], c2, -mc)), fast_exp2(fmaf(sc[h][3], c2, -mc)));
+            l_sum = T::add_pair(pk[2 * h + 1], T::add_pair(pk[2 * h], l_sum));   // sums the rounded weights that are multiplied
+        }
+        // O^T += V^T P^T: row d = 16db + l16, keys 4 quad + 0..3 (and 16 + 4 quad + 0..3)
+        const int row = 4 * quad + (l16 >> 2);
+        const char* rowp = my_v + row * RB;
+        const int sw = GEO::swz_v(row);   // rows 16 apart share a swizzle
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            const int dcol = 16 * db + 4 * (l16 & 3), at = 16 * ((dcol >> 3) ^ sw) + 2 * (dcol & 7);
+            const s16x4 a0 = lds_read_tr16(rowp + at);
+            if constexpr (NH == 2) {
+                const s16x4 a1 = lds_read_tr16(rowp + 16 * RB + at);
+                o_acc[db] = T::mfma16(s16x8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
+                                      __builtin_bit_cast(s16x8, u32x4{pk[0], pk[1], pk[2 * NH - 2], pk[2 * NH - 1]}), o_acc[db]);
+            } else {
+                uint2 pu; pu.x = pk[0]; pu.y = pk[1];
+                o_acc[db] = T::mfma16k16(a0, __builtin_bit_cast(s16x4, pu), o_acc[db]);
+            }
+        }
+    };
+
+    Ids next = ids_of(g0);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const Ids now = next;
+        next = ids_of(g0 + i + 1);
+        load_group(g0 + i, now, ring[i]);
+    }
+    for (int t0 = g0; t0 < g1; t0 += NS) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            if (t0 + i < g1 && ring[i].there) consume(t0 + i, ring[i]);
+            const Ids now = next;
+            next = ids_of(t0 + i + NS + 1);
+            load_group(t0 + i + NS, now, ring[i]);
+        }
+    }
+    acc.m = m_ref;
+    acc.l = sum_across_quads(l_sum);
+}
+
+MA_DEV int64_t part_row(const DecodeWork& w, int s, int g, int col) { return ((int64_t)s * w.p.Hkv + g) * w.n_col + col; }
+
+// A wave's partial result of every column, into the workspace.
+template <int D> MA_DEV void store_part(const DecodeWork& w, int s, int g, int hg, int slot, const ColumnAcc<D>& acc) {
+    const int lane = threadIdx.x & 63, col = hg * 16 + (lane & 15), quad = lane >> 4;
+    if (col >= w.n_col) return;
+    const int64_t at = part_row(w, s, g, col) * w.p.slots + slot;
+    float* dst = w.p.part_o + at * D + 4 * quad;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc.o[db];
+    if (quad == 0) { w.p.part_ml[at * 2] = acc.m; w.p.part_ml[at * 2 + 1] = acc.l; }
+}
+
+// ---- the line ------------------------------------------------------------------------------------------------------
+// Lengths in groups: every sequence's (zero without tokens) times its pairs, one after the other.  The quota: an equal share for
+// every wave, 128 rows at least, and as much as leaves no pair with more partial results than there are slots.
+struct LineSeq { SeqInfo info; int groups; };
+template <int GR> MA_DEV LineSeq line_seq(const DecodeWork& w, int s) {   // (per lane)
+    const PagedParams& p = w.p;
+    LineSeq r{{0, 0, 0}, 0};
+    if (s < p.n_seqs) {
+        const TokenRange t = token_range(p.cu[s], p.cu[s + 1], p.T);
+        r.info = SeqInfo{t.lo, t.len, min(max(p.ctx[s], 0), p.c.width << p.c.page_log2)};
+        r.groups = t.len > 0 ? (r.info.ctx + GR - 1) / GR : 0;
+    }
+    return r;
+}
+
+template <class T, int D, bool FP8>
+__global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const DecodeWork work) {
+    __shared__ __attribute__((aligned(1024))) char lds[kLineWaves][kWaveLds<D, FP8>];
+    constexpr int GR = kRows<FP8>;
+    const PagedParams& p = work.p;
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int pairs = p.Hkv * work.n_hg, n_waves = work.n_wg * kLineWaves;
+    const bool first = blockIdx.x == 0 && w == 0;   // the wave that leaves the sequences' places for the merge
+    int total = 0, longest = 0;
+    for (int base = 0; base < p.n_seqs; base += 64) {
+        const LineSeq q = line_seq<GR>(work, base + lane);
+        const int incl = wave_inclusive_scan(q.groups * pairs);
+        if (first && base + lane < p.n_seqs) work.seq_off[base + lane] = total + incl - q.groups * pairs;
+        total += lane_value(incl, 63);
+        longest = max(longest, q.groups);
+    }
+    longest = (int)wave_max((float)longest);   // (below 2^24 exactly, and above rounded up or down by less than the slots to spare)
+    const int quota = max(max((total + n_waves - 1) / n_waves, 128 / GR), longest / (p.slots - 3) + 1);
+    if (first && lane == 0) { work.seq_off[p.n_seqs] = total; work.seq_off[p.n_seqs + 1] = quota; }
+    // shares to the waves of a workgroup in turn; where there are no more shares than workgroups, one to each
+    const int n_shares = (total + quota - 1) / quota;
+    const int wave = n_shares <= (int)gridDim.x ? w * (int)gridDim.x + (int)blockIdx.x : (int)blockIdx.x * kLineWaves + w;
+    int x = wave * quota;
+    const int x_end = min(total, x + quota);
+    if (wave >= n_shares) return;
+    // the sequence that holds position x
+    int s = 0, off = 0, groups = 0;
+    for (int base = 0, start = 0; base < p.n_seqs; base += 64) {
+        const LineSeq q = line_seq<GR>(work, base + lane);
+        const int incl = wave_inclusive_scan(q.groups * pairs), sum = lane_value(incl, 63);
+        if (x < start + sum) {
+            const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < start + incl)) - 1);
+            s = base + src;
+            groups = lane_value(q.groups, src);
+            off = start + lane_value(incl, src) - groups * pairs;
+            break;
+        }
+        start += sum;
+    }
+    SeqInfo info = seq_info(p, s);
+    while (x < x_end) {
+        if (x >= off + pairs * groups) {   // the sequence is done: on to the next that has rows
+            off += pairs * groups;
+            do {
+                info = seq_info(p, ++s);
+                groups = info.len > 0 ? (info.ctx + GR - 1) / GR : 0;
+            } while (groups == 0);
+        }
+        const int y = x - off, pair = y / groups, g0 = y - pair * groups, g1 = min(groups, g0 + (x_end - x));
+        const int slot = wave - (off + pair * groups) / quota;
+        const int hg = work.n_hg == 1 ? 0 : pair / p.Hkv, g = pair - hg * p.Hkv;
+        ColumnAcc<D> acc;
+        stream_pages<T, D, FP8>(work, s, info, g, hg, g0, g1, lds[w], acc);
+        store_part<D>(work, s, g, hg, slot, acc);
+        x += g1 - g0;
+    }
+}
+
+// out = sum_i O_i w_i / sum_i l_i w_i, w_i = 2^(m_i - max m), over the parts of a row; a wave per row (sequence, token, head), lane i holding part i's
+// reference and sum.  A part whose scores are all NaN has a weight of zero and sums of NaN and is multiplied like any other.
+template <class T, int D, int GR>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work) {
+    const PagedParams& p = work.p;
+    constexpr int EPL = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
+    const int per_seq = p.Hkv * work.n_col;
+    if (row >= (int64_t)p.n_seqs * per_seq) return;
+    const int s = (int)(row / per_seq), in = (int)(row - (int64_t)s * per_seq), g = in / work.n_col, col = in - g * work.n_col;
+    const float* src = p.part_o + row * p.slots * D + EPL * lane;
+    auto load_o = [&](int slot, float (&x)[EPL]) __attribute__((always_inline)) {
+        const float* at = src + (int64_t)slot * D;
+        if (EPL == 2) { const f32x2 v = *reinterpret_cast<const f32x2*>(at); x[0] = v[0]; x[EPL - 1] = v[1]; }
+        else x[0] = at[0];
+    };
+    // requested before the number of parts is known (what is past it is discarded)
+    const int sl = min(lane, p.slots - 1);
+    const float m_raw = p.part_ml[(row * p.slots + sl) * 2], l_raw = p.part_ml[(row * p.slots + sl) * 2 + 1];
+    constexpr int kEarly = 4;
+    float x[8][EPL];
+#pragma unroll
+    for (int u = 0; u < kEarly; ++u) load_o(min(u, p.slots - 1), x[u]);
+    const SeqInfo info = seq_info(p, s);
+    const int tok = col / p.n_rep;
+    if (tok >= info.len) return;
+    const int groups = (info.ctx + GR - 1) / GR, quota = const_load(work.seq_off + p.n_seqs + 1);
+    const int start = const_load(work.seq_off + s) + ((col / 16) * p.Hkv + g) * groups;
+    const int ns = groups > 0 ? min((start + groups - 1) / quota - start / quota + 1, p.slots) : 0;
+    const float m = lane < ns ? m_raw : -INFINITY, l = lane < ns ? l_raw : 0.f;
+    const float top = wave_max(m);
+    const float wgt = m > -INFINITY ? fast_exp2(m - top) : 0.f;
+    const float total = lane_sum<64>(l * wgt);
+    float acc[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
+    for (int s0 = 0; s0 < ns; s0 += 8) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (s0 > 0 || u >= kEarly) load_o(min(s0 + u, ns - 1), x[u]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float wi = lane_value(wgt, min(s0 + u, 63));
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[e] += s0 + u < ns ? x[u][e] * wi : 0.f;
+        }
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + EPL * lane;
+    if (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = T::pack2(acc[0] * inv, acc[EPL - 1] * inv);
+    else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
+}
+
+// Workgroups of the line: as many as the chip holds at once.
+static int compute_units() {
+    static std::atomic<int> cached[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    int n = cached[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+        cached[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// Slots of a row: enough for shares of 128 rows, 64 at most (longer contexts get longer shares).
+static int64_t slots_of(int64_t max_context) { return std::min<int64_t>(kMaxSlots, max_context / 128 + 4); }
+
+bool paged_decode_takes(int64_t Hq, int64_t Hkv, int64_t max_q) { return max_q == 1 || max_q * (Hq / Hkv) <= 16; }
+
+static size_t part_bytes(int64_t rows, int64_t slots, int64_t floats) { return ((size_t)(rows * slots * floats * 4) + 255) / 256 * 256; }
+size_t paged_decode_workspace_bytes(int64_t n_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
+    (void)Hkv;
+    const int64_t rows = n_seqs * Hq * max_q, slots = slots_of(max_context);
+    return part_bytes(rows, slots, D) + part_bytes(rows, slots, 2) + ((size_t)(n_seqs + 2) * 4 + 255) / 256 * 256;
+}
+
+template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_line_kernel<T, D, FP8>), dim3((unsigned)w.n_wg), dim3(kLineWaves * 64), 0, stream, w);
+    if (int rc = check_launch("paged_line_kernel")) return rc;
+    const int64_t rows = (int64_t)w.p.n_seqs * w.p.Hkv * w.n_col;
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
+    return check_launch("paged_merge_kernel");
+}
+template <class T> static int launch_decode_as(const DecodeWork& w, int64_t D, bool eight, hipStream_t stream) {
+    if (eight) return D == 128 ? launch_line<T, 128, true>(w, stream) : launch_line<T, 64, true>(w, stream);
+    return D == 128 ? launch_line<T, 128, false>(w, stream) : launch_line<T, 64, false>(w, stream);
+}
+
+int launch_paged_decode(PagedParams p, int dtype, int64_t D, bool eight, int64_t max_context, void* workspace, hipStream_t stream) {
+    DecodeWork w{};
+    w.n_col = p.max_q * p.n_rep;
+    w.n_hg = (w.n_col + 15) / 16;
+    w.n_wg = compute_units() * kLineWgPerCu;
+    const int64_t rows = (int64_t)p.n_seqs * p.Hkv * w.n_col, slots = slots_of(max_context);
+    if (rows > 0x7fffffffLL || (int64_t)p.n_seqs * p.Hkv * w.n_hg * ((max_context + 15) / 16 + 1) > 0x7fffffffLL - 65536)
+        return fail(MINFER_ATTN_EINVAL, "flash_attn_paged: problem too large for one launch");
+    p.slots = (int)slots;
+    p.part_o = (float*)workspace;
+    p.part_ml = (float*)((char*)workspace + part_bytes(rows, slots, D));
+    w.seq_off = (int32_t*)((char*)p.part_ml + part_bytes(rows, slots, 2));
+    w.p = p;
+    return dtype == MINFER_ATTN_F16 ? launch_decode_as<F16>(w, D, eight, stream) : launch_decode_as<BF16>(w, D, eight, stream);
+}
+
+}  // namespace minfer_attn
