@@ -420,6 +420,185 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work)
     else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
 }
 
+// ---- chunks ----------------------------------------------------------------------------------------------------------
+// What the line costs a small problem is latency: a wave streams 128 rows one group after the other, and a second launch merges.  Here the eight waves of
+// a workgroup share a chunk and merge in LDS.  A pair that is one chunk long is done with that; otherwise the chunk's result goes to
+// the workspace, and the workgroup that comes last (a counter per pair) merges the pair's.  Results cross from one XCD's L2 to
+// another's: they are written and read with device-scope accesses, which go past the L2s on both sides, and a workgroup counts itself
+// only when its own have arrived; the reader's loads stand behind a barrier that thread 0 reaches with the count's value in hand.
+MA_DEV void store_shared(float* p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+MA_DEV float load_shared(const float* p) { return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Every pair of a sequence is cut into the same number of chunks, equal to within a group; the chunk's size, the same for all sequences, is the
+// smallest (256 rows at least) that leaves no more chunks than workgroups.  Up to 64 sequences, one to a lane; all waves
+// work it out for themselves.
+template <int GR> struct ChunkPlan {
+    LineSeq q;        // per lane: the sequence
+    int each, incl;   // per lane: chunks of each of its pairs; chunks of the sequences up to and with it
+    int total;
+    MA_DEV ChunkPlan(const DecodeWork& w, int n_wg) {
+        const int lane = threadIdx.x & 63, pairs = w.p.Hkv * w.n_hg;
+        q = line_seq<GR>(w, lane);
+        const bool on = lane < w.p.n_seqs && q.info.len > 0;
+        const int sum = lane_value(wave_inclusive_scan(q.groups * pairs), 63), active = __popcll(__ballot(on));
+        const int longest = (int)wave_max((float)q.groups);
+        // a pair's last chunk is half full on average: that many workgroups are as good as not there
+        int size = max(max((sum + n_wg - 1) / max(n_wg - active * pairs / 2, 1), 256 / GR), longest / w.p.slots + 1);
+        for (;; size += 1 + size / 16) {   // (ends: with the longest context as the size there is one chunk a pair, and no more pairs than workgroups)
+            each = on ? max((q.groups + size - 1) / size, 1) : 0;
+            incl = wave_inclusive_scan(each * pairs);
+            total = lane_value(incl, 63);
+            if (total <= n_wg) break;
+        }
+    }
+};
+
+MA_DEV float merge_weight(float m, float top) { return m > -INFINITY ? fast_exp2(m - top) : 0.f; }
+
+// Merges the n chunks of the columns of (s, g, hg) from the workspace and stores the output rows; all threads of the workgroup.  The order of
+// the sums depends on nothing but n.
+template <class T, int D>
+MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g, int hg, int n, float* lds_w /* [128][16] */, float* lds_inv /* [16] */) {
+    const PagedParams& p = w.p;
+    const int tid = threadIdx.x, cols = min(16, w.n_col - hg * 16);
+    const int64_t at0 = part_row(w, s, g, hg * 16) * p.slots;
+    for (int i = tid; i < n * cols; i += kChunkWaves * 64) {
+        const int c = i / n, k = i - c * n;
+        lds_w[k * 16 + c] = load_shared(p.part_ml + (at0 + (int64_t)c * p.slots + k) * 2);
+        lds_w[(64 + k) * 16 + c] = load_shared(p.part_ml + (at0 + (int64_t)c * p.slots + k) * 2 + 1);
+    }
+    // an output element's first parts are requested while the weights are made
+    constexpr int PER = 16 * D / (kChunkWaves * 64);
+    float x[PER][8];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int idx = tid + e * kChunkWaves * 64;
+        if (idx < cols * D) {
+            const float* src = p.part_o + (at0 + (int64_t)(idx / D) * p.slots) * D + idx % D;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + (int64_t)min(u, n - 1) * D);
+        }
+    }
+    __syncthreads();
+    if (tid < cols) {
+        float top = -INFINITY, l = 0.f;
+        for (int i = 0; i < n; ++i) top = fmaxf(top, lds_w[i * 16 + tid]);
+        for (int i = 0; i < n; ++i) {
+            const float wi = merge_weight(lds_w[i * 16 + tid], top);
+            l += lds_w[(64 + i) * 16 + tid] * wi;
+            lds_w[i * 16 + tid] = wi;
+        }
+        lds_inv[tid] = l > 0.f ? 1.f / l : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int idx = tid + e * kChunkWaves * 64;
+        if (idx >= cols * D) break;
+        const int c = idx / D, d = idx % D, col = hg * 16 + c, tok = col / p.n_rep;
+        const float* src = p.part_o + (at0 + (int64_t)c * p.slots) * D + d;
+        float sum = 0.f;
+        for (int s0 = 0; s0 < n; s0 += 8) {
+            if (s0 > 0) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + (int64_t)min(s0 + u, n - 1) * D);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (s0 + u < n) sum += x[e][u] * lds_w[(s0 + u) * 16 + c];
+        }
+        if (tok < info.len)
+            reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * lds_inv[c], 0.f) & 0xffffu);
+    }
+}
+
+template <class T, int D, bool FP8>
+__global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const DecodeWork work) {
+    const PagedParams& p = work.p;
+    constexpr int NW = kChunkWaves, DB = D / 16, GR = kRows<FP8>, WAVE_LDS = kWaveLds<D, FP8>;
+    constexpr int ORS = D + 4;   // floats between two columns of a wave's result: their 16-byte pieces start in different banks
+    constexpr int LDS = NW * WAVE_LDS > NW * 16 * ORS * 4 ? NW * WAVE_LDS : NW * 16 * ORS * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];   // the waves' row areas, then their results
+    __shared__ float ml_s[128 * 16], inv_s[16];
+    __shared__ int last_s;
+    const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), l16 = lane & 15, quad = lane >> 4;
+    const int pairs = p.Hkv * work.n_hg;
+    const ChunkPlan<GR> plan(work, (int)gridDim.x);
+    const int x = (int)blockIdx.x;
+    if (x >= plan.total) return;
+    const int s = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < plan.incl)) - 1);
+    const SeqInfo info{lane_value(plan.q.info.lo, s), lane_value(plan.q.info.len, s), lane_value(plan.q.info.ctx, s)};
+    const int n = lane_value(plan.each, s), all = lane_value(plan.q.groups, s);   // chunks and groups of the pair
+    const int local = x - (lane_value(plan.incl, s) - n * pairs), pair = local / n, split = local - pair * n;
+    const int hg = work.n_hg == 1 ? 0 : pair / p.Hkv, g = pair - hg * p.Hkv;
+    const int size = all / n, longer = all - size * n;   // the first `longer` chunks are a group longer
+    const int first = split * size + min(split, longer), groups = size + (split < longer ? 1 : 0);
+    const int per = (groups + NW - 1) / NW;
+    const int g_lo = min(w * per, groups), g_hi = min(g_lo + per, groups);
+    ColumnAcc<D> acc;
+    acc.m = -INFINITY; acc.l = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc.o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (g_hi > g_lo) stream_pages<T, D, FP8>(work, s, info, g, hg, first + g_lo, first + g_hi, lds + w * WAVE_LDS, acc);
+    __syncthreads();   // every wave is done with its row area
+    const int cols = min(16, work.n_col - hg * 16);
+    float* o_s = reinterpret_cast<float*>(lds);   // [wave][column][ORS]
+    if (l16 < cols) {
+        float* dst = o_s + (w * 16 + l16) * ORS + 4 * quad;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc.o[db];
+        if (quad == 0) { ml_s[w * 16 + l16] = acc.m; ml_s[(64 + w) * 16 + l16] = acc.l; }
+    }
+    __syncthreads();
+    const bool whole = n <= 1;   // the chunk is the whole context: its result is the output
+    const int64_t at0 = part_row(work, s, g, hg * 16) * p.slots + split;
+    for (int idx = tid; idx < cols * D; idx += NW * 64) {
+        const int c = idx / D, d = idx % D;
+        float top = -INFINITY, l = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) top = fmaxf(top, ml_s[i * 16 + c]);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float wi = merge_weight(ml_s[i * 16 + c], top);
+            l += ml_s[(64 + i) * 16 + c] * wi;
+            sum += o_s[(i * 16 + c) * ORS + d] * wi;
+        }
+        if (whole) {
+            const int col = hg * 16 + c, tok = col / p.n_rep;
+            if (tok < info.len)
+                reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * (l > 0.f ? 1.f / l : 0.f), 0.f) & 0xffffu);
+        } else {
+            store_shared(p.part_o + (at0 + (int64_t)c * p.slots) * D + d, sum);
+            if (d == 0) {
+                store_shared(p.part_ml + (at0 + (int64_t)c * p.slots) * 2, top);
+                store_shared(p.part_ml + (at0 + (int64_t)c * p.slots) * 2 + 1, l);
+            }
+        }
+    }
+    if (whole || !work.done) return;
+    wait_vmcnt<0>();   // the thread's stores have arrived
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t* done = work.done + s * pairs + pair;
+        const uint32_t before = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_s = before == (uint32_t)(n - 1);
+        if (last_s) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (last_s) merge_chunks<T, D>(work, s, info, g, hg, n, ml_s, inv_s);
+}
+
+// (where there are no counters) grid (column groups x KV heads, sequences)
+template <class T, int D, int GR>
+__global__ __launch_bounds__(kChunkWaves * 64) void paged_chunk_merge_kernel(const DecodeWork work, int n_wg) {
+    const PagedParams& p = work.p;
+    __shared__ float ml_s[128 * 16], inv_s[16];
+    const int s = blockIdx.y, hg = (int)blockIdx.x / p.Hkv, g = (int)blockIdx.x - hg * p.Hkv;
+    const ChunkPlan<GR> plan(work, n_wg);
+    const int n = lane_value(plan.each, s);
+    if (n > 1) merge_chunks<T, D>(work, s, seq_info(p, s), g, hg, n, ml_s, inv_s);
+}
+
 // Workgroups of the line: as many as the chip holds at once.
 static int compute_units() {
     static std::atomic<int> cached[64];
@@ -452,9 +631,24 @@ template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStre
     hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
     return check_launch("paged_merge_kernel");
 }
+// Whether a call is one for chunks: a workgroup for every pair at least, one to a unit.
+static bool takes_chunks(const DecodeWork& w) { return w.p.n_seqs <= 64 && (int64_t)w.p.n_seqs * w.p.Hkv * w.n_hg <= compute_units(); }
+template <class T, int D, bool FP8> static int launch_chunks(DecodeWork w, hipStream_t stream) {
+    const int n_wg = compute_units();
+    static_assert(kStreamCounters >= 256, "a counter for every pair");
+    w.done = stream_counters(stream);
+    hipLaunchKernelGGL((paged_chunk_kernel<T, D, FP8>), dim3((unsigned)n_wg), dim3(kChunkWaves * 64), 0, stream, w);
+    if (int rc = check_launch("paged_chunk_kernel")) return rc;
+    if (w.done) return MINFER_ATTN_OK;
+    hipLaunchKernelGGL((paged_chunk_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)(w.p.Hkv * w.n_hg), (unsigned)w.p.n_seqs), dim3(kChunkWaves * 64), 0, stream, w, n_wg);
+    return check_launch("paged_chunk_merge_kernel");
+}
+template <class T, int D, bool FP8> static int launch_rows(const DecodeWork& w, hipStream_t stream) {
+    return takes_chunks(w) ? launch_chunks<T, D, FP8>(w, stream) : launch_line<T, D, FP8>(w, stream);
+}
 template <class T> static int launch_decode_as(const DecodeWork& w, int64_t D, bool eight, hipStream_t stream) {
-    if (eight) return D == 128 ? launch_line<T, 128, true>(w, stream) : launch_line<T, 64, true>(w, stream);
-    return D == 128 ? launch_line<T, 128, false>(w, stream) : launch_line<T, 64, false>(w, stream);
+    if (eight) return D == 128 ? launch_rows<T, 128, true>(w, stream) : launch_rows<T, 64, true>(w, stream);
+    return D == 128 ? launch_rows<T, 128, false>(w, stream) : launch_rows<T, 64, false>(w, stream);
 }
 
 int launch_paged_decode(PagedParams p, int dtype, int64_t D, bool eight, int64_t max_context, void* workspace, hipStream_t stream) {
