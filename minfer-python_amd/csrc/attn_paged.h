@@ -107,12 +107,15 @@ struct PagedParams {
     PagedCache c;
     const void* q; void* out;
     const int32_t* cu; const int32_t* ctx;
-    float* part_o;     // partial results, un-normalised, [row][slot][D] ...
-    float* part_ml;    // ... with their reference (log2 units) and sum, [row][slot][2]
+    float* part_o;     // partial results, un-normalised: decode [row][slot][D], tiles [piece][KV head][row of the block][D] ...
+    float* part_ml;    // ... with their reference (log2 units) and sum
     int64_t q1, q2, o1, o2;
     int n_seqs, T, Hq, Hkv, n_rep;
     int max_q;         // tokens of a sequence past this many are not computed
-    int slots;         // partial results a row can have
+    int slots;         // decode: partial results a row can have
+    int pieces;        // tiles: pieces that the blocks of rows may be cut into, per KV head; 0: none is cut
+    int max_blocks;    // tiles: bound of the blocks of rows
+    int32_t* blocks;   // tiles: (sequence, block, first piece, pieces) of every block, their number four entries in front of them
     float scale_log2, inv_scale_log2;  // softmax scale * log2(e), and one over it
 };
 

@@ -3,8 +3,8 @@
 // Rows.  The new tokens of a sequence and the query heads of a KV head's group are one list of rows, token by token, heads innermost
 // (row = token * n_rep + head): whatever the group's size, 32 rows of a wave attend one KV head, and a sequence of a few tokens
 // fills its rows with heads.  A workgroup takes NW * 32 rows and walks the sequence's 64-key tiles up to its last row's position;
-// where there are fewer workgroups than the chip holds the tiles are cut into n_split ranges with a workgroup each, which leave
-// un-normalised sums in the workspace for paged_combine_kernel.
+// where that makes fewer workgroups than two rounds of the chip, blocks of many tiles are cut into pieces of about equal size with a
+// workgroup each (PiecePlan), which leave un-normalised sums in the workspace for paged_combine_kernel.
 //
 // Per tile a wave computes S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32, the scores staying in registers as the second
 // product's operand; tiles are double-buffered in LDS, 16-bit rows copied there directly, 8-bit codes through registers, in which
@@ -44,6 +44,133 @@ template <class T> MA_DEV void widen16(u32x4 codes, float scale, s16x8 (&to)[2])
     for (int h = 0; h < 2; ++h) to[h] = __builtin_bit_cast(s16x8, u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]});
 }
 
+// The first 64-key tile of a sequence with a page that is there (its number of tiles if there is none): a window that moved on has given the pages
+// in front of it back.  Looked for only where the first page is missing, 64 pages at a time; the whole wave.
+MA_DEV int first_tile(const PagedCache& c, int seq, int ctx) {
+    const int32_t* table = c.table + (int64_t)seq * c.table_stride;
+    const int lane = threadIdx.x & 63, n = (ctx + (1 << c.page_log2) - 1) >> c.page_log2;
+    for (int base = 0; base < n; base += 64) {
+        const int i = base + lane;
+        const uint64_t hit = __ballot(i < n && (unsigned)table[min(i, n - 1)] < (unsigned)c.n_pages);
+        if (hit) return ((base + __ffsll((unsigned long long)hit) - 1) << c.page_log2) >> 6;
+    }
+    return (ctx + 63) >> 6;
+}
+
+// What a workgroup does: tiles t_lo .. t_hi - 1 for a block of rows of a sequence; n_pieces of the block's, this one the part-th of all pieces.
+struct PieceOf { int seq, block, lo, len, ctx, t_lo, t_hi, n_pieces, part; };
+
+// How the blocks of rows (NW * 32 each) of up to kPlanBlocks of them are cut into pieces, worked out by every workgroup for itself: the size of a piece is
+// the smallest, in tiles, that leaves no more pieces than `most`; a block is cut evenly.  Sequences, then blocks, are shared out to the threads.
+constexpr int kPlanBlocks = 1024;
+struct PieceTable { int seq_first[kPlanBlocks + 1], rows[kPlanBlocks], pos0[kPlanBlocks], tile0[kPlanBlocks], wave_sum[16]; float wave_total[16], wave_longest[16]; PieceOf found; };
+
+// Sum of x over all threads before this one (and of all): 256 threads, two barriers.
+MA_DEV int block_scan(int x, int* wave_sum, int& total) {
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int incl = wave_inclusive_scan(x);
+    if (lane == 63) wave_sum[w] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < (int)(blockDim.x >> 6); ++i) { before += i < w ? wave_sum[i] : 0; total += wave_sum[i]; }
+    __syncthreads();
+    return before + incl - x;
+}
+
+MA_DEV int tiles_of(int pos0, int rows, int n_rep, int block, int BR) { return (max(pos0 + min(block * BR + BR - 1, rows - 1) / n_rep + 1, 0) + 63) >> 6; }
+
+// The x-th piece (found.seq < 0: there is none).  With `publish`, also leaves every block's (sequence, block, first piece, pieces) for the combine kernel.
+template <int BR> MA_DEV void find_piece(const PagedParams& p, PieceTable& t, int x, int most, bool publish) {
+    const int tid = threadIdx.x, threads = blockDim.x, w = wave_id();
+    constexpr int kPer = kPlanBlocks / 256;
+    // sequences: four in a row per thread
+    int mine[kPer], sum = 0, n_blocks;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int s = tid * kPer + k;
+        mine[k] = 0;
+        if (tid < 256 && s < p.n_seqs) {
+            const TokenRange r = token_range(p.cu[s], p.cu[s + 1], p.T);
+            const int ctx = min(max(p.ctx[s], 0), p.c.width << p.c.page_log2);
+            t.rows[s] = min(r.len, p.max_q) * p.n_rep;
+            t.pos0[s] = ctx - r.len;
+            t.tile0[s] = ctx > 0 && r.len > 0 && (unsigned)p.c.table[(int64_t)s * p.c.table_stride] >= (unsigned)p.c.n_pages ? -1 : 0;
+            mine[k] = (t.rows[s] + BR - 1) / BR;
+        }
+        sum += mine[k];
+    }
+    int at = block_scan(sum, t.wave_sum, n_blocks);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        if (tid < 256 && tid * kPer + k < p.n_seqs) t.seq_first[tid * kPer + k] = at;
+        at += mine[k];
+    }
+    if (tid == 0) { t.seq_first[p.n_seqs] = n_blocks; t.found.seq = -1; }
+    n_blocks = min(n_blocks, p.max_blocks);   // (sequences that overlap, which no valid call has, could make more than there is room for)
+    __syncthreads();
+    for (int s = w; s < p.n_seqs; s += threads >> 6)
+        if (t.tile0[s] < 0) {
+            const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
+            const int tile = first_tile(p.c, s, t.pos0[s] + r.len);
+            if ((tid & 63) == 0) t.tile0[s] = tile;
+        }
+    __syncthreads();
+    // blocks: as many in a row per thread as that takes
+    const int per = (n_blocks + 255) >> 8;   // <= kPer
+    int seq[kPer], blk[kPer], lo[kPer], n_tiles[kPer], all = 0, longest = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int i = tid * per + k;
+        n_tiles[k] = 0;
+        if (tid < 256 && k < per && i < n_blocks) {
+            int a = 0, b = p.n_seqs - 1;   // the last sequence whose first block is not behind i
+            while (a < b) { const int m = (a + b + 1) >> 1; if (t.seq_first[m] <= i) a = m; else b = m - 1; }
+            seq[k] = a;
+            blk[k] = t.seq_first[a + 1] - 1 - i;   // most keys first
+            lo[k] = t.tile0[a];
+            n_tiles[k] = max(tiles_of(t.pos0[a], t.rows[a], p.n_rep, blk[k], BR) - lo[k], 1);
+        }
+        all += n_tiles[k];
+        longest = max(longest, n_tiles[k]);
+    }
+    float total = 0.f, most_tiles = 0.f;   // (sums that the size alone goes by: the same in every workgroup)
+    {
+        const float sum_w = lane_sum<64>((float)all), max_w = wave_max((float)longest);
+        if ((tid & 63) == 0) { t.wave_total[w] = sum_w; t.wave_longest[w] = max_w; }
+        __syncthreads();
+        for (int i = 0; i < (threads >> 6); ++i) { total += t.wave_total[i]; most_tiles = fmaxf(most_tiles, t.wave_longest[i]); }
+    }
+    constexpr int kLeastTiles = 4;
+    int size = max((int)ceilf(total / (float)most), kLeastTiles), n, before;
+    for (;; size += 1 + size / 16) {
+        n = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) n += (n_tiles[k] + size - 1) / size;
+        int pieces;
+        before = block_scan(n, t.wave_sum, pieces);
+        if (pieces <= most || (float)size >= most_tiles) break;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int pieces = (n_tiles[k] + size - 1) / size;
+        if (pieces > 0) {
+            if (x >= before && x < before + pieces) {
+                const int i = x - before, each = n_tiles[k] / pieces, longer = n_tiles[k] - each * pieces;
+                PieceOf f;
+                f.seq = seq[k]; f.block = blk[k]; f.n_pieces = pieces; f.part = x;
+                f.t_lo = lo[k] + i * each + min(i, longer);
+                f.t_hi = f.t_lo + each + (i < longer ? 1 : 0);
+                t.found = f;
+            }
+            if (publish) reinterpret_cast<int4*>(p.blocks)[tid * per + k] = make_int4(seq[k], blk[k], before, pieces);
+            before += pieces;
+        }
+    }
+    if (publish && tid == 0) p.blocks[-4] = n_blocks;
+    __syncthreads();
+}
+
 template <class T, int D, bool FP8, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParams p) {
     using GEO = PagedGeom<D, NW>;
@@ -69,35 +196,50 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
         g = (int)blockIdx.x % p.Hkv;
         rank = (int)blockIdx.x / p.Hkv;
     }
-    const int split = rank % p.slots;
-    int x = rank / p.slots, seq = -1, seq_lo = 0, seq_len = 0, blocks = 0;
-    for (int base = 0; base < p.n_seqs; base += 64) {
-        const int s = base + lane;
-        TokenRange r{0, 0};
-        if (s < p.n_seqs) r = token_range(p.cu[s], p.cu[s + 1], p.T);
-        const int n = (min(r.len, p.max_q) * p.n_rep + BR - 1) / BR;
-        const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
-        if (x < total) {
-            const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
-            seq = base + src;
-            seq_lo = lane_value(r.lo, src);
-            seq_len = lane_value(r.len, src);
-            blocks = lane_value(n, src);
-            x -= lane_value(incl - n, src);
-            break;
+    PieceOf me;
+    me.seq = -1;
+    if (p.pieces > 0) {
+        PieceTable& table = *reinterpret_cast<PieceTable*>(&kv_lds[0][0]);
+        static_assert(sizeof(PieceTable) <= 2 * STAGE_BYTES, "in the stages, before any tile or row is there");
+        find_piece<BR>(p, table, rank, p.pieces, blockIdx.x == 0);
+        me = table.found;
+        __syncthreads();   // the stages are free
+        if (me.seq < 0) return;
+    } else {
+        int x = rank;
+        for (int base = 0; base < p.n_seqs; base += 64) {
+            const int s = base + lane;
+            TokenRange r{0, 0};
+            if (s < p.n_seqs) r = token_range(p.cu[s], p.cu[s + 1], p.T);
+            const int n = (min(r.len, p.max_q) * p.n_rep + BR - 1) / BR;
+            const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
+            if (x < total) {
+                const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
+                me.seq = base + src;
+                me.block = lane_value(n, src) - 1 - (x - lane_value(incl - n, src));   // most keys first
+                break;
+            }
+            x -= total;
         }
-        x -= total;
+        if (me.seq < 0) return;
+        me.n_pieces = 1;
     }
-    if (seq < 0) return;
-    const int block = blocks - 1 - x;                                    // most keys first
+    const int seq = __builtin_amdgcn_readfirstlane(me.seq), block = __builtin_amdgcn_readfirstlane(me.block);
+    const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
+    const int seq_lo = range.lo, seq_len = range.len;
     const int ctx = min(max(const_load(p.ctx + seq), 0), p.c.width << p.c.page_log2);
     const int pos0 = ctx - seq_len;                                      // position of the sequence's token 0
     const int rows = min(seq_len, p.max_q) * p.n_rep, last_row = rows - 1;
     const int row0 = block * BR + w * 32;                                // the wave's first row
     const bool wave_on = row0 < rows;
-    const int keys = max(pos0 + min(block * BR + BR - 1, last_row) / p.n_rep + 1, 0);   // of the workgroup's last row
-    const int n_tiles = (keys + 63) >> 6, per = (n_tiles + p.slots - 1) / p.slots;
-    const int t_lo = min(split * per, n_tiles), n_own = min(t_lo + per, n_tiles) - t_lo;
+    int t_lo = 0, t_hi = tiles_of(pos0, rows, p.n_rep, block, BR);
+    if (p.pieces > 0) {
+        t_lo = __builtin_amdgcn_readfirstlane(me.t_lo);
+        t_hi = min(t_hi, __builtin_amdgcn_readfirstlane(me.t_hi));
+    } else if (t_hi > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages) {
+        t_lo = first_tile(p.c, seq, ctx);
+    }
+    const int n_own = max(t_hi - t_lo, 0);
     const int wave_first = pos0 + min(row0, last_row) / p.n_rep, wave_last = pos0 + min(row0 + 31, last_row) / p.n_rep;
 
     // positions of the lane's two rows (one per block of 16)
@@ -386,7 +528,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
                 pg = pages_of(kt + 2);
             }
         }
-        if (wave_on && kt * 64 <= wave_last) process_tile(stage_tag, kt, there);
+        if (wave_on && there && kt * 64 <= wave_last) process_tile(stage_tag, kt, there);
         there = there_1;
         there_1 = there_2;
     };
@@ -399,12 +541,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     float l_all[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) l_all[qb] = sum_across_quads(l_sum[qb]);
-    if (p.slots > 1) {
+    if (me.n_pieces > 1) {
+        const int64_t part = (int64_t)(__builtin_amdgcn_readfirstlane(me.part) * p.Hkv + g) * BR;
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-            const int r = row0 + 16 * qb + l16, t = r / p.n_rep;
-            if (r > last_row) continue;
-            const int64_t slot = ((int64_t)(seq_lo + t) * p.Hq + g * p.n_rep + r - t * p.n_rep) * p.slots + split;
+            if (row0 + 16 * qb + l16 > last_row) continue;
+            const int64_t slot = part + w * 32 + 16 * qb + l16;
             float* dst = p.part_o + slot * D + 4 * quad;
 #pragma unroll
             for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = o_acc[db][qb];
@@ -441,35 +583,43 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     }
 }
 
-// out = sum_i O_i w_i / sum_i l_i w_i with w_i = 2^(m_i - max m) over the n_split parts of a row; a wave per row (token, head), lane i
-// holding part i's reference and sum.  A part without keys has a sum of zero and is left out; one whose scores are all NaN has
-// sums of NaN and is multiplied like any other.  grid (n_seqs * blocks_per_seq), 4 waves.
-template <class T, int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p, int blocks_per_seq) {
+// out = sum_i O_i w_i / sum_i l_i w_i with w_i = 2^(m_i - max m) over the pieces of a block that was cut; a wave per row, lane i holding
+// piece i's reference and sum.  A piece without keys has a sum of zero and is left out; one whose scores are all NaN has sums of
+// NaN and is multiplied like any other.  grid (rows of a block / 4, KV heads, blocks), 4 waves.
+template <class T, int D, int BR>
+__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
     constexpr int EPL = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int s = (int)blockIdx.x / blocks_per_seq, row = ((int)blockIdx.x - s * blocks_per_seq) * 4 + wave_id();
-    const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
-    if (row >= min(r.len, p.max_q) * p.Hq) return;
-    const int t = row / p.Hq, head = row - t * p.Hq;
-    const int64_t slot0 = ((int64_t)(r.lo + t) * p.Hq + head) * p.slots;
-    float m = -INFINITY, l = 0.f;
-    if (lane < p.slots) { m = p.part_ml[(slot0 + lane) * 2]; l = p.part_ml[(slot0 + lane) * 2 + 1]; }
-    const float top = wave_max(m);
-    const float wgt = m > -INFINITY ? fast_exp2(m - top) : 0.f;
-    const float total = lane_sum<64>(l * wgt);
-    float acc[EPL];
+    const int lane = threadIdx.x & 63, row = (int)blockIdx.x * 4 + wave_id(), g = blockIdx.y, b = blockIdx.z;
+    if (b >= const_load(p.blocks - 4)) return;
+    const int seq = const_load(p.blocks + 4 * b), block = const_load(p.blocks + 4 * b + 1), first = const_load(p.blocks + 4 * b + 2), n = const_load(p.blocks + 4 * b + 3);
+    const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
+    const int r = block * BR + row;
+    if (n <= 1 || r >= min(range.len, p.max_q) * p.n_rep) return;
+    const int64_t step = (int64_t)p.Hkv * BR, at0 = ((int64_t)first * p.Hkv + g) * BR + row;
+    float top = -INFINITY, total = 0.f, acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-    for (int i = 0; i < p.slots; ++i) {
-        if (lane_value(l, i) == 0.f) continue;
-        const float wi = lane_value(wgt, i);
-        const float* src = p.part_o + (slot0 + i) * D + EPL * lane;
+    for (int base = 0; base < n; base += 64) {   // (a block of more than 64 pieces: what is there so far takes the new reference)
+        float m = -INFINITY, l = 0.f;
+        if (base + lane < n) { m = p.part_ml[(at0 + (base + lane) * step) * 2]; l = p.part_ml[(at0 + (base + lane) * step) * 2 + 1]; }
+        const float now = fmaxf(top, wave_max(m));
+        const float was = top > -INFINITY ? fast_exp2(top - now) : (now > -INFINITY ? 0.f : 1.f);
+        const float wgt = m > -INFINITY ? fast_exp2(m - now) : 0.f;
+        total = total * was + lane_sum<64>(l * wgt);
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) acc[e] += src[e] * wi;
+        for (int e = 0; e < EPL; ++e) acc[e] *= was;
+        top = now;
+        for (int i = 0; i < min(n - base, 64); ++i) {
+            if (lane_value(l, i) == 0.f) continue;
+            const float wi = lane_value(wgt, i);
+            const float* src = p.part_o + (at0 + (base + i) * step) * D + EPL * lane;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[e] += src[e] * wi;
+        }
     }
     const float inv = total > 0.f ? 1.f / total : 0.f;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(r.lo + t) * p.o2 + (int64_t)head * p.o1 + EPL * lane;
+    const int t = r / p.n_rep;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(range.lo + t) * p.o2 + (int64_t)(g * p.n_rep + r - t * p.n_rep) * p.o1 + EPL * lane;
     if (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = T::pack2(acc[0] * inv, acc[EPL - 1] * inv);
     else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
 }
@@ -479,18 +629,20 @@ static int64_t bounded_tokens(int64_t T, int64_t max_q_len) { return max_q_len >
 // How a call is laid out, from its sizes alone (contexts and lengths are on the device).
 struct PagedPlan {
     int64_t blocks;    // bound of the blocks of rows of all sequences
-    int64_t n_split;
-    size_t o_bytes, ml_bytes;
+    int64_t pieces;    // pieces per KV head that they may be cut into; 0: none is cut
+    size_t o_bytes, ml_bytes, table_bytes;
 };
-static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q, int rows_per_wg) {
+constexpr int64_t kRound = 512;   // workgroups that the chip holds at once
+static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int rows_per_wg) {
     PagedPlan r{};
     const int64_t n_rep = Hq / Hkv;
     r.blocks = std::min(n_seqs * ((max_q * n_rep + rows_per_wg - 1) / rows_per_wg), T * n_rep / rows_per_wg + n_seqs);
-    const int64_t wgs = r.blocks * Hkv, most = std::min<int64_t>(64, max_context / 256);
-    r.n_split = std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(wgs, 1)));
-    if (r.n_split > 1) {
-        r.o_bytes = ((size_t)(T * Hq * r.n_split * D * 4) + 255) / 256 * 256;
-        r.ml_bytes = ((size_t)(T * Hq * r.n_split * 2 * 4) + 255) / 256 * 256;
+    const int64_t wgs = r.blocks * Hkv;
+    if (wgs <= 2 * kRound && r.blocks <= kPlanBlocks && n_seqs <= kPlanBlocks) {
+        r.pieces = std::max((wgs + kRound - 1) / kRound * kRound / Hkv, r.blocks);
+        r.o_bytes = (size_t)(r.pieces * Hkv * rows_per_wg * D * 4);
+        r.ml_bytes = (size_t)(r.pieces * Hkv * rows_per_wg * 2 * 4);
+        r.table_bytes = (size_t)(r.blocks + 1) * 16;
     }
     return r;
 }
@@ -499,11 +651,12 @@ constexpr int kPagedWaves = 4;
 
 template <class T, int D, bool FP8>
 static int launch_paged(const PagedParams& p, const PagedPlan& plan, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, FP8, kPagedWaves>), dim3((unsigned)(plan.blocks * p.Hkv * plan.n_split)), dim3(kPagedWaves * 64), 0, stream, p);
+    const int64_t wgs = (plan.pieces > 0 ? plan.pieces : plan.blocks) * p.Hkv;
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, FP8, kPagedWaves>), dim3((unsigned)wgs), dim3(kPagedWaves * 64), 0, stream, p);
     if (int rc = check_launch("paged_tile_kernel")) return rc;
-    if (plan.n_split == 1) return MINFER_ATTN_OK;
-    const int64_t per = ((int64_t)p.max_q * p.Hq + 3) / 4;
-    hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3((unsigned)(per * p.n_seqs)), dim3(256), 0, stream, p, (int)per);
+    if (plan.pieces == 0) return MINFER_ATTN_OK;
+    constexpr int BR = kPagedWaves * 32;
+    hipLaunchKernelGGL((paged_combine_kernel<T, D, BR>), dim3(BR / 4, (unsigned)p.Hkv, (unsigned)plan.blocks), dim3(256), 0, stream, p);
     return check_launch("paged_combine_kernel");
 }
 template <class T> static int launch_paged_as(const PagedParams& p, const PagedPlan& plan, int64_t D, bool eight, hipStream_t stream) {
@@ -520,8 +673,8 @@ MINFER_ATTN_EXPORT size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs
     if (n_seqs <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_context < 0 || Hq % Hkv != 0) return 0;
     const int64_t max_q = bounded_tokens(T, max_q_len);
     if (paged_decode_takes(Hq, Hkv, max_q)) return paged_decode_workspace_bytes(n_seqs, Hq, Hkv, D, max_context, max_q);
-    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_context, max_q, kPagedWaves * 32);
-    return r.o_bytes + r.ml_bytes;
+    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_q, kPagedWaves * 32);
+    return r.o_bytes + r.ml_bytes + r.table_bytes;
 }
 
 MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const void* q, const minfer_kv_pages* pages, const int32_t* cu_seqlens,
@@ -558,14 +711,15 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
             return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
         return launch_paged_decode(p, dtype, D, eight, max_context, workspace, (hipStream_t)stream_v);
     }
-    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_context, max_q, kPagedWaves * 32);
+    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_q, kPagedWaves * 32);
     // (workgroups and their ids are 32-bit numbers)
-    if (plan.blocks * Hkv * plan.n_split > 0x7fffffffLL || (max_q * Hq + 3) / 4 * n_seqs > 0x7fffffffLL)
-        return bad("flash_attn_paged: problem too large for one launch");
-    if (plan.n_split > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes))
+    if (plan.blocks * Hkv > 0x7fffffffLL) return bad("flash_attn_paged: problem too large for one launch");
+    if (plan.pieces > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes + plan.table_bytes))
         return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
-    p.slots = (int)plan.n_split;
+    p.pieces = (int)plan.pieces;
+    p.max_blocks = (int)plan.blocks;
     p.part_o = (float*)workspace;
     p.part_ml = (float*)((char*)workspace + plan.o_bytes);
+    p.blocks = plan.pieces > 0 ? (int32_t*)((char*)workspace + plan.o_bytes + plan.ml_bytes) + 4 : nullptr;
     return dtype == MINFER_ATTN_F16 ? launch_paged_as<F16>(p, plan, D, eight, (hipStream_t)stream_v) : launch_paged_as<BF16>(p, plan, D, eight, (hipStream_t)stream_v);
 }

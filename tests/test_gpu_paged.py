@@ -97,6 +97,32 @@ def test_attend_bad_tables(kerns, seqs, eight):
         check_attend(kerns, c, 4)
 
 
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("seqs,Hq,Hkv,D,page,gone", [
+    ([(20, 38000)], 4, 1, 64, 64, 0),                              # one block of rows in more pieces than lanes
+    ([(60, 5000), (33, 90), (200, 0)], 4, 1, 128, 16, 0),          # pieces of long and short blocks together
+    ([(60, 5000), (33, 3000)], 6, 2, 64, 32, 40),                  # their first pages given back
+    ([(17 + i % 3, (37 * i) % 200) for i in range(150)], 2, 1, 64, 16, 0),   # more sequences than lanes
+    ([(260, 2000)], 24, 8, 64, 16, 0),                             # more blocks than one round
+    ([(700, 0), (300, 40)], 32, 8, 64, 16, 1),                     # blocks of two rounds
+], ids=["many pieces", "long and short", "given back", "many sequences", "a round", "two rounds"])
+def test_attend_pieces(kerns, seqs, Hq, Hkv, D, page, gone, eight):
+    c = ref.Paged(seqs, page, Hkv, D, torch.float16, DEV, gone={(s, i) for s in range(len(seqs)) for i in range(gone)}, eight=eight)
+    check_attend(kerns, c, Hq)
+
+
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("seqs,Hq,Hkv", [([(1, 9000), (1, 70), (1, 2500)], 8, 1), ([(1, (53 * i) % 700) for i in range(70)], 4, 1),
+                                         ([(1, 3000 + 37 * i) for i in range(40)], 16, 8), ([(2, 5000), (4, 700), (0, 40)], 8, 2), ([(1, 20000)], 2, 1)],
+                         ids=["uneven", "more than lanes", "the line", "drafts", "long"])
+def test_attend_shares(kerns, seqs, Hq, Hkv, eight):
+    """Chunks and shares: contexts that differ, more sequences than lanes, more pairs than units, many parts of a row; a table that is wider than the
+    longest context needs."""
+    for width in (None, 4000):
+        c = ref.Paged(seqs, 16, Hkv, 64, torch.float16, DEV, eight=eight, width=width)
+        check_attend(kerns, c, Hq)
+
+
 @pytest.mark.parametrize("n_tokens", [1, 3, 50])
 def test_attend_leaves_other_rows(kerns, n_tokens):
     """Rows of out behind the last sequence, and tokens past max_q_len, are left as they were."""
