@@ -180,8 +180,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     constexpr int BR = NW * 32;  // rows of a workgroup
     constexpr int STAGE_BYTES = 2 * GEO::TILE_BYTES;   // the K tile followed by the V tile
     constexpr int ROWS_BYTES = 32 * RB;
-    static_assert(NW * ROWS_BYTES == STAGE_BYTES, "a workgroup's query or output rows fill a stage");
+    // The waves' query rows on their way in and output rows on their way out: with four waves inside a stage (the query rows in stage 1, which no
+    // tile touches before the barrier of tile 0; the output rows in the stage that the last tile did not use), with eight beside them.
+    constexpr bool kAliasRows = NW * ROWS_BYTES <= STAGE_BYTES;
     __shared__ __attribute__((aligned(1024))) char kv_lds[2][STAGE_BYTES];
+    __shared__ __attribute__((aligned(1024))) char rows_lds[kAliasRows ? 1 : NW][kAliasRows ? 16 : ROWS_BYTES];
 
     const int lane = threadIdx.x & 63, w = wave_id();
     const int l16 = lane & 15, quad = lane >> 4;
@@ -237,7 +240,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
         t_lo = __builtin_amdgcn_readfirstlane(me.t_lo);
         t_hi = min(t_hi, __builtin_amdgcn_readfirstlane(me.t_hi));
     } else if (t_hi > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages) {
-        t_lo = first_tile(p.c, seq, ctx);
+        t_lo = __builtin_amdgcn_readfirstlane(first_tile(p.c, seq, ctx));
     }
     const int n_own = max(t_hi - t_lo, 0);
     const int wave_first = pos0 + min(row0, last_row) / p.n_rep, wave_last = pos0 + min(row0 + 31, last_row) / p.n_rep;
@@ -245,8 +248,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     // positions of the lane's two rows (one per block of 16)
     const int pos[2] = {pos0 + min(row0 + l16, last_row) / p.n_rep, pos0 + min(row0 + 16 + l16, last_row) / p.n_rep};
 
-    // ---- the wave's query rows, copied global->LDS as whole rows into stage 1, which no tile touches before the barrier of tile 0 ----
-    char* const q_stage = &kv_lds[1][w * ROWS_BYTES];
+    // ---- the wave's query rows, copied global->LDS as whole rows ----
+    char* const q_stage = kAliasRows ? &kv_lds[1][w * ROWS_BYTES] : &rows_lds[kAliasRows ? 0 : w][0];
 #pragma unroll
     for (int j = 0; j < 32 / RPI; ++j) {
         const int row = j * RPI + lane / G, r = min(row0 + row, last_row), t = r / p.n_rep;
@@ -310,7 +313,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     constexpr int NR = FP8 ? GEO::NLD8 : 1, RPI8 = GEO::RPI8;
     __shared__ __attribute__((aligned(1024))) char raw_lds[FP8 ? NW : 1][FP8 ? 2 * NR * 1024 : 16];
     const uint32_t raw0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(&raw_lds[FP8 ? w : 0][0]));
-    struct Scales { float k[NR], v[NR]; } scales;   // of the tile in the raw area
+    struct Scales { uint32_t k[NR], v[NR]; } scales{};   // of the tile in the raw area, as their bytes
     const uint32_t c_off = (uint32_t)((lane / (D / 16)) * (int)p.c.row_stride + 16 * (lane % (D / 16)));
     auto block_of = [&](int j) __attribute__((always_inline)) { return ((j * NW + w) * RPI8) >> 4; };
     auto request_codes = [&](int kt, const Pages& pg) __attribute__((always_inline)) {
@@ -320,10 +323,18 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
             const int64_t at = rows_at(id, kt * 64 + (j * NW + w) * RPI8);
             copy16_global_to_lds_at<2 * j * 1024, true>((const char*)p.c.k + at, c_off, raw0);
             copy16_global_to_lds_at<(2 * j + 1) * 1024, true>((const char*)p.c.v + at, c_off, raw0);
-            const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
-            scales.k[j] = scale_value(const_byte(p.c.k_scales + sc));
-            scales.v[j] = scale_value(const_byte(p.c.v_scales + sc));
         });
+    };
+    auto scales_of = [&](const Pages& pg) __attribute__((always_inline)) {
+        Scales r;
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            const int b = block_of(j), id = b == 0 ? pg.id[0] : b == 1 ? pg.id[1] : b == 2 ? pg.id[2] : pg.id[3];
+            const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
+            r.k[j] = const_byte(p.c.k_scales + sc);
+            r.v[j] = const_byte(p.c.v_scales + sc);
+        }
+        return r;
     };
     auto widen_tile = [&](int kt, int there, int stage) __attribute__((always_inline)) {
         // (the lane's places are worked out for every tile: ten instructions; kept across tiles they do not fit the registers at D = 128)
@@ -337,10 +348,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
             constexpr int j = decltype(j_tag)::value, AT = j * NW * RPI8 * RB;
             const bool on = (there >> block_of(j) & 1) && kt * 64 + j * NW * RPI8 + row_w < ctx;
             s16x8 x[2];
-            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw0 + 16 * ln, 2 * j * 1024)), scales.k[j], x);
+            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw0 + 16 * ln, 2 * j * 1024)), scale_value(scales.k[j]), x);
             lds_write_b128(k_to, AT, x[0]);
             lds_write_b128(k_to ^ 16u, AT, x[1]);
-            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw0 + 16 * ln, (2 * j + 1) * 1024)), scales.v[j], x);
+            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw0 + 16 * ln, (2 * j + 1) * 1024)), scale_value(scales.v[j]), x);
             lds_write_b128(v_to, AT, on ? x[0] : s16x8{0, 0, 0, 0, 0, 0, 0, 0});
             lds_write_b128(v_to ^ 16u, AT, on ? x[1] : s16x8{0, 0, 0, 0, 0, 0, 0, 0});
         });
@@ -486,7 +497,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     if (n_own > 0) {
         pg = pages_of(t_lo);
         there = there_of(pg);
-        if (FP8) request_codes(t_lo, pg);
+        if (FP8) { request_codes(t_lo, pg); scales = scales_of(pg); }
         else copy_tile(t_lo, pg, std::integral_constant<int, 0>{});
         pg = pages_of(t_lo + 1);
     }
@@ -502,7 +513,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     }
     if (FP8 && n_own > 0) {
         widen_tile(t_lo, there, 0);
-        if (n_own > 1) request_codes(t_lo + 1, pg);
+        if (n_own > 1) { request_codes(t_lo + 1, pg); scales = scales_of(pg); }
         there_1 = there_of(pg);
         pg = pages_of(t_lo + 2);
     }
@@ -510,9 +521,19 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
         constexpr int STAGE = decltype(stage_tag)::value;
         const int kt = t_lo + it;
         int there_2 = 0;
+        // The table's entries, and the scales of codes about to be sent for, are asked for here and waited for in front of the barrier, where the wave
+        // waits anyway: scalar loads return in no order, so that with one on its way every wait for an LDS read is one for all of them.
+        Pages after = pages_of(FP8 ? kt + 3 : kt + 2);
+        Scales scales_2{};
+        if (FP8) scales_2 = scales_of(pg);
         if (!FP8) {
             wait_vmcnt<0>();       // this wave's share of the tile has landed
             if (!whole(kt, there)) clear_rows(kt, there, STAGE);
+        }
+        asm volatile("" : "+s"(after.id[0]), "+s"(after.id[1]), "+s"(after.id[2]), "+s"(after.id[3]));
+        if (FP8) {
+#pragma unroll
+            for (int j = 0; j < NR; ++j) asm volatile("" : "+s"(scales_2.k[j]), "+s"(scales_2.v[j]));
         }
         __syncthreads();           // everyone's has; the other stage is no longer being read
         if (it + 1 < n_own) {
@@ -521,12 +542,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
                 widen_tile(kt + 1, there_1, STAGE ^ 1);
                 if (it + 2 < n_own) request_codes(kt + 2, pg);
                 there_2 = there_of(pg);
-                pg = pages_of(kt + 3);
+                scales = scales_2;
             } else {
                 copy_tile(kt + 1, pg, std::integral_constant<int, STAGE ^ 1>{});
                 there_1 = there_of(pg);
-                pg = pages_of(kt + 2);
             }
+            pg = after;
         }
         if (wave_on && there && kt * 64 <= wave_last) process_tile(stage_tag, kt, there);
         there = there_1;
@@ -554,8 +575,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
         }
         return;
     }
-    // normalised rows through LDS (the stage that the last tile did not use), so that a store instruction writes whole rows
-    const uint32_t so = lds_addr(&kv_lds[0][0]) + (n_own & 1) * STAGE_BYTES + w * ROWS_BYTES;
+    // normalised rows through LDS, so that a store instruction writes whole rows
+    const uint32_t so = kAliasRows ? lds_addr(&kv_lds[0][0]) + (n_own & 1) * STAGE_BYTES + w * ROWS_BYTES : lds_addr(q_stage);
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
     wave_lds_order();
@@ -583,85 +604,104 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     }
 }
 
-// out = sum_i O_i w_i / sum_i l_i w_i with w_i = 2^(m_i - max m) over the pieces of a block that was cut; a wave per row, lane i holding
-// piece i's reference and sum.  A piece without keys has a sum of zero and is left out; one whose scores are all NaN has sums of
-// NaN and is multiplied like any other.  grid (rows of a block / 4, KV heads, blocks), 4 waves.
+// out = sum_i O_i w_i / sum_i l_i w_i with w_i = 2^(m_i - max m) over the pieces of a block that was cut; D/4 lanes per row, four pieces requested at a
+// time, references and sums with them.  A piece without keys has a sum of zero and is left out; one whose scores are all NaN has sums of NaN and
+// is multiplied like any other.  grid (rows of a block / rows of a workgroup, KV heads, blocks).
 template <class T, int D, int BR>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
-    constexpr int EPL = D / 64;
-    const int lane = threadIdx.x & 63, row = (int)blockIdx.x * 4 + wave_id(), g = blockIdx.y, b = blockIdx.z;
+    constexpr int LPR = D / 4, RPW = 256 / LPR;   // lanes per row, rows per workgroup
+    const int row = (int)blockIdx.x * RPW + (int)threadIdx.x / LPR, d = 4 * ((int)threadIdx.x % LPR), g = blockIdx.y, b = blockIdx.z;
     if (b >= const_load(p.blocks - 4)) return;
     const int seq = const_load(p.blocks + 4 * b), block = const_load(p.blocks + 4 * b + 1), first = const_load(p.blocks + 4 * b + 2), n = const_load(p.blocks + 4 * b + 3);
+    if (n <= 1) return;
     const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
     const int r = block * BR + row;
-    if (n <= 1 || r >= min(range.len, p.max_q) * p.n_rep) return;
+    if (r >= min(range.len, p.max_q) * p.n_rep) return;
     const int64_t step = (int64_t)p.Hkv * BR, at0 = ((int64_t)first * p.Hkv + g) * BR + row;
-    float top = -INFINITY, total = 0.f, acc[EPL];
+    float top = -INFINITY, total = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < n; i0 += 4) {
+        f32x2 ml[4];
+        f32x4 o[4];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-    for (int base = 0; base < n; base += 64) {   // (a block of more than 64 pieces: what is there so far takes the new reference)
-        float m = -INFINITY, l = 0.f;
-        if (base + lane < n) { m = p.part_ml[(at0 + (base + lane) * step) * 2]; l = p.part_ml[(at0 + (base + lane) * step) * 2 + 1]; }
-        const float now = fmaxf(top, wave_max(m));
+        for (int u = 0; u < 4; ++u) {
+            const int64_t at = at0 + min(i0 + u, n - 1) * step;
+            ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + at * 2);
+            o[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + d);
+        }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) now = fmaxf(now, ml[u][0]);
         const float was = top > -INFINITY ? fast_exp2(top - now) : (now > -INFINITY ? 0.f : 1.f);
-        const float wgt = m > -INFINITY ? fast_exp2(m - now) : 0.f;
-        total = total * was + lane_sum<64>(l * wgt);
+        total *= was;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) acc[e] *= was;
+        for (int e = 0; e < 4; ++e) acc[e] *= was;
         top = now;
-        for (int i = 0; i < min(n - base, 64); ++i) {
-            if (lane_value(l, i) == 0.f) continue;
-            const float wi = lane_value(wgt, i);
-            const float* src = p.part_o + (at0 + (base + i) * step) * D + EPL * lane;
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) acc[e] += src[e] * wi;
+        for (int u = 0; u < 4; ++u) {
+            const bool on = i0 + u < n && !(ml[u][1] == 0.f);
+            const float w = ml[u][0] > -INFINITY ? fast_exp2(ml[u][0] - now) : 0.f;
+            total += on ? ml[u][1] * w : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += on ? o[u][e] * w : 0.f;
         }
     }
     const float inv = total > 0.f ? 1.f / total : 0.f;
     const int t = r / p.n_rep;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(range.lo + t) * p.o2 + (int64_t)(g * p.n_rep + r - t * p.n_rep) * p.o1 + EPL * lane;
-    if (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = T::pack2(acc[0] * inv, acc[EPL - 1] * inv);
-    else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
+    uint2 pk;
+    pk.x = T::pack2(acc[0] * inv, acc[1] * inv);
+    pk.y = T::pack2(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>((uint16_t*)p.out + (int64_t)(range.lo + t) * p.o2 + (int64_t)(g * p.n_rep + r - t * p.n_rep) * p.o1 + d) = pk;
 }
 
 static int64_t bounded_tokens(int64_t T, int64_t max_q_len) { return max_q_len > 0 && max_q_len < T ? max_q_len : T; }
 
 // How a call is laid out, from its sizes alone (contexts and lengths are on the device).
 struct PagedPlan {
+    int waves;         // per workgroup
     int64_t blocks;    // bound of the blocks of rows of all sequences
     int64_t pieces;    // pieces per KV head that they may be cut into; 0: none is cut
     size_t o_bytes, ml_bytes, table_bytes;
 };
-constexpr int64_t kRound = 512;   // workgroups that the chip holds at once
-static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int rows_per_wg) {
+// Rows of a workgroup: 256 share a tile's copies at head_dim 128 where they fill the chip's units, one workgroup to a unit, one and a half times; 128, two to
+// a unit (three at head_dim 64), else.
+constexpr int kWavesBig = 8, kWavesSmall = 4;
+constexpr int64_t kUnits = 256;
+static int64_t blocks_of(int64_t n_seqs, int64_t T, int64_t n_rep, int64_t max_q, int waves) {
+    const int64_t rows = waves * 32;
+    return std::min(n_seqs * ((max_q * n_rep + rows - 1) / rows), T * n_rep / rows + n_seqs);
+}
+#ifndef MINFER_PAGED_BIG
+#define MINFER_PAGED_BIG 384
+#endif
+static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q) {
     PagedPlan r{};
     const int64_t n_rep = Hq / Hkv;
-    r.blocks = std::min(n_seqs * ((max_q * n_rep + rows_per_wg - 1) / rows_per_wg), T * n_rep / rows_per_wg + n_seqs);
-    const int64_t wgs = r.blocks * Hkv;
-    if (wgs <= 2 * kRound && r.blocks <= kPlanBlocks && n_seqs <= kPlanBlocks) {
-        r.pieces = std::max((wgs + kRound - 1) / kRound * kRound / Hkv, r.blocks);
-        r.o_bytes = (size_t)(r.pieces * Hkv * rows_per_wg * D * 4);
-        r.ml_bytes = (size_t)(r.pieces * Hkv * rows_per_wg * 2 * 4);
+    r.waves = D == 128 && T * n_rep / (kWavesBig * 32) * Hkv >= MINFER_PAGED_BIG ? kWavesBig : kWavesSmall;
+    r.blocks = blocks_of(n_seqs, T, n_rep, max_q, r.waves);
+    const int64_t wgs = r.blocks * Hkv, round = r.waves == kWavesBig ? kUnits : 2 * kUnits;   // workgroups that the chip holds at once
+    if (wgs <= 2 * round && r.blocks <= kPlanBlocks && n_seqs <= kPlanBlocks) {
+        r.pieces = std::max((wgs + round - 1) / round * round / Hkv, r.blocks);
+        r.o_bytes = (size_t)(r.pieces * Hkv * r.waves * 32 * D * 4);
+        r.ml_bytes = (size_t)(r.pieces * Hkv * r.waves * 32 * 2 * 4);
         r.table_bytes = (size_t)(r.blocks + 1) * 16;
     }
     return r;
 }
 
-constexpr int kPagedWaves = 4;
-
-template <class T, int D, bool FP8>
+template <class T, int D, bool FP8, int NW>
 static int launch_paged(const PagedParams& p, const PagedPlan& plan, hipStream_t stream) {
     const int64_t wgs = (plan.pieces > 0 ? plan.pieces : plan.blocks) * p.Hkv;
-    hipLaunchKernelGGL((paged_tile_kernel<T, D, FP8, kPagedWaves>), dim3((unsigned)wgs), dim3(kPagedWaves * 64), 0, stream, p);
+    hipLaunchKernelGGL((paged_tile_kernel<T, D, FP8, NW>), dim3((unsigned)wgs), dim3(NW * 64), 0, stream, p);
     if (int rc = check_launch("paged_tile_kernel")) return rc;
     if (plan.pieces == 0) return MINFER_ATTN_OK;
-    constexpr int BR = kPagedWaves * 32;
-    hipLaunchKernelGGL((paged_combine_kernel<T, D, BR>), dim3(BR / 4, (unsigned)p.Hkv, (unsigned)plan.blocks), dim3(256), 0, stream, p);
+    constexpr int BR = NW * 32;
+    hipLaunchKernelGGL((paged_combine_kernel<T, D, BR>), dim3(BR * (D / 4) / 256, (unsigned)p.Hkv, (unsigned)plan.blocks), dim3(256), 0, stream, p);
     return check_launch("paged_combine_kernel");
 }
-template <class T> static int launch_paged_as(const PagedParams& p, const PagedPlan& plan, int64_t D, bool eight, hipStream_t stream) {
-    if (eight) return D == 128 ? launch_paged<T, 128, true>(p, plan, stream) : launch_paged<T, 64, true>(p, plan, stream);
-    return D == 128 ? launch_paged<T, 128, false>(p, plan, stream) : launch_paged<T, 64, false>(p, plan, stream);
+template <class T, bool FP8> static int launch_paged_as(const PagedParams& p, const PagedPlan& plan, int64_t D, hipStream_t stream) {
+    if (D == 64) return launch_paged<T, 64, FP8, kWavesSmall>(p, plan, stream);
+    return plan.waves == kWavesBig ? launch_paged<T, 128, FP8, kWavesBig>(p, plan, stream) : launch_paged<T, 128, FP8, kWavesSmall>(p, plan, stream);
 }
 
 }  // namespace minfer_attn
@@ -673,7 +713,7 @@ MINFER_ATTN_EXPORT size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs
     if (n_seqs <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_context < 0 || Hq % Hkv != 0) return 0;
     const int64_t max_q = bounded_tokens(T, max_q_len);
     if (paged_decode_takes(Hq, Hkv, max_q)) return paged_decode_workspace_bytes(n_seqs, Hq, Hkv, D, max_context, max_q);
-    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_q, kPagedWaves * 32);
+    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_q);
     return r.o_bytes + r.ml_bytes + r.table_bytes;
 }
 
@@ -711,7 +751,7 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
             return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
         return launch_paged_decode(p, dtype, D, eight, max_context, workspace, (hipStream_t)stream_v);
     }
-    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_q, kPagedWaves * 32);
+    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_q);
     // (workgroups and their ids are 32-bit numbers)
     if (plan.blocks * Hkv > 0x7fffffffLL) return bad("flash_attn_paged: problem too large for one launch");
     if (plan.pieces > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes + plan.table_bytes))
@@ -721,5 +761,7 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
     p.part_o = (float*)workspace;
     p.part_ml = (float*)((char*)workspace + plan.o_bytes);
     p.blocks = plan.pieces > 0 ? (int32_t*)((char*)workspace + plan.o_bytes + plan.ml_bytes) + 4 : nullptr;
-    return dtype == MINFER_ATTN_F16 ? launch_paged_as<F16>(p, plan, D, eight, (hipStream_t)stream_v) : launch_paged_as<BF16>(p, plan, D, eight, (hipStream_t)stream_v);
+    hipStream_t stream = (hipStream_t)stream_v;
+    if (dtype == MINFER_ATTN_F16) return eight ? launch_paged_as<F16, true>(p, plan, D, stream) : launch_paged_as<F16, false>(p, plan, D, stream);
+    return eight ? launch_paged_as<BF16, true>(p, plan, D, stream) : launch_paged_as<BF16, false>(p, plan, D, stream);
 }
