@@ -113,9 +113,8 @@ struct PagedParams {
     int n_seqs, T, Hq, Hkv, n_rep;
     int max_q;         // tokens of a sequence past this many are not computed
     int slots;         // decode: partial results a row can have
-    int pieces;        // tiles: pieces that the blocks of rows may be cut into, per KV head; 0: none is cut
-    int max_blocks;    // tiles: bound of the blocks of rows
-    int32_t* blocks;   // tiles: (sequence, block, first piece, pieces) of every block, their number four entries in front of them
+    int round;         // tiles: workgroups per KV head that the chip holds at once, which blocks of rows are cut up to fill; 0: none is cut
+    int32_t* table;    // tiles: the number of pieces, and from the fourth entry on (sequence, block, part, parts) of each
     float scale_log2, inv_scale_log2;  // softmax scale * log2(e), and one over it
 };
 

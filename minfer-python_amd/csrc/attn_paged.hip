@@ -3,8 +3,8 @@
 // Rows.  The new tokens of a sequence and the query heads of a KV head's group are one list of rows, token by token, heads innermost
 // (row = token * n_rep + head): whatever the group's size, 32 rows of a wave attend one KV head, and a sequence of a few tokens
 // fills its rows with heads.  A workgroup takes NW * 32 rows and walks the sequence's 64-key tiles up to its last row's position;
-// where that makes fewer workgroups than two rounds of the chip, blocks of many tiles are cut into pieces of about equal size with a
-// workgroup each (PiecePlan), which leave un-normalised sums in the workspace for paged_combine_kernel.
+// where that makes few workgroups the tiles of a long sequence's blocks are cut into pieces with a workgroup each (find_piece), which
+// leave un-normalised sums in the workspace for paged_combine_kernel.
 //
 // Per tile a wave computes S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32, the scores staying in registers as the second
 // product's operand; tiles are double-buffered in LDS, 16-bit rows copied there directly, 8-bit codes through registers, in which
@@ -57,118 +57,61 @@ MA_DEV int first_tile(const PagedCache& c, int seq, int ctx) {
     return (ctx + 63) >> 6;
 }
 
-// What a workgroup does: tiles t_lo .. t_hi - 1 for a block of rows of a sequence; n_pieces of the block's, this one the part-th of all pieces.
-struct PieceOf { int seq, block, lo, len, ctx, t_lo, t_hi, n_pieces, part; };
-
-// How the blocks of rows (NW * 32 each) of up to kPlanBlocks of them are cut into pieces, worked out by every workgroup for itself: the size of a piece is
-// the smallest, in tiles, that leaves no more pieces than `most`; a block is cut evenly.  Sequences, then blocks, are shared out to the threads.
-constexpr int kPlanBlocks = 1024;
-struct PieceTable { int seq_first[kPlanBlocks + 1], rows[kPlanBlocks], pos0[kPlanBlocks], tile0[kPlanBlocks], wave_sum[16]; float wave_total[16], wave_longest[16]; PieceOf found; };
-
-// Sum of x over all threads before this one (and of all): 256 threads, two barriers.
-MA_DEV int block_scan(int x, int* wave_sum, int& total) {
-    const int lane = threadIdx.x & 63, w = wave_id();
-    const int incl = wave_inclusive_scan(x);
-    if (lane == 63) wave_sum[w] = incl;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 6); ++i) { before += i < w ? wave_sum[i] : 0; total += wave_sum[i]; }
-    __syncthreads();
-    return before + incl - x;
-}
-
 MA_DEV int tiles_of(int pos0, int rows, int n_rep, int block, int BR) { return (max(pos0 + min(block * BR + BR - 1, rows - 1) / n_rep + 1, 0) + 63) >> 6; }
 
-// The x-th piece (found.seq < 0: there is none).  With `publish`, also leaves every block's (sequence, block, first piece, pieces) for the combine kernel.
-template <int BR> MA_DEV void find_piece(const PagedParams& p, PieceTable& t, int x, int most, bool publish) {
-    const int tid = threadIdx.x, threads = blockDim.x, w = wave_id();
-    constexpr int kPer = kPlanBlocks / 256;
-    // sequences: four in a row per thread
-    int mine[kPer], sum = 0, n_blocks;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int s = tid * kPer + k;
-        mine[k] = 0;
-        if (tid < 256 && s < p.n_seqs) {
-            const TokenRange r = token_range(p.cu[s], p.cu[s + 1], p.T);
-            const int ctx = min(max(p.ctx[s], 0), p.c.width << p.c.page_log2);
-            t.rows[s] = min(r.len, p.max_q) * p.n_rep;
-            t.pos0[s] = ctx - r.len;
-            t.tile0[s] = ctx > 0 && r.len > 0 && (unsigned)p.c.table[(int64_t)s * p.c.table_stride] >= (unsigned)p.c.n_pages ? -1 : 0;
-            mine[k] = (t.rows[s] + BR - 1) / BR;
-        }
-        sum += mine[k];
-    }
-    int at = block_scan(sum, t.wave_sum, n_blocks);
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        if (tid < 256 && tid * kPer + k < p.n_seqs) t.seq_first[tid * kPer + k] = at;
-        at += mine[k];
-    }
-    if (tid == 0) { t.seq_first[p.n_seqs] = n_blocks; t.found.seq = -1; }
-    n_blocks = min(n_blocks, p.max_blocks);   // (sequences that overlap, which no valid call has, could make more than there is room for)
-    __syncthreads();
-    for (int s = w; s < p.n_seqs; s += threads >> 6)
-        if (t.tile0[s] < 0) {
-            const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
-            const int tile = first_tile(p.c, s, t.pos0[s] + r.len);
-            if ((tid & 63) == 0) t.tile0[s] = tile;
-        }
-    __syncthreads();
-    // blocks: as many in a row per thread as that takes
-    const int per = (n_blocks + 255) >> 8;   // <= kPer
-    int seq[kPer], blk[kPer], lo[kPer], n_tiles[kPer], all = 0, longest = 0;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int i = tid * per + k;
-        n_tiles[k] = 0;
-        if (tid < 256 && k < per && i < n_blocks) {
-            int a = 0, b = p.n_seqs - 1;   // the last sequence whose first block is not behind i
-            while (a < b) { const int m = (a + b + 1) >> 1; if (t.seq_first[m] <= i) a = m; else b = m - 1; }
-            seq[k] = a;
-            blk[k] = t.seq_first[a + 1] - 1 - i;   // most keys first
-            lo[k] = t.tile0[a];
-            n_tiles[k] = max(tiles_of(t.pos0[a], t.rows[a], p.n_rep, blk[k], BR) - lo[k], 1);
-        }
-        all += n_tiles[k];
-        longest = max(longest, n_tiles[k]);
-    }
-    float total = 0.f, most_tiles = 0.f;   // (sums that the size alone goes by: the same in every workgroup)
-    {
-        const float sum_w = lane_sum<64>((float)all), max_w = wave_max((float)longest);
-        if ((tid & 63) == 0) { t.wave_total[w] = sum_w; t.wave_longest[w] = max_w; }
-        __syncthreads();
-        for (int i = 0; i < (threads >> 6); ++i) { total += t.wave_total[i]; most_tiles = fmaxf(most_tiles, t.wave_longest[i]); }
-    }
-    constexpr int kLeastTiles = 4;
-    int size = max((int)ceilf(total / (float)most), kLeastTiles), n, before;
-    for (;; size += 1 + size / 16) {
-        n = 0;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) n += (n_tiles[k] + size - 1) / size;
-        int pieces;
-        before = block_scan(n, t.wave_sum, pieces);
-        if (pieces <= most || (float)size >= most_tiles) break;
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int pieces = (n_tiles[k] + size - 1) / size;
-        if (pieces > 0) {
-            if (x >= before && x < before + pieces) {
-                const int i = x - before, each = n_tiles[k] / pieces, longer = n_tiles[k] - each * pieces;
-                PieceOf f;
-                f.seq = seq[k]; f.block = blk[k]; f.n_pieces = pieces; f.part = x;
-                f.t_lo = lo[k] + i * each + min(i, longer);
-                f.t_hi = f.t_lo + each + (i < longer ? 1 : 0);
-                t.found = f;
+// What a workgroup does: the `part`-th of `parts` equal pieces of the tiles of a block of rows (NW * 32 of them); piece `x` of the launch.
+struct Piece { int seq, block, part, parts; };
+
+// The x-th piece (seq < 0: there is none) and, with it, how many there are.  The blocks of a sequence are cut into the same number of pieces, its last
+// block's tiles over a size that is the same for all sequences: the smallest that leaves no more pieces than workgroups which the chip
+// holds at once (p.round, or a multiple of it where the blocks alone are more).  Every wave works it out for itself, a sequence to a lane: with sums over
+// all blocks in LDS it took 14 us in front of a launch's first tile, this 1.
+template <int BR> MA_DEV Piece find_piece(const PagedParams& p, int x, int& all) {
+    const int lane = threadIdx.x & 63;
+    Piece r{-1, 0, 0, 1};
+    if (p.round == 0) {   // whole blocks, of any number of sequences
+        all = 0;
+        for (int base = 0; base < p.n_seqs; base += 64) {
+            TokenRange t{0, 0};
+            if (base + lane < p.n_seqs) t = token_range(p.cu[base + lane], p.cu[base + lane + 1], p.T);
+            const int n = (min(t.len, p.max_q) * p.n_rep + BR - 1) / BR;
+            const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
+            if (x < total) {
+                const int s = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
+                r.seq = base + s;
+                r.block = lane_value(n, s) - 1 - (x - lane_value(incl - n, s));   // most keys first
+                return r;
             }
-            if (publish) reinterpret_cast<int4*>(p.blocks)[tid * per + k] = make_int4(seq[k], blk[k], before, pieces);
-            before += pieces;
+            x -= total;
         }
+        return r;
     }
-    if (publish && tid == 0) p.blocks[-4] = n_blocks;
-    __syncthreads();
+    int n = 0, tiles = 0;   // the lane's sequence: blocks, tiles of the last one
+    if (lane < p.n_seqs) {
+        const TokenRange t = token_range(p.cu[lane], p.cu[lane + 1], p.T);
+        const int ctx = min(max(p.ctx[lane], 0), p.c.width << p.c.page_log2), rows = min(t.len, p.max_q) * p.n_rep;
+        n = (rows + BR - 1) / BR;
+        tiles = n > 0 ? max(tiles_of(ctx - t.len, rows, p.n_rep, n - 1, BR), 1) : 0;
+        // (a window that moved on: half of the pages, a guess, which only the number of pieces goes by)
+        if (n > 0 && ctx > 0 && (unsigned)p.c.table[(int64_t)lane * p.c.table_stride] >= (unsigned)p.c.n_pages) tiles = (tiles + 1) / 2;
+    }
+    const int blocks = lane_value(wave_inclusive_scan(n), 63), most = (blocks + p.round - 1) / p.round * p.round;
+    const float sum = lane_sum<64>((float)n * (float)tiles);
+    constexpr int kLeastTiles = 4;
+    int size = max((int)(sum / (float)max(most, 1)), kLeastTiles), parts, incl;
+    for (;; size += 1 + size / 8) {   // (ends: with the most tiles of a sequence as the size there is a piece for every block, and `most` is no less)
+        parts = (tiles + size - 1) / size;
+        incl = wave_inclusive_scan(n * parts);
+        all = lane_value(incl, 63);
+        if (all <= most) break;
+    }
+    if (x >= all) return r;
+    r.seq = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
+    r.parts = lane_value(parts, r.seq);
+    const int blocks_of = lane_value(n, r.seq), local = x - (lane_value(incl, r.seq) - blocks_of * r.parts);
+    r.block = blocks_of - 1 - local / r.parts;
+    r.part = local % r.parts;
+    return r;
 }
 
 template <class T, int D, bool FP8, int NW>
@@ -199,35 +142,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
         g = (int)blockIdx.x % p.Hkv;
         rank = (int)blockIdx.x / p.Hkv;
     }
-    PieceOf me;
-    me.seq = -1;
-    if (p.pieces > 0) {
-        PieceTable& table = *reinterpret_cast<PieceTable*>(&kv_lds[0][0]);
-        static_assert(sizeof(PieceTable) <= 2 * STAGE_BYTES, "in the stages, before any tile or row is there");
-        find_piece<BR>(p, table, rank, p.pieces, blockIdx.x == 0);
-        me = table.found;
-        __syncthreads();   // the stages are free
-        if (me.seq < 0) return;
-    } else {
-        int x = rank;
-        for (int base = 0; base < p.n_seqs; base += 64) {
-            const int s = base + lane;
-            TokenRange r{0, 0};
-            if (s < p.n_seqs) r = token_range(p.cu[s], p.cu[s + 1], p.T);
-            const int n = (min(r.len, p.max_q) * p.n_rep + BR - 1) / BR;
-            const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
-            if (x < total) {
-                const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
-                me.seq = base + src;
-                me.block = lane_value(n, src) - 1 - (x - lane_value(incl - n, src));   // most keys first
-                break;
-            }
-            x -= total;
-        }
-        if (me.seq < 0) return;
-        me.n_pieces = 1;
+    int all;
+    const Piece me = find_piece<BR>(p, rank, all);
+    if (me.seq < 0) return;
+    const int seq = me.seq, block = me.block;
+    if (p.round > 0 && g == 0 && threadIdx.x == 0) {   // for the combine kernel
+        reinterpret_cast<int4*>(p.table)[1 + rank] = make_int4(me.seq, me.block, me.part, me.parts);
+        if (rank == 0) p.table[0] = all;
     }
-    const int seq = __builtin_amdgcn_readfirstlane(me.seq), block = __builtin_amdgcn_readfirstlane(me.block);
     const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
     const int seq_lo = range.lo, seq_len = range.len;
     const int ctx = min(max(const_load(p.ctx + seq), 0), p.c.width << p.c.page_log2);
@@ -235,14 +157,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     const int rows = min(seq_len, p.max_q) * p.n_rep, last_row = rows - 1;
     const int row0 = block * BR + w * 32;                                // the wave's first row
     const bool wave_on = row0 < rows;
-    int t_lo = 0, t_hi = tiles_of(pos0, rows, p.n_rep, block, BR);
-    if (p.pieces > 0) {
-        t_lo = __builtin_amdgcn_readfirstlane(me.t_lo);
-        t_hi = min(t_hi, __builtin_amdgcn_readfirstlane(me.t_hi));
-    } else if (t_hi > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages) {
-        t_lo = __builtin_amdgcn_readfirstlane(first_tile(p.c, seq, ctx));
-    }
-    const int n_own = max(t_hi - t_lo, 0);
+    const int tiles = tiles_of(pos0, rows, p.n_rep, block, BR);
+    int t_first = 0;
+    if (tiles > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages)
+        t_first = __builtin_amdgcn_readfirstlane(first_tile(p.c, seq, ctx));
+    const int n_tiles = max(tiles - t_first, 0), each = n_tiles / me.parts, longer = n_tiles - each * me.parts;
+    const int t_lo = t_first + me.part * each + min(me.part, longer), n_own = each + (me.part < longer ? 1 : 0);
     const int wave_first = pos0 + min(row0, last_row) / p.n_rep, wave_last = pos0 + min(row0 + 31, last_row) / p.n_rep;
 
     // positions of the lane's two rows (one per block of 16)
@@ -562,8 +482,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     float l_all[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) l_all[qb] = sum_across_quads(l_sum[qb]);
-    if (me.n_pieces > 1) {
-        const int64_t part = (int64_t)(__builtin_amdgcn_readfirstlane(me.part) * p.Hkv + g) * BR;
+    if (me.parts > 1) {
+        const int64_t part = (int64_t)(rank * p.Hkv + g) * BR;
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
             if (row0 + 16 * qb + l16 > last_row) continue;
@@ -606,14 +526,16 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
 
 // out = sum_i O_i w_i / sum_i l_i w_i with w_i = 2^(m_i - max m) over the pieces of a block that was cut; D/4 lanes per row, four pieces requested at a
 // time, references and sums with them.  A piece without keys has a sum of zero and is left out; one whose scores are all NaN has sums of NaN and
-// is multiplied like any other.  grid (rows of a block / rows of a workgroup, KV heads, blocks).
+// is multiplied like any other.  grid (rows of a block / rows of a workgroup, KV heads, pieces): a block's first piece does it.
 template <class T, int D, int BR>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
     constexpr int LPR = D / 4, RPW = 256 / LPR;   // lanes per row, rows per workgroup
-    const int row = (int)blockIdx.x * RPW + (int)threadIdx.x / LPR, d = 4 * ((int)threadIdx.x % LPR), g = blockIdx.y, b = blockIdx.z;
-    if (b >= const_load(p.blocks - 4)) return;
-    const int seq = const_load(p.blocks + 4 * b), block = const_load(p.blocks + 4 * b + 1), first = const_load(p.blocks + 4 * b + 2), n = const_load(p.blocks + 4 * b + 3);
-    if (n <= 1) return;
+    const int row = (int)blockIdx.x * RPW + (int)threadIdx.x / LPR, d = 4 * ((int)threadIdx.x % LPR), g = blockIdx.y, first = blockIdx.z;
+    if (first >= const_load(p.table)) return;
+    const int32_t* me = p.table + 4 * (1 + first);
+    // (sequences that overlap, which no valid call has, could have more pieces than there is room for)
+    const int seq = const_load(me), block = const_load(me + 1), n = min(const_load(me + 3), (int)gridDim.z - first);
+    if (n <= 1 || const_load(me + 2) != 0) return;
     const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
     const int r = block * BR + row;
     if (r >= min(range.len, p.max_q) * p.n_rep) return;
@@ -660,7 +582,8 @@ static int64_t bounded_tokens(int64_t T, int64_t max_q_len) { return max_q_len >
 struct PagedPlan {
     int waves;         // per workgroup
     int64_t blocks;    // bound of the blocks of rows of all sequences
-    int64_t pieces;    // pieces per KV head that they may be cut into; 0: none is cut
+    int64_t round;     // workgroups per KV head that the chip holds at once where blocks may be cut, 0 where none is
+    int64_t pieces;    // bound of the pieces, per KV head
     size_t o_bytes, ml_bytes, table_bytes;
 };
 // Rows of a workgroup: 256 share a tile's copies at head_dim 128 where they fill the chip's units, one workgroup to a unit, one and a half times; 128, two to
@@ -680,23 +603,25 @@ static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, 
     r.waves = D == 128 && T * n_rep / (kWavesBig * 32) * Hkv >= MINFER_PAGED_BIG ? kWavesBig : kWavesSmall;
     r.blocks = blocks_of(n_seqs, T, n_rep, max_q, r.waves);
     const int64_t wgs = r.blocks * Hkv, round = r.waves == kWavesBig ? kUnits : 2 * kUnits;   // workgroups that the chip holds at once
-    if (wgs <= 2 * round && r.blocks <= kPlanBlocks && n_seqs <= kPlanBlocks) {
-        r.pieces = std::max((wgs + round - 1) / round * round / Hkv, r.blocks);
+    r.pieces = r.blocks;
+    if (wgs <= 2 * round && n_seqs <= 64) {
+        r.round = std::max<int64_t>(round / Hkv, 1);
+        r.pieces = (r.blocks + r.round - 1) / r.round * r.round;
         r.o_bytes = (size_t)(r.pieces * Hkv * r.waves * 32 * D * 4);
         r.ml_bytes = (size_t)(r.pieces * Hkv * r.waves * 32 * 2 * 4);
-        r.table_bytes = (size_t)(r.blocks + 1) * 16;
+        r.table_bytes = (size_t)(r.pieces + 1) * 16;
     }
     return r;
 }
 
 template <class T, int D, bool FP8, int NW>
 static int launch_paged(const PagedParams& p, const PagedPlan& plan, hipStream_t stream) {
-    const int64_t wgs = (plan.pieces > 0 ? plan.pieces : plan.blocks) * p.Hkv;
+    const int64_t wgs = plan.pieces * p.Hkv;
     hipLaunchKernelGGL((paged_tile_kernel<T, D, FP8, NW>), dim3((unsigned)wgs), dim3(NW * 64), 0, stream, p);
     if (int rc = check_launch("paged_tile_kernel")) return rc;
-    if (plan.pieces == 0) return MINFER_ATTN_OK;
+    if (plan.round == 0) return MINFER_ATTN_OK;
     constexpr int BR = NW * 32;
-    hipLaunchKernelGGL((paged_combine_kernel<T, D, BR>), dim3(BR * (D / 4) / 256, (unsigned)p.Hkv, (unsigned)plan.blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((paged_combine_kernel<T, D, BR>), dim3(BR * (D / 4) / 256, (unsigned)p.Hkv, (unsigned)plan.pieces), dim3(256), 0, stream, p);
     return check_launch("paged_combine_kernel");
 }
 template <class T, bool FP8> static int launch_paged_as(const PagedParams& p, const PagedPlan& plan, int64_t D, hipStream_t stream) {
@@ -753,14 +678,13 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
     }
     const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_q);
     // (workgroups and their ids are 32-bit numbers)
-    if (plan.blocks * Hkv > 0x7fffffffLL) return bad("flash_attn_paged: problem too large for one launch");
-    if (plan.pieces > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes + plan.table_bytes))
+    if (plan.pieces * Hkv > 0x7fffffffLL) return bad("flash_attn_paged: problem too large for one launch");
+    if (plan.round > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes + plan.table_bytes))
         return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
-    p.pieces = (int)plan.pieces;
-    p.max_blocks = (int)plan.blocks;
+    p.round = (int)plan.round;
     p.part_o = (float*)workspace;
     p.part_ml = (float*)((char*)workspace + plan.o_bytes);
-    p.blocks = plan.pieces > 0 ? (int32_t*)((char*)workspace + plan.o_bytes + plan.ml_bytes) + 4 : nullptr;
+    p.table = (int32_t*)((char*)workspace + plan.o_bytes + plan.ml_bytes);
     hipStream_t stream = (hipStream_t)stream_v;
     if (dtype == MINFER_ATTN_F16) return eight ? launch_paged_as<F16, true>(p, plan, D, stream) : launch_paged_as<F16, false>(p, plan, D, stream);
     return eight ? launch_paged_as<BF16, true>(p, plan, D, stream) : launch_paged_as<BF16, false>(p, plan, D, stream);
