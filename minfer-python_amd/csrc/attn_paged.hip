@@ -668,7 +668,7 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
     p.inv_scale_log2 = (float)(sqrt((double)D) / 1.4426950408889634);
     const bool eight = page_type == MINFER_FP8_E4M3;
     const int64_t max_q = bounded_tokens(T, max_q_len);
-    if (T > (1 << 30) || T * Hq > 0x7fffffffLL || n_seqs > (1 << 24)) return bad("flash_attn_paged: problem too large for one launch");
+    if (T > (1 << 30) || T * Hq > 0x7fffffffLL - 4096 || n_seqs > (1 << 24)) return bad("flash_attn_paged: problem too large for one launch");
     p.max_q = (int)max_q;
     if (paged_decode_takes(Hq, Hkv, max_q)) {
         const size_t need = paged_decode_workspace_bytes(n_seqs, Hq, Hkv, D, max_context, max_q);

@@ -78,7 +78,7 @@ MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg)
 
 // Streams groups g0 .. g1 - 1 (at least one) of (sequence s, KV head g) for the columns of group hg; `area` is the wave's own LDS.
 template <class T, int D, bool FP8>
-MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, int g1, char* area, ColumnAcc<D>& acc) {
+MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D>& acc) {
     const PagedParams& p = work.p;
     using GEO = DecodeGeom<D>;
     constexpr int RB = GEO::RB, G = GEO::G, RPI = GEO::RPI, NI = GEO::NI, RPI8 = GEO::RPI8, NI8 = GEO::NI8;
@@ -260,7 +260,26 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
         }
     };
 
+    acc.m = -INFINITY;
+    acc.l = 0.f;
     Ids next = ids_of(g0);
+    bool any = false;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) any = any || is_there(next.id[h]);
+    if (!any) {   // pages given back by a window that moved on: on to the first group that is there, 64 at a time (64 sequences to 8192 rows 183 us, the first half of them gone 116)
+        int at = g1;
+        for (int base = g0; base < g1; base += 64) {
+            const Ids mine = ids_of(base + lane);
+            bool on = false;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) on = on || is_there(mine.id[h]);
+            const uint64_t hit = __ballot(on && base + lane < g1);
+            if (hit) { at = base + __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)hit) - 1); break; }
+        }
+        if (at >= g1) return;
+        g0 = __builtin_amdgcn_readfirstlane(at);
+        next = ids_of(g0);
+    }
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const Ids now = next;
@@ -316,13 +335,24 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
     const int lane = threadIdx.x & 63, w = wave_id();
     const int pairs = p.Hkv * work.n_hg, n_waves = work.n_wg * kLineWaves;
     const bool first = blockIdx.x == 0 && w == 0;   // the wave that leaves the sequences' places for the merge
+    // 64 sequences at a time, 256 requested together; the first 64 are kept
+    constexpr int UN = 4;
+    LineSeq kept{{0, 0, 0}, 0};
     int total = 0, longest = 0;
-    for (int base = 0; base < p.n_seqs; base += 64) {
-        const LineSeq q = line_seq<GR>(work, base + lane);
-        const int incl = wave_inclusive_scan(q.groups * pairs);
-        if (first && base + lane < p.n_seqs) work.seq_off[base + lane] = total + incl - q.groups * pairs;
-        total += lane_value(incl, 63);
-        longest = max(longest, q.groups);
+    for (int base = 0; base < p.n_seqs; base += 64 * UN) {
+        LineSeq q[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) q[u] = line_seq<GR>(work, base + 64 * u + lane);
+        if (base == 0) kept = q[0];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int b = base + 64 * u;
+            if (b >= p.n_seqs) break;
+            const int incl = wave_inclusive_scan(q[u].groups * pairs);
+            if (first && b + lane < p.n_seqs) work.seq_off[b + lane] = total + incl - q[u].groups * pairs;
+            total += lane_value(incl, 63);
+            longest = max(longest, q[u].groups);
+        }
     }
     longest = (int)wave_max((float)longest);   // (below 2^24 exactly, and above rounded up or down by less than the slots to spare)
     const int quota = max(max((total + n_waves - 1) / n_waves, 128 / GR), longest / (p.slots - 3) + 1);
@@ -330,13 +360,13 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
     // shares to the waves of a workgroup in turn; where there are no more shares than workgroups, one to each
     const int n_shares = (total + quota - 1) / quota;
     const int wave = n_shares <= (int)gridDim.x ? w * (int)gridDim.x + (int)blockIdx.x : (int)blockIdx.x * kLineWaves + w;
+    if (wave >= n_shares) return;
     int x = wave * quota;
     const int x_end = min(total, x + quota);
-    if (wave >= n_shares) return;
     // the sequence that holds position x
     int s = 0, off = 0, groups = 0;
     for (int base = 0, start = 0; base < p.n_seqs; base += 64) {
-        const LineSeq q = line_seq<GR>(work, base + lane);
+        const LineSeq q = base == 0 ? kept : line_seq<GR>(work, base + lane);
         const int incl = wave_inclusive_scan(q.groups * pairs), sum = lane_value(incl, 63);
         if (x < start + sum) {
             const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < start + incl)) - 1);
@@ -631,11 +661,18 @@ template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStre
     hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
     return check_launch("paged_merge_kernel");
 }
-// Whether a call is one for chunks: a workgroup for every pair at least, one to a unit.
-static bool takes_chunks(const DecodeWork& w) { return w.p.n_seqs <= 64 && (int64_t)w.p.n_seqs * w.p.Hkv * w.n_hg <= compute_units(); }
-template <class T, int D, bool FP8> static int launch_chunks(DecodeWork w, hipStream_t stream) {
-    const int n_wg = compute_units();
-    static_assert(kStreamCounters >= 256, "a counter for every pair");
+// Whether a call is one for chunks.  Up to a pair for every unit always (us, chunks / line, contexts alike and from a sixteenth up: one of 4000 12.2 / 15.7, 10.8 /
+// 14.7; 4 of 30000 79 / 86, 41 / 46; 16 of 4000 45 / 51, 32 / 35, of 20000 e4m3 111 / 120, 66 / 66; 32 of 300 10.9 / 17.4, 8.9 / 18.5, of 1500 e4m3
+// 23 / 32, 20 / 25; where every unit has one long context, contexts that differ leave units idle: 32 of 6000 121 / 127, 79 / 74, e4m3 68 / 79, 57 / 50).
+// Two rounds of whole contexts where the table has no room for long ones: 64 of 100 14.3 / 16.7, 12.7 / 24.4, of 400 26.2 / 28.6, 20.7 / 22.1, of 1000
+// 47.2 / 50.9, 32.1 / 32.6, of 3000 123 / 128, 82 / 79; e4m3 of 100 14.3 / 18.6, 13.6 / 24.1, of 400 22.0 / 25.3, 20.0 / 19.0, of 1000 36.6 / 32.8.
+static int chunk_rounds(const DecodeWork& w, int64_t max_context, bool eight) {
+    const int64_t pairs = (int64_t)w.p.n_seqs * w.p.Hkv * w.n_hg, units = compute_units();
+    if (w.p.n_seqs > 64 || pairs > kStreamCounters) return 0;
+    return pairs <= units ? 1 : pairs <= 2 * units && max_context <= (eight ? 384 : 1024) ? 2 : 0;
+}
+template <class T, int D, bool FP8> static int launch_chunks(DecodeWork w, int rounds, hipStream_t stream) {
+    const int n_wg = rounds * compute_units();
     w.done = stream_counters(stream);
     hipLaunchKernelGGL((paged_chunk_kernel<T, D, FP8>), dim3((unsigned)n_wg), dim3(kChunkWaves * 64), 0, stream, w);
     if (int rc = check_launch("paged_chunk_kernel")) return rc;
@@ -643,12 +680,12 @@ template <class T, int D, bool FP8> static int launch_chunks(DecodeWork w, hipSt
     hipLaunchKernelGGL((paged_chunk_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)(w.p.Hkv * w.n_hg), (unsigned)w.p.n_seqs), dim3(kChunkWaves * 64), 0, stream, w, n_wg);
     return check_launch("paged_chunk_merge_kernel");
 }
-template <class T, int D, bool FP8> static int launch_rows(const DecodeWork& w, hipStream_t stream) {
-    return takes_chunks(w) ? launch_chunks<T, D, FP8>(w, stream) : launch_line<T, D, FP8>(w, stream);
+template <class T, int D, bool FP8> static int launch_rows(const DecodeWork& w, int rounds, hipStream_t stream) {
+    return rounds > 0 ? launch_chunks<T, D, FP8>(w, rounds, stream) : launch_line<T, D, FP8>(w, stream);
 }
-template <class T> static int launch_decode_as(const DecodeWork& w, int64_t D, bool eight, hipStream_t stream) {
-    if (eight) return D == 128 ? launch_rows<T, 128, true>(w, stream) : launch_rows<T, 64, true>(w, stream);
-    return D == 128 ? launch_rows<T, 128, false>(w, stream) : launch_rows<T, 64, false>(w, stream);
+template <class T> static int launch_decode_as(const DecodeWork& w, int64_t D, bool eight, int rounds, hipStream_t stream) {
+    if (eight) return D == 128 ? launch_rows<T, 128, true>(w, rounds, stream) : launch_rows<T, 64, true>(w, rounds, stream);
+    return D == 128 ? launch_rows<T, 128, false>(w, rounds, stream) : launch_rows<T, 64, false>(w, rounds, stream);
 }
 
 int launch_paged_decode(PagedParams p, int dtype, int64_t D, bool eight, int64_t max_context, void* workspace, hipStream_t stream) {
@@ -664,7 +701,8 @@ int launch_paged_decode(PagedParams p, int dtype, int64_t D, bool eight, int64_t
     p.part_ml = (float*)((char*)workspace + part_bytes(rows, slots, D));
     w.seq_off = (int32_t*)((char*)p.part_ml + part_bytes(rows, slots, 2));
     w.p = p;
-    return dtype == MINFER_ATTN_F16 ? launch_decode_as<F16>(w, D, eight, stream) : launch_decode_as<BF16>(w, D, eight, stream);
+    const int rounds = chunk_rounds(w, max_context, eight);
+    return dtype == MINFER_ATTN_F16 ? launch_decode_as<F16>(w, D, eight, rounds, stream) : launch_decode_as<BF16>(w, D, eight, rounds, stream);
 }
 
 }  // namespace minfer_attn

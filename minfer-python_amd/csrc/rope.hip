@@ -626,29 +626,38 @@ __global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Para
     int x = (int)blockIdx.x / ap.n_hg;
     const int hg = (int)blockIdx.x - x * ap.n_hg;
     int seq = -1, first_tok = 0, pos0 = 0, a = 0, b = 0;
-    for (int base = 0; base < p.n_seqs; base += 64) {
-        const int s = base + lane;
-        TokenRange r{0, 0};
-        int at = 0, lo = 0, hi = 0;
-        if (s < p.n_seqs) {
-            r = token_range(p.cu[s], p.cu[s + 1], p.L);
-            at = p.positions[s];
-            lo = max(at, 0);                                                        // rows lo .. hi - 1 of the sequence are written
-            hi = (int)min((int64_t)at + r.len, (int64_t)pc.width << S_log2);
+    constexpr int UN = 4;   // 64 sequences at a time, 256 requested together
+    for (int base = 0; base < p.n_seqs && seq < 0; base += 64 * UN) {
+        TokenRange r[UN];
+        int at[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int s = base + 64 * u + lane;
+            r[u] = TokenRange{0, 0};
+            at[u] = 0;
+            if (s < p.n_seqs) {
+                r[u] = token_range(p.cu[s], p.cu[s + 1], p.L);
+                at[u] = p.positions[s];
+            }
         }
-        const int n = hi > lo ? ((hi - 1) >> S_log2) - (lo >> S_log2) + 1 : 0;
-        const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
-        if (x < total) {
-            const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
-            seq = base + src;
-            x -= lane_value(incl - n, src);
-            first_tok = lane_value(r.lo, src);
-            pos0 = lane_value(at, src);
-            a = lane_value(lo, src);
-            b = lane_value(hi, src);
-            break;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            if (seq >= 0) break;
+            const int lo = max(at[u], 0), hi = (int)min((int64_t)at[u] + r[u].len, (int64_t)pc.width << S_log2);   // rows lo .. hi - 1 of the sequence are written
+            const int n = r[u].len > 0 && hi > lo ? ((hi - 1) >> S_log2) - (lo >> S_log2) + 1 : 0;
+            const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
+            if (x < total) {
+                const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
+                seq = base + 64 * u + src;
+                x -= lane_value(incl - n, src);
+                first_tok = lane_value(r[u].lo, src);
+                pos0 = lane_value(at[u], src);
+                a = lane_value(lo, src);
+                b = lane_value(hi, src);
+            } else {
+                x -= total;
+            }
         }
-        x -= total;
     }
     if (seq < 0) return;
     const int page = (a >> S_log2) + x;

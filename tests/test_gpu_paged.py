@@ -152,6 +152,24 @@ def test_attend_bound_unknown(kerns, eight):
         check_attend(kerns, c, 8, max_q=0)
 
 
+@pytest.mark.parametrize("n,Hq", [(1, 4), (4, 4), (70, 4)], ids=["decode", "drafts", "chunks"])
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+def test_attend_fewer_rows_than_tokens(kerns, n, Hq, eight):
+    """A context shorter than the tokens: the first ones stand in front of row 0 and yield zeros, the others attend what is there."""
+    c = ref.Paged([(n, 0), (n, 30)], 16, 2, 64, torch.float16, DEV, eight=eight)
+    q = make_q(c.T, Hq, 64, torch.float16)
+    held = n // 2
+    c.ctx[0] = held
+    out = torch.full_like(q, 7.0)
+    run_attend(kerns, c, q, out)
+    assert (out[0, :n - held] == 0).all()
+    short = ref.Paged([(held, 0), (n, 30)], 16, 2, 64, torch.float16, DEV, eight=eight)
+    short.k_dense = [c.k_dense[0][:, :held], c.k_dense[1]]
+    short.v_dense = [c.v_dense[0][:, :held], c.v_dense[1]]
+    want, bound = ref.attend(short, q[0, n - held:].transpose(0, 1))
+    assert ((out[0, n - held:].transpose(0, 1).double().cpu() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("seqs", [[(1, 40), (1, 900)], [(3, 40), (2, 1900)], [(80, 5), (3, 70)]], ids=["decode", "drafts", "chunks"])
 def test_attend_malformed_index_tensors_stay_in_bounds(kerns, seqs):
     """cu_seqlens and ctx_lens that make no sense: q, out and the pools lie between guards that stay as they are (what such a call
