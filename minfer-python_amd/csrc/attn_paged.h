@@ -65,6 +65,61 @@ MA_DEV void lds_write_b128(uint32_t addr, int imm, s16x8 x) {
     *(lds_s16x8*)(uintptr_t)(addr + imm) = x;
 }
 
+// Four values of a cached row, from element `at` of a pool on.
+template <class T, bool FP8> MA_DEV f32x4 row_values(const void* pool, int64_t at, uint32_t scale) {
+    uint32_t lo, hi;
+    if constexpr (FP8) {
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>((const char*)pool + at);
+        lo = widen2<T, false>(codes, scale_value(scale));
+        hi = widen2<T, true>(codes, scale_value(scale));
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>((const short*)pool + at);
+        lo = x.x; hi = x.y;
+    }
+    return f32x4{T::to_float((short)(lo & 0xffffu)), T::to_float((short)(lo >> 16)), T::to_float((short)(hi & 0xffffu)), T::to_float((short)(hi >> 16))};
+}
+
+// Keys first .. end - 1 of a sequence for NQ columns of a wave, key by key and without matrix products, in which a V row with an infinity or a NaN would
+// meet the weights of zero of columns that do not attend it: for the few keys from the first such row on that some columns attend and others do not.
+// Lane (l16, quad) holds column l16's O at d = 16db + 4 quad + 0..3 (o(db, i) of column i), its reference m (log2 units) and a
+// share l of its sum; q[i] is its query row (null: no column), limit[i] the rows that it attends.  The test in front of it costs 0 to 2 % (prompt of 8192 f16 508 to
+// 519 us, four drafts 27.7 to 28.2); the keys themselves about a microsecond each, which only a cache that holds such rows pays.
+template <class T, int D, bool FP8, int NQ, class Acc>
+MA_DEV void attend_key_by_key(const PagedCache& c, int Hkv, int seq, int g, int first, int end, const short* const (&q)[NQ], const int (&limit)[NQ], float c2,
+                              Acc o, float (&m)[NQ], float (&l)[NQ]) {
+    const int quad = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
+    for (int key = first; key < end; ++key) {
+        const int id = const_load(c.table + (int64_t)seq * c.table_stride + min(key >> c.page_log2, c.width - 1));
+        if ((unsigned)id >= (unsigned)c.n_pages) continue;
+        const int64_t at = (int64_t)id * c.page_stride + (int64_t)g * c.head_stride + (int64_t)(key & ((1 << c.page_log2) - 1)) * c.row_stride + 4 * quad;
+        const uint32_t ks = FP8 ? const_byte(c.k_scales + (int64_t)id * Hkv + g) : 0u, vs = FP8 ? const_byte(c.v_scales + (int64_t)id * Hkv + g) : 0u;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            float score = 0.f;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 16) {
+                const f32x4 x = row_values<T, FP8>(c.k, at + d, ks), y = q[i] ? row_values<T, false>(q[i], 4 * quad + d, 0u) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) score = fmaf(x[e], y[e], score);
+            }
+            score = sum_across_quads(score) * c2;
+            const bool on = q[i] && key < limit[i];
+            const float m_new = on ? fmaxf(m[i], score) : m[i], base = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = m[i] == -INFINITY ? (on ? 0.f : 1.f) : fast_exp2(m[i] - base);
+            const float w = T::to_float((short)(T::pack2(fast_exp2(score - base), 0.f) & 0xffffu));
+            m[i] = m_new;
+            l[i] = on ? l[i] * alpha + (quad == 0 ? w : 0.f) : l[i];
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) {
+                const f32x4 x = row_values<T, FP8>(c.v, at + 16 * db, vs);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o(db, i)[e] = on ? fmaf(w, x[e], o(db, i)[e] * alpha) : o(db, i)[e];
+            }
+        }
+    }
+}
+
 // Checks of a cache's description, for an operator called `op`; fills `c`.
 inline int check_pages(const char* op, int dtype, int page_type, const minfer_kv_pages* pages, int64_t n_seqs, int64_t Hkv, int64_t D, PagedCache& c) {
     char msg[256];

@@ -12,7 +12,8 @@
 // as scalars: pages have at least 16 rows, so a copy instruction's rows lie in one.
 //
 // Rows that nothing was written to, behind the context in its last page, and rows of pages that are not there may hold NaN, which a weight of zero would
-// not take out of a sum: their scores are replaced, and their V rows are cleared in LDS, in the few tiles that have any.
+// not take out of a sum: their scores are replaced, and their V rows are cleared in LDS, in the few tiles that have any.  A row with an infinity or a NaN
+// that a sequence's later tokens attend is kept from its earlier ones as well (attend_key_by_key).
 #include <algorithm>
 
 #include "attn_paged.h"
@@ -305,6 +306,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     constexpr float kLazyLog2 = 8.f;
     const float c2 = p.scale_log2, inv_c2 = p.inv_scale_log2;
     s16x8 qf[2][KC];
+    int by_key = 0x7fffffff;   // the tile from which on the wave's keys are taken one by one
 
     auto process_tile = [&](auto stage_tag, int kt, int there) __attribute__((always_inline)) {
         constexpr int SOFF = decltype(stage_tag)::value * STAGE_BYTES;
@@ -337,6 +339,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
                 }
                 pin();
             });
+        }
+        if (key0 + 63 > wave_first) {
+            // V rows that some of the wave's tokens attend and others do not: whether all are finite is what products with zero say
+            f32x4 probe = {0.f, 0.f, 0.f, 0.f};
+            const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int db = 0; db < DB; ++db) probe = T::mfma16(read_v(1, db), zero, T::mfma16(va[db], zero, probe));
+            if (__any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.f))) { by_key = kt; return; }
         }
         if (key0 + 63 > wave_first || !whole(kt, there)) {
 #pragma unroll
@@ -469,7 +479,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
             }
             pg = after;
         }
-        if (wave_on && there && kt * 64 <= wave_last) process_tile(stage_tag, kt, there);
+        if (wave_on && there && kt * 64 <= wave_last && kt < by_key) process_tile(stage_tag, kt, there);
         there = there_1;
         there_1 = there_2;
     };
@@ -479,6 +489,17 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     }
 
     if (!wave_on) return;
+    if (by_key < t_lo + n_own) {
+        const short* q[2];
+        const int limit[2] = {pos[0] + 1, pos[1] + 1};
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            const int r = min(row0 + 16 * qb + l16, last_row), t = r / p.n_rep;
+            q[qb] = (const short*)p.q + (int64_t)(seq_lo + t) * p.q2 + (int64_t)(g * p.n_rep + r - t * p.n_rep) * p.q1;
+        }
+        attend_key_by_key<T, D, FP8, 2>(p.c, p.Hkv, seq, g, by_key * 64, min(wave_last + 1, (t_lo + n_own) * 64), q, limit, c2,
+                                        [&](int db, int qb) __attribute__((always_inline)) -> f32x4& { return o_acc[db][qb]; }, m_ref, l_sum);
+    }
     float l_all[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) l_all[qb] = sum_across_quads(l_sum[qb]);

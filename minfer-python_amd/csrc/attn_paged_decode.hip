@@ -65,9 +65,9 @@ template <int D, bool FP8> constexpr int kWaveLds = FP8 ? 32 * D * 2 : 2 * 16 * 
 
 // The columns of a group: what lane l16 needs of its own.
 struct Column { const short* q; int limit; };   // its query row (null: no column), and the rows that it attends: 0 .. limit - 1
-MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg) {
+MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg, int l16) {
     const PagedParams& p = w.p;
-    const int col = hg * 16 + ((int)threadIdx.x & 15), tok = p.n_rep > 16 || p.max_q == 1 ? 0 : col / p.n_rep;
+    const int col = hg * 16 + l16, tok = p.n_rep > 16 || p.max_q == 1 ? 0 : col / p.n_rep;
     Column c{nullptr, 0};
     if (col < w.n_col && tok < info.len) {
         c.q = (const short*)p.q + (int64_t)(info.lo + tok) * p.q2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.q1;
@@ -87,7 +87,9 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
     const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
     const int ctx = info.ctx, page_mask = (1 << p.c.page_log2) - 1;
     const int32_t* const table = p.c.table + (int64_t)s * p.c.table_stride;
-    const Column col = column_of(work, info, g, hg);
+    const Column col = column_of(work, info, g, hg, l16);
+    const int edge = ctx - info.len + 1;   // from this row on some columns attend what others do not
+    int by_key = 0x7fffffff;               // the group from which on keys are taken one by one
 
     // Q^T fragments (B operand): column l16; contraction step c takes d = 32c + 8 quad + 0..7, or for codes, whose 16-byte pieces hold
     // two steps, d = 64 (c / 2) + 16 quad + 8 (c % 2) + 0..7
@@ -214,6 +216,20 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
                 *reinterpret_cast<u32x4*>(my_v + row * RB + 16 * ((lane % G) ^ GEO::swz_v(row))) = st.v[j];
             }
         }
+        const int row = 4 * quad + (l16 >> 2);
+        const char* rowp_v = my_v + row * RB;
+        const int sw_v = GEO::swz_v(row);   // rows 16 apart share a swizzle
+        if (edge < min(t * GR + GR, ctx)) {
+            // V rows that some columns attend and others do not: whether all are finite is what products with zero say
+            f32x4 probe = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                const int dcol = 16 * db + 4 * (l16 & 3), at = 16 * ((dcol >> 3) ^ sw_v) + 2 * (dcol & 7);
+#pragma unroll
+                for (int h = 0; h < NH; ++h) probe = T::mfma16k16(lds_read_tr16(rowp_v + 16 * h * RB + at), s16x4{0, 0, 0, 0}, probe);
+            }
+            if (__any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.f))) { by_key = t; return; }
+        }
         // rows that the column does not attend
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
@@ -242,15 +258,12 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
             l_sum = T::add_pair(pk[2 * h + 1], T::add_pair(pk[2 * h], l_sum));   // sums the rounded weights that are multiplied
         }
         // O^T += V^T P^T: row d = 16db + l16, keys 4 quad + 0..3 (and 16 + 4 quad + 0..3)
-        const int row = 4 * quad + (l16 >> 2);
-        const char* rowp = my_v + row * RB;
-        const int sw = GEO::swz_v(row);   // rows 16 apart share a swizzle
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-            const int dcol = 16 * db + 4 * (l16 & 3), at = 16 * ((dcol >> 3) ^ sw) + 2 * (dcol & 7);
-            const s16x4 a0 = lds_read_tr16(rowp + at);
+            const int dcol = 16 * db + 4 * (l16 & 3), at = 16 * ((dcol >> 3) ^ sw_v) + 2 * (dcol & 7);
+            const s16x4 a0 = lds_read_tr16(rowp_v + at);
             if constexpr (NH == 2) {
-                const s16x4 a1 = lds_read_tr16(rowp + 16 * RB + at);
+                const s16x4 a1 = lds_read_tr16(rowp_v + 16 * RB + at);
                 o_acc[db] = T::mfma16(s16x8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
                                       __builtin_bit_cast(s16x8, u32x4{pk[0], pk[1], pk[2 * NH - 2], pk[2 * NH - 1]}), o_acc[db]);
             } else {
@@ -289,11 +302,23 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
     for (int t0 = g0; t0 < g1; t0 += NS) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            if (t0 + i < g1 && ring[i].there) consume(t0 + i, ring[i]);
+            if (t0 + i < g1 && ring[i].there && t0 + i < by_key) consume(t0 + i, ring[i]);
             const Ids now = next;
             next = ids_of(t0 + i + NS + 1);
             load_group(t0 + i + NS, now, ring[i]);
         }
+    }
+    if (by_key < g1) {
+        int l = l16;   // (worked out again: kept over the loop, the column's query row does not fit the registers of codes at D = 128)
+        asm volatile("" : "+v"(l));
+        const Column again = column_of(work, info, g, hg, l);
+        const short* const q[1] = {again.q};
+        const int limit[1] = {again.limit};
+        float m[1] = {m_ref}, sum[1] = {l_sum};
+        attend_key_by_key<T, D, FP8, 1>(p.c, p.Hkv, s, g, by_key * GR, min(g1 * GR, ctx), q, limit, c2,
+                                        [&](int db, int) __attribute__((always_inline)) -> f32x4& { return o_acc[db]; }, m, sum);
+        m_ref = m[0];
+        l_sum = sum[0];
     }
     acc.m = m_ref;
     acc.l = sum_across_quads(l_sum);

@@ -235,6 +235,56 @@ def test_attend_nan_and_infinities_of_attended_rows(kerns, seqs):
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("seqs,Hq,Hkv,D,max_q", [
+    ([(4, 300), (3, 9)], 4, 1, 64, None), ([(2, 61), (3, 4)] + [(2, (41 * i) % 300) for i in range(70)], 6, 2, 128, None), ([(9, 130), (1, 7)], 8, 1, 128, 1),
+    ([(90, 40), (70, 0)], 4, 2, 128, None), ([(50, 2100), (5, 5)], 12, 1, 64, None), ([(1030, 0), (1040, 9)], 48, 24, 128, None)],
+    ids=["drafts", "drafts of many", "first tokens only", "chunks", "pieces", "prompts"])
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("dtype,value", [(torch.float16, float("inf")), (torch.bfloat16, float("nan"))], ids=["f16-inf", "bf16-nan"])
+def test_attend_rows_that_are_not_finite_reach_who_attends_them(kerns, seqs, Hq, Hkv, D, max_q, eight, dtype, value):
+    """V rows of some tokens hold an infinity (a NaN, which is all that e4m3 has): the tokens before them are as if they were not there,
+    and those behind have it in its column and nowhere else."""
+    c = ref.Paged(seqs, 16, Hkv, D, dtype, DEV, eight=eight)
+    q = make_q(c.T, Hq, D, dtype)
+    bad = {}   # sequence: first token that attends a bad row
+    for s, (n, past) in enumerate(seqs[:2]):
+        bad[s] = max(n // 2, 1) if n > 1 else n
+        for i in range(bad[s], n, 3):
+            page, row = c.table_list[s][(past + i) // 16], (past + i) % 16
+            if eight:
+                c.v_pages.view(torch.uint8)[page, :, row, 3] = 0x7f
+            else:
+                c.v_pages[page, :, row, 3] = value
+    out = torch.full_like(q, 7.0)
+    run_attend(kerns, c, q, out, max_q)
+    want, bound = ref.attend(c, q[0].transpose(0, 1))
+    got = out[0].transpose(0, 1).double().cpu()
+    for s, (n, _) in enumerate(seqs):
+        lo, done = c.cu_list[s], n if max_q is None else min(n, max_q)
+        reached = torch.zeros(Hq, n, D, dtype=torch.bool)
+        reached[:, bad.get(s, n):, 3] = True
+        here = slice(lo, lo + done)
+        reached = reached[:, :done]
+        ok = (got[:, here] - want[:, here]).abs() <= bound[:, here]
+        assert (ok | reached).all(), f"sequence {s}"
+        x = got[:, here][reached]
+        assert not torch.isfinite(x).any() and (value == value and not eight or torch.isnan(x).all()), f"sequence {s}"
+
+
+@pytest.mark.parametrize("n", [3, 60], ids=["drafts", "chunks"])
+def test_attend_a_page_whose_scale_is_no_number(kerns, n):
+    """A scale of NaN makes NaN of the page's rows, for the tokens that attend one of them and no others."""
+    c = ref.Paged([(n, 30), (2, 40)], 16, 1, 64, torch.bfloat16, DEV, eight=True)
+    q = make_q(c.T, 4, 64, torch.bfloat16)
+    c.v_scales.view(torch.uint8)[c.table_list[0][2]] = 255   # rows 32 .. 47: the tokens from the third on
+    out = torch.full_like(q, 7.0)
+    run_attend(kerns, c, q, out)
+    want, bound = ref.attend(c, q[0].transpose(0, 1))
+    got = out[0].transpose(0, 1).double().cpu()
+    ok = (got - want).abs() <= bound
+    assert ok[:, :2].all() and ok[:, n:].all() and torch.isnan(got[:, 2:n]).all()
+
+
 @pytest.mark.parametrize("seqs,Hq", [([(1, 700), (1, 64)], 8), ([(4, 300), (3, 9)], 8), ([(90, 40)], 4)], ids=["decode", "drafts", "chunks"])
 @pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
 def test_attend_repeats_and_streams(kerns, seqs, Hq, eight):
