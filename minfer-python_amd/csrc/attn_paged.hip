@@ -607,25 +607,32 @@ struct PagedPlan {
     int64_t pieces;    // bound of the pieces, per KV head
     size_t o_bytes, ml_bytes, table_bytes;
 };
-// Rows of a workgroup: 256 share a tile's copies at head_dim 128 where they fill the chip's units, one workgroup to a unit, one and a half times; 128, two to
-// a unit (three at head_dim 64), else.
+// Waves of a workgroup, 32 rows each.  16-bit rows: four, and two workgroups to a unit (three at head_dim 64); eight, one to a unit, take 226 us / 243
+// for 2 x 700 tokens behind 8000, 58 / 68 for a prompt of 2048, 488 / 494 for one of 8192.  Codes at head_dim 128: eight where a sequence can fill them, which widen a tile
+// for twice as many rows (us, four / eight: 2 x 700 behind 8000 339 / 296, a prompt of 2048 behind 20000 833 / 730, of 4096 190 / 165, of 512
+// 24.6 / 27.3; where it cannot, 60 x 20 tokens of 4 heads behind 2000 to 8000, 300 / 356).
 constexpr int kWavesBig = 8, kWavesSmall = 4;
 constexpr int64_t kUnits = 256;
 static int64_t blocks_of(int64_t n_seqs, int64_t T, int64_t n_rep, int64_t max_q, int waves) {
     const int64_t rows = waves * 32;
     return std::min(n_seqs * ((max_q * n_rep + rows - 1) / rows), T * n_rep / rows + n_seqs);
 }
-#ifndef MINFER_PAGED_BIG
-#define MINFER_PAGED_BIG 384
-#endif
-static PagedPlan plan_paged(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q) {
+// Blocks of rows are cut where whole ones would leave more than a quarter of the chip's rounds of workgroups empty, of two rounds at most: the combine's
+// launch and the sums' way through memory cost 4 to 8 us where that gains nothing (us, whole / cut: 700 tokens behind 8000, a third of a
+// round 126 / 86, 3 x 700 a little over one 275 / 214, 4 x 700 280 / 238, of codes 374 / 293; 4 x 1000 behind 2000, two full rounds 120 / 127; 60 x 20, one round
+// 263 / 280), and not where contexts are short (a prompt of 512 16.7 / 21.7, of 1024 28.2 / 31.3, of codes 22.1 / 24.7 and 42.1 / 38.9).
+static bool cuts_blocks(bool eight, int64_t wgs, int64_t round, int64_t n_seqs, int64_t max_context) {
+    const int64_t rounds = (wgs + round - 1) / round;
+    return rounds <= 2 && 4 * wgs <= 3 * rounds * round && n_seqs <= 64 && max_context > (eight ? 512 : 1024);
+}
+static PagedPlan plan_paged(bool eight, int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_context) {
     PagedPlan r{};
     const int64_t n_rep = Hq / Hkv;
-    r.waves = D == 128 && T * n_rep / (kWavesBig * 32) * Hkv >= MINFER_PAGED_BIG ? kWavesBig : kWavesSmall;
+    r.waves = eight && D == 128 && max_q * n_rep > kWavesSmall * 32 ? kWavesBig : kWavesSmall;
     r.blocks = blocks_of(n_seqs, T, n_rep, max_q, r.waves);
     const int64_t wgs = r.blocks * Hkv, round = r.waves == kWavesBig ? kUnits : 2 * kUnits;   // workgroups that the chip holds at once
     r.pieces = r.blocks;
-    if (wgs <= 2 * round && n_seqs <= 64) {
+    if (cuts_blocks(eight, wgs, round, n_seqs, max_context)) {
         r.round = std::max<int64_t>(round / Hkv, 1);
         r.pieces = (r.blocks + r.round - 1) / r.round * r.round;
         r.o_bytes = (size_t)(r.pieces * Hkv * r.waves * 32 * D * 4);
@@ -647,7 +654,9 @@ static int launch_paged(const PagedParams& p, const PagedPlan& plan, hipStream_t
 }
 template <class T, bool FP8> static int launch_paged_as(const PagedParams& p, const PagedPlan& plan, int64_t D, hipStream_t stream) {
     if (D == 64) return launch_paged<T, 64, FP8, kWavesSmall>(p, plan, stream);
-    return plan.waves == kWavesBig ? launch_paged<T, 128, FP8, kWavesBig>(p, plan, stream) : launch_paged<T, 128, FP8, kWavesSmall>(p, plan, stream);
+    if constexpr (FP8)
+        if (plan.waves == kWavesBig) return launch_paged<T, 128, FP8, kWavesBig>(p, plan, stream);
+    return launch_paged<T, 128, FP8, kWavesSmall>(p, plan, stream);
 }
 
 }  // namespace minfer_attn
@@ -659,8 +668,12 @@ MINFER_ATTN_EXPORT size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs
     if (n_seqs <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_context < 0 || Hq % Hkv != 0) return 0;
     const int64_t max_q = bounded_tokens(T, max_q_len);
     if (paged_decode_takes(Hq, Hkv, max_q)) return paged_decode_workspace_bytes(n_seqs, Hq, Hkv, D, max_context, max_q);
-    const PagedPlan r = plan_paged(n_seqs, T, Hq, Hkv, D, max_q);
-    return r.o_bytes + r.ml_bytes + r.table_bytes;
+    size_t most = 0;   // of both kinds of pages
+    for (const bool eight : {false, true}) {
+        const PagedPlan r = plan_paged(eight, n_seqs, T, Hq, Hkv, D, max_q, max_context);
+        most = std::max(most, r.o_bytes + r.ml_bytes + r.table_bytes);
+    }
+    return most;
 }
 
 MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const void* q, const minfer_kv_pages* pages, const int32_t* cu_seqlens,
@@ -697,7 +710,7 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged(int dtype, int page_type, const v
             return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged: workspace too small or misaligned (see minfer_flash_attn_paged_workspace_bytes)");
         return launch_paged_decode(p, dtype, D, eight, max_context, workspace, (hipStream_t)stream_v);
     }
-    const PagedPlan plan = plan_paged(n_seqs, T, Hq, Hkv, D, max_q);
+    const PagedPlan plan = plan_paged(eight, n_seqs, T, Hq, Hkv, D, max_q, max_context);
     // (workgroups and their ids are 32-bit numbers)
     if (plan.pieces * Hkv > 0x7fffffffLL) return bad("flash_attn_paged: problem too large for one launch");
     if (plan.round > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.o_bytes + plan.ml_bytes + plan.table_bytes))
