@@ -217,7 +217,8 @@ typedef struct minfer_kv_pages {
  * <= 7 (fp16) or 119 (bf16), -100 where all are zero; magnitudes beyond 448 * 2^e are cut to it, and what is infinite or NaN becomes NaN.  A page whose row 0
  * is among the new rows gets the scale that its new rows need; another page keeps the larger of its scale and that, and where its scale grows the codes of
  * its rows in front of the new ones move to it (rounded again only where they leave e4m3's normal numbers; NaN stays NaN).  Rows behind the new ones keep their bytes.
- * The result does not depend on the order in which anything runs.  A page that a call writes to must belong to one sequence of that call.
+ * The result does not depend on the order in which anything runs.  A page that a call writes to must belong to one sequence of that call,
+ * once.
  *
  * All pointers 16-byte aligned; D is 64 or 128; rotary_dim a multiple of 8 (interleaved) or 16 (NeoX).
  */

@@ -85,6 +85,63 @@ def flash_attn_decode_q8_0(backend: str, which: str, workload: str, repeat: int)
     torch.cuda.synchronize()
 
 
+def flash_attn_paged(backend: str, which: str, workload: str, repeat: int, eight: bool = False):
+    """The decode workload with its caches in pages of 16 rows, or, with --workload long, the last 1024 tokens of each of four of its
+    sequences as chunks behind 7168 cached rows; `ref` is the op over the slab caches (decode workload only)."""
+    kerns = KernelBackend(backend)
+    q, kc, vc, ctx = workloads.decode_cache(device="cuda")
+    if workload == "long":
+        kc, vc, ctx = kc[:4], vc[:4], torch.full((4,), 8192, dtype=torch.int32, device="cuda")
+        q = torch.randn(1, q.shape[1], 4 * 1024, q.shape[3], device="cuda").to(q.dtype)
+    else:
+        q = q.squeeze(2).transpose(0, 1)[None]
+    n, per = ctx.numel(), q.shape[2] // ctx.numel()
+    kp, vp, table = workloads.in_pages(kc, vc)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda") * per
+    out = torch.zeros_like(q)
+    if which != "minfer":
+        assert per == 1, "ref: the decode workload only"
+        rows, slab = q[0].transpose(0, 1)[:, :, None].contiguous(), torch.zeros(n, q.shape[1], 1, q.shape[3], dtype=q.dtype, device="cuda")
+        fn = lambda: kerns.flash_attn_decode(QT, QB, QS, rows, kc, vc, ctx, slab)
+    elif eight:
+        (kp, ks), (vp, vs) = workloads.e4m3_pages(kp), workloads.e4m3_pages(vp)
+        fn = lambda: kerns.flash_attn_paged_fp8(QT, QB, QS, q, kp, vp, ks, vs, table, cu, ctx, per, out)
+    else:
+        fn = lambda: kerns.flash_attn_paged(QT, QB, QS, q, kp, vp, table, cu, ctx, per, out)
+    for _ in range(repeat):
+        fn()
+    torch.cuda.synchronize()
+
+
+def flash_attn_paged_fp8(backend: str, which: str, workload: str, repeat: int):
+    """flash_attn_paged over e4m3 pages."""
+    flash_attn_paged(backend, which, workload, repeat, True)
+
+
+def rope_kv_append_paged(backend: str, which: str, workload: str, repeat: int, eight: bool = False):
+    """The rope_kv_append shape (eight prompts of 4096 tokens) into pages of 16 rows; `ref` is the op into slab caches."""
+    kerns = KernelBackend(backend)
+    q, k, v, pos, kc, vc = workloads.kv_append(device="cuda", B=8, L=4096)
+    kp, vp, table = workloads.in_pages(kc, vc)
+    cu = torch.arange(9, dtype=torch.int32, device="cuda") * 4096
+    packed = [x.reshape(1, -1, *x.shape[2:]) for x in (q, k, v)]
+    if which != "minfer":
+        fn = lambda: kerns.rope_kv_append(1, 128, 5e5, q, k, v, pos, kc, vc)
+    elif eight:
+        (kp, ks), (vp, vs) = workloads.e4m3_pages(kp), workloads.e4m3_pages(vp)
+        fn = lambda: kerns.rope_kv_append_paged_fp8(1, 128, 5e5, *packed, cu, pos, table, kp, vp, ks, vs)
+    else:
+        fn = lambda: kerns.rope_kv_append_paged(1, 128, 5e5, *packed, cu, pos, table, kp, vp)
+    for _ in range(repeat):
+        fn()
+    torch.cuda.synchronize()
+
+
+def rope_kv_append_paged_fp8(backend: str, which: str, workload: str, repeat: int):
+    """rope_kv_append_paged into e4m3 pages."""
+    rope_kv_append_paged(backend, which, workload, repeat, True)
+
+
 def flash_attn_varlen(backend: str, which: str, workload: str, repeat: int):
     kerns = KernelBackend(backend)
     q, k, v, cu = workloads.ragged_prefill(device="cuda")
@@ -289,7 +346,9 @@ def mfma_rate(backend: str, which: str, workload: str, repeat: int):
 if __name__ == "__main__":
     KERNELS = {"mfma_rate": mfma_rate, "gemm_q8_0": gemm_q8_0, "flash_attn": flash_attn, "flash_attn_decode": flash_attn_decode, "flash_attn_varlen": flash_attn_varlen,
                "flash_attn_decode_q8_0": flash_attn_decode_q8_0, "il_rope": il_rope, "rope_kv_append": rope_kv_append,
-               "rope_kv_append_q8_0": rope_kv_append_q8_0, "rope_kv_append_norm": rope_kv_append_norm, "qkv": qkv, "quant": quant, "rmsnorm": rmsnorm, "gemm": gemm, "gemm_decode": gemm_decode, "copy": copy}
+               "rope_kv_append_q8_0": rope_kv_append_q8_0, "rope_kv_append_norm": rope_kv_append_norm,
+               "flash_attn_paged": flash_attn_paged, "flash_attn_paged_fp8": flash_attn_paged_fp8, "rope_kv_append_paged": rope_kv_append_paged,
+               "rope_kv_append_paged_fp8": rope_kv_append_paged_fp8, "qkv": qkv, "quant": quant, "rmsnorm": rmsnorm, "gemm": gemm, "gemm_decode": gemm_decode, "copy": copy}
     parser = argparse.ArgumentParser()
     parser.add_argument("--backend", choices=["torch_ext"], default="torch_ext")
     parser.add_argument("--kernel", choices=sorted(KERNELS), required=True)

@@ -99,6 +99,25 @@ def decode_cache(seed=0, device="cpu", B=64, Hq=32, Hkv=8, Lmax=8192, D=128, dty
     return q, kc, vc, ctx
 
 
+def in_pages(kc, vc, page=16, seed=0):
+    """Slab caches [B,Hkv,Lmax,D] cut into pages of `page` rows that lie in the pool in no order: k_pages, v_pages
+    [B*Lmax/page, Hkv, page, D] and the int32 table [B, Lmax/page]."""
+    B, Hkv, Lmax, D = kc.shape
+    order = torch.randperm(B * Lmax // page, generator=torch.Generator().manual_seed(seed)).to(kc.device)   # slab page i lies in page order[i]
+    pools = []
+    for x in (kc, vc):
+        pool = torch.empty(B * Lmax // page, Hkv, page, D, dtype=x.dtype, device=x.device)
+        pool[order] = x.view(B, Hkv, Lmax // page, page, D).transpose(1, 2).reshape(pool.shape)
+        pools.append(pool)
+    return pools[0], pools[1], order.to(torch.int32).view(B, Lmax // page)
+
+
+def e4m3_pages(pages, exponent=-6):
+    """Codes of pages and their scales, all 2^exponent (values of unit variance need 2^-7 or 2^-6)."""
+    codes = (pages * 2.0 ** -exponent).to(torch.float8_e4m3fn)
+    return codes, torch.full(pages.shape[:2], exponent + 127, dtype=torch.uint8, device=pages.device).view(torch.float8_e8m0fnu)
+
+
 def q8_0_rows(x):
     """Device tensor [..., D] (D a multiple of 32) -> its rows as Q8_0 blocks, uint8 [..., D/32*34], quantised on the
     device by the library's own quantiser (reference format: common/types.hpp:141-146)."""

