@@ -120,7 +120,8 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
 
     // ---- a ring of groups on their way ----
     constexpr int NK = FP8 ? NH * D / 64 : NI, NV = FP8 ? NH * NI8 : NI;
-    struct Stage { u32x4 k[NK], v[NV]; float ks[NH], vs[NH]; int there; } ring[NS];
+    // (scales as the words that hold their bytes: to take them out is to wait for them.  there: bit h half h's page is, above bit 8 which bytes)
+    struct Stage { u32x4 k[NK], v[NV]; uint32_t ks[NH], vs[NH]; int there; } ring[NS];
     // a lane's place inside the 16 rows: its row and chunk of load j, and its key's pieces of K's codes
     const int stride = (int)p.c.row_stride;
     constexpr int VPI = FP8 ? RPI8 : RPI, CPR = 64 / VPI;   // rows a load covers, 16-byte pieces per row
@@ -143,8 +144,10 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
 #pragma unroll
                 for (int j = 0; j < NI8; ++j) st.v[h * NI8 + j] = stream_load(reinterpret_cast<const u32x4*>(vb + (uint32_t)((j * RPI8 + v_row) * step + v_piece)));
                 const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
-                st.ks[h] = scale_value(const_byte(p.c.k_scales + sc));
-                st.vs[h] = scale_value(const_byte(p.c.v_scales + sc));
+                const uintptr_t ka = (uintptr_t)(p.c.k_scales + sc), va = (uintptr_t)(p.c.v_scales + sc);
+                st.ks[h] = const_load((const uint32_t*)(ka & ~(uintptr_t)3));
+                st.vs[h] = const_load((const uint32_t*)(va & ~(uintptr_t)3));
+                st.there |= ((int)(ka & 3) | (int)(va & 3) << 2) << (8 + 4 * h);
             } else {
                 const short* kb = (const short*)p.c.k + at;
                 const short* vb = (const short*)p.c.v + at;
@@ -166,6 +169,9 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
     char* const my_k = area + 16 * RB;   // 16-bit rows only
 
     auto consume = [&](int t, Stage& st) __attribute__((always_inline)) {
+        int ln = threadIdx.x & 63;
+        if (FP8 && D == 128) asm volatile("" : "+v"(ln));   // (places in LDS are worked out for every group: kept, they do not fit the registers of codes)
+        const int lane = ln, l16 = ln & 15, quad = ln >> 4;
         f32x4 sc[NH];
         // V rows behind the context may hold anything, NaN too, and their weight of zero would not take it out of the sums (of K only the
         // row's own scores are made, which are replaced)
@@ -178,18 +184,19 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
                 sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                const float ks = scale_value(st.ks[h] >> 8 * (st.there >> (8 + 4 * h) & 3) & 255u);
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
                     const u32x4 x = st.k[h * (D / 64) + c / 2];
                     const uint32_t lo = x[2 * (c % 2)], hi = x[2 * (c % 2) + 1];
-                    const u32x4 a = {widen2<T, false>(lo, st.ks[h]), widen2<T, true>(lo, st.ks[h]), widen2<T, false>(hi, st.ks[h]), widen2<T, true>(hi, st.ks[h])};
+                    const u32x4 a = {widen2<T, false>(lo, ks), widen2<T, true>(lo, ks), widen2<T, false>(hi, ks), widen2<T, true>(hi, ks)};
                     sc[h] = T::mfma16(__builtin_bit_cast(s16x8, a), qf[c], sc[h]);
                 }
             }
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
                 const bool on = (st.there >> h & 1) != 0;   // (a page that is not there: what was loaded in its place is not multiplied)
-                const float vs = on ? st.vs[h] : 1.f;
+                const float vs = on ? scale_value(st.vs[h] >> 8 * (st.there >> (10 + 4 * h) & 3) & 255u) : 1.f;
 #pragma unroll
                 for (int j = 0; j < NI8; ++j) {
                     const int row = 16 * h + j * RPI8 + lane / (D / 16), gr = 2 * (lane % (D / 16));
@@ -278,10 +285,12 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
 
     acc.m = -INFINITY;
     acc.l = 0.f;
-    Ids next = ids_of(g0);
+    Ids first[NS + 1];   // requested together: one wait
+#pragma unroll
+    for (int i = 0; i <= NS; ++i) first[i] = ids_of(g0 + i);
     bool any = false;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) any = any || is_there(next.id[h]);
+    for (int h = 0; h < NH; ++h) any = any || is_there(first[0].id[h]);
     if (!any) {   // pages given back by a window that moved on: on to the first group that is there, 64 at a time (64 sequences to 8192 rows 183 us, the first half of them gone 116)
         int at = g1;
         for (int base = g0; base < g1; base += 64) {
@@ -294,23 +303,27 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
         }
         if (at >= g1) return;
         g0 = __builtin_amdgcn_readfirstlane(at);
-        next = ids_of(g0);
+#pragma unroll
+        for (int i = 0; i <= NS; ++i) first[i] = ids_of(g0 + i);
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const Ids now = next;
-        next = ids_of(g0 + i + 1);
-        load_group(g0 + i, now, ring[i]);
-    }
-    for (int t0 = g0; t0 < g1; t0 += NS) {
+    for (int i = 0; i < NS; ++i) load_group(g0 + i, first[i], ring[i]);
+    Ids next = first[NS];
+    // the last round requests nothing: what a workgroup's barrier, or the next pair, would wait for (3 x 200 to 3000 rows of codes 11.9 us / 10.4, 64 x 50 to 300
+    // 18.3 / 15.4, 64 x 512 to 8192 182.6 / 181.4)
+    int t0 = g0;
+    for (; t0 + NS < g1; t0 += NS) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            if (t0 + i < g1 && ring[i].there && t0 + i < by_key) consume(t0 + i, ring[i]);
+            if ((ring[i].there & 3) && t0 + i < by_key) consume(t0 + i, ring[i]);
             const Ids now = next;
             next = ids_of(t0 + i + NS + 1);
             load_group(t0 + i + NS, now, ring[i]);
         }
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+        if (t0 + i < g1 && (ring[i].there & 3) && t0 + i < by_key) consume(t0 + i, ring[i]);
     if (by_key < g1) {
         int l = l16;   // (worked out again: kept over the loop, the column's query row does not fit the registers of codes at D = 128)
         asm volatile("" : "+v"(l));
@@ -424,8 +437,19 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
     }
 }
 
+// Weights of a column's partial results, lane i holding part i's reference and sum (-inf and 0 in lanes without): w_i = 2^(m_i - max m), and the sum of
+// l_i w_i.  A part whose scores are all NaN has a weight of zero and sums of NaN and is multiplied like any other.
+struct PartWeights { float w, top, total; };
+MA_DEV PartWeights part_weights(float m, float l) {
+    PartWeights r;
+    r.top = wave_max(m);
+    r.w = m > -INFINITY ? fast_exp2(m - r.top) : 0.f;
+    r.total = lane_sum<64>(l * r.w);
+    return r;
+}
+
 // out = sum_i O_i w_i / sum_i l_i w_i, w_i = 2^(m_i - max m), over the parts of a row; a wave per row (sequence, token, head), lane i holding part i's
-// reference and sum.  A part whose scores are all NaN has a weight of zero and sums of NaN and is multiplied like any other.
+// reference and sum.
 template <class T, int D, int GR>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work) {
     const PagedParams& p = work.p;
@@ -455,9 +479,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work)
     const int start = const_load(work.seq_off + s) + ((col / 16) * p.Hkv + g) * groups;
     const int ns = groups > 0 ? min((start + groups - 1) / quota - start / quota + 1, p.slots) : 0;
     const float m = lane < ns ? m_raw : -INFINITY, l = lane < ns ? l_raw : 0.f;
-    const float top = wave_max(m);
-    const float wgt = m > -INFINITY ? fast_exp2(m - top) : 0.f;
-    const float total = lane_sum<64>(l * wgt);
+    const PartWeights pw = part_weights(m, l);
     float acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
@@ -467,12 +489,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work)
             if (s0 > 0 || u >= kEarly) load_o(min(s0 + u, ns - 1), x[u]);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float wi = lane_value(wgt, min(s0 + u, 63));
+            const float wi = lane_value(pw.w, min(s0 + u, 63));
 #pragma unroll
             for (int e = 0; e < EPL; ++e) acc[e] += s0 + u < ns ? x[u][e] * wi : 0.f;
         }
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = pw.total > 0.f ? 1.f / pw.total : 0.f;
     uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + EPL * lane;
     if (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = T::pack2(acc[0] * inv, acc[EPL - 1] * inv);
     else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
@@ -486,6 +508,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work)
 // only when its own have arrived; the reader's loads stand behind a barrier that thread 0 reaches with the count's value in hand.
 MA_DEV void store_shared(float* p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 MA_DEV float load_shared(const float* p) { return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+MA_DEV void store_shared2(float* p, f32x2 x) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+MA_DEV f32x2 load_shared2(const float* p) {
+    return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float*>(p)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
 
 // Every pair of a sequence is cut into the same number of chunks, equal to within a group; the chunk's size, the same for all sequences, is the
 // smallest (256 rows at least) that leaves no more chunks than workgroups.  Up to 64 sequences, one to a lane; all waves
@@ -511,49 +539,34 @@ template <int GR> struct ChunkPlan {
     }
 };
 
-MA_DEV float merge_weight(float m, float top) { return m > -INFINITY ? fast_exp2(m - top) : 0.f; }
-
-// Merges the n chunks of the columns of (s, g, hg) from the workspace and stores the output rows; all threads of the workgroup.  The order of
+// Merges the n chunks of the columns of (s, g, hg) from the workspace and stores the output rows; all threads of the workgroup, a wave 64
+// elements of a column at a time, without LDS and barriers (with the weights made by 16 threads in LDS it took twice the time).  The order of
 // the sums depends on nothing but n.
 template <class T, int D>
-MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g, int hg, int n, float* lds_w /* [128][16] */, float* lds_inv /* [16] */) {
+MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g, int hg, int n) {
     const PagedParams& p = w.p;
-    const int tid = threadIdx.x, cols = min(16, w.n_col - hg * 16);
+    const int lane = threadIdx.x & 63, wave = wave_id(), cols = min(16, w.n_col - hg * 16);
     const int64_t at0 = part_row(w, s, g, hg * 16) * p.slots;
-    for (int i = tid; i < n * cols; i += kChunkWaves * 64) {
-        const int c = i / n, k = i - c * n;
-        lds_w[k * 16 + c] = load_shared(p.part_ml + (at0 + (int64_t)c * p.slots + k) * 2);
-        lds_w[(64 + k) * 16 + c] = load_shared(p.part_ml + (at0 + (int64_t)c * p.slots + k) * 2 + 1);
-    }
-    // an output element's first parts are requested while the weights are made
     constexpr int PER = 16 * D / (kChunkWaves * 64);
     float x[PER][8];
+    f32x2 ml[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int idx = tid + e * kChunkWaves * 64;
+        const int idx = (wave + e * kChunkWaves) * 64;
         if (idx < cols * D) {
-            const float* src = p.part_o + (at0 + (int64_t)(idx / D) * p.slots) * D + idx % D;
+            const int64_t at = at0 + (int64_t)(idx / D) * p.slots;
+            ml[e] = load_shared2(p.part_ml + (at + min(lane, n - 1)) * 2);
+            const float* src = p.part_o + at * D + idx % D + lane;
 #pragma unroll
             for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + (int64_t)min(u, n - 1) * D);
         }
     }
-    __syncthreads();
-    if (tid < cols) {
-        float top = -INFINITY, l = 0.f;
-        for (int i = 0; i < n; ++i) top = fmaxf(top, lds_w[i * 16 + tid]);
-        for (int i = 0; i < n; ++i) {
-            const float wi = merge_weight(lds_w[i * 16 + tid], top);
-            l += lds_w[(64 + i) * 16 + tid] * wi;
-            lds_w[i * 16 + tid] = wi;
-        }
-        lds_inv[tid] = l > 0.f ? 1.f / l : 0.f;
-    }
-    __syncthreads();
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int idx = tid + e * kChunkWaves * 64;
+        const int idx = (wave + e * kChunkWaves) * 64;
         if (idx >= cols * D) break;
-        const int c = idx / D, d = idx % D, col = hg * 16 + c, tok = col / p.n_rep;
+        const int c = idx / D, d = idx % D + lane, col = hg * 16 + c, tok = col / p.n_rep;
+        const PartWeights pw = part_weights(lane < n ? ml[e][0] : -INFINITY, lane < n ? ml[e][1] : 0.f);
         const float* src = p.part_o + (at0 + (int64_t)c * p.slots) * D + d;
         float sum = 0.f;
         for (int s0 = 0; s0 < n; s0 += 8) {
@@ -562,11 +575,13 @@ MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g,
                 for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + (int64_t)min(s0 + u, n - 1) * D);
             }
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (s0 + u < n) sum += x[e][u] * lds_w[(s0 + u) * 16 + c];
+            for (int u = 0; u < 8; ++u) {
+                const float wi = lane_value(pw.w, min(s0 + u, 63));
+                sum += s0 + u < n ? x[e][u] * wi : 0.f;
+            }
         }
         if (tok < info.len)
-            reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * lds_inv[c], 0.f) & 0xffffu);
+            reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * (pw.total > 0.f ? 1.f / pw.total : 0.f), 0.f) & 0xffffu);
     }
 }
 
@@ -577,7 +592,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const 
     constexpr int ORS = D + 4;   // floats between two columns of a wave's result: their 16-byte pieces start in different banks
     constexpr int LDS = NW * WAVE_LDS > NW * 16 * ORS * 4 ? NW * WAVE_LDS : NW * 16 * ORS * 4;
     __shared__ __attribute__((aligned(1024))) char lds[LDS];   // the waves' row areas, then their results
-    __shared__ float ml_s[128 * 16], inv_s[16];
+    __shared__ float ml_s[2 * NW * 16];
     __shared__ int last_s;
     const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), l16 = lane & 15, quad = lane >> 4;
     const int pairs = p.Hkv * work.n_hg;
@@ -605,32 +620,24 @@ __global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const 
         float* dst = o_s + (w * 16 + l16) * ORS + 4 * quad;
 #pragma unroll
         for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc.o[db];
-        if (quad == 0) { ml_s[w * 16 + l16] = acc.m; ml_s[(64 + w) * 16 + l16] = acc.l; }
+        if (quad == 0) { ml_s[w * 16 + l16] = acc.m; ml_s[(NW + w) * 16 + l16] = acc.l; }
     }
     __syncthreads();
     const bool whole = n <= 1;   // the chunk is the whole context: its result is the output
     const int64_t at0 = part_row(work, s, g, hg * 16) * p.slots + split;
-    for (int idx = tid; idx < cols * D; idx += NW * 64) {
-        const int c = idx / D, d = idx % D;
-        float top = -INFINITY, l = 0.f, sum = 0.f;
+    for (int idx = w * 64; idx < cols * D; idx += NW * 64) {   // a wave 64 elements of a column
+        const int c = idx / D, d = idx % D + lane;
+        const PartWeights pw = part_weights(lane < NW ? ml_s[lane * 16 + c] : -INFINITY, lane < NW ? ml_s[(NW + lane) * 16 + c] : 0.f);
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) top = fmaxf(top, ml_s[i * 16 + c]);
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            const float wi = merge_weight(ml_s[i * 16 + c], top);
-            l += ml_s[(64 + i) * 16 + c] * wi;
-            sum += o_s[(i * 16 + c) * ORS + d] * wi;
-        }
+        for (int i = 0; i < NW; ++i) sum += o_s[(i * 16 + c) * ORS + d] * lane_value(pw.w, i);
         if (whole) {
             const int col = hg * 16 + c, tok = col / p.n_rep;
             if (tok < info.len)
-                reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * (l > 0.f ? 1.f / l : 0.f), 0.f) & 0xffffu);
+                reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * (pw.total > 0.f ? 1.f / pw.total : 0.f), 0.f) & 0xffffu);
         } else {
             store_shared(p.part_o + (at0 + (int64_t)c * p.slots) * D + d, sum);
-            if (d == 0) {
-                store_shared(p.part_ml + (at0 + (int64_t)c * p.slots) * 2, top);
-                store_shared(p.part_ml + (at0 + (int64_t)c * p.slots) * 2 + 1, l);
-            }
+            if (idx % D == 0 && lane == 0) store_shared2(p.part_ml + (at0 + (int64_t)c * p.slots) * 2, f32x2{pw.top, pw.total});
         }
     }
     if (whole || !work.done) return;
@@ -643,18 +650,17 @@ __global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const 
         if (last_s) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (last_s) merge_chunks<T, D>(work, s, info, g, hg, n, ml_s, inv_s);
+    if (last_s) merge_chunks<T, D>(work, s, info, g, hg, n);
 }
 
 // (where there are no counters) grid (column groups x KV heads, sequences)
 template <class T, int D, int GR>
 __global__ __launch_bounds__(kChunkWaves * 64) void paged_chunk_merge_kernel(const DecodeWork work, int n_wg) {
     const PagedParams& p = work.p;
-    __shared__ float ml_s[128 * 16], inv_s[16];
     const int s = blockIdx.y, hg = (int)blockIdx.x / p.Hkv, g = (int)blockIdx.x - hg * p.Hkv;
     const ChunkPlan<GR> plan(work, n_wg);
     const int n = lane_value(plan.each, s);
-    if (n > 1) merge_chunks<T, D>(work, s, seq_info(p, s), g, hg, n, ml_s, inv_s);
+    if (n > 1) merge_chunks<T, D>(work, s, seq_info(p, s), g, hg, n);
 }
 
 // Workgroups of the line: as many as the chip holds at once.
