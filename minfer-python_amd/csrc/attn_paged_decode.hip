@@ -14,11 +14,11 @@
 // * the line: all rows to be read, sequence by sequence, KV head by KV head, cut into as many equal shares as the launch has waves; a
 //   wave's share covers parts of a few (sequence, KV head) pairs, each of which leaves a partial result that
 //   paged_merge_kernel puts together.  Whatever the mix of contexts, all waves end together.  64 sequences of 512 to 8192 rows, 32 query
-//   heads on 8 of 128: 182 us, 6.0 TB/s, of which the merge 5; over codes 102 us, 5.4 TB/s.
+//   heads on 8 of 128: 180 us, 6.1 TB/s, of which the merge 5; over codes 99 us, 5.6 TB/s.
 // * chunks, for few pairs: eight waves of a workgroup share one chunk of a pair and merge in LDS, and the last workgroup of a pair merges its
 //   chunks (on the null stream; elsewhere paged_chunk_merge_kernel does).  A sequence is cut by its own context, which the host does not know.
-//   12 sequences of 3 or 4 drafts, 28964 rows: 28 us, 4.2 TB/s; one token, 8 heads on 2 of 64, against 1501 rows 8 us, three against 5570 rows of
-//   codes 13 us, which is latency: a launch, two dependent loads of tables, the first rows, the merge in LDS.
+//   12 sequences of 3 or 4 drafts, 28964 rows: 27 us, 4.4 TB/s; one token, 8 heads on 2 of 64, against 1501 rows 8 us, three against 5570 rows of
+//   codes 10 us, which is latency: a launch, two dependent loads of tables, the first rows, the merge in LDS.
 #include <algorithm>
 #include <atomic>
 
@@ -29,6 +29,9 @@ namespace minfer_attn {
 constexpr int kLineWaves = 4;          // waves per workgroup of the line
 constexpr int kLineWgPerCu = 2;
 constexpr int kChunkWaves = 8;
+// Least rows of a wave's share of the line (us, 128 / 64 / 32: 64 sequences of 6 to 100 21.8 / 14.9 / 12.9, of 100 15.8 / 14.1 / 15.9, of codes 15.9 / 14.5 /
+// 12.1; one of 4000 15.1 / 14.7 / 14.8; 64 of up to 2000 on one KV head 16.0 / 16.5 / 19.4; where every wave has more nothing changes).
+constexpr int kLeastShare = 64;
 constexpr int kMaxSlots = 64;          // partial results a row can have: a wave merges them, one to a lane
 
 struct DecodeWork {
@@ -355,7 +358,7 @@ template <int D> MA_DEV void store_part(const DecodeWork& w, int s, int g, int h
 
 // ---- the line ------------------------------------------------------------------------------------------------------
 // Lengths in groups: every sequence's (zero without tokens) times its pairs, one after the other.  The quota: an equal share for
-// every wave, 128 rows at least, and as much as leaves no pair with more partial results than there are slots.
+// every wave, kLeastShare rows at least, and as much as leaves no pair with more partial results than there are slots.
 struct LineSeq { SeqInfo info; int groups; };
 template <int GR> MA_DEV LineSeq line_seq(const DecodeWork& w, int s) {   // (per lane)
     const PagedParams& p = w.p;
@@ -396,7 +399,7 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
         }
     }
     longest = (int)wave_max((float)longest);   // (below 2^24 exactly, and above rounded up or down by less than the slots to spare)
-    const int quota = max(max((total + n_waves - 1) / n_waves, 128 / GR), longest / (p.slots - 3) + 1);
+    const int quota = max(max((total + n_waves - 1) / n_waves, kLeastShare / GR), longest / (p.slots - 3) + 1);
     if (first && lane == 0) { work.seq_off[p.n_seqs] = total; work.seq_off[p.n_seqs + 1] = quota; }
     // shares to the waves of a workgroup in turn; where there are no more shares than workgroups, one to each
     const int n_shares = (total + quota - 1) / quota;
@@ -501,7 +504,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work)
 }
 
 // ---- chunks ----------------------------------------------------------------------------------------------------------
-// What the line costs a small problem is latency: a wave streams 128 rows one group after the other, and a second launch merges.  Here the eight waves of
+// What the line costs a small problem is latency: a wave streams its rows one group after the other, and a second launch merges.  Here the eight waves of
 // a workgroup share a chunk and merge in LDS.  A pair that is one chunk long is done with that; otherwise the chunk's result goes to
 // the workspace, and the workgroup that comes last (a counter per pair) merges the pair's.  Results cross from one XCD's L2 to
 // another's: they are written and read with device-scope accesses, which go past the L2s on both sides, and a workgroup counts itself
@@ -676,8 +679,8 @@ static int compute_units() {
     return n;
 }
 
-// Slots of a row: enough for shares of 128 rows, 64 at most (longer contexts get longer shares).
-static int64_t slots_of(int64_t max_context) { return std::min<int64_t>(kMaxSlots, max_context / 128 + 4); }
+// Slots of a row: enough for the least shares, 64 at most (longer contexts get longer shares).
+static int64_t slots_of(int64_t max_context) { return std::min<int64_t>(kMaxSlots, max_context / kLeastShare + 4); }
 
 bool paged_decode_takes(int64_t Hq, int64_t Hkv, int64_t max_q) { return max_q == 1 || max_q * (Hq / Hkv) <= 16; }
 
@@ -695,15 +698,16 @@ template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStre
     hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
     return check_launch("paged_merge_kernel");
 }
-// Whether a call is one for chunks.  Up to a pair for every unit always (us, chunks / line, contexts alike and from a sixteenth up: one of 4000 12.2 / 15.7, 10.8 /
-// 14.7; 4 of 30000 79 / 86, 41 / 46; 16 of 4000 45 / 51, 32 / 35, of 20000 e4m3 111 / 120, 66 / 66; 32 of 300 10.9 / 17.4, 8.9 / 18.5, of 1500 e4m3
-// 23 / 32, 20 / 25; where every unit has one long context, contexts that differ leave units idle: 32 of 6000 121 / 127, 79 / 74, e4m3 68 / 79, 57 / 50).
-// Two rounds of whole contexts where the table has no room for long ones: 64 of 100 14.3 / 16.7, 12.7 / 24.4, of 400 26.2 / 28.6, 20.7 / 22.1, of 1000
-// 47.2 / 50.9, 32.1 / 32.6, of 3000 123 / 128, 82 / 79; e4m3 of 100 14.3 / 18.6, 13.6 / 24.1, of 400 22.0 / 25.3, 20.0 / 19.0, of 1000 36.6 / 32.8.
+// Whether a call is one for chunks.  Up to a pair for every unit always (us, chunks / line, contexts alike and from a sixteenth up: one of 4000 10.5 / 14.7, 9.6 /
+// 14; 4 of 30000 78 / 85, 39 / 45; 16 of 4000 44 / 49, 32 / 34, of 20000 e4m3 110 / 118, 65 / 63; 32 of 300 10.2 / 16, 8.2 / 13, of 1500 e4m3
+// 22 / 29, 19 / 22; where every unit has one long context, contexts that differ leave units idle: 32 of 6000 121 / 128, 79 / 74, e4m3 67 / 76, 56 / 47).
+// Two rounds of whole contexts where the table has no room for long ones: 64 of 100 13.1 / 14.1, 11.8 / 14.9, of 400 25.2 / 27.4, 19.9 / 20.1, of 1000
+// 45.7 / 50.3, 31.0 / 31.4, of 2000 84 / 91, 53 / 53, of 6000 237 / 244, 156 / 146; e4m3 of 100 12.0 / 14.5, 10.9 / 14.8, of 400 19.2 / 22.4, 17.9 / 17.6, of 700 24.8 /
+// 28.8, 22.2 / 22.2, of 1000 33.7 / 31.7, 28.7 / 25.7.
 static int chunk_rounds(const DecodeWork& w, int64_t max_context, bool eight) {
     const int64_t pairs = (int64_t)w.p.n_seqs * w.p.Hkv * w.n_hg, units = compute_units();
     if (w.p.n_seqs > 64 || pairs > kStreamCounters) return 0;
-    return pairs <= units ? 1 : pairs <= 2 * units && max_context <= (eight ? 384 : 1024) ? 2 : 0;
+    return pairs <= units ? 1 : pairs <= 2 * units && max_context <= (eight ? 768 : 2048) ? 2 : 0;
 }
 template <class T, int D, bool FP8> static int launch_chunks(DecodeWork w, int rounds, hipStream_t stream) {
     const int n_wg = rounds * compute_units();
