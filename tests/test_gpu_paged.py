@@ -285,6 +285,60 @@ def test_attend_a_page_whose_scale_is_no_number(kerns, n):
     assert ok[:, :2].all() and ok[:, n:].all() and torch.isnan(got[:, 2:n]).all()
 
 
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 40)], [(3, 100), (4, 30)], [(70, 50), (9, 0)]], ids=["decode", "drafts", "chunks"])
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+def test_pages_whose_offsets_pass_32_bits(kerns, seqs, eight):
+    """Pages that lie 2^32 elements behind a pool's first one: the same bits as in a small pool, appended and attended."""
+    c = ref.Paged(seqs, 64, 2, 128, torch.float16, DEV, eight=eight)
+    n_big = 2 ** 32 // c.k_pages[0].numel() + 50 * c.n_pages
+    pools = [torch.empty((n_big,) + c.k_pages.shape[1:], dtype=c.k_pages.dtype, device=DEV) for _ in range(2)]
+    ids = n_big - 1 - 50 * torch.arange(c.n_pages, device=DEV)
+    table = torch.where(c.table >= 0, ids.to(torch.int32)[c.table.long().clamp(min=0)], -1)
+    scales = ()
+    for pool, small in zip(pools, (c.k_pages, c.v_pages)):
+        bits(pool)[ids] = bits(small)
+    if eight:
+        scales = tuple(torch.zeros(n_big, 2, dtype=torch.uint8, device=DEV) for _ in range(2))
+        for big, small in zip(scales, c.scales()):
+            big[ids] = small.view(torch.uint8)
+        scales = tuple(x.view(torch.float8_e8m0fnu) for x in scales)
+    q = make_q(c.T, 8, 128, torch.float16)
+    k, v = make_q(c.T, 2, 128, torch.float16, 2), make_q(c.T, 2, 128, torch.float16, 3)
+    outs = []
+    for t, (kp, vp), sc in ((c.table, (c.k_pages, c.v_pages), c.scales()), (table, pools, scales)):
+        mine, out = q.clone(), torch.empty_like(q)
+        append, attend = (kerns.rope_kv_append_paged_fp8, kerns.flash_attn_paged_fp8) if eight else (kerns.rope_kv_append_paged, kerns.flash_attn_paged)
+        append(1, 128, BASE, mine, k, v, c.cu, c.past, t, kp, vp, *sc)
+        attend(*QT[q.dtype], mine.transpose(1, 2), kp, vp, *sc, t, c.cu, c.ctx, max(n for n, _ in seqs), out.transpose(1, 2))
+        outs.append((mine, out))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1]) and torch.isfinite(outs[0][1]).all()
+    for pool, small in zip(pools, (c.k_pages, c.v_pages)):
+        assert torch.equal(bits(pool)[ids], bits(small))
+
+
+@pytest.mark.parametrize("n", [1, 3, 40], ids=["decode", "drafts", "chunks"])
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+def test_attend_one_page_many_times(kerns, n, eight):
+    """A table that names one page again and again, 2^17 rows, behind them one page of its own: a context is read by its table, however
+    long; many times the same rows are the weights of one of them, many times.  Beside the bound of rounded weights, fp32 sums of up
+    to 2^17 / 4 weights a lane and as many products are off by half a step a term."""
+    c = ref.Paged([(n, 64)], 64, 1, 64, torch.float16, DEV, eight=eight)
+    times = 2 ** 17 // 64
+    table = torch.cat([c.table[:, :1].expand(1, times), c.table[:, 1:2]], 1).contiguous()
+    ctx = torch.tensor([times * 64 + n], dtype=torch.int32, device=DEV)
+    q = make_q(n, 4, 64, torch.float16)
+    out = torch.full_like(q, 7.0)
+    call = kerns.flash_attn_paged_fp8 if eight else kerns.flash_attn_paged
+    call(*QT[q.dtype], q.transpose(1, 2), c.k_pages, c.v_pages, *c.scales(), table, c.cu, ctx, n, out.transpose(1, 2))
+    big = ref.Paged([(n, 64)], 64, 1, 64, torch.float16, DEV, eight=eight)
+    big.seqs, big.table_list = [(n, times * 64)], [[0] * (times + 1)]
+    big.k_dense = [torch.cat([c.k_dense[0][:, :64].repeat(1, times, 1), c.k_dense[0][:, 64:]], 1)]
+    big.v_dense = [torch.cat([c.v_dense[0][:, :64].repeat(1, times, 1), c.v_dense[0][:, 64:]], 1)]
+    want, bound = ref.attend(big, q[0].transpose(0, 1))
+    sums = 2 * 2.0 ** 15 * 2.0 ** -24 * float(big.v_dense[0].abs().max())
+    assert ((out[0].transpose(0, 1).double().cpu() - want).abs() <= bound + sums).all()
+
+
 @pytest.mark.parametrize("seqs,Hq", [([(1, 700), (1, 64)], 8), ([(4, 300), (3, 9)], 8), ([(90, 40)], 4)], ids=["decode", "drafts", "chunks"])
 @pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
 def test_attend_repeats_and_streams(kerns, seqs, Hq, eight):
