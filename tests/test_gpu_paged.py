@@ -339,6 +339,36 @@ def test_attend_one_page_many_times(kerns, n, eight):
     assert ((out[0].transpose(0, 1).double().cpu() - want).abs() <= bound + sums).all()
 
 
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+def test_attend_pieces_of_two_rounds(kerns, eight):
+    """A little more blocks than the chip holds at once: 73 of 128 rows, or 37 of 256, for each of eight KV heads."""
+    c = ref.Paged([(2300, 0), (10, 1500)], 16, 8, 128, torch.bfloat16, DEV, eight=eight)
+    check_attend(kerns, c, 32)
+
+
+@pytest.mark.parametrize("seqs", [[(1, 4000), (1, 300)], [(3, 900), (2, 70)], [(50, 3000)]], ids=["decode", "drafts", "chunks"])
+def test_attend_on_two_streams_at_once(kerns, seqs):
+    """Calls in flight on the null stream and on another at the same time, of the same cache and of different ones: the bits of calls alone."""
+    caches = [ref.Paged(seqs, 16, 2, 64, torch.float16, DEV, seed=s) for s in range(2)]
+    qs = [make_q(c.T, 8, 64, torch.float16, 5 + i) for i, c in enumerate(caches)]
+    alone = []
+    for c, q in zip(caches, qs):
+        out = torch.empty_like(q)
+        run_attend(kerns, c, q, out)
+        torch.cuda.synchronize()
+        alone.append(out)
+    side = torch.cuda.Stream()
+    outs = [[torch.full_like(qs[0], 7.0) for _ in range(40)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(40):
+        run_attend(kerns, caches[i % 2], qs[i % 2], outs[0][i])
+        with torch.cuda.stream(side):
+            run_attend(kerns, caches[(i // 2) % 2], qs[(i // 2) % 2], outs[1][i])
+    torch.cuda.synchronize()
+    for i in range(40):
+        assert torch.equal(outs[0][i], alone[i % 2]) and torch.equal(outs[1][i], alone[(i // 2) % 2])
+
+
 @pytest.mark.parametrize("seqs,Hq", [([(1, 700), (1, 64)], 8), ([(4, 300), (3, 9)], 8), ([(90, 40)], 4)], ids=["decode", "drafts", "chunks"])
 @pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
 def test_attend_repeats_and_streams(kerns, seqs, Hq, eight):
