@@ -148,12 +148,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     }
     int all;
     const Piece me = find_piece<BR>(p, rank, all);
+    if (p.round > 0 && blockIdx.x == 0 && threadIdx.x == 0) p.table[0] = all;   // for the combine kernel (of no sequences, too)
     if (me.seq < 0) return;
     const int seq = me.seq, block = me.block;
-    if (p.round > 0 && g == 0 && threadIdx.x == 0) {   // for the combine kernel
-        reinterpret_cast<int4*>(p.table)[1 + rank] = make_int4(me.seq, me.block, me.part, me.parts);
-        if (rank == 0) p.table[0] = all;
-    }
+    if (p.round > 0 && g == 0 && threadIdx.x == 0) reinterpret_cast<int4*>(p.table)[1 + rank] = make_int4(me.seq, me.block, me.part, me.parts);
     const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
     const int seq_lo = range.lo, seq_len = range.len;
     const int ctx = min(max(const_load(p.ctx + seq), 0), p.c.width << p.c.page_log2);

@@ -339,6 +339,24 @@ def test_attend_one_page_many_times(kerns, n, eight):
     assert ((out[0].transpose(0, 1).double().cpu() - want).abs() <= bound + sums).all()
 
 
+@pytest.mark.parametrize("n", [1, 3, 80], ids=["decode", "drafts", "chunks"])
+def test_attend_tokens_of_no_sequence(kerns, n):
+    """Tokens that belong to no sequence, all of them empty, over a table wide enough for blocks to be cut: nothing is written, whatever the
+    memory held that the call's workspace gets."""
+    c = ref.Paged([(n, 40), (n, 90)], 16, 2, 64, torch.float16, DEV, width=300)
+    q = make_q(c.T, 4, 64, torch.float16)
+    out = torch.full_like(q, 7.0)
+    for fill in (0x00, 0x7f):
+        for cu in ([0, 0, 0], [c.T, c.T, c.T]):
+            c.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+            before = [torch.full((size,), fill, dtype=torch.uint8, device=DEV) for size in (1 << 16, 1 << 20, 1 << 24, 1 << 26)]
+            torch.cuda.synchronize()
+            del before   # to the allocator, which hands it out again as it is
+            run_attend(kerns, c, q, out, n)
+            torch.cuda.synchronize()
+            assert (out == 7).all()
+
+
 @pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
 def test_attend_pieces_of_two_rounds(kerns, eight):
     """A little more blocks than the chip holds at once: 73 of 128 rows, or 37 of 256, for each of eight KV heads."""
