@@ -520,10 +520,16 @@ void append_paged(const char* op, int64_t style, int64_t rotary_dim, double freq
     const int64_t n_seqs = cu_seqlens.size(0) - 1, T = q.size(1), D = q.size(3);
     check_index(cu_seqlens, n_seqs + 1, q, op, "cu_seqlens");
     check_index(positions, n_seqs, q, op, "positions");
-    const minfer_kv_pages pages = pages_of(q, n_seqs, D, block_table, k_pages, v_pages, scales, op);
+    minfer_kv_pages pages = pages_of(q, n_seqs, D, block_table, k_pages, v_pages, scales, op);
     STD_TORCH_CHECK(k_pages.size(1) == k.size(2), op, ": the pages' number of heads is not k's");
     STD_TORCH_CHECK(rotary_dim <= D, op, ": rotary_dim exceeds head_dim");
     if (T == 0 || n_seqs == 0) return;
+    pages.k = k_pages.mutable_data_ptr();   // (a lazily copied tensor gets memory of its own)
+    pages.v = v_pages.mutable_data_ptr();
+    if (scales.k) {
+        pages.k_scales = scales.k->mutable_data_ptr();
+        pages.v_scales = scales.v->mutable_data_ptr();
+    }
     const OnDeviceOf on(q);
     check_rc(minfer_rope_kv_append_paged(dtype, (int)style, scales.k ? MINFER_FP8_E4M3 : dtype, q.mutable_data_ptr(), k.const_data_ptr(),
                                          v.const_data_ptr(), static_cast<const int32_t*>(cu_seqlens.const_data_ptr()),
