@@ -212,8 +212,8 @@ typedef struct minfer_kv_pages {
  * belong to none are left alone, and rows whose position is negative or whose page is not there are not written (q is still rotated).
  * page_type is the activations' dtype, and the rows are those that minfer_rope_kv_append would write, or MINFER_FP8_E4M3.
  *
- * 8-bit pages: what a 16-bit cache would have held is rounded to e4m3 (to nearest, ties to even) after division by the scale of
- * its page and head.  The scale that rows need is the smallest power of two 2^e with their largest finite magnitude <= 448 * 2^e, -100 <= e
+ * 8-bit pages: k, rotated in 64 bits and rounded to the activations' type, and v are rounded to e4m3 (to nearest, ties to even) after division by
+ * the scale of their page and head.  The scale that rows need is the smallest power of two 2^e with their largest finite magnitude <= 448 * 2^e, -100 <= e
  * <= 7 (fp16) or 119 (bf16), -100 where all are zero; magnitudes beyond 448 * 2^e are cut to it, and what is infinite or NaN becomes NaN.  A page whose row 0
  * is among the new rows gets the scale that its new rows need; another page keeps the larger of its scale and that, and where its scale grows the codes of
  * its rows in front of the new ones move to it (rounded again only where they leave e4m3's normal numbers; NaN stays NaN).  Rows behind the new ones keep their bytes.

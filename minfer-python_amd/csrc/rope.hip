@@ -532,12 +532,24 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_append_kernel(const No
 // ------------------------------------------------------------------------------------------------
 // The producer into 8-bit pages (csrc/attn_paged.h).  A page's scale needs the largest of all its new rows, so a workgroup takes one page that
 // the call writes to, for HPW KV heads: D/8 lanes hold one row of one (head, tensor), 16 rows one after the other in registers, and
-// the groups of lanes that the heads leave over share the rows out (`parts`).  k is rotated as it is loaded; then the largest
-// magnitude, the scale, the codes.  Pages with more rows than parts * 16 go through their rows twice.  One workgroup reads, moves and writes
+// the groups of lanes that the heads leave over share the rows out (`parts`).  k is rotated as it is loaded, the NeoX partner from the lane that holds it; then the largest
+// magnitude, the scale, the codes.  The rotation is exact to its rounding to the 16-bit type (angles in 64 bits, kept as fp32 and a rest): with angles and sums in fp32
+// a few values in a million end in the code beside theirs, a sixteenth off, which no later step is as coarse as (25.1 us then, 26.4 now).  Pages with more rows than parts * 16 go through their rows twice.  One workgroup reads, moves and writes
 // all of a (page, head)'s rows and its scale, so nothing depends on an order.  The launch's further workgroups rotate q, a token each.
-// Bound by memory, few tokens by the chain of loads: 3398 tokens of 64 heads on 8 of 128 25 us, 5.3 TB/s; 40 of 32 on 8 7.6 us.
+// Bound by memory, few tokens by the chain of loads: 3398 tokens of 64 heads on 8 of 128 26 us, 5.0 TB/s with three waves to a
+// SIMD (with two 30.6); 40 of 32 on 8 7.6 us.
 // ------------------------------------------------------------------------------------------------
 constexpr int kAppendRows = 16;   // rows a group of lanes holds
+
+// The cosine and sine of pos * inv_freq in 64 bits: a quarter turn about zero, by its series, whose first terms left out are below 1e-11.
+MA_DEV void angle64(double inv_freq, int pos, double& c, double& s) {
+    const double quarters = (double)pos * inv_freq * 0.6366197723675814, q = rint(quarters), a = (quarters - q) * 1.5707963267948966, b = a * a;
+    const double si = a * fma(b, fma(b, fma(b, fma(b, fma(b, -1.0 / 39916800, 1.0 / 362880), -1.0 / 5040), 1.0 / 120), -1.0 / 6), 1.0);
+    const double co = fma(b, fma(b, fma(b, fma(b, fma(b, fma(b, 1.0 / 479001600, -1.0 / 3628800), 1.0 / 40320), -1.0 / 720), 1.0 / 24), -1.0 / 2), 1.0);
+    const int k = (int)(int64_t)q & 3;
+    c = k == 0 ? co : k == 1 ? -si : k == 2 ? -co : si;
+    s = k == 0 ? si : k == 1 ? co : k == 2 ? -si : -co;
+}
 
 struct Append8Params {
     RopeParams r;
@@ -571,11 +583,11 @@ MA_DEV uint32_t move4(uint32_t codes, float factor) {
 }
 
 template <class T, int STYLE, int D>
-__global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Params ap) {
+__global__ __launch_bounds__(kRopeThreads, 3) void append8_kernel(const Append8Params ap) {
     const RopeParams& p = ap.r;
     const PagedCache& pc = p.pages;
     constexpr int GL = D / 8, NG = kRopeThreads / GL;   // lanes per row, groups of lanes
-    extern __shared__ f32x2 tab[];                       // [rows of a round][rd/2]: cosine and sine
+    extern __shared__ f32x2 tab[];                       // [rows of a round][rd/2]: cosine and sine, and behind all of them, as pairs of bf16, what fp32 leaves of each
     __shared__ float most[NG];
     const int tid = threadIdx.x, lane = tid & 63;
     const int half_rd = p.rd >> 1;
@@ -678,7 +690,7 @@ __global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Para
     const bool hi_half = STYLE == ROPE_NEOX && c >= rot_chunks;              // holds the second elements of its pairs
     const bool rotates = !is_v && (STYLE == ROPE_IL ? c < rot_chunks : c < 2 * rot_chunks);
     const int pair0 = STYLE == ROPE_IL ? 4 * c : 8 * (hi_half ? c - rot_chunks : c);
-    const int partner = hi_half ? -half_rd : half_rd;                        // NeoX: where the other elements of the pairs are
+    const int partner = 4 * (lane + (hi_half ? -rot_chunks : rot_chunks));   // NeoX: address of the lane that holds the other elements of the pairs
     const int64_t tok0 = first_tok + (row_lo - pos0);
     const short* src = (const short*)(is_v ? p.v : p.k) + (tok0 * p.Hkv + (on ? head : 0)) * D + 8 * c;
     char* rows = (char*)(is_v ? pc.v : pc.k) + (int64_t)id * pc.page_stride + (int64_t)(on ? head : 0) * pc.head_stride + 8 * c;
@@ -686,6 +698,17 @@ __global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Para
     const int e_held = n_old > 0 ? (int)*scale_at - 127 : -128;              // a page's first rows ask nobody
 
     const int per_round = kAppendRows * parts, rounds = (n_rows + per_round - 1) / per_round;
+    uint32_t* const rest = reinterpret_cast<uint32_t*>(tab + min(per_round, S) * half_rd);
+    // cosine and sine of entry i, and mine * cosine + other * sine, rounded once
+    struct Angle { double c, s; };
+    auto angle = [&](int i) __attribute__((always_inline)) {
+        const f32x2 hi = tab[i];
+        const uint32_t lo = rest[i];
+        return Angle{(double)hi[0] + (double)BF16::to_float((short)(lo & 0xffffu)), (double)hi[1] + (double)BF16::to_float((short)(lo >> 16))};
+    };
+    auto turned = [&](double c, double s, short mine, short other) __attribute__((always_inline)) {
+        return (float)fma(c, (double)T::to_float(mine), s * (double)T::to_float(other));
+    };
     s16x8 xs[kAppendRows];
     // rows part, part + parts, .. of a round, rotated; those past the last row are zero
     auto load_round = [&](int round) __attribute__((always_inline)) {
@@ -693,7 +716,10 @@ __global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Para
         __syncthreads();   // the table of the round before has been read
         for (int i = tid; i < min(per_round, n_rows - r0) * half_rd; i += kRopeThreads) {
             const int row = i / half_rd, pair = i - row * half_rd;
-            tab[i] = table_entry(p.inv_freq[pair], row_lo + r0 + row);
+            double co, si;
+            angle64(p.inv_freq[pair], row_lo + r0 + row, co, si);
+            tab[i] = f32x2{(float)co, (float)si};
+            rest[i] = BF16::pack2((float)(co - (double)(float)co), (float)(si - (double)(float)si));
         }
 #pragma unroll
         for (int i = 0; i < kAppendRows; ++i) {
@@ -707,57 +733,70 @@ __global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Para
             for (int i = 0; i < kAppendRows; ++i) {
                 const int row = part + i * parts;
                 if (r0 + row >= n_rows) continue;
-                const f32x2* cs = tab + row * half_rd + pair0;
+                int at = row * half_rd + pair0;
+                asm volatile("" : "+v"(at));   // (rows one after the other: their angles all at once do not leave registers for three waves)
                 uint32_t r[4];
                 if (STYLE == ROPE_IL) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) r[j] = rotate_pair<T>(cs[j][0], cs[j][1], xs[i][2 * j], xs[i][2 * j + 1]);
+                    for (int j = 0; j < 4; ++j) {
+                        const Angle t = angle(at + j);
+                        r[j] = T::pack2(turned(t.c, -t.s, xs[i][2 * j], xs[i][2 * j + 1]), turned(t.c, t.s, xs[i][2 * j + 1], xs[i][2 * j]));
+                    }
                 } else {
-                    const s16x8 o = *reinterpret_cast<const s16x8*>(src + (int64_t)(r0 + row) * p.Hkv * D + partner);
+                    const u32x4 mine = __builtin_bit_cast(u32x4, xs[i]);
+                    u32x4 theirs;   // the other elements of the pairs, from the lane that holds them
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) theirs[j] = (uint32_t)__builtin_amdgcn_ds_bpermute(partner, (int)mine[j]);
+                    const s16x8 o = __builtin_bit_cast(s16x8, theirs);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float s0 = cs[2 * j][1], s1 = cs[2 * j + 1][1];
-                        r[j] = T::pack2(rotate_one<T>(cs[2 * j][0], hi_half ? s0 : -s0, xs[i][2 * j], o[2 * j]),
-                                        rotate_one<T>(cs[2 * j + 1][0], hi_half ? s1 : -s1, xs[i][2 * j + 1], o[2 * j + 1]));
+                        const Angle t0 = angle(at + 2 * j), t1 = angle(at + 2 * j + 1);
+                        r[j] = T::pack2(turned(t0.c, hi_half ? t0.s : -t0.s, xs[i][2 * j], o[2 * j]), turned(t1.c, hi_half ? t1.s : -t1.s, xs[i][2 * j + 1], o[2 * j + 1]));
                     }
                 }
                 xs[i] = __builtin_bit_cast(s16x8, u32x4{r[0], r[1], r[2], r[3]});
             }
         }
     };
-    float amax = 0.f;
-    for (int round = 0; round < rounds; ++round) {
+    // the rounds for their largest value, and, the last one's rows being there still, again the others
+    float amax = 0.f, down = 0.f;
+#pragma unroll 1
+    for (int step = 0; step < 2 * rounds - 1; ++step) {
+        const int round = step < rounds ? step : step - rounds;
         load_round(round);
+        if (step < rounds) {
 #pragma unroll
-        for (int i = 0; i < kAppendRows; ++i)
+            for (int i = 0; i < kAppendRows; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float f = __builtin_fabsf(T::to_float(xs[i][j]));
-                amax = f < INFINITY ? fmaxf(amax, f) : amax;
-            }
-    }
-    // over the lanes of the row, then over the parts
-    amax = fmaxf(amax, row_exchange<0xb1>(amax));
-    amax = fmaxf(amax, row_exchange<0x4e>(amax));
-    amax = fmaxf(amax, row_exchange<0x141>(amax));
-    if (GL > 8) amax = fmaxf(amax, row_exchange<0x140>(amax));
-    if (c == 0) most[gi] = amax;
-    __syncthreads();
-    for (int i = 0; i < parts; ++i) amax = fmaxf(amax, most[i * units + unit]);
-    const int e = max(e_held, scale_exponent(amax, ap.max_e));
-    if (on && part == 0 && c == 0) *scale_at = (uint8_t)(e + 127);
-    if (on && n_old > 0 && e > e_held) {
-        const float factor = power_of_two(e_held - e);
-        for (int row = part; row < n_old; row += parts) {
-            uint2* at = reinterpret_cast<uint2*>(rows + row * (int)pc.row_stride);
-            uint2 codes = *at;
-            codes.x = move4(codes.x, factor);
-            codes.y = move4(codes.y, factor);
-            *at = codes;
+                for (int j = 0; j < 8; ++j) {
+                    const float f = __builtin_fabsf(T::to_float(xs[i][j]));
+                    amax = f < INFINITY ? fmaxf(amax, f) : amax;
+                }
         }
-    }
-    const float down = e == 128 ? __builtin_nanf("") : power_of_two(-e);
-    auto store_round = [&](int round) __attribute__((always_inline)) {
+        if (step < rounds - 1) continue;
+        if (step == rounds - 1) {
+            // over the lanes of the row, then over the parts
+            amax = fmaxf(amax, row_exchange<0xb1>(amax));
+            amax = fmaxf(amax, row_exchange<0x4e>(amax));
+            amax = fmaxf(amax, row_exchange<0x141>(amax));
+            if (GL > 8) amax = fmaxf(amax, row_exchange<0x140>(amax));
+            if (c == 0) most[gi] = amax;
+            __syncthreads();
+            for (int i = 0; i < parts; ++i) amax = fmaxf(amax, most[i * units + unit]);
+            const int e = max(e_held, scale_exponent(amax, ap.max_e));
+            if (on && part == 0 && c == 0) *scale_at = (uint8_t)(e + 127);
+            if (on && n_old > 0 && e > e_held) {
+                const float factor = power_of_two(e_held - e);
+                for (int row = part; row < n_old; row += parts) {
+                    uint2* at = reinterpret_cast<uint2*>(rows + row * (int)pc.row_stride);
+                    uint2 codes = *at;
+                    codes.x = move4(codes.x, factor);
+                    codes.y = move4(codes.y, factor);
+                    *at = codes;
+                }
+            }
+            down = e == 128 ? __builtin_nanf("") : power_of_two(-e);
+        }
 #pragma unroll
         for (int i = 0; i < kAppendRows; ++i) {
             const int row = round * per_round + part + i * parts;
@@ -767,11 +806,6 @@ __global__ __launch_bounds__(kRopeThreads) void append8_kernel(const Append8Para
             for (int j = 0; j < 8; ++j) f[j] = T::to_float(xs[i][j]);
             *reinterpret_cast<uint2*>(rows + (n_old + row) * (int)pc.row_stride) = narrow8(f, down);
         }
-    };
-    store_round(rounds - 1);   // the last round's rows are still there
-    for (int round = 0; round + 1 < rounds; ++round) {
-        load_round(round);
-        store_round(round);
     }
 }
 
@@ -998,7 +1032,7 @@ MINFER_ATTN_EXPORT int minfer_rope_kv_append_paged(int dtype, int style, int pag
     const int64_t S = pages->page_size;
     const int64_t items = p.pages.width > 0 ? std::min(T, T / S + 2 * n_seqs) : 0;
     // KV heads per workgroup: all the groups of lanes have a row where pages get few rows; where they get many, fewer heads and more rows
-    // at a time (two heads at least: a round's table of angles is then 32 KiB at most)
+    // at a time (two heads at least: a round's table of angles is then 48 KiB at most)
     const int64_t rows = std::min(S, T / n_seqs + 1);
     const int groups = kRopeThreads / ((int)D / 8);
     int hpw_log2 = 3;
@@ -1010,7 +1044,7 @@ MINFER_ATTN_EXPORT int minfer_rope_kv_append_paged(int dtype, int style, int pag
     const int64_t q_wgs = std::min<int64_t>(T, 256 * 16), grid = items * ap.n_hg + q_wgs;
     if (grid > 0x7fffffffLL) return bad("rope_kv_append_paged: problem too large for one launch");
     const int parts = groups / (2 << hpw_log2);
-    const size_t lds = (size_t)std::max<int64_t>(1, std::min<int64_t>(kAppendRows * parts, S)) * (rotary_dim / 2) * sizeof(f32x2) + sizeof(f32x2);
+    const size_t lds = (size_t)std::max<int64_t>(1, std::min<int64_t>(kAppendRows * parts, S)) * (rotary_dim / 2) * (sizeof(f32x2) + sizeof(uint32_t)) + sizeof(f32x2);
 #define MINFER_APPEND8(T_, STYLE_) \
     if (D == 128) hipLaunchKernelGGL((append8_kernel<T_, STYLE_, 128>), dim3((unsigned)grid), dim3(kRopeThreads), lds, stream, ap); \
     else hipLaunchKernelGGL((append8_kernel<T_, STYLE_, 64>), dim3((unsigned)grid), dim3(kRopeThreads), lds, stream, ap)

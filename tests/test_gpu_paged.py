@@ -520,11 +520,13 @@ def same_codes(a, b):
 @pytest.mark.parametrize("style,rd,D,page,order,Hkv", [(0, 128, 128, 16, "heads", 8), (1, 128, 128, 32, "rows", 3), (1, 64, 64, 16, "heads", 1), (0, 64, 128, 64, "rows", 2),
                                                        (1, 32, 64, 256, "heads", 5), (1, 64, 128, 128, "heads", 8)])
 def test_append_e4m3(kerns, batch, dtype, style, rd, D, page, order, Hkv):
-    """Codes and scales from the definition, given the 16-bit rows that rope_kv_append makes; every other byte stays."""
+    """Codes and scales from the definition, the rotated k rounded from 64 bits to the 16-bit type; every other byte stays.  q as
+    rope_kv_append makes it."""
     c = ref.Paged([(n, p % 3000) for n, p in APPENDS[batch]], page, Hkv, D, dtype, DEV, order=order, held_only=True, eight=True)
     q = make_q(c.T, 2 * Hkv, D, dtype)
     k, v = make_kv(c.T, Hkv, D, dtype)
-    want_q, rows_k, rows_v = slab_append(kerns, c, style, rd, q, k, v)
+    want_q, _, rows_v = slab_append(kerns, c, style, rd, q, k, v)
+    rows_k = torch.cat([ref.rotated(k[0, c.cu_list[s]:c.cu_list[s] + n].double().cpu(), past, style, rd, BASE).to(dtype) for s, (n, past) in enumerate(c.seqs)])
     max_e = 7 if dtype == torch.float16 else 119
     want = [expected_e4m3(c, r.double().cpu(), pool, sc, max_e) for r, pool, sc in ((rows_k, c.k_pages, c.k_scales), (rows_v, c.v_pages, c.v_scales))]
     kerns.rope_kv_append_paged_fp8(style, rd, BASE, q, k, v, c.cu, c.past, c.table, c.k_pages, c.v_pages, c.k_scales, c.v_scales)
