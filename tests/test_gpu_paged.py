@@ -358,6 +358,15 @@ def test_attend_tokens_of_no_sequence(kerns, n):
 
 
 @pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 5, 11], ids=["decode", "drafts", "chunks"])
+def test_attend_hundreds_of_sequences(kerns, n, eight):
+    """More sequences than are looked up at a time, some of them without tokens or without rows held."""
+    seqs = [((i * 7) % (n + 1), (37 * i) % 90) for i in range(700)]
+    c = ref.Paged(seqs, 16, 1, 64, torch.float16, DEV, eight=eight)
+    check_attend(kerns, c, 2, max_q=n)
+
+
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "e4m3"])
 def test_attend_pieces_of_two_rounds(kerns, eight):
     """A little more blocks than the chip holds at once: 73 of 128 rows, or 37 of 256, for each of eight KV heads."""
     c = ref.Paged([(2300, 0), (10, 1500)], 16, 8, 128, torch.bfloat16, DEV, eight=eight)
