@@ -208,8 +208,11 @@ typedef struct minfer_kv_pages {
 /*
  * minfer_rope_kv_append into a paged cache, for packed tokens: q [T,Hq,D] is rotated in place; token cu_seqlens[s] + i stands at
  * position positions[s] + i of sequence s, and its rotated k and its v [T,Hkv,D] go to that row of the sequence's pages.  cu_seqlens
- * int32 [n_seqs + 1] and positions int32 [n_seqs] are on the device; sequences are cut to their part inside [0, T), tokens that
- * belong to none are left alone, and rows whose position is negative or whose page is not there are not written (q is still rotated).
+ * int32 [n_seqs + 1] and positions int32 [n_seqs] are on the device and not trusted; tokens that
+ * belong to no sequence are left alone, and rows whose position is negative or whose page is not there are not written (q is still rotated).
+ * Sequence s is the tokens cu_seqlens[s] .. cu_seqlens[s+1]-1 that lie in [0, T), none where the second is not larger; what is cut off moves no
+ * other token.  (So entries of zero, or of T or more, behind the last sequence are sequences without tokens.)  Where sequences
+ * overlap it is not defined which of them has a token.
  * page_type is the activations' dtype, and the rows are those that minfer_rope_kv_append would write, or MINFER_FP8_E4M3.
  *
  * 8-bit pages: k, rotated in 64 bits and rounded to the activations' type, and v are rounded to e4m3 (to nearest, ties to even) after division by
@@ -239,7 +242,8 @@ size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs, int64_t T, int64_
  * token a sequence is a decode step, a few are drafts, many a chunk of a prompt or all of it; sequences of a call may differ.  A token without rows
  * (a negative position, no page there) yields zeros.  max_q_len: an upper bound of the sequences' numbers of tokens (0 = not known); it
  * sizes the launch, and tokens of a sequence past it are not computed.  cu_seqlens int32 [n_seqs + 1] and ctx_lens int32 [n_seqs] are
- * read on the device only and not trusted: sequences are cut to their part inside [0, T), contexts to 0 .. pages_per_seq * page_size.
+ * read on the device only and not trusted: a sequence is its tokens inside [0, T), as in minfer_rope_kv_append_paged (n counts those cut off, too, which have
+ * rows; max_q_len does not), contexts are cut to 0 .. pages_per_seq * page_size.
  * out is written for the tokens of the sequences only.  The order of the sums depends on the sizes given here and the device data, not on timing: a call
  * repeated on the same stream gives the same bits.  Rows that nothing was written to may hold anything.
  * Over 8-bit pages the result is that over the 16-bit rows code * scale, as far as dtype holds them.

@@ -40,13 +40,16 @@ MA_DEV uint32_t const_byte(const uint8_t* p) {
     return (const_load((const uint32_t*)(at & ~(uintptr_t)3)) >> (8 * (at & 3))) & 255u;
 }
 
-// The two numbers that say where a sequence's tokens of this call are, whatever cu_seqlens holds: a start in [0, T] and a length that
-// stays inside.
-struct TokenRange { int lo, len; };
+// Where a sequence's tokens of this call are, whatever cu_seqlens holds: those of lo .. hi - 1 that lie in [0, T), a start and a length.  What is
+// cut off moves no other token: the first one's position is (lo cut) - lo further on, the last one's `behind` in front of the context's end.
+struct TokenRange { int lo, len, behind; };
 MA_DEV TokenRange token_range(int lo, int hi, int T) {
     lo = min(max(lo, 0), T);
-    return TokenRange{lo, min(max(hi, lo), T) - lo};
+    return TokenRange{lo, min(max(hi, lo), T) - lo, max(hi, T) - T};
 }
+
+// Rows of a sequence up to its last token that is there: ctx_lens' entry, cut to the table, without the rows of tokens behind T.
+MA_DEV int context_of(const PagedCache& c, int ctx, const TokenRange& t) { return max(min(max(ctx, 0), c.width << c.page_log2) - t.behind, 0); }
 
 // 2^(bits - 127) for a scale's byte; 255 is no number.  (2^-127 is a subnormal fp32.)
 MA_DEV float scale_value(uint32_t bits) {

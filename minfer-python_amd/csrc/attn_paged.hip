@@ -73,7 +73,7 @@ template <int BR> MA_DEV Piece find_piece(const PagedParams& p, int x, int& all)
     if (p.round == 0) {   // whole blocks, of any number of sequences
         all = 0;
         for (int base = 0; base < p.n_seqs; base += 64) {
-            TokenRange t{0, 0};
+            TokenRange t{0, 0, 0};
             if (base + lane < p.n_seqs) t = token_range(p.cu[base + lane], p.cu[base + lane + 1], p.T);
             const int n = (min(t.len, p.max_q) * p.n_rep + BR - 1) / BR;
             const int incl = wave_inclusive_scan(n), total = lane_value(incl, 63);
@@ -90,7 +90,7 @@ template <int BR> MA_DEV Piece find_piece(const PagedParams& p, int x, int& all)
     int n = 0, tiles = 0;   // the lane's sequence: blocks, tiles of the last one
     if (lane < p.n_seqs) {
         const TokenRange t = token_range(p.cu[lane], p.cu[lane + 1], p.T);
-        const int ctx = min(max(p.ctx[lane], 0), p.c.width << p.c.page_log2), rows = min(t.len, p.max_q) * p.n_rep;
+        const int ctx = context_of(p.c, p.ctx[lane], t), rows = min(t.len, p.max_q) * p.n_rep;
         n = (rows + BR - 1) / BR;
         tiles = n > 0 ? max(tiles_of(ctx - t.len, rows, p.n_rep, n - 1, BR), 1) : 0;
         // (a window that moved on: half of the pages, a guess, which only the number of pieces goes by)
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     if (p.round > 0 && g == 0 && threadIdx.x == 0) reinterpret_cast<int4*>(p.table)[1 + rank] = make_int4(me.seq, me.block, me.part, me.parts);
     const TokenRange range = token_range(const_load(p.cu + seq), const_load(p.cu + seq + 1), p.T);
     const int seq_lo = range.lo, seq_len = range.len;
-    const int ctx = min(max(const_load(p.ctx + seq), 0), p.c.width << p.c.page_log2);
+    const int ctx = context_of(p.c, const_load(p.ctx + seq), range);
     const int pos0 = ctx - seq_len;                                      // position of the sequence's token 0
     const int rows = min(seq_len, p.max_q) * p.n_rep, last_row = rows - 1;
     const int row0 = block * BR + w * 32;                                // the wave's first row

@@ -46,10 +46,10 @@ struct DecodeWork {
 template <bool FP8> constexpr int kRows = FP8 ? 32 : 16;   // rows of a group
 
 // What a wave has to know about a sequence.
-struct SeqInfo { int lo, len, ctx; };   // first token, tokens that are computed against .. and the rows they have
+struct SeqInfo { int lo, len, ctx; };   // its first token, its number of tokens, the rows up to its last token
 MA_DEV SeqInfo seq_info(const PagedParams& p, int s) {
     const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
-    return SeqInfo{r.lo, r.len, min(max(const_load(p.ctx + s), 0), p.c.width << p.c.page_log2)};
+    return SeqInfo{r.lo, r.len, context_of(p.c, const_load(p.ctx + s), r)};
 }
 
 template <int D> struct ColumnAcc {
@@ -365,7 +365,7 @@ template <int GR> MA_DEV LineSeq line_seq(const DecodeWork& w, int s) {   // (pe
     LineSeq r{{0, 0, 0}, 0};
     if (s < p.n_seqs) {
         const TokenRange t = token_range(p.cu[s], p.cu[s + 1], p.T);
-        r.info = SeqInfo{t.lo, t.len, min(max(p.ctx[s], 0), p.c.width << p.c.page_log2)};
+        r.info = SeqInfo{t.lo, t.len, context_of(p.c, p.ctx[s], t)};
         r.groups = t.len > 0 ? (r.info.ctx + GR - 1) / GR : 0;
     }
     return r;

@@ -84,17 +84,17 @@ MA_DEV f32x2 table_entry(double inv_freq, int pos) {
     return f32x2{c, s};
 }
 
-// The sequence that packed token `tok` belongs to and its first token, or seq = -1; the same for all lanes of the wave.  The last start that
-// is not behind the token, 64 candidates at a time (up to 64 sequences one load, up to 4096 two); whatever cu_seqlens holds, the result is a
-// sequence that contains the token or none.
+// The sequence s that packed token `tok` belongs to, cu[s] <= tok < cu[s + 1], and cu[s], or seq = -1; the same for all lanes of the wave.  Looked for
+// as the last start that is not behind the token, 64 candidates at a time (up to 64 sequences one load, up to 4096 two).  Where that is none
+// that contains it, the token belongs to nobody or the starts do not ascend (zeros behind the last sequence): then one after the other.
 struct TokenOwner { int seq, first; };
 MA_DEV TokenOwner owner_of(const int32_t* cu, int n_seqs, int tok) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, n = n_seqs;
-    while (n > 0) {
+    int lo = 0;
+    for (int n = n_seqs; n > 0;) {
         const int step = (n + 63) >> 6, i = lane * step;
         const uint64_t hit = __ballot(i < n && cu[lo + min(i, n - 1)] <= tok);
-        if (hit == 0) return TokenOwner{-1, 0};
+        if (hit == 0) break;
         const int at = __builtin_amdgcn_readfirstlane(63 - __clzll((long long)hit)) * step;
         lo += at;
         if (step == 1) break;
@@ -102,7 +102,29 @@ MA_DEV TokenOwner owner_of(const int32_t* cu, int n_seqs, int tok) {
     }
     if (n_seqs <= 0) return TokenOwner{-1, 0};
     const int first = const_load(cu + lo), end = const_load(cu + lo + 1);
-    return first <= tok && tok < end && first >= 0 ? TokenOwner{lo, first} : TokenOwner{-1, 0};
+    if (first <= tok && tok < end) return TokenOwner{lo, first};
+    constexpr int UN = 4;   // 256 sequences requested together
+#pragma unroll 1
+    for (int base = 0; base < n_seqs; base += 64 * UN) {
+        bool here[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int s = min(base + 64 * u + lane, n_seqs - 1);
+            here[u] = cu[s] <= tok && tok < cu[s + 1];
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const uint64_t hit = __ballot(here[u]);
+            if (hit == 0) continue;
+            const int s = min(base + 64 * u + __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)hit)) - 1, n_seqs - 1);
+            return TokenOwner{s, const_load(cu + s)};
+        }
+    }
+    return TokenOwner{-1, 0};
+}
+// Its position, whatever the two say.
+MA_DEV int64_t position_of(const int32_t* positions, const TokenOwner& o, int tok) {
+    return (int64_t)const_load(positions + max(o.seq, 0)) + ((int64_t)tok - o.first);
 }
 
 // Per token: every thread requests the 16-byte chunks it owns (a few in flight), the first rd/2 threads
@@ -153,10 +175,10 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
         const TokenOwner o = owner_of(p.cu, p.n_seqs, tok);
         k.owned = o.seq >= 0;
         const int s = max(o.seq, 0);
-        k.pos = (int)((uint32_t)const_load(p.positions + s) + (uint32_t)(tok - o.first));
-        const int at = k.pos >> p.pages.page_log2;
+        const int64_t pos = position_of(p.positions, o, tok), at = pos >> p.pages.page_log2;
+        k.pos = (int)pos;
         int id = -1;
-        if (k.owned && k.pos >= 0 && at < p.pages.width) id = const_load(p.pages.table + (int64_t)s * p.pages.table_stride + at);
+        if (k.owned && pos >= 0 && at < p.pages.width) id = const_load(p.pages.table + (int64_t)s * p.pages.table_stride + at);
         k.row_ok = (unsigned)id < (unsigned)p.pages.n_pages;
         const int64_t row = (int64_t)id * p.pages.page_stride + (int64_t)(k.pos & ((1 << p.pages.page_log2) - 1)) * p.pages.row_stride;
         k.ck = (short*)p.pages.k + row;
@@ -599,7 +621,7 @@ __global__ __launch_bounds__(kRopeThreads, 3) void append8_kernel(const Append8P
         for (int tok = (int)blockIdx.x - ap.items * ap.n_hg; tok < p.L; tok += q_wgs) {
             const TokenOwner o = owner_of(p.cu, p.n_seqs, tok);
             if (o.seq >= 0) {
-                const int pos = (int)((uint32_t)const_load(p.positions + o.seq) + (uint32_t)(tok - o.first));
+                const int pos = (int)position_of(p.positions, o, tok);
                 if (tid < half_rd) tab[tid] = table_entry(p.inv_freq[tid], pos);
             }
             __syncthreads();
@@ -647,11 +669,12 @@ __global__ __launch_bounds__(kRopeThreads, 3) void append8_kernel(const Append8P
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const int s = base + 64 * u + lane;
-            r[u] = TokenRange{0, 0};
+            r[u] = TokenRange{0, 0, 0};
             at[u] = 0;
             if (s < p.n_seqs) {
-                r[u] = token_range(p.cu[s], p.cu[s + 1], p.L);
-                at[u] = p.positions[s];
+                const int start = p.cu[s];
+                r[u] = token_range(start, p.cu[s + 1], p.L);
+                at[u] = (int)min(max((int64_t)p.positions[s] + ((int64_t)r[u].lo - start), (int64_t)INT32_MIN), (int64_t)INT32_MAX);   // of the first token that is there
             }
         }
 #pragma unroll

@@ -236,7 +236,9 @@ def rope_kv_append_paged(
     k [1,T,n_kv_heads,D] and v into k_pages/v_pages [n_pages,n_kv_heads,page_size,D].  Tokens cu_seqlens[s] ..
     cu_seqlens[s+1]-1 are sequence s's rows positions[s], positions[s]+1, ..; row r lies in page block_table[s, r // page_size]
     at row r % page_size.  All index tensors int32 (cu_seqlens [n_seqs+1], positions [n_seqs], block_table [n_seqs, pages]).
-    A table entry outside the pool (-1) means no page: its rows are not written.  page_size is a power of two in 16..1024."""
+    A table entry outside the pool (-1) means no page: its rows are not written.  page_size is a power of two in 16..1024.
+    Sequences that end at or in front of their start have no tokens (so cu_seqlens may end in zeros or in T), and what lies
+    outside [0, T) is cut off without moving the other tokens; they must not overlap."""
     return torch.ops.minfer.rope_kv_append_paged.default(style, rotary_dim, freq_base, q, k, v, cu_seqlens, positions,
                                                          block_table, k_pages, v_pages)
 
