@@ -402,11 +402,12 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
     const int quota = max(max((total + n_waves - 1) / n_waves, kLeastShare / GR), longest / (p.slots - 3) + 1);
     if (first && lane == 0) { work.seq_off[p.n_seqs] = total; work.seq_off[p.n_seqs + 1] = quota; }
     // shares to the waves of a workgroup in turn; where there are no more shares than workgroups, one to each
-    const int n_shares = (total + quota - 1) / quota;
+    // (the line's length and a share of it may together pass 31 bits)
+    const int n_shares = total > 0 ? (total - 1) / quota + 1 : 0;
     const int wave = n_shares <= (int)gridDim.x ? w * (int)gridDim.x + (int)blockIdx.x : (int)blockIdx.x * kLineWaves + w;
     if (wave >= n_shares) return;
     int x = wave * quota;
-    const int x_end = min(total, x + quota);
+    const int x_end = x + min(quota, total - x);
     // the sequence that holds position x
     int s = 0, off = 0, groups = 0;
     for (int base = 0, start = 0; base < p.n_seqs; base += 64) {
