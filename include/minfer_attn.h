@@ -231,7 +231,7 @@ int minfer_rope_kv_append_paged(int dtype, int style, int page_type, void* q, co
                                 int64_t rotary_dim, double freq_base, void* stream);
 
 /* Bytes of workspace for minfer_flash_attn_paged (partial results of a sequence's rows that are split); max_context is
- * pages_per_seq * page_size. */
+ * pages_per_seq * page_size.  For launches on the device that is current. */
 size_t minfer_flash_attn_paged_workspace_bytes(int64_t n_seqs, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                                int64_t max_context, int64_t max_q_len);
 

@@ -165,12 +165,11 @@ struct PagedParams {
     PagedCache c;
     const void* q; void* out;
     const int32_t* cu; const int32_t* ctx;
-    float* part_o;     // partial results, un-normalised: decode [row][slot][D], tiles [piece][KV head][row of the block][D] ...
+    float* part_o;     // partial results, un-normalised: decode [part][column][D], tiles [piece][KV head][row of the block][D] ...
     float* part_ml;    // ... with their reference (log2 units) and sum
     int64_t q1, q2, o1, o2;
     int n_seqs, T, Hq, Hkv, n_rep;
     int max_q;         // tokens of a sequence past this many are not computed
-    int slots;         // decode: partial results a row can have
     int round;         // tiles: workgroups per KV head that the chip holds at once, which blocks of rows are cut up to fill; 0: none is cut
     int32_t* table;    // tiles: the number of pieces, and from the fourth entry on (sequence, block, part, parts) of each
     float scale_log2, inv_scale_log2;  // softmax scale * log2(e), and one over it

@@ -32,13 +32,14 @@ constexpr int kChunkWaves = 8;
 // Least rows of a wave's share of the line (us, 128 / 64 / 32: 64 sequences of 6 to 100 21.8 / 14.9 / 12.9, of 100 15.8 / 14.1 / 15.9, of codes 15.9 / 14.5 /
 // 12.1; one of 4000 15.1 / 14.7 / 14.8; 64 of up to 2000 on one KV head 16.0 / 16.5 / 19.4; where every wave has more nothing changes).
 constexpr int kLeastShare = 64;
-constexpr int kMaxSlots = 64;          // partial results a row can have: a wave merges them, one to a lane
+constexpr int kMaxParts = 64;          // partial results a column can have: a wave merges them, one to a lane
 
 struct DecodeWork {
     PagedParams p;
     int32_t* seq_off;   // line: [n_seqs + 2] start of every sequence on the line, its length, the quota; written by workgroup 0
     int n_col;          // columns per KV head: max_q * n_rep
     int n_hg;           // groups of <= 16 columns per KV head
+    int per_part;       // columns of a partial result: those of a group
     int n_wg;           // line: workgroups
     uint32_t* done;     // chunks: zeroed counters, one per pair, left zero; or null
 };
@@ -343,13 +344,16 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
     acc.l = sum_across_quads(l_sum);
 }
 
-MA_DEV int64_t part_row(const DecodeWork& w, int s, int g, int col) { return ((int64_t)s * w.p.Hkv + g) * w.n_col + col; }
+// Where column c of a column group's partial result `part` lies.  Partial results are numbered through the launch, those of a (sequence, KV head,
+// column group) one after the other: there is room for as many as there can be of all of them together, not for the most that each could have
+// (which for 256 sequences of 64 heads was 0.5 GiB, now 16 MiB; 4096 of 32 4 GiB, now 69 MiB).
+MA_DEV int64_t part_row(const DecodeWork& w, int64_t part, int c) { return part * w.per_part + c; }
 
 // A wave's partial result of every column, into the workspace.
-template <int D> MA_DEV void store_part(const DecodeWork& w, int s, int g, int hg, int slot, const ColumnAcc<D>& acc) {
-    const int lane = threadIdx.x & 63, col = hg * 16 + (lane & 15), quad = lane >> 4;
-    if (col >= w.n_col) return;
-    const int64_t at = part_row(w, s, g, col) * w.p.slots + slot;
+template <int D> MA_DEV void store_part(const DecodeWork& w, int hg, int64_t part, const ColumnAcc<D>& acc) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    if (hg * 16 + l16 >= w.n_col) return;
+    const int64_t at = part_row(w, part, l16);
     float* dst = w.p.part_o + at * D + 4 * quad;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc.o[db];
@@ -358,7 +362,8 @@ template <int D> MA_DEV void store_part(const DecodeWork& w, int s, int g, int h
 
 // ---- the line ------------------------------------------------------------------------------------------------------
 // Lengths in groups: every sequence's (zero without tokens) times its pairs, one after the other.  The quota: an equal share for
-// every wave, kLeastShare rows at least, and as much as leaves no pair with more partial results than there are slots.
+// every wave, kLeastShare rows at least, and as much as leaves no pair with more partial results than a merge takes.  Along the line either the share's
+// number or the pair's, or both, go up by one from one partial result to the next: their sum numbers the partial results.
 struct LineSeq { SeqInfo info; int groups; };
 template <int GR> MA_DEV LineSeq line_seq(const DecodeWork& w, int s) {   // (per lane)
     const PagedParams& p = w.p;
@@ -398,8 +403,8 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
             longest = max(longest, q[u].groups);
         }
     }
-    longest = (int)wave_max((float)longest);   // (below 2^24 exactly, and above rounded up or down by less than the slots to spare)
-    const int quota = max(max((total + n_waves - 1) / n_waves, kLeastShare / GR), longest / (p.slots - 3) + 1);
+    longest = (int)wave_max((float)longest);   // (below 2^24 exactly, and above rounded up or down by less than the parts to spare)
+    const int quota = max(max((total + n_waves - 1) / n_waves, kLeastShare / GR), longest / (kMaxParts - 3) + 1);
     if (first && lane == 0) { work.seq_off[p.n_seqs] = total; work.seq_off[p.n_seqs + 1] = quota; }
     // shares to the waves of a workgroup in turn; where there are no more shares than workgroups, one to each
     // (the line's length and a share of it may together pass 31 bits)
@@ -432,11 +437,10 @@ __global__ __launch_bounds__(kLineWaves * 64, 2) void paged_line_kernel(const De
             } while (groups == 0);
         }
         const int y = x - off, pair = y / groups, g0 = y - pair * groups, g1 = min(groups, g0 + (x_end - x));
-        const int slot = wave - (off + pair * groups) / quota;
         const int hg = work.n_hg == 1 ? 0 : pair / p.Hkv, g = pair - hg * p.Hkv;
         ColumnAcc<D> acc;
         stream_pages<T, D, FP8>(work, s, info, g, hg, g0, g1, lds[w], acc);
-        store_part<D>(work, s, g, hg, slot, acc);
+        store_part<D>(work, hg, (int64_t)s * pairs + pair + wave, acc);
         x += g1 - g0;
     }
 }
@@ -463,27 +467,31 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const DecodeWork work)
     const int per_seq = p.Hkv * work.n_col;
     if (row >= (int64_t)p.n_seqs * per_seq) return;
     const int s = (int)(row / per_seq), in = (int)(row - (int64_t)s * per_seq), g = in / work.n_col, col = in - g * work.n_col;
-    const float* src = p.part_o + row * p.slots * D + EPL * lane;
-    auto load_o = [&](int slot, float (&x)[EPL]) __attribute__((always_inline)) {
-        const float* at = src + (int64_t)slot * D;
-        if (EPL == 2) { const f32x2 v = *reinterpret_cast<const f32x2*>(at); x[0] = v[0]; x[EPL - 1] = v[1]; }
-        else x[0] = at[0];
-    };
-    // requested before the number of parts is known (what is past it is discarded)
-    const int sl = min(lane, p.slots - 1);
-    const float m_raw = p.part_ml[(row * p.slots + sl) * 2], l_raw = p.part_ml[(row * p.slots + sl) * 2 + 1];
-    constexpr int kEarly = 4;
-    float x[8][EPL];
-#pragma unroll
-    for (int u = 0; u < kEarly; ++u) load_o(min(u, p.slots - 1), x[u]);
     const SeqInfo info = seq_info(p, s);
     const int tok = col / p.n_rep;
     if (tok >= info.len) return;
-    const int groups = (info.ctx + GR - 1) / GR, quota = const_load(work.seq_off + p.n_seqs + 1);
-    const int start = const_load(work.seq_off + s) + ((col / 16) * p.Hkv + g) * groups;
-    const int ns = groups > 0 ? min((start + groups - 1) / quota - start / quota + 1, p.slots) : 0;
-    const float m = lane < ns ? m_raw : -INFINITY, l = lane < ns ? l_raw : 0.f;
-    const PartWeights pw = part_weights(m, l);
+    const int groups = (info.ctx + GR - 1) / GR, quota = const_load(work.seq_off + p.n_seqs + 1), pair = (col / 16) * p.Hkv + g;
+    const int start = const_load(work.seq_off + s) + pair * groups, first = start / quota;   // the pair's first group and its share
+    const int ns = groups > 0 ? min((start + groups - 1) / quota - first + 1, kMaxParts) : 0;
+    const int64_t at0 = part_row(work, (int64_t)s * p.Hkv * work.n_hg + pair + first, col % 16);
+    const float* src = p.part_o + at0 * D + EPL * lane;
+    auto load_o = [&](int part, float (&x)[EPL]) __attribute__((always_inline)) {
+        const float* at = src + (int64_t)part * work.per_part * D;
+        if (EPL == 2) { const f32x2 v = *reinterpret_cast<const f32x2*>(at); x[0] = v[0]; x[EPL - 1] = v[1]; }
+        else x[0] = at[0];
+    };
+    // the first parts' rows beside their references and sums
+    f32x2 ml = {-INFINITY, 0.f};
+    if (lane < ns) ml = *reinterpret_cast<const f32x2*>(p.part_ml + (at0 + (int64_t)lane * work.per_part) * 2);
+    constexpr int kEarly = 4;
+    float x[8][EPL];
+#pragma unroll
+    for (int u = 0; u < kEarly; ++u) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[u][e] = 0.f;
+        if (ns > 0) load_o(min(u, ns - 1), x[u]);
+    }
+    const PartWeights pw = part_weights(ml[0], ml[1]);
     float acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
@@ -533,7 +541,7 @@ template <int GR> struct ChunkPlan {
         const int sum = lane_value(wave_inclusive_scan(q.groups * pairs), 63), active = __popcll(__ballot(on));
         const int longest = (int)wave_max((float)q.groups);
         // a pair's last chunk is half full on average: that many workgroups are as good as not there
-        int size = max(max((sum + n_wg - 1) / max(n_wg - active * pairs / 2, 1), 256 / GR), longest / w.p.slots + 1);
+        int size = max(max((sum + n_wg - 1) / max(n_wg - active * pairs / 2, 1), 256 / GR), longest / kMaxParts + 1);
         for (;; size += 1 + size / 16) {   // (ends: with the longest context as the size there is one chunk a pair, and no more pairs than workgroups)
             each = on ? max((q.groups + size - 1) / size, 1) : 0;
             incl = wave_inclusive_scan(each * pairs);
@@ -543,14 +551,14 @@ template <int GR> struct ChunkPlan {
     }
 };
 
-// Merges the n chunks of the columns of (s, g, hg) from the workspace and stores the output rows; all threads of the workgroup, a wave 64
+// Merges the n chunks, from number `first` of the launch on, of the columns of (s, g, hg) from the workspace and stores the output rows; all threads of the workgroup, a wave 64
 // elements of a column at a time, without LDS and barriers (with the weights made by 16 threads in LDS it took twice the time).  The order of
 // the sums depends on nothing but n.
 template <class T, int D>
-MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g, int hg, int n) {
+MA_DEV void merge_chunks(const DecodeWork& w, const SeqInfo& info, int g, int hg, int first, int n) {
     const PagedParams& p = w.p;
     const int lane = threadIdx.x & 63, wave = wave_id(), cols = min(16, w.n_col - hg * 16);
-    const int64_t at0 = part_row(w, s, g, hg * 16) * p.slots;
+    const int64_t at0 = part_row(w, first, 0), step = (int64_t)w.per_part * D;
     constexpr int PER = 16 * D / (kChunkWaves * 64);
     float x[PER][8];
     f32x2 ml[PER];
@@ -558,11 +566,11 @@ MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g,
     for (int e = 0; e < PER; ++e) {
         const int idx = (wave + e * kChunkWaves) * 64;
         if (idx < cols * D) {
-            const int64_t at = at0 + (int64_t)(idx / D) * p.slots;
-            ml[e] = load_shared2(p.part_ml + (at + min(lane, n - 1)) * 2);
+            const int64_t at = at0 + idx / D;
+            ml[e] = load_shared2(p.part_ml + (at + (int64_t)min(lane, n - 1) * w.per_part) * 2);
             const float* src = p.part_o + at * D + idx % D + lane;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + (int64_t)min(u, n - 1) * D);
+            for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + min(u, n - 1) * step);
         }
     }
 #pragma unroll
@@ -571,12 +579,12 @@ MA_DEV void merge_chunks(const DecodeWork& w, int s, const SeqInfo& info, int g,
         if (idx >= cols * D) break;
         const int c = idx / D, d = idx % D + lane, col = hg * 16 + c, tok = col / p.n_rep;
         const PartWeights pw = part_weights(lane < n ? ml[e][0] : -INFINITY, lane < n ? ml[e][1] : 0.f);
-        const float* src = p.part_o + (at0 + (int64_t)c * p.slots) * D + d;
+        const float* src = p.part_o + (at0 + c) * D + d;
         float sum = 0.f;
         for (int s0 = 0; s0 < n; s0 += 8) {
             if (s0 > 0) {
 #pragma unroll
-                for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + (int64_t)min(s0 + u, n - 1) * D);
+                for (int u = 0; u < 8; ++u) x[e][u] = load_shared(src + min(s0 + u, n - 1) * step);
             }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
@@ -628,7 +636,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const 
     }
     __syncthreads();
     const bool whole = n <= 1;   // the chunk is the whole context: its result is the output
-    const int64_t at0 = part_row(work, s, g, hg * 16) * p.slots + split;
+    const int64_t at0 = part_row(work, x, 0);
     for (int idx = w * 64; idx < cols * D; idx += NW * 64) {   // a wave 64 elements of a column
         const int c = idx / D, d = idx % D + lane;
         const PartWeights pw = part_weights(lane < NW ? ml_s[lane * 16 + c] : -INFINITY, lane < NW ? ml_s[(NW + lane) * 16 + c] : 0.f);
@@ -640,8 +648,8 @@ __global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const 
             if (tok < info.len)
                 reinterpret_cast<uint16_t*>(p.out)[(int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + col - tok * p.n_rep) * p.o1 + d] = (uint16_t)(T::pack2(sum * (pw.total > 0.f ? 1.f / pw.total : 0.f), 0.f) & 0xffffu);
         } else {
-            store_shared(p.part_o + (at0 + (int64_t)c * p.slots) * D + d, sum);
-            if (idx % D == 0 && lane == 0) store_shared2(p.part_ml + (at0 + (int64_t)c * p.slots) * 2, f32x2{pw.top, pw.total});
+            store_shared(p.part_o + (at0 + c) * D + d, sum);
+            if (idx % D == 0 && lane == 0) store_shared2(p.part_ml + (at0 + c) * 2, f32x2{pw.top, pw.total});
         }
     }
     if (whole || !work.done) return;
@@ -654,7 +662,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 2) void paged_chunk_kernel(const 
         if (last_s) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (last_s) merge_chunks<T, D>(work, s, info, g, hg, n);
+    if (last_s) merge_chunks<T, D>(work, info, g, hg, x - split, n);
 }
 
 // (where there are no counters) grid (column groups x KV heads, sequences)
@@ -663,8 +671,8 @@ __global__ __launch_bounds__(kChunkWaves * 64) void paged_chunk_merge_kernel(con
     const PagedParams& p = work.p;
     const int s = blockIdx.y, hg = (int)blockIdx.x / p.Hkv, g = (int)blockIdx.x - hg * p.Hkv;
     const ChunkPlan<GR> plan(work, n_wg);
-    const int n = lane_value(plan.each, s);
-    if (n > 1) merge_chunks<T, D>(work, s, seq_info(p, s), g, hg, n);
+    const int n = lane_value(plan.each, s), pairs = p.Hkv * work.n_hg;
+    if (n > 1) merge_chunks<T, D>(work, seq_info(p, s), g, hg, lane_value(plan.incl, s) - n * (pairs - (int)blockIdx.x), n);
 }
 
 // Workgroups of the line: as many as the chip holds at once.
@@ -680,17 +688,7 @@ static int compute_units() {
     return n;
 }
 
-// Slots of a row: enough for the least shares, 64 at most (longer contexts get longer shares).
-static int64_t slots_of(int64_t max_context) { return std::min<int64_t>(kMaxSlots, max_context / kLeastShare + 4); }
-
 bool paged_decode_takes(int64_t Hq, int64_t Hkv, int64_t max_q) { return max_q == 1 || max_q * (Hq / Hkv) <= 16; }
-
-static size_t part_bytes(int64_t rows, int64_t slots, int64_t floats) { return ((size_t)(rows * slots * floats * 4) + 255) / 256 * 256; }
-size_t paged_decode_workspace_bytes(int64_t n_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
-    (void)Hkv;
-    const int64_t rows = n_seqs * Hq * max_q, slots = slots_of(max_context);
-    return part_bytes(rows, slots, D) + part_bytes(rows, slots, 2) + ((size_t)(n_seqs + 2) * 4 + 255) / 256 * 256;
-}
 
 template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStream_t stream) {
     hipLaunchKernelGGL((paged_line_kernel<T, D, FP8>), dim3((unsigned)w.n_wg), dim3(kLineWaves * 64), 0, stream, w);
@@ -705,11 +703,37 @@ template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStre
 // Two rounds of whole contexts where the table has no room for long ones: 64 of 100 13.1 / 14.1, 11.8 / 14.9, of 400 25.2 / 27.4, 19.9 / 20.1, of 1000
 // 45.7 / 50.3, 31.0 / 31.4, of 2000 84 / 91, 53 / 53, of 6000 237 / 244, 156 / 146; e4m3 of 100 12.0 / 14.5, 10.9 / 14.8, of 400 19.2 / 22.4, 17.9 / 17.6, of 700 24.8 /
 // 28.8, 22.2 / 22.2, of 1000 33.7 / 31.7, 28.7 / 25.7.
-static int chunk_rounds(const DecodeWork& w, int64_t max_context, bool eight) {
-    const int64_t pairs = (int64_t)w.p.n_seqs * w.p.Hkv * w.n_hg, units = compute_units();
-    if (w.p.n_seqs > 64 || pairs > kStreamCounters) return 0;
+static int chunk_rounds(int64_t n_seqs, int64_t pairs, int64_t max_context, bool eight) {
+    const int64_t units = compute_units();
+    if (n_seqs > 64 || pairs > kStreamCounters) return 0;
     return pairs <= units ? 1 : pairs <= 2 * units && max_context <= (eight ? 768 : 2048) ? 2 : 0;
 }
+
+// How a call is laid out, from its sizes alone.
+struct DecodePlan {
+    int64_t n_col, n_hg, per_part;   // as in DecodeWork
+    int rounds;                      // chunk_rounds
+    int64_t parts;                   // partial results: chunks, a workgroup each; of the line, shares and pairs
+    size_t o_bytes, ml_bytes, bytes;
+};
+static size_t whole_lines(int64_t bytes) { return ((size_t)bytes + 255) / 256 * 256; }
+static DecodePlan plan_decode(bool eight, int64_t n_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
+    DecodePlan r{};
+    r.n_col = max_q * (Hq / Hkv);
+    r.n_hg = (r.n_col + 15) / 16;
+    r.per_part = std::min<int64_t>(r.n_col, 16);
+    const int64_t pairs = n_seqs * Hkv * r.n_hg, units = compute_units();
+    r.rounds = chunk_rounds(n_seqs, pairs, max_context, eight);
+    r.parts = r.rounds > 0 ? r.rounds * units : units * kLineWgPerCu * kLineWaves + pairs;
+    r.o_bytes = whole_lines(r.parts * r.per_part * D * 4);
+    r.ml_bytes = whole_lines(r.parts * r.per_part * 2 * 4);
+    r.bytes = r.o_bytes + r.ml_bytes + (r.rounds > 0 ? 0 : whole_lines((n_seqs + 2) * 4));
+    return r;
+}
+size_t paged_decode_workspace_bytes(int64_t n_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
+    return std::max(plan_decode(false, n_seqs, Hq, Hkv, D, max_context, max_q).bytes, plan_decode(true, n_seqs, Hq, Hkv, D, max_context, max_q).bytes);
+}
+
 template <class T, int D, bool FP8> static int launch_chunks(DecodeWork w, int rounds, hipStream_t stream) {
     const int n_wg = rounds * compute_units();
     w.done = stream_counters(stream);
@@ -729,19 +753,19 @@ template <class T> static int launch_decode_as(const DecodeWork& w, int64_t D, b
 
 int launch_paged_decode(PagedParams p, int dtype, int64_t D, bool eight, int64_t max_context, void* workspace, hipStream_t stream) {
     DecodeWork w{};
-    w.n_col = p.max_q * p.n_rep;
-    w.n_hg = (w.n_col + 15) / 16;
+    const DecodePlan plan = plan_decode(eight, p.n_seqs, p.Hq, p.Hkv, D, max_context, p.max_q);
+    w.n_col = (int)plan.n_col;
+    w.n_hg = (int)plan.n_hg;
+    w.per_part = (int)plan.per_part;
     w.n_wg = compute_units() * kLineWgPerCu;
-    const int64_t rows = (int64_t)p.n_seqs * p.Hkv * w.n_col, slots = slots_of(max_context);
+    const int64_t rows = (int64_t)p.n_seqs * p.Hkv * w.n_col;
     if (rows > 0x7fffffffLL || (int64_t)p.n_seqs * p.Hkv * w.n_hg * ((max_context + 15) / 16 + 1) > 0x7fffffffLL - 65536)
         return fail(MINFER_ATTN_EINVAL, "flash_attn_paged: problem too large for one launch");
-    p.slots = (int)slots;
     p.part_o = (float*)workspace;
-    p.part_ml = (float*)((char*)workspace + part_bytes(rows, slots, D));
-    w.seq_off = (int32_t*)((char*)p.part_ml + part_bytes(rows, slots, 2));
+    p.part_ml = (float*)((char*)workspace + plan.o_bytes);
+    w.seq_off = plan.rounds > 0 ? nullptr : (int32_t*)((char*)p.part_ml + plan.ml_bytes);
     w.p = p;
-    const int rounds = chunk_rounds(w, max_context, eight);
-    return dtype == MINFER_ATTN_F16 ? launch_decode_as<F16>(w, D, eight, rounds, stream) : launch_decode_as<BF16>(w, D, eight, rounds, stream);
+    return dtype == MINFER_ATTN_F16 ? launch_decode_as<F16>(w, D, eight, plan.rounds, stream) : launch_decode_as<BF16>(w, D, eight, plan.rounds, stream);
 }
 
 }  // namespace minfer_attn
