@@ -24,6 +24,7 @@
 // sequence's table of pages, while its chunks are on their way.  8-bit pages have a kernel of their own (append8_kernel).
 // 64 tokens of 32 heads on 8 of 128 4.4 us, 7157 of 48 on 8 31 us, 4.7 TB/s where a large copy has 4.9.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 #include "attn_host.h"
@@ -37,7 +38,7 @@ constexpr int kMaxPairs = 128;    // rotary_dim <= 256
 
 enum { ROPE_IL = MINFER_ROPE_INTERLEAVED, ROPE_NEOX = MINFER_ROPE_NEOX };
 
-struct RopeParams {
+struct RopeCommon {
     void* x;                  // [B, L, H, D], rotated in place (q of the fused producer)
     const void* k;            // fused: [B, L, Hkv, D]
     const void* v;            // fused: [B, L, Hkv, D]
@@ -47,9 +48,16 @@ struct RopeParams {
     int64_t c0, c1, c2;
     int B, L, H, Hkv, D, rd, Lmax;
     int start_pos;            // not fused: position of token l is start_pos + l
-    int n_seqs;               // paged: B = 1, L = the packed tokens; positions [n_seqs]
-    const int32_t* cu;        // paged: [n_seqs + 1]
-    PagedCache pages;         // paged: the cache, in place of the fields above
+};
+struct RopeParams : RopeCommon {
+    double inv_freq[kMaxPairs];
+};
+// Paged caches: B = 1, L = the packed tokens, positions [n_seqs].  (A struct of its own, with its fields next to the others: behind the frequencies
+// they cost the paged producers of few tokens 0.2 to 0.5 us of 3.8 and 7.2, in front of them in every launch the one into Q8_0 caches 0.15 of 4.)
+struct PagedRopeParams : RopeCommon {
+    int n_seqs;
+    const int32_t* cu;        // [n_seqs + 1]
+    PagedCache pages;         // the cache, in place of the fields above
     double inv_freq[kMaxPairs];
 };
 
@@ -136,7 +144,7 @@ MA_DEV int64_t position_of(const int32_t* positions, const TokenOwner& o, int to
 // elements 8c..8c+7 and their partners rd/2 + 8c.., rd/16 chunks per head.  Sections, in order: q rotary,
 // then (fused only) k rotary, k tail (elements rd..D-1, copied), v (copied).
 template <class T, int STYLE, bool FUSED, bool Q8, bool STREAM, bool PAGED = false>
-__global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const RopeParams p) {
+__global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const std::conditional_t<PAGED, PagedRopeParams, RopeParams> p) {
     static_assert(FUSED || (!Q8 && !PAGED), "only the fused producer writes a cache");
     __shared__ f32x2 tab[2][kMaxPairs];
     __shared__ double freq[kMaxPairs];   // the kernel argument array, where a thread can index it cheaply
@@ -169,20 +177,23 @@ __global__ __launch_bounds__(kRopeThreads, FUSED ? 1 : 8) void rope_kernel(const
         char* qk; char* qv;        // ... or byte pointers (Q8_0)
         bool owned;                // paged: the token belongs to a sequence
     };
-    const int64_t head_stride = PAGED ? p.pages.head_stride : p.c1;
+    int64_t head_stride = p.c1;
+    if constexpr (PAGED) head_stride = p.pages.head_stride;
     // (paged: the token's sequence, position and cache row; after its chunks have been requested)
     auto locate = [&](Token& k, int tok) __attribute__((always_inline)) {
-        const TokenOwner o = owner_of(p.cu, p.n_seqs, tok);
-        k.owned = o.seq >= 0;
-        const int s = max(o.seq, 0);
-        const int64_t pos = position_of(p.positions, o, tok), at = pos >> p.pages.page_log2;
-        k.pos = (int)pos;
-        int id = -1;
-        if (k.owned && pos >= 0 && at < p.pages.width) id = const_load(p.pages.table + (int64_t)s * p.pages.table_stride + at);
-        k.row_ok = (unsigned)id < (unsigned)p.pages.n_pages;
-        const int64_t row = (int64_t)id * p.pages.page_stride + (int64_t)(k.pos & ((1 << p.pages.page_log2) - 1)) * p.pages.row_stride;
-        k.ck = (short*)p.pages.k + row;
-        k.cv = (short*)p.pages.v + row;
+        if constexpr (PAGED) {
+            const TokenOwner o = owner_of(p.cu, p.n_seqs, tok);
+            k.owned = o.seq >= 0;
+            const int s = max(o.seq, 0);
+            const int64_t pos = position_of(p.positions, o, tok), at = pos >> p.pages.page_log2;
+            k.pos = (int)pos;
+            int id = -1;
+            if (k.owned && pos >= 0 && at < p.pages.width) id = const_load(p.pages.table + (int64_t)s * p.pages.table_stride + at);
+            k.row_ok = (unsigned)id < (unsigned)p.pages.n_pages;
+            const int64_t row = (int64_t)id * p.pages.page_stride + (int64_t)(k.pos & ((1 << p.pages.page_log2) - 1)) * p.pages.row_stride;
+            k.ck = (short*)p.pages.k + row;
+            k.cv = (short*)p.pages.v + row;
+        }
     };
     auto token_at = [&](int tok) __attribute__((always_inline)) {
         Token k;
@@ -574,7 +585,7 @@ MA_DEV void angle64(double inv_freq, int pos, double& c, double& s) {
 }
 
 struct Append8Params {
-    RopeParams r;
+    PagedRopeParams r;
     int hpw_log2, n_hg;    // KV heads per workgroup = 1 << hpw_log2, workgroups per page
     int items;             // bound of the pages that the call writes to
     int max_e;             // largest scale exponent: 448 * 2^max_e is a finite number of the activations' type
@@ -606,7 +617,7 @@ MA_DEV uint32_t move4(uint32_t codes, float factor) {
 
 template <class T, int STYLE, int D>
 __global__ __launch_bounds__(kRopeThreads, 3) void append8_kernel(const Append8Params ap) {
-    const RopeParams& p = ap.r;
+    const PagedRopeParams& p = ap.r;
     const PagedCache& pc = p.pages;
     constexpr int GL = D / 8, NG = kRopeThreads / GL;   // lanes per row, groups of lanes
     extern __shared__ f32x2 tab[];                       // [rows of a round][rd/2]: cosine and sine, and behind all of them, as pairs of bf16, what fp32 leaves of each
@@ -846,7 +857,8 @@ static void inverse_frequencies(double* out, int64_t rotary_dim, double freq_bas
     std::copy(kept.inv_freq, kept.inv_freq + n, out);
 }
 
-static int fill_rope(RopeParams& p, int dtype, int style, int64_t B, int64_t L, int64_t H, int64_t D,
+template <class Params>
+static int fill_rope(Params& p, int dtype, int style, int64_t B, int64_t L, int64_t H, int64_t D,
                      int64_t rotary_dim, double freq_base, const char* op) {
     char msg[160];
     auto bad = [&](const char* what) {
@@ -871,7 +883,7 @@ static bool vector_ok(int style, int64_t D, int64_t rd) {
 }
 
 template <bool FUSED, bool Q8, bool STREAM, bool PAGED>
-static void launch_rope_as(int dtype, int style, const RopeParams& p, int grid, hipStream_t stream) {
+static void launch_rope_as(int dtype, int style, const std::conditional_t<PAGED, PagedRopeParams, RopeParams>& p, int grid, hipStream_t stream) {
     if (dtype == MINFER_ATTN_F16) {
         if (style == ROPE_IL) hipLaunchKernelGGL((rope_kernel<F16, ROPE_IL, FUSED, Q8, STREAM, PAGED>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
         else hipLaunchKernelGGL((rope_kernel<F16, ROPE_NEOX, FUSED, Q8, STREAM, PAGED>), dim3(grid), dim3(kRopeThreads), 0, stream, p);
@@ -882,7 +894,7 @@ static void launch_rope_as(int dtype, int style, const RopeParams& p, int grid, 
 }
 
 template <bool FUSED, bool Q8 = false, bool PAGED = false>
-static int launch_rope(int dtype, int style, const RopeParams& p, hipStream_t stream) {
+static int launch_rope(int dtype, int style, const std::conditional_t<PAGED, PagedRopeParams, RopeParams>& p, hipStream_t stream) {
     const int tokens = p.B * p.L;
     const int grid = std::min(tokens, 256 * 16);
     // distinct bytes the launch touches: q's rotary part (in place), and for the producer k, v and their cache rows
@@ -1035,7 +1047,7 @@ MINFER_ATTN_EXPORT int minfer_rope_kv_append_paged(int dtype, int style, int pag
                                                    double freq_base, void* stream_v) {
     clear_error();
     Append8Params ap{};
-    RopeParams& p = ap.r;
+    PagedRopeParams& p = ap.r;
     if (int rc = fill_rope(p, dtype, style, 1, T, Hq, D, rotary_dim, freq_base, "rope_kv_append_paged")) return rc;
     if (int rc = check_pages("rope_kv_append_paged", dtype, page_type, pages, n_seqs, Hkv, D, p.pages)) return rc;
     const bool eight = page_type == MINFER_FP8_E4M3;
