@@ -110,6 +110,7 @@ MA_DEV void attend_key_by_key(const PagedCache& c, int Hkv, int seq, int g, int 
             const bool on = q[i] && key < limit[i];
             const float m_new = on ? fmaxf(m[i], score) : m[i], base = m_new == -INFINITY ? 0.f : m_new;
             const float alpha = m[i] == -INFINITY ? (on ? 0.f : 1.f) : fast_exp2(m[i] - base);
+            // (the weight as a product with V has it in front of these keys: rounded to the 16-bit type)
             const float w = T::to_float((short)(T::pack2(fast_exp2(score - base), 0.f) & 0xffffu));
             m[i] = m_new;
             l[i] = on ? l[i] * alpha + (quad == 0 ? w : 0.f) : l[i];

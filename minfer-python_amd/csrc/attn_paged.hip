@@ -116,7 +116,7 @@ template <int BR> MA_DEV Piece find_piece(const PagedParams& p, int x, int& all)
 }
 
 // Bound by the matrix unit with the exponentials and, over codes, the widening between its instructions.  A prompt of 8192, 32 query heads on 8 of 128, f16:
-// 521 us, 1055 TFLOP/s, nine tenths of what a library product of 8192^3 reaches; 4 chunks, 1257 tokens to 13795 rows, 24 heads on 8, bf16: 67 us, 770; 5 chunks,
+// 515 us, 1067 TFLOP/s, nine tenths of what a library product of 8192^3 reaches; 4 chunks, 1257 tokens to 13795 rows, 24 heads on 8, bf16: 66 us, 774; 2 chunks,
 // 1778 tokens to 12315 rows of codes, 64 heads on 8, a window that moved on: 226 us, 804.  Prompts of 512 and 1024 take 17 and 28: 5 us and 1.4 a tile.
 template <class T, int D, bool FP8, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParams p) {
@@ -392,7 +392,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
                 }
             }
         }
-        // P = 2^E and O^T += V^T P^T, 32 keys and 16 rows at a time, the next weights made between the MFMAs of the current ones
+        // P = 2^E and O^T += V^T P^T, 32 keys and 16 rows at a time, the next weights made between the MFMAs of the current ones.  The weights are rounded to the
+        // 16-bit type, since an MFMA takes both operands in one type and V is there in that: error against 64 bits 2.5e-4 (f16) and 2.2e-3 (bf16) of the output's scale, of
+        // which the output's own rounding makes 2.0e-4 and 1.7e-3.  What the rounding leaves as a second operand would be half as many MFMAs again.
         float ls[2] = {0.f, 0.f};
         auto weights_quarter = [&](int ck, int qb, int i) __attribute__((always_inline)) -> uint32_t {
             const int kb = 2 * ck + (i >> 1), r = 2 * (i & 1);
@@ -609,10 +611,10 @@ struct PagedPlan {
     int64_t pieces;    // bound of the pieces, per KV head
     size_t o_bytes, ml_bytes, table_bytes;
 };
-// Waves of a workgroup, 32 rows each.  16-bit rows: four, and two workgroups to a unit (three at head_dim 64); eight, one to a unit, take 226 us / 243
-// for 2 x 700 tokens behind 8000, 58 / 68 for a prompt of 2048, 488 / 494 for one of 8192.  Codes at head_dim 128: eight where a sequence can fill them, which widen a tile
-// for twice as many rows (us, four / eight: 2 x 700 behind 8000 339 / 296, a prompt of 2048 behind 20000 833 / 730, of 4096 190 / 165, of 512
-// 24.6 / 27.3; where it cannot, 60 x 20 tokens of 4 heads behind 2000 to 8000, 300 / 356).
+// Waves of a workgroup, 32 rows each (times in us, four / eight; 32 heads on 8 of 128, bf16).  16-bit rows: four, and two workgroups to a unit (three at head_dim
+// 64), eight being one to a unit: 2 x 700 tokens behind 8000 224 / 244, a prompt of 512 16.6 / 21.0, of 2048 53.5 / 62.9, of 8192 492 / 494, of 16384 1925 / 1911.  Codes
+// at head_dim 128: eight where a sequence can fill them, which widen a tile for twice as many rows: 2 x 700 behind 8000 338 / 295, 2048 behind 20000 827 / 725, a
+// prompt of 4096 184 / 158, of 512 21.8 / 24.5; where it cannot, 60 x 20 behind 2000 to 8000, 277 / 361.
 constexpr int kWavesBig = 8, kWavesSmall = 4;
 constexpr int64_t kUnits = 256;
 static int64_t blocks_of(int64_t n_seqs, int64_t T, int64_t n_rep, int64_t max_q, int waves) {
@@ -620,9 +622,12 @@ static int64_t blocks_of(int64_t n_seqs, int64_t T, int64_t n_rep, int64_t max_q
     return std::min(n_seqs * ((max_q * n_rep + rows - 1) / rows), T * n_rep / rows + n_seqs);
 }
 // Blocks of rows are cut where whole ones would leave more than a quarter of the chip's rounds of workgroups empty, of two rounds at most: the combine's
-// launch and the sums' way through memory cost 4 to 8 us where that gains nothing (us, whole / cut: 700 tokens behind 8000, a third of a
-// round 126 / 86, 3 x 700 a little over one 275 / 214, 4 x 700 280 / 238, of codes 374 / 293; 4 x 1000 behind 2000, two full rounds 120 / 127; 60 x 20, one round
-// 263 / 280), and not where contexts are short (a prompt of 512 16.7 / 21.7, of 1024 28.2 / 31.3, of codes 22.1 / 24.7 and 42.1 / 38.9).
+// launch and the sums' way through memory cost 4 to 8 us where that gains nothing (us, whole / cut, heads as above: 350 tokens behind 8000, a sixth of a round 179 / 63, 700
+// behind 8000, a third, 185 / 122, of codes 289 / 159; 8 x 330 behind 250 to 16000, 1.5 rounds 425 / 360, of codes 616 / 499, but 4 x 700 behind 8000, 1.4 rounds of equal
+// contexts 444 / 451; 60 x 20 behind 2000 to 8000, one round, 258 / 262), and not where contexts are short (a prompt of 512 16.6 / 21.2, of 1024 27.7 / 31.3, of codes 24.5
+// / 27.0 and 41.8 / 38.7).  The host knows sizes, not contexts: where the blocks fill the chip and one context is far longer than the others, its
+// blocks end alone (64 x 20 tokens, 63 behind 2000 and one behind 60000: 1270, behind 2000 all of them 102; 2048 tokens with 60 single ones, one of them at 60000 rows, 1298, in two
+// calls 110 and 133).  So it is with more than 64 sequences, which are not cut (64 x 5 tokens of 16 heads on 2 behind 8000 106, 65 of them 168).
 static bool cuts_blocks(bool eight, int64_t wgs, int64_t round, int64_t n_seqs, int64_t max_context) {
     const int64_t rounds = (wgs + round - 1) / round;
     return rounds <= 2 && 4 * wgs <= 3 * rounds * round && n_seqs <= 64 && max_context > (eight ? 512 : 1024);

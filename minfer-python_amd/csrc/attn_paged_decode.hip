@@ -14,7 +14,7 @@
 // * the line: all rows to be read, sequence by sequence, KV head by KV head, cut into as many equal shares as the launch has waves; a
 //   wave's share covers parts of a few (sequence, KV head) pairs, each of which leaves a partial result that
 //   paged_merge_kernel puts together.  Whatever the mix of contexts, all waves end together.  64 sequences of 512 to 8192 rows, 32 query
-//   heads on 8 of 128: 180 us, 6.1 TB/s, of which the merge 5; over codes 99 us, 5.6 TB/s.
+//   heads on 8 of 128: 179 us, 6.1 TB/s, of which the merge 5; over codes 98 us, 5.6 TB/s.
 // * chunks, for few pairs: eight waves of a workgroup share one chunk of a pair and merge in LDS, and the last workgroup of a pair merges its
 //   chunks (on the null stream; elsewhere paged_chunk_merge_kernel does).  A sequence is cut by its own context, which the host does not know.
 //   12 sequences of 3 or 4 drafts, 28964 rows: 27 us, 4.4 TB/s; one token, 8 heads on 2 of 64, against 1501 rows 8 us, three against 5570 rows of
@@ -29,8 +29,8 @@ namespace minfer_attn {
 constexpr int kLineWaves = 4;          // waves per workgroup of the line
 constexpr int kLineWgPerCu = 2;
 constexpr int kChunkWaves = 8;
-// Least rows of a wave's share of the line (us, 128 / 64 / 32: 64 sequences of 6 to 100 21.8 / 14.9 / 12.9, of 100 15.8 / 14.1 / 15.9, of codes 15.9 / 14.5 /
-// 12.1; one of 4000 15.1 / 14.7 / 14.8; 64 of up to 2000 on one KV head 16.0 / 16.5 / 19.4; where every wave has more nothing changes).
+// Least rows of a wave's share of the line (us, 128 / 64 / 32, 32 heads on 8 of 128: 80 sequences of 6 to 100 21.2 / 16.3 / 13.9, of codes 17.1 / 13.2 / 12.9; 80 of
+// 100 16.8 / 16.8 / 16.1; 4 heads on 1: 80 of up to 2000 15.8 / 14.8 / 17.5, one of 4000 with 69 of 6 22.6 / 19.3 / 19.3; where every wave has more nothing changes).
 constexpr int kLeastShare = 64;
 constexpr int kMaxParts = 64;          // partial results a column can have: a wave merges them, one to a lane
 
@@ -269,7 +269,7 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
         for (int h = 0; h < NH; ++h) {
             pk[2 * h] = T::pack2(fast_exp2(fmaf(sc[h][0], c2, -mc)), fast_exp2(fmaf(sc[h][1], c2, -mc)));
             pk[2 * h + 1] = T::pack2(fast_exp2(fmaf(sc[h][2], c2, -mc)), fast_exp2(fmaf(sc[h][3], c2, -mc)));
-            l_sum = T::add_pair(pk[2 * h + 1], T::add_pair(pk[2 * h], l_sum));   // sums the rounded weights that are multiplied
+            l_sum = T::add_pair(pk[2 * h + 1], T::add_pair(pk[2 * h], l_sum));   // sums the rounded weights that are multiplied (as in paged_tile_kernel)
         }
         // O^T += V^T P^T: row d = 16db + l16, keys 4 quad + 0..3 (and 16 + 4 quad + 0..3)
 #pragma unroll
@@ -697,12 +697,12 @@ template <class T, int D, bool FP8> static int launch_line(DecodeWork w, hipStre
     hipLaunchKernelGGL((paged_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
     return check_launch("paged_merge_kernel");
 }
-// Whether a call is one for chunks.  Up to a pair for every unit always (us, chunks / line, contexts alike and from a sixteenth up: one of 4000 10.5 / 14.7, 9.6 /
-// 14; 4 of 30000 78 / 85, 39 / 45; 16 of 4000 44 / 49, 32 / 34, of 20000 e4m3 110 / 118, 65 / 63; 32 of 300 10.2 / 16, 8.2 / 13, of 1500 e4m3
-// 22 / 29, 19 / 22; where every unit has one long context, contexts that differ leave units idle: 32 of 6000 121 / 128, 79 / 74, e4m3 67 / 76, 56 / 47).
-// Two rounds of whole contexts where the table has no room for long ones: 64 of 100 13.1 / 14.1, 11.8 / 14.9, of 400 25.2 / 27.4, 19.9 / 20.1, of 1000
-// 45.7 / 50.3, 31.0 / 31.4, of 2000 84 / 91, 53 / 53, of 6000 237 / 244, 156 / 146; e4m3 of 100 12.0 / 14.5, 10.9 / 14.8, of 400 19.2 / 22.4, 17.9 / 17.6, of 700 24.8 /
-// 28.8, 22.2 / 22.2, of 1000 33.7 / 31.7, 28.7 / 25.7.
+// Whether a call is one for chunks.  Up to a pair for every unit always (us, chunks / line, contexts alike and from a sixteenth up, 32 heads on 8 of 128: one of 4000
+// 10.0 / 14.0, 8.2 / 10.6; 4 of 30000 78 / 87, 43 / 62; 16 of 4000 44 / 48, 26 / 31, of 20000 e4m3 109 / 114, 87 / 76; 32 of 300 8.4 / 15.9, 7.2 / 12.3, of 1500
+// e4m3 21 / 28, 18 / 21; where every unit has one long context, contexts that differ leave units idle: 32 of 6000 123 / 131, 79 / 72, e4m3 66 / 73, 55 / 45).
+// Two rounds of whole contexts where the table has no room for long ones: 64 of 100 11.5 / 13.2, 10.7 / 14.0, of 400 23.0 / 24.6, 17.0 / 17.6, of 1000
+// 44.5 / 48.8, 30.2 / 30.4, of 2000 82 / 88, 55 / 53, of 6000 242 / 251, 148 / 141; e4m3 of 100 11.4 / 11.4, 10.9 / 12.5, of 400 18.1 / 21.1, 16.8 / 15.6, of 700 23.4 /
+// 27.1, 20.7 / 20.8, of 1000 32.0 / 31.0, 27.9 / 24.4.
 static int chunk_rounds(int64_t n_seqs, int64_t pairs, int64_t max_context, bool eight) {
     const int64_t units = compute_units();
     if (n_seqs > 64 || pairs > kStreamCounters) return 0;

@@ -570,7 +570,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_append_kernel(const No
 // a few values in a million end in the code beside theirs, a sixteenth off, which no later step is as coarse as (25.1 us then, 26.4 now).  Pages with more rows than parts * 16 go through their rows twice.  One workgroup reads, moves and writes
 // all of a (page, head)'s rows and its scale, so nothing depends on an order.  The launch's further workgroups rotate q, a token each.
 // Bound by memory, few tokens by the chain of loads: 3398 tokens of 64 heads on 8 of 128 26 us, 5.0 TB/s with three waves to a
-// SIMD (with two 30.6); 40 of 32 on 8 7.6 us.
+// SIMD (with two 30.6); 40 of 32 on 8 7.5 us.
 // ------------------------------------------------------------------------------------------------
 constexpr int kAppendRows = 16;   // rows a group of lanes holds
 
