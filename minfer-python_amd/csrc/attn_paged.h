@@ -137,7 +137,8 @@ inline int check_pages(const char* op, int dtype, int page_type, const minfer_kv
     if (pages->page_size < 16 || pages->page_size > 1024 || (pages->page_size & (pages->page_size - 1)) != 0)
         return bad("page_size must be a power of two in 16..1024");
     if (pages->n_pages < 0 || pages->n_pages > 0x7fffffffLL || pages->pages_per_seq < 0) return bad("bad number of pages");
-    if (pages->pages_per_seq * pages->page_size > (int64_t)1 << 30) return bad("pages_per_seq * page_size > 2^30 unsupported");
+    const int64_t most = ((int64_t)1 << 30) / pages->page_size;   // (the products themselves need not fit 64 bits)
+    if (pages->pages_per_seq > most) return bad("pages_per_seq * page_size > 2^30 unsupported");
     if (pages->table_stride < 0) return bad("table_stride must be non-negative");
     if (n_seqs > 0 && pages->pages_per_seq > 0 && !pages->block_table) return bad("block_table is null");
     if (pages->n_pages > 0) {
@@ -149,7 +150,7 @@ inline int check_pages(const char* op, int dtype, int page_type, const minfer_kv
     for (int i = 0; i < 3; ++i)
         if (s[i] < 0 || s[i] % unit != 0) return bad(eight ? "page strides must be non-negative multiples of 16 bytes" : "page strides must be non-negative multiples of 8 elements");
     // (a lane's offset from a page's first row is 32 bits)
-    if (pages->page_size * pages->stride_row >= (int64_t)1 << 30) return bad("page_size * stride_row >= 2^30 unsupported");
+    if (pages->stride_row >= most) return bad("page_size * stride_row >= 2^30 unsupported");
     c.k = pages->k; c.v = pages->v;
     c.k_scales = (uint8_t*)pages->k_scales; c.v_scales = (uint8_t*)pages->v_scales;
     c.table = pages->block_table;
