@@ -36,8 +36,8 @@ APPEND_TRAFFIC_BYTES = 786534 * 1024        # rope_kv_append, B=8 L=4096 Llama-3
 NORM_TRAFFIC_BYTES = 786669 * 1024          # rmsnorm on [8,4096,6144]
 GEMM_TRAFFIC_BYTES = 229726 * 1024          # gemm 4096^3 (A and B panels are re-read by several XCDs)
 DECODE_Q8_TRAFFIC_BYTES = 597506 * 1024     # decode over Q8_0 caches (split + combine)
-APPEND_Q8_TRAFFIC_BYTES = 737576 * 1024     # rope_kv_append into Q8_0 caches
-APPEND_NORM_TRAFFIC_BYTES = 786622 * 1024   # rope_kv_append_norm, the same shape
+APPEND_Q8_TRAFFIC_BYTES = 737581 * 1024     # rope_kv_append into Q8_0 caches
+APPEND_NORM_TRAFFIC_BYTES = 786629 * 1024   # rope_kv_append_norm, the same shape
 QKV_TRAFFIC_BYTES = 377747 * 1024           # qkv in one launch, M=K=4096, N=4096+1024+1024
 LONG_TRAFFIC_BYTES = 2721679 * 1024         # long-context prefill (classify + main), S=32768 bf16: the 1 GiB mask once, K/V re-fetched past the 4 MiB L2s
 RAGGED_TRAFFIC_BYTES = 747918 * 1024        # packed ragged prefill (T=20514, Hq=64)
@@ -51,7 +51,7 @@ TRAFFIC_MEASURED_AGAINST = {
     "attn_decode.hip": "35cbde39fc19",
     "quant_q8.h": "4fea6a94e300",
     "rope.hip": "531e784a5a11",
-    "attn_paged.h": "ebc343c708b7",
+    "attn_paged.h": "9febe38c9fdd",
     "rmsnorm.hip": "90740d99856e",
     "gemm.hip": "87632e517cc6",
     "gemm_common.h": "efc44e77d7fe",
