@@ -415,6 +415,69 @@ int minfer_rope_kv_append_q8_0(int dtype, int style, void* q, const void* k, con
                                int64_t rotary_dim, double freq_base, void* stream);
 
 /*
+ * The free pages of a paged cache's pool, a ring of n_pages entries on the device: `count` free pages from entry `head` on, around the
+ * ring's end.  state is {head, count, anything}, int32; state_after gets the state behind a call, its third entry the pages that the call could not
+ * have (minfer_paged_tables) or had no room for (minfer_paged_release).  state_after must not be state: a program keeps two and exchanges
+ * them.  Pages are taken from the front and given back behind the last.  n_pages is the pool's number of pages.
+ */
+typedef struct minfer_page_ring {
+    int32_t* pages;
+    const int32_t* state;
+    int32_t* state_after;
+    int64_t n_pages;
+} minfer_page_ring;
+
+/*
+ * Block tables and slot maps for a step of a paged cache, from lengths: sequence s holds past_lens[s] rows in its table's first
+ * pages_held[s] pages and gets new_lens[s] new rows.  Where these need more pages they are taken from the ring, sequence by sequence, page by
+ * page, and written to the table behind those that are there; where the ring has no more, -1 is.  Written besides:
+ *   cu_seqlens [n_seqs + 1]  sums of new_lens, as the operators over packed tokens take them
+ *   ctx_lens [n_seqs]        past_lens + new_lens, as the attention takes them (the append's positions are past_lens)
+ *   slots [n_slots]          of token cu_seqlens[s] + i its row past_lens[s] + i in the pool, page * page_size + row of the page, -1 where it has no
+ *                            page; entries behind the last token are left alone, tokens behind the last entry have none
+ *   held_after [n_seqs]      pages_held with the pages that were had
+ * int32 but for slots, int64; all contiguous, the table's rows table_stride apart.  Nothing of it is trusted: negative lengths are zero, lengths past 2^30
+ * are cut to it, sums saturate; pages_held is cut to 0 .. pages_per_seq, and rows behind the table get no page; a page outside the pool is no slot.
+ * Entries of the table behind held_after are not cleared.  Outputs must not overlap inputs.  page_size is a power of two in 16..1024; n_seqs at most 2^24.
+ */
+int minfer_paged_tables(int64_t page_size, const int32_t* past_lens, const int32_t* new_lens, const int32_t* pages_held,
+                        const minfer_page_ring* ring, int32_t* block_table, int64_t table_stride, int64_t pages_per_seq,
+                        int32_t* cu_seqlens, int32_t* ctx_lens, int64_t* slots, int64_t n_slots, int32_t* held_after,
+                        int64_t n_seqs, void* stream);
+
+/*
+ * Pages given back: sequence s keeps the pages of its first keep_lens[s] rows (0: it ended; a large number: it keeps all), and its pages behind them, up to
+ * pages_held[s], go to the ring, sequence by sequence, page by page, those whose table entry names no page of the pool left out.
+ * held_after [n_seqs] are the pages that each holds then; the table is not written, its entries behind held_after mean nothing any more.  A page that
+ * several sequences share must be among the rows that all but one of them keep.  Not trusted, and not overlapping, as in minfer_paged_tables.
+ */
+size_t minfer_paged_release_workspace_bytes(int64_t n_seqs);
+int minfer_paged_release(int64_t page_size, const int32_t* keep_lens, const int32_t* pages_held, const minfer_page_ring* ring,
+                         const int32_t* block_table, int64_t table_stride, int64_t pages_per_seq, int32_t* held_after, int64_t n_seqs,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Drafted tokens against the target's probabilities.  tokens [T] are a step's, packed: of sequence s, cu_seqlens[s] .. cu_seqlens[s+1]-1, the first
+ * is known and the others are drafts.  target_probs row t [V] is the target's distribution of the token behind token t, draft_probs row t the
+ * one that the draft behind it was drawn from (its rows at last tokens are not read; null: drafts without probabilities, each as if drawn with
+ * probability one).  The draft x behind token t is kept while accept_u[t] * draft_probs[t][x] < target_probs[t][x] and all drafts in front of it are.  Then
+ *   out_tokens[t]  of token t its kept draft; at the first that is not kept, or at the last token where all are, the next token; -1 behind
+ *   n_accepted[s]  the drafts that are kept
+ * The next token is the least j with w_0 + .. + w_j > sample_u[s] * (w_0 + .. + w_{V-1}), w = max(target - draft, 0) of the row where a draft was not
+ * kept, and the target's row where all were or where the former is zero everywhere; the last j with w_j > 0 where no sum is larger (sample_u of
+ * one or more), -1 where all are zero.  Sums are held in 64 bits.  Probabilities need not add up to one; negative ones and NaN count as zero there, and a draft
+ * whose comparison is with NaN, or that is no token (outside 0..V-1), is not kept; infinite ones are not meant.  Sequences without tokens get n_accepted 0.
+ * prob_dtype MINFER_ATTN_F32, F16 or BF16, for both; rows contiguous, *_stride elements apart, at any address of the type's alignment; tokens and
+ * out_tokens of token_bits 32 or 64; accept_u [T] and sample_u [n_seqs] fp32 in [0, 1); cu_seqlens and n_accepted int32, cu_seqlens not trusted, as
+ * in minfer_rope_kv_append_paged.  out_tokens must not overlap tokens.  n_seqs at most 65535.
+ */
+size_t minfer_verify_drafts_workspace_bytes(int64_t n_seqs, int64_t V);
+int minfer_verify_drafts(int prob_dtype, int token_bits, const void* tokens, const int32_t* cu_seqlens, const void* target_probs,
+                         const void* draft_probs, const float* accept_u, const float* sample_u, void* out_tokens, int32_t* n_accepted,
+                         int64_t n_seqs, int64_t T, int64_t V, int64_t target_stride, int64_t draft_stride, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
  * Calibration, not an operator (no counterpart in the reference): `workgroups` workgroups of 8 waves issue
  * 16 * iters v_mfma_f32_16x16x32 (f16 or bf16) each, the instruction the prefill and GEMM kernels are built on, back to
  * back on eight accumulator blocks, from 16 operand fragments (64 lanes x 16 bytes each, 16 KiB in all) that every wave

@@ -12,6 +12,7 @@
 // fails in the dispatcher instead of falling back to anything.
 #include <Python.h>
 
+#include <algorithm>
 #include <optional>
 
 #include <torch/csrc/inductor/aoti_torch/c/shim.h>
@@ -49,6 +50,7 @@ void* current_stream() {
 // 0.1 to 0.3).
 const int32_t kHalf = aoti_torch_dtype_float16(), kBFloat16 = aoti_torch_dtype_bfloat16(), kFloat = aoti_torch_dtype_float32(),
               kByte = aoti_torch_dtype_uint8(), kInt = aoti_torch_dtype_int32(), kBool = aoti_torch_dtype_bool(),
+              kLong = aoti_torch_dtype_int64(),
               kE4m3 = aoti_torch_dtype_float8_e4m3fn(), kE8m0 = (int32_t)ScalarType::Float8_e8m0fnu;   // (the ABI has no name for the last)
 
 // The types that these operators take; Undefined for any other.
@@ -59,6 +61,7 @@ ScalarType type_of(const Tensor& t) {
     if (d == kBFloat16) return ScalarType::BFloat16;
     if (d == kByte) return ScalarType::Byte;
     if (d == kInt) return ScalarType::Int;
+    if (d == kLong) return ScalarType::Long;
     if (d == kBool) return ScalarType::Bool;
     if (d == kE4m3) return ScalarType::Float8_e4m3fn;
     if (d == kE8m0) return ScalarType::Float8_e8m0fnu;
@@ -591,6 +594,106 @@ void flash_attn_paged_fp8_hip(int64_t qtype_int, int64_t qblock_size, int64_t qt
     attend_paged("flash_attn_paged_fp8", qtype_int, q, k_pages, v_pages, ScalePair{&k_scales, &v_scales}, block_table, cu_seqlens, ctx_lens, max_q_len, out);
 }
 
+// ---- a serving step around the paged cache -----------------------------------------------------------------------
+// Page tables from lengths, pages given back, drafted tokens checked.  No counterpart in the reference.
+namespace {
+int32_t* int_ptr(const Tensor& t) { return const_cast<int32_t*>(static_cast<const int32_t*>(t.const_data_ptr())); }
+int32_t* int_out(Tensor& t) { return static_cast<int32_t*>(t.mutable_data_ptr()); }
+
+void check_table(const Tensor& t, int64_t n_seqs, const Tensor& like, const char* op) {
+    STD_TORCH_CHECK(t.is_cuda() && t.get_device_index() == like.get_device_index() && type_of(t) == ScalarType::Int && t.dim() == 2 && t.size(0) == n_seqs &&
+                    (t.size(1) <= 1 || t.stride(1) == 1), op, ": block_table must be int32 [n_seqs, pages per sequence], contiguous in its last dimension");
+}
+minfer_page_ring ring_of(const Tensor& ring, const Tensor& state, Tensor& state_after, const Tensor& like, const char* op) {
+    STD_TORCH_CHECK(ring.dim() == 1, op, ": free_ring must be 1-D, an entry for every page of the pool");
+    check_index(ring, ring.size(0), like, op, "free_ring");
+    check_index(state, 3, like, op, "ring_state");
+    check_index(state_after, 3, like, op, "state_after");
+    return minfer_page_ring{int_ptr(ring), int_ptr(state), int_out(state_after), ring.size(0)};
+}
+}  // namespace
+
+void paged_tables_hip(int64_t page_size, const Tensor& past_lens, const Tensor& new_lens, const Tensor& pages_held, const Tensor& free_ring,
+                      const Tensor& ring_state, Tensor& block_table, Tensor& cu_seqlens, Tensor& ctx_lens, Tensor& slots, Tensor& held_after,
+                      Tensor& state_after) {
+    const char* const op = "paged_tables";
+    STD_TORCH_CHECK(on_gpu(past_lens) && past_lens.dim() == 1, op, ": past_lens must be 1-D and on the GPU");
+    const int64_t n_seqs = past_lens.size(0);
+    check_index(past_lens, n_seqs, past_lens, op, "past_lens");
+    check_index(new_lens, n_seqs, past_lens, op, "new_lens");
+    check_index(pages_held, n_seqs, past_lens, op, "pages_held");
+    check_index(cu_seqlens, n_seqs + 1, past_lens, op, "cu_seqlens");
+    check_index(ctx_lens, n_seqs, past_lens, op, "ctx_lens");
+    check_index(held_after, n_seqs, past_lens, op, "held_after");
+    check_table(block_table, n_seqs, past_lens, op);
+    STD_TORCH_CHECK(slots.is_cuda() && slots.get_device_index() == past_lens.get_device_index() && type_of(slots) == ScalarType::Long && slots.dim() == 1 &&
+                    slots.is_contiguous(), op, ": slots must be contiguous int64 [T] on past_lens' device");
+    const minfer_page_ring ring = ring_of(free_ring, ring_state, state_after, past_lens, op);
+    const OnDeviceOf on(past_lens);
+    check_rc(minfer_paged_tables(page_size, int_ptr(past_lens), int_ptr(new_lens), int_ptr(pages_held), &ring, int_out(block_table), block_table.stride(0),
+                                 block_table.size(1), int_out(cu_seqlens), int_out(ctx_lens), static_cast<int64_t*>(slots.mutable_data_ptr()), slots.size(0),
+                                 int_out(held_after), n_seqs, current_stream()),
+             op);
+}
+
+void paged_release_hip(int64_t page_size, const Tensor& keep_lens, const Tensor& pages_held, const Tensor& block_table, Tensor& free_ring,
+                       const Tensor& ring_state, Tensor& held_after, Tensor& state_after) {
+    const char* const op = "paged_release";
+    STD_TORCH_CHECK(on_gpu(keep_lens) && keep_lens.dim() == 1, op, ": keep_lens must be 1-D and on the GPU");
+    const int64_t n_seqs = keep_lens.size(0);
+    check_index(keep_lens, n_seqs, keep_lens, op, "keep_lens");
+    check_index(pages_held, n_seqs, keep_lens, op, "pages_held");
+    check_index(held_after, n_seqs, keep_lens, op, "held_after");
+    check_table(block_table, n_seqs, keep_lens, op);
+    minfer_page_ring ring = ring_of(free_ring, ring_state, state_after, keep_lens, op);
+    ring.pages = int_out(free_ring);   // (a lazily copied tensor gets memory of its own)
+    const OnDeviceOf on(keep_lens);
+    const size_t ws_bytes = minfer_paged_release_workspace_bytes(n_seqs);
+    const Workspace ws(keep_lens, ws_bytes);
+    check_rc(minfer_paged_release(page_size, int_ptr(keep_lens), int_ptr(pages_held), &ring, int_ptr(block_table), block_table.stride(0), block_table.size(1),
+                                  int_out(held_after), n_seqs, ws.ptr(), ws_bytes, current_stream()),
+             op);
+}
+
+void verify_drafts_hip(const Tensor& tokens, const Tensor& cu_seqlens, const Tensor& target_probs, const std::optional<Tensor>& draft_probs,
+                       const Tensor& accept_u, const Tensor& sample_u, Tensor& out_tokens, Tensor& n_accepted) {
+    const char* const op = "verify_drafts";
+    STD_TORCH_CHECK(on_gpu(tokens) && tokens.dim() == 1 && tokens.is_contiguous(), op, ": tokens must be 1-D, contiguous and on the GPU");
+    const ScalarType t = type_of(tokens), pt = type_of(target_probs);
+    const int64_t T = tokens.size(0);
+    auto here = [&](const Tensor& x) { return x.is_cuda() && x.get_device_index() == tokens.get_device_index(); };
+    STD_TORCH_CHECK(t == ScalarType::Int || t == ScalarType::Long, op, ": tokens must be int32 or int64");
+    STD_TORCH_CHECK(here(out_tokens) && type_of(out_tokens) == t && out_tokens.dim() == 1 && out_tokens.is_contiguous() && out_tokens.size(0) == T, op,
+                    ": out_tokens must be contiguous, of tokens' type, size and device");
+    STD_TORCH_CHECK(pt == ScalarType::Float || pt == ScalarType::Half || pt == ScalarType::BFloat16, op, ": target_probs must be float32, float16 or bfloat16");
+    auto check_probs = [&](const Tensor& x, const char* name) {
+        STD_TORCH_CHECK(here(x) && type_of(x) == pt && x.dim() == 2 && x.size(0) == T && x.size(1) == target_probs.size(1) && (x.size(1) <= 1 || x.stride(1) == 1), op,
+                        ": ", name, " must be [T, vocabulary] on tokens' device, both of one type and contiguous in the last dimension");
+    };
+    check_probs(target_probs, "target_probs");
+    if (draft_probs) check_probs(*draft_probs, "draft_probs");
+    STD_TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) >= 1, op, ": cu_seqlens must be 1-D with at least one entry");
+    const int64_t n_seqs = cu_seqlens.size(0) - 1, V = target_probs.size(1);
+    check_index(cu_seqlens, n_seqs + 1, tokens, op, "cu_seqlens");
+    check_index(n_accepted, n_seqs, tokens, op, "n_accepted");
+    STD_TORCH_CHECK(here(accept_u) && type_of(accept_u) == ScalarType::Float && accept_u.dim() == 1 && accept_u.is_contiguous() && accept_u.size(0) == T, op,
+                    ": accept_u must be contiguous float32 with an entry for every token");
+    STD_TORCH_CHECK(here(sample_u) && type_of(sample_u) == ScalarType::Float && sample_u.dim() == 1 && sample_u.is_contiguous() && sample_u.size(0) == n_seqs, op,
+                    ": sample_u must be contiguous float32 with an entry for every sequence");
+    if (n_seqs == 0) return;
+    const OnDeviceOf on(tokens);
+    const size_t ws_bytes = minfer_verify_drafts_workspace_bytes(n_seqs, V);
+    const Workspace ws(tokens, ws_bytes);
+    // (a single row may have any stride; rows one element apart are those of a vocabulary of one)
+    auto row_stride = [&](const Tensor& x) { return T > 1 ? x.stride(0) : std::max(V, x.stride(0)); };
+    check_rc(minfer_verify_drafts(pt == ScalarType::Float ? MINFER_ATTN_F32 : pt == ScalarType::Half ? MINFER_ATTN_F16 : MINFER_ATTN_BF16,
+                                  t == ScalarType::Long ? 64 : 32, tokens.const_data_ptr(), int_ptr(cu_seqlens), target_probs.const_data_ptr(),
+                                  draft_probs ? draft_probs->const_data_ptr() : nullptr, static_cast<const float*>(accept_u.const_data_ptr()),
+                                  static_cast<const float*>(sample_u.const_data_ptr()), out_tokens.mutable_data_ptr(), int_out(n_accepted), n_seqs, T, V,
+                                  row_stride(target_probs), draft_probs ? row_stride(*draft_probs) : V, ws.ptr(), ws_bytes, current_stream()),
+             op);
+}
+
 // Same signature, argument meaning and checks as the reference's rmsnorm_cuda
 // (reference: src/minfer/kernels/torch_ext/csrc/cuda/rmsnorm/op.cuh:20-70); bfloat16 is admitted as well.
 void rmsnorm_hip(double eps,
@@ -820,6 +923,9 @@ STABLE_TORCH_LIBRARY(minfer, m) {
     m.def("rope_kv_append_norm(int style, int rotary_dim, float freq_base, float eps, Tensor(a!) q, Tensor k, Tensor v, Tensor wq_norm, Tensor wk_norm, Tensor positions, Tensor(b!) k_cache, Tensor(c!) v_cache) -> ()");
     m.def("rope_kv_append_paged(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor positions, Tensor block_table, Tensor(b!) k_pages, Tensor(c!) v_pages) -> ()");
     m.def("rope_kv_append_paged_fp8(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor positions, Tensor block_table, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor(d!) k_scales, Tensor(e!) v_scales) -> ()");
+    m.def("paged_tables(int page_size, Tensor past_lens, Tensor new_lens, Tensor pages_held, Tensor free_ring, Tensor ring_state, Tensor(a!) block_table, Tensor(b!) cu_seqlens, Tensor(c!) ctx_lens, Tensor(d!) slots, Tensor(e!) held_after, Tensor(f!) state_after) -> ()");
+    m.def("paged_release(int page_size, Tensor keep_lens, Tensor pages_held, Tensor block_table, Tensor(a!) free_ring, Tensor ring_state, Tensor(b!) held_after, Tensor(c!) state_after) -> ()");
+    m.def("verify_drafts(Tensor tokens, Tensor cu_seqlens, Tensor target_probs, Tensor? draft_probs, Tensor accept_u, Tensor sample_u, Tensor(a!) out_tokens, Tensor(b!) n_accepted) -> ()");
     m.def("flash_attn_paged(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cu_seqlens, Tensor ctx_lens, int max_q_len, Tensor(a!) out) -> ()");
     m.def("flash_attn_paged_fp8(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor cu_seqlens, Tensor ctx_lens, int max_q_len, Tensor(a!) out) -> ()");
 }
@@ -839,6 +945,9 @@ STABLE_TORCH_LIBRARY_IMPL(minfer, CUDA, m) {  // "CUDA" is PyTorch's dispatch-ke
     m.impl("rope_kv_append_norm", TORCH_BOX(&rope_kv_append_norm_hip));
     m.impl("rope_kv_append_paged", TORCH_BOX(&rope_kv_append_paged_hip));
     m.impl("rope_kv_append_paged_fp8", TORCH_BOX(&rope_kv_append_paged_fp8_hip));
+    m.impl("paged_tables", TORCH_BOX(&paged_tables_hip));
+    m.impl("paged_release", TORCH_BOX(&paged_release_hip));
+    m.impl("verify_drafts", TORCH_BOX(&verify_drafts_hip));
     m.impl("flash_attn_paged", TORCH_BOX(&flash_attn_paged_hip));
     m.impl("flash_attn_paged_fp8", TORCH_BOX(&flash_attn_paged_fp8_hip));
 }

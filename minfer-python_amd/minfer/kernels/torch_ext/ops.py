@@ -2,6 +2,8 @@
 before them, mirroring the reference's wrapper layer (reference:
 src/minfer/kernels/torch_ext/ops.py:60-266): positional pass-through
 to ``torch.ops.minfer.<op>.default``; the result is written into ``out``."""
+from typing import Optional
+
 import torch
 
 _ACT_DTYPES = (torch.float16, torch.bfloat16)
@@ -333,6 +335,97 @@ def flash_attn_paged_fp8(
 def _(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, ctx_lens, max_q_len, out):
     _check_pages(q, k_pages, v_pages, (k_scales, v_scales), block_table, cu_seqlens, ctx_lens)
     torch._check(out.dtype == q.dtype and out.shape == q.shape)
+
+
+_IDS = (torch.int32, torch.int64)
+
+
+def paged_tables(
+    page_size: int,
+    past_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    pages_held: torch.Tensor,
+    free_ring: torch.Tensor,
+    ring_state: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    slots: torch.Tensor,
+    held_after: torch.Tensor,
+    state_after: torch.Tensor,
+):
+    """The index tensors of a step over a paged cache, made on the device from lengths.  Sequence s holds past_lens[s] rows in
+    the first pages_held[s] pages of block_table[s] and gets new_lens[s] rows; the pages that it lacks are taken from the pool's free ones
+    and written behind those (-1 where there are no more).  free_ring [n_pages] holds them as a ring whose ring_state is {first entry, free
+    pages, unused}.  Written: cu_seqlens [n_seqs+1] and ctx_lens [n_seqs] as the paged operators take them (their `positions`
+    are past_lens), slots [T] int64 (the row of the pool of every new token, page * page_size + row, or -1), held_after [n_seqs]
+    and state_after [3] = {first entry, free pages, pages that were lacking}; these two go into the next call, in place of
+    pages_held and ring_state, which must be other tensors.  All other tensors int32."""
+    return torch.ops.minfer.paged_tables.default(page_size, past_lens, new_lens, pages_held, free_ring, ring_state, block_table, cu_seqlens,
+                                                 ctx_lens, slots, held_after, state_after)
+
+
+@torch.library.register_fake("minfer::paged_tables")
+def _(page_size, past_lens, new_lens, pages_held, free_ring, ring_state, block_table, cu_seqlens, ctx_lens, slots, held_after, state_after):
+    ints = (past_lens, new_lens, pages_held, free_ring, ring_state, block_table, cu_seqlens, ctx_lens, held_after, state_after)
+    torch._check(all(t.dtype == torch.int32 for t in ints) and slots.dtype == torch.int64)
+    torch._check(past_lens.device.type == "cuda" and all(t.device == past_lens.device for t in (*ints, slots)))
+    torch._check(block_table.dim() == 2 and all(t.dim() == 1 for t in (*ints[:5], *ints[6:], slots)))
+
+
+def paged_release(
+    page_size: int,
+    keep_lens: torch.Tensor,
+    pages_held: torch.Tensor,
+    block_table: torch.Tensor,
+    free_ring: torch.Tensor,
+    ring_state: torch.Tensor,
+    held_after: torch.Tensor,
+    state_after: torch.Tensor,
+):
+    """Gives pages back to the ring that paged_tables takes them from: sequence s keeps the pages of its first keep_lens[s] rows
+    (0: it ended; a large number: all of them), and those behind, up to pages_held[s], are added to free_ring in the order of sequences and
+    pages; entries that name no page (a window that moved on) are left out.  held_after and state_after as in paged_tables; the
+    table itself is not written.  A page that sequences share must be kept by all of them but one.  All tensors int32."""
+    return torch.ops.minfer.paged_release.default(page_size, keep_lens, pages_held, block_table, free_ring, ring_state, held_after, state_after)
+
+
+@torch.library.register_fake("minfer::paged_release")
+def _(page_size, keep_lens, pages_held, block_table, free_ring, ring_state, held_after, state_after):
+    ints = (keep_lens, pages_held, block_table, free_ring, ring_state, held_after, state_after)
+    torch._check(all(t.dtype == torch.int32 for t in ints))
+    torch._check(keep_lens.device.type == "cuda" and all(t.device == keep_lens.device for t in ints))
+    torch._check(block_table.dim() == 2)
+
+
+def verify_drafts(
+    tokens: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    target_probs: torch.Tensor,
+    draft_probs: Optional[torch.Tensor],
+    accept_u: torch.Tensor,
+    sample_u: torch.Tensor,
+    out_tokens: torch.Tensor,
+    n_accepted: torch.Tensor,
+):
+    """Checks drafted tokens against the target's probabilities, so that what is kept or drawn is distributed as the target says.
+    tokens [T] (int32 or int64) are a step's: of sequence s, cu_seqlens[s] .. cu_seqlens[s+1]-1, the first is known, the others drafts.
+    target_probs [T, V] row t is the target's distribution behind token t, draft_probs row t the one that the draft behind it was drawn
+    from (None: drafts without probabilities, from a look-up).  The draft x behind token t is kept while accept_u[t] *
+    draft_probs[t, x] < target_probs[t, x]; the next token is drawn with sample_u[s] from max(target - draft, 0) of the first row whose
+    draft is not kept, or from the last row's target.  out_tokens [T]: kept drafts, the next token, -1 behind it;
+    n_accepted [n_seqs] int32: the drafts kept.  Random numbers are float32 in [0, 1)."""
+    return torch.ops.minfer.verify_drafts.default(tokens, cu_seqlens, target_probs, draft_probs, accept_u, sample_u, out_tokens, n_accepted)
+
+
+@torch.library.register_fake("minfer::verify_drafts")
+def _(tokens, cu_seqlens, target_probs, draft_probs, accept_u, sample_u, out_tokens, n_accepted):
+    torch._check(tokens.dtype in _IDS and out_tokens.dtype == tokens.dtype and out_tokens.shape == tokens.shape)
+    torch._check(target_probs.dtype in (torch.float32, *_ACT_DTYPES) and target_probs.dim() == 2)
+    torch._check(draft_probs is None or (draft_probs.dtype == target_probs.dtype and draft_probs.shape == target_probs.shape))
+    torch._check(accept_u.dtype == torch.float32 and sample_u.dtype == torch.float32)
+    torch._check(cu_seqlens.dtype == torch.int32 and n_accepted.dtype == torch.int32)
+    torch._check(tokens.device.type == "cuda")
 
 
 def rmsnorm(eps: float, input: torch.Tensor, w: torch.Tensor, out: torch.Tensor):
