@@ -415,6 +415,24 @@ int minfer_rope_kv_append_q8_0(int dtype, int style, void* q, const void* k, con
                                int64_t rotary_dim, double freq_base, void* stream);
 
 /*
+ * minfer_flash_attn_paged for sequences of which groups share their first rows, in pages that all their tables name: the result is that of
+ * minfer_flash_attn_paged up to the order of the sums, and a prefix is read once for a group instead of once for each sequence.  Group i are the sequences
+ * cu_groups[i] .. cu_groups[i+1]-1, the first prefix_lens[i] rows of which lie in the same pages (read through the table of the group's first sequence, in
+ * whole pieces of 64 rows; what is left of a prefix is read through each sequence's own table); sequences in front of the first group and behind the
+ * last have none.  A prefix may reach beyond a sequence's context or into its new tokens: each token attends the rows up to its own.
+ * cu_groups int32 [n_groups + 1] and prefix_lens int32 [n_groups] are on the device and not trusted: what they hold is cut to the sequences and to the table, and no
+ * address is made from more; but the result is that above only where cu_groups does not fall, and cu_seqlens does not either, except for
+ * entries behind the last sequence with tokens.  max_q_len, where it is small, makes the call one for single tokens and drafts (max_q_len * Hq / Hkv <= 64); longer
+ * chunks of prompts are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
+ */
+size_t minfer_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                                      int64_t max_context, int64_t max_q_len);
+int minfer_flash_attn_paged_shared(int dtype, int page_type, const void* q, const minfer_kv_pages* pages,
+                                   const int32_t* cu_seqlens, const int32_t* ctx_lens, const int32_t* cu_groups, const int32_t* prefix_lens,
+                                   void* out, int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len,
+                                   const minfer_attn_strides* st, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * The free pages of a paged cache's pool, a ring of n_pages entries on the device: `count` free pages from entry `head` on, around the
  * ring's end.  state is {head, count, anything}, int32; state_after gets the state behind a call, its third entry the pages that the call could not
  * have (minfer_paged_tables) or had no room for (minfer_paged_release).  state_after must not be state: a program keeps two and exchanges

@@ -542,7 +542,8 @@ void append_paged(const char* op, int64_t style, int64_t rotary_dim, double freq
 }
 
 void attend_paged(const char* op, int64_t qtype_int, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, ScalePair scales,
-                  const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& ctx_lens, int64_t max_q_len, Tensor& out) {
+                  const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& ctx_lens, int64_t max_q_len, Tensor& out,
+                  const Tensor* cu_groups = nullptr, const Tensor* prefix_lens = nullptr) {   // null: no groups that share a prefix
     STD_TORCH_CHECK(on_gpu(q) && on_gpu(out) && out.get_device_index() == q.get_device_index(), op, ": all tensors must be on one GPU");
     STD_TORCH_CHECK(qtype_int != MINFER_Q8_0, op, ": pages of Q8_0 blocks are not built; 8-bit pages are float8_e4m3fn (flash_attn_paged_fp8)");
     const int dtype = activation_code(q, op);
@@ -557,11 +558,29 @@ void attend_paged(const char* op, int64_t qtype_int, const Tensor& q, const Tens
     const minfer_kv_pages pages = pages_of(q, n_seqs, D, block_table, k_pages, v_pages, scales, op);
     const int64_t Hkv = k_pages.size(1);
     STD_TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0, op, ": n_heads must be a multiple of n_kv_heads");
+    int64_t n_groups = 0;
+    if (cu_groups) {
+        STD_TORCH_CHECK(cu_groups->dim() == 1 && cu_groups->size(0) >= 1, op, ": cu_groups must be 1-D with at least one entry");
+        n_groups = cu_groups->size(0) - 1;
+        check_index(*cu_groups, n_groups + 1, q, op, "cu_groups");
+        check_index(*prefix_lens, n_groups, q, op, "prefix_lens");
+        STD_TORCH_CHECK(n_groups <= n_seqs, op, ": more groups than sequences");
+    }
     if (T == 0 || n_seqs == 0) return;
     const OnDeviceOf on(q);
     const minfer_attn_strides st{0, q.stride(1), q.stride(2), 0, 0, 0, 0, out.stride(1), out.stride(2)};
-    const size_t ws_bytes = minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, pages.n_pages > 0 ? pages.pages_per_seq * pages.page_size : 0, max_q_len);
+    const int64_t max_context = pages.n_pages > 0 ? pages.pages_per_seq * pages.page_size : 0;
+    const size_t ws_bytes = cu_groups ? minfer_flash_attn_paged_shared_workspace_bytes(n_seqs, n_groups, T, Hq, Hkv, D, max_context, max_q_len)
+                                      : minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, max_context, max_q_len);
     const Workspace ws(q, ws_bytes);
+    if (cu_groups) {
+        check_rc(minfer_flash_attn_paged_shared(dtype, scales.k ? MINFER_FP8_E4M3 : dtype, q.const_data_ptr(), &pages,
+                                                static_cast<const int32_t*>(cu_seqlens.const_data_ptr()), static_cast<const int32_t*>(ctx_lens.const_data_ptr()),
+                                                static_cast<const int32_t*>(cu_groups->const_data_ptr()), static_cast<const int32_t*>(prefix_lens->const_data_ptr()),
+                                                out.mutable_data_ptr(), n_seqs, n_groups, T, Hq, Hkv, D, max_q_len, &st, ws.ptr(), ws_bytes, current_stream()),
+                 op);
+        return;
+    }
     check_rc(minfer_flash_attn_paged(dtype, scales.k ? MINFER_FP8_E4M3 : dtype, q.const_data_ptr(), &pages,
                                      static_cast<const int32_t*>(cu_seqlens.const_data_ptr()), static_cast<const int32_t*>(ctx_lens.const_data_ptr()),
                                      out.mutable_data_ptr(), n_seqs, T, Hq, Hkv, D, max_q_len, &st, ws.ptr(), ws_bytes, current_stream()),
@@ -592,6 +611,22 @@ void flash_attn_paged_fp8_hip(int64_t qtype_int, int64_t qblock_size, int64_t qt
                               int64_t max_q_len, Tensor& out) {
     (void)qblock_size; (void)qtype_size;
     attend_paged("flash_attn_paged_fp8", qtype_int, q, k_pages, v_pages, ScalePair{&k_scales, &v_scales}, block_table, cu_seqlens, ctx_lens, max_q_len, out);
+}
+
+// The same for groups of sequences that share their first rows (cu_groups [n_groups + 1], prefix_lens [n_groups]), which are read once for a group.
+void flash_attn_paged_shared_hip(int64_t qtype_int, int64_t qblock_size, int64_t qtype_size, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                                 const Tensor& block_table, const Tensor& cu_seqlens, const Tensor& ctx_lens, const Tensor& cu_groups,
+                                 const Tensor& prefix_lens, int64_t max_q_len, Tensor& out) {
+    (void)qblock_size; (void)qtype_size;
+    attend_paged("flash_attn_paged_shared", qtype_int, q, k_pages, v_pages, ScalePair{nullptr, nullptr}, block_table, cu_seqlens, ctx_lens, max_q_len, out, &cu_groups,
+                 &prefix_lens);
+}
+void flash_attn_paged_shared_fp8_hip(int64_t qtype_int, int64_t qblock_size, int64_t qtype_size, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                                     const Tensor& k_scales, const Tensor& v_scales, const Tensor& block_table, const Tensor& cu_seqlens,
+                                     const Tensor& ctx_lens, const Tensor& cu_groups, const Tensor& prefix_lens, int64_t max_q_len, Tensor& out) {
+    (void)qblock_size; (void)qtype_size;
+    attend_paged("flash_attn_paged_shared_fp8", qtype_int, q, k_pages, v_pages, ScalePair{&k_scales, &v_scales}, block_table, cu_seqlens, ctx_lens, max_q_len, out,
+                 &cu_groups, &prefix_lens);
 }
 
 // ---- a serving step around the paged cache -----------------------------------------------------------------------
@@ -923,6 +958,8 @@ STABLE_TORCH_LIBRARY(minfer, m) {
     m.def("rope_kv_append_norm(int style, int rotary_dim, float freq_base, float eps, Tensor(a!) q, Tensor k, Tensor v, Tensor wq_norm, Tensor wk_norm, Tensor positions, Tensor(b!) k_cache, Tensor(c!) v_cache) -> ()");
     m.def("rope_kv_append_paged(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor positions, Tensor block_table, Tensor(b!) k_pages, Tensor(c!) v_pages) -> ()");
     m.def("rope_kv_append_paged_fp8(int style, int rotary_dim, float freq_base, Tensor(a!) q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor positions, Tensor block_table, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor(d!) k_scales, Tensor(e!) v_scales) -> ()");
+    m.def("flash_attn_paged_shared(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cu_seqlens, Tensor ctx_lens, Tensor cu_groups, Tensor prefix_lens, int max_q_len, Tensor(a!) out) -> ()");
+    m.def("flash_attn_paged_shared_fp8(int qtype_int, int qblock_size, int qtype_size, Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor cu_seqlens, Tensor ctx_lens, Tensor cu_groups, Tensor prefix_lens, int max_q_len, Tensor(a!) out) -> ()");
     m.def("paged_tables(int page_size, Tensor past_lens, Tensor new_lens, Tensor pages_held, Tensor free_ring, Tensor ring_state, Tensor(a!) block_table, Tensor(b!) cu_seqlens, Tensor(c!) ctx_lens, Tensor(d!) slots, Tensor(e!) held_after, Tensor(f!) state_after) -> ()");
     m.def("paged_release(int page_size, Tensor keep_lens, Tensor pages_held, Tensor block_table, Tensor(a!) free_ring, Tensor ring_state, Tensor(b!) held_after, Tensor(c!) state_after) -> ()");
     m.def("verify_drafts(Tensor tokens, Tensor cu_seqlens, Tensor target_probs, Tensor? draft_probs, Tensor accept_u, Tensor sample_u, Tensor(a!) out_tokens, Tensor(b!) n_accepted) -> ()");
@@ -945,6 +982,8 @@ STABLE_TORCH_LIBRARY_IMPL(minfer, CUDA, m) {  // "CUDA" is PyTorch's dispatch-ke
     m.impl("rope_kv_append_norm", TORCH_BOX(&rope_kv_append_norm_hip));
     m.impl("rope_kv_append_paged", TORCH_BOX(&rope_kv_append_paged_hip));
     m.impl("rope_kv_append_paged_fp8", TORCH_BOX(&rope_kv_append_paged_fp8_hip));
+    m.impl("flash_attn_paged_shared", TORCH_BOX(&flash_attn_paged_shared_hip));
+    m.impl("flash_attn_paged_shared_fp8", TORCH_BOX(&flash_attn_paged_shared_fp8_hip));
     m.impl("paged_tables", TORCH_BOX(&paged_tables_hip));
     m.impl("paged_release", TORCH_BOX(&paged_release_hip));
     m.impl("verify_drafts", TORCH_BOX(&verify_drafts_hip));

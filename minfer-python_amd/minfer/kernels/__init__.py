@@ -7,7 +7,7 @@ class KernelBackend:
     def __init__(self, backend: str):
         if backend == "torch_ext":
             from .torch_ext import (_dequant, _quant, flash_attn, flash_attn_decode, flash_attn_paged, flash_attn_paged_fp8,
-                                    flash_attn_varlen, gemm, il_rope, neox_rope, paged_release, paged_tables, qkv, rmsnorm, rope_kv_append,
+                                    flash_attn_paged_shared, flash_attn_paged_shared_fp8, flash_attn_varlen, gemm, il_rope, neox_rope, paged_release, paged_tables, qkv, rmsnorm, rope_kv_append,
                                     rope_kv_append_norm, rope_kv_append_paged, rope_kv_append_paged_fp8, verify_drafts)
             self._dequant = _dequant
             self._quant = _quant
@@ -25,6 +25,8 @@ class KernelBackend:
             self.rope_kv_append_paged_fp8 = rope_kv_append_paged_fp8
             self.flash_attn_paged = flash_attn_paged
             self.flash_attn_paged_fp8 = flash_attn_paged_fp8
+            self.flash_attn_paged_shared = flash_attn_paged_shared
+            self.flash_attn_paged_shared_fp8 = flash_attn_paged_shared_fp8
             self.paged_tables = paged_tables
             self.paged_release = paged_release
             self.verify_drafts = verify_drafts

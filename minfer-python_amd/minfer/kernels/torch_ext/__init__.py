@@ -8,7 +8,7 @@ except ImportError as e:  # pragma: no cover
         "minfer.kernels.torch_ext._C is not built; run `python minfer-python_amd/build.py` "
         "(hipcc, gfx950) first"
     ) from e
-from .ops import (flash_attn, flash_attn_decode, flash_attn_paged, flash_attn_paged_fp8, flash_attn_varlen,  # noqa: E402,F401
-                  gemm, il_rope, neox_rope, paged_release, paged_tables, qkv, rmsnorm, rope_kv_append, rope_kv_append_norm,
+from .ops import (flash_attn, flash_attn_decode, flash_attn_paged, flash_attn_paged_fp8, flash_attn_paged_shared,  # noqa: E402,F401
+                  flash_attn_paged_shared_fp8, flash_attn_varlen, gemm, il_rope, neox_rope, paged_release, paged_tables, qkv, rmsnorm, rope_kv_append, rope_kv_append_norm,
                   rope_kv_append_paged, rope_kv_append_paged_fp8, verify_drafts)
 from .ops import dequant as _dequant, quant as _quant  # noqa: E402,F401  (reference: torch_ext/__init__.py:2)

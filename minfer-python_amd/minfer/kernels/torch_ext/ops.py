@@ -337,6 +337,68 @@ def _(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, k_scales, v_scale
     torch._check(out.dtype == q.dtype and out.shape == q.shape)
 
 
+def flash_attn_paged_shared(
+    qtype_int: int,
+    qblock_size: int,
+    qtype_size: int,
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    cu_groups: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    max_q_len: int,
+    out: torch.Tensor,
+):
+    """flash_attn_paged where groups of sequences share their first rows, a prompt that a whole batch stands behind: sequences
+    cu_groups[i] .. cu_groups[i+1]-1 name the same pages for their first prefix_lens[i] rows, which are then read once for the group
+    instead of once for each of them; sequences in front of the first group and behind the last share nothing.  The result is
+    flash_attn_paged's up to the order of the sums.  cu_groups int32 [n_groups+1] and prefix_lens int32 [n_groups] on the device.  Meant for single
+    tokens and drafts: max_q_len, the bound of a sequence's tokens, times the query heads of a KV head up to 64; above that it is flash_attn_paged."""
+    return torch.ops.minfer.flash_attn_paged_shared.default(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages,
+                                           block_table, cu_seqlens, ctx_lens, cu_groups, prefix_lens, max_q_len, out)
+
+
+@torch.library.register_fake("minfer::flash_attn_paged_shared")
+def _(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, block_table, cu_seqlens, ctx_lens, cu_groups, prefix_lens, max_q_len, out):
+    _check_pages(q, k_pages, v_pages, None, block_table, cu_seqlens, ctx_lens)
+    torch._check(all(t.dtype == torch.int32 and t.dim() == 1 and t.device == q.device for t in (cu_groups, prefix_lens)))
+    torch._check(cu_groups.size(0) == prefix_lens.size(0) + 1)
+    torch._check(out.dtype == q.dtype and out.shape == q.shape)
+
+
+def flash_attn_paged_shared_fp8(
+    qtype_int: int,
+    qblock_size: int,
+    qtype_size: int,
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    cu_groups: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    max_q_len: int,
+    out: torch.Tensor,
+):
+    """flash_attn_paged_shared over 8-bit pages, as flash_attn_paged_fp8 takes them."""
+    return torch.ops.minfer.flash_attn_paged_shared_fp8.default(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, k_scales, v_scales,
+                                           block_table, cu_seqlens, ctx_lens, cu_groups, prefix_lens, max_q_len, out)
+
+
+@torch.library.register_fake("minfer::flash_attn_paged_shared_fp8")
+def _(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages, k_scales, v_scales, block_table, cu_seqlens, ctx_lens, cu_groups, prefix_lens, max_q_len, out):
+    _check_pages(q, k_pages, v_pages, (k_scales, v_scales), block_table, cu_seqlens, ctx_lens)
+    torch._check(all(t.dtype == torch.int32 and t.dim() == 1 and t.device == q.device for t in (cu_groups, prefix_lens)))
+    torch._check(cu_groups.size(0) == prefix_lens.size(0) + 1)
+    torch._check(out.dtype == q.dtype and out.shape == q.shape)
+
+
 _IDS = (torch.int32, torch.int64)
 
 
