@@ -73,7 +73,7 @@ template <int BR> MA_DEV Piece find_piece(const PagedParams& p, int x, int& all)
 // 1778 tokens to 12315 rows of codes, 64 heads on 8, a window that moved on: 226 us, 804.  Prompts of 512 and 1024 take 17 and 28: 5 us and 1.4 a tile.
 template <class T, int D, bool FP8, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParams p) {
-    __shared__ __attribute__((aligned(1024))) char lds[TileLds<D, FP8, NW>::BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<D, FP8, NW, false>::BYTES];
     constexpr int BR = NW * 32;
     // ---- which KV head, range of tiles and block of rows; a KV head's workgroups on one XCD (ids go round-robin) ----
     int g, rank;
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(const PagedParam
     if (p.round > 0 && g == 0 && threadIdx.x == 0) reinterpret_cast<int4*>(p.table)[1 + rank] = make_int4(me.seq, me.block, me.part, me.parts);
     const TokenRange range = token_range(const_load(p.cu + me.seq), const_load(p.cu + me.seq + 1), p.T);
     const int ctx = context_of(p.c, const_load(p.ctx + me.seq), range);
-    const TileJob job{g, me.seq, range.lo, ctx, ctx - range.len, min(range.len, p.max_q) * p.n_rep, me.block, me.part, me.parts, rank, 0, 0, false};
+    const TileJob job{g, me.seq, range.lo, ctx, ctx - range.len, min(range.len, p.max_q) * p.n_rep, me.block * BR, 0, me.part, me.parts, rank, 0, 0, 0, 0, false, false};
     attend_tiles<T, D, FP8, NW, false>(p, job, lds);
 }
 

@@ -40,37 +40,44 @@ template <class T> MA_DEV void widen16(u32x4 codes, float scale, s16x8 (&to)[2])
     for (int h = 0; h < 2; ++h) to[h] = __builtin_bit_cast(s16x8, u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]});
 }
 
-// The first 64-key tile of a sequence with a page that is there (its number of tiles if there is none): a window that moved on has given the pages
+// The first row of a sequence in a page that is there (its context if there is none): a window that moved on has given the pages
 // in front of it back.  Looked for only where the first page is missing, 64 pages at a time; the whole wave.
-MA_DEV int first_tile(const PagedCache& c, int seq, int ctx) {
+MA_DEV int first_row(const PagedCache& c, int seq, int ctx) {
     const int32_t* table = c.table + (int64_t)seq * c.table_stride;
     const int lane = threadIdx.x & 63, n = (ctx + (1 << c.page_log2) - 1) >> c.page_log2;
     for (int base = 0; base < n; base += 64) {
         const int i = base + lane;
         const uint64_t hit = __ballot(i < n && (unsigned)table[min(i, n - 1)] < (unsigned)c.n_pages);
-        if (hit) return ((base + __ffsll((unsigned long long)hit) - 1) << c.page_log2) >> 6;
+        if (hit) return (base + __ffsll((unsigned long long)hit) - 1) << c.page_log2;
     }
-    return (ctx + 63) >> 6;
+    return ctx + 63;   // behind the last tile
 }
 
-// LDS of a workgroup: two stages, the rows' area where it has one of its own, the codes' areas.
-template <int D, bool FP8, int NW> struct TileLds {
+// LDS of a workgroup: its stages, the rows' area where it has one of its own, the codes' areas.  A block of one sequence's rows meets tiles that blocks beside
+// it have just read, and two stages do: a tile is on its way for the time of one.  The rows of a group that shares a prefix are few and read tiles
+// nobody has (SHARED): three tiles are on their way, into four stages of 16-bit rows, or into four areas of codes in front of two stages.
+template <int D, bool FP8, int NW, bool SHARED> struct TileLds {
     using GEO = PagedGeom<D, NW>;
     static constexpr int STAGE_BYTES = 2 * GEO::TILE_BYTES;   // the K tile followed by the V tile
     static constexpr int ROWS_BYTES = 32 * GEO::RB;
+    static constexpr int RING = 4;                            // SHARED: stages, or areas of codes
+    static constexpr int STAGES = SHARED && !FP8 ? RING : 2;
     // The waves' query rows on their way in and output rows on their way out: with four waves inside a stage (the query rows in stage 1, which no
     // tile touches before the barrier of tile 0; the output rows in the stage that the last tile did not use), with eight beside them.
-    static constexpr bool kAliasRows = NW * ROWS_BYTES <= STAGE_BYTES;
+    // SHARED: the query rows in the last two stages.
+    static constexpr bool kAliasRows = SHARED || NW * ROWS_BYTES <= STAGE_BYTES;
+    static constexpr int ROWS_AT = SHARED ? (STAGES - 2) * STAGE_BYTES : kAliasRows ? STAGE_BYTES : 2 * STAGE_BYTES;
+    static_assert(!SHARED || NW * ROWS_BYTES <= 2 * STAGE_BYTES, "query rows in two stages");
     static constexpr int NR = FP8 ? GEO::NLD8 : 1;            // loads of codes per wave, tile and tensor
-    static constexpr int RAW_BYTES = FP8 ? 2 * NR * 1024 : 0, RAW_AT = 2 * STAGE_BYTES + (kAliasRows ? 0 : NW * ROWS_BYTES);
-    static constexpr int BYTES = RAW_AT + NW * RAW_BYTES;
+    static constexpr int RAW_BYTES = FP8 ? 2 * NR * 1024 : 0, RAW_AT = STAGES * STAGE_BYTES + (kAliasRows ? 0 : NW * ROWS_BYTES);
+    static constexpr int BYTES = RAW_AT + NW * RAW_BYTES * (SHARED ? RING : 1);
 };
 
-// What a workgroup walks: the `part`-th of `parts` equal pieces of the tiles of a block of rows of KV head g.
-// The rows are `rows` (token, head) pairs from token `lo` on, those of a sequence, whose table row and context these are and whose token 0 stands at pos0; or
-// those of the sequences first .. last - 1 that share a prefix (SHARED): ctx are then the prefix's rows, whole tiles, all of which every row attends, but for
-// tokens that stand inside them (`inside`: there are some).
-struct TileJob { int g, seq, lo, ctx, pos0, rows, block, part, parts, slot, first, last; bool inside; };
+// What a workgroup walks: the tiles of a block of rows of KV head g, the `part`-th of `parts` equal pieces of them; or (SHARED) n_own of them, from tile t_lo on.
+// The rows are (token, head) pairs from token `lo` on, `rows` in all, of which the workgroup's are row0 .. row_end - 1: those of a sequence, whose table row and
+// context these are and whose token 0 stands at pos0; or (`prefix`) those of the sequences first .. last - 1 that share one, ctx being its rows, whole tiles, all
+// of which every row attends, but for tokens that stand inside them (`inside`: there are some).
+struct TileJob { int g, seq, lo, ctx, pos0, rows, row0, row_end, part, parts, slot, t_lo, n_own, first, last; bool prefix, inside; };
 
 MA_DEV int tiles_of(int pos0, int rows, int n_rep, int block, int BR) { return (max(pos0 + min(block * BR + BR - 1, rows - 1) / n_rep + 1, 0) + 63) >> 6; }
 
@@ -85,8 +92,9 @@ MA_DEV int position_of(const PagedParams& p, int first, int last, int t) {
 }
 
 template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tiles(const PagedParams& p, const TileJob& job, char* const lds) {
-    using GEO = PagedGeom<D, NW>;
-    using LDS = TileLds<D, FP8, NW>;
+    using LDS = TileLds<D, FP8, NW, SHARED>;
+    using GEO = typename LDS::GEO;
+    constexpr int KEYS = 64, NB = KEYS / 16;   // of a tile: keys, blocks of 16
     constexpr int RB = GEO::RB, G = GEO::G, RPI = GEO::RPI, NLD = GEO::NLD;
     constexpr int KC = D / 32;   // 32-wide contraction chunks of Q K^T
     constexpr int DB = D / 16;   // 16-row blocks of O^T
@@ -97,35 +105,12 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
     const int lane = threadIdx.x & 63, w = wave_id();
     const int l16 = lane & 15, quad = lane >> 4;
     const int g = job.g, seq = job.seq, ctx = job.ctx;
-    const int last_row = job.rows - 1;
-    const int row0 = job.block * BR + w * 32;                            // the wave's first row
-    const bool wave_on = row0 < job.rows;
-    const int tiles = SHARED ? ctx >> 6 : tiles_of(job.pos0, job.rows, p.n_rep, job.block, BR);
-    int t_first = 0;
-    if (tiles > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages)
-        t_first = __builtin_amdgcn_readfirstlane(first_tile(p.c, seq, ctx));
-    const int n_tiles = max(tiles - t_first, 0), each = n_tiles / job.parts, longer = n_tiles - each * job.parts;
-    const int t_lo = t_first + job.part * each + min(job.part, longer), n_own = each + (job.part < longer ? 1 : 0);
-
-    // positions of the lane's two rows (one per block of 16), cut to the last key, and the wave's least and greatest
-    int pos[2], wave_first, wave_last;
-    if constexpr (SHARED) {
-        pos[0] = pos[1] = wave_first = wave_last = ctx - 1;
-        if (job.inside) {
-#pragma unroll
-            for (int qb = 0; qb < 2; ++qb) pos[qb] = min(ctx - 1, position_of(p, job.first, job.last, job.lo + min(row0 + 16 * qb + l16, last_row) / p.n_rep));
-            wave_first = __builtin_amdgcn_readfirstlane(-(int)wave_max((float)-min(pos[0], pos[1])));   // (rounded, it is off by less than a tile)
-            wave_first -= 64;
-        }
-    } else {
-        wave_first = job.pos0 + min(row0, last_row) / p.n_rep;
-        wave_last = job.pos0 + min(row0 + 31, last_row) / p.n_rep;
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) pos[qb] = job.pos0 + min(row0 + 16 * qb + l16, last_row) / p.n_rep;
-    }
+    const int last_row = (SHARED ? job.row_end : job.rows) - 1;
+    const int row0 = job.row0 + w * 32;                                  // the wave's first row
+    const bool wave_on = row0 <= last_row;
 
     // ---- the wave's query rows, copied global->LDS as whole rows ----
-    char* const q_stage = lds + (kAliasRows ? STAGE_BYTES : 2 * STAGE_BYTES) + w * ROWS_BYTES;
+    char* const q_stage = lds + LDS::ROWS_AT + w * ROWS_BYTES;
 #pragma unroll
     for (int j = 0; j < 32 / RPI; ++j) {
         const int row = j * RPI + lane / G, r = min(row0 + row, last_row), t = r / p.n_rep;
@@ -133,22 +118,63 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         copy16_global_to_lds(src, q_stage + j * RPI * RB);
     }
 
-    // ---- pages: the four 16-row blocks of a tile -----------------------------------------------------------------
+    // ---- pages: the 16-row blocks of a tile -----------------------------------------------------------------
     const int32_t* const table = p.c.table + (int64_t)seq * p.c.table_stride;
-    struct Pages { int id[4]; };
+    struct Pages { int id[NB]; };
     auto pages_of = [&](int kt) __attribute__((always_inline)) {
         Pages r;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) r.id[b] = const_load(table + min((kt * 64 + 16 * b) >> p.c.page_log2, p.c.width - 1));
+        for (int b = 0; b < NB; ++b) r.id[b] = const_load(table + min((kt * KEYS + 16 * b) >> p.c.page_log2, p.c.width - 1));
         return r;
     };
+    int t_lo, n_own;
+    Pages next3[3];
+    if constexpr (SHARED) {
+        t_lo = job.t_lo;
+        n_own = job.n_own;
+        next3[0] = pages_of(t_lo);   // asked for together with the table's first entry
+        next3[1] = pages_of(t_lo + 1);
+        next3[2] = pages_of(t_lo + 2);
+        // (tiles in front of the first page that is there)
+        if (n_own > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages) {
+            const int t_first = min(max(__builtin_amdgcn_readfirstlane(first_row(p.c, seq, ctx)) / KEYS, t_lo), t_lo + n_own);
+            n_own -= t_first - t_lo;
+            t_lo = t_first;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) next3[i] = pages_of(t_lo + i);
+        }
+    } else {
+        const int tiles = tiles_of(job.pos0, job.rows, p.n_rep, job.row0 / BR, BR);
+        int t_first = 0;
+        if (tiles > 0 && (unsigned)const_load(p.c.table + (int64_t)seq * p.c.table_stride) >= (unsigned)p.c.n_pages)
+            t_first = __builtin_amdgcn_readfirstlane(first_row(p.c, seq, ctx)) / KEYS;
+        const int n_tiles = max(tiles - t_first, 0), each = n_tiles / job.parts, longer = n_tiles - each * job.parts;
+        t_lo = t_first + job.part * each + min(job.part, longer);
+        n_own = each + (job.part < longer ? 1 : 0);
+    }
+
+    // positions of the lane's two rows (one per block of 16), cut to the last key, and the wave's least and greatest
+    int pos[2] = {job.pos0 + min(row0 + l16, last_row) / p.n_rep, job.pos0 + min(row0 + 16 + l16, last_row) / p.n_rep};
+    int wave_first = job.pos0 + min(row0, last_row) / p.n_rep, wave_last = job.pos0 + min(row0 + 31, last_row) / p.n_rep;
+    if (SHARED && job.prefix) {
+        pos[0] = pos[1] = wave_first = wave_last = ctx - 1;
+        if (job.inside) {
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) pos[qb] = min(ctx - 1, position_of(p, job.first, job.last, job.lo + min(row0 + 16 * qb + l16, last_row) / p.n_rep));
+            wave_first = __builtin_amdgcn_readfirstlane(-(int)wave_max((float)-min(pos[0], pos[1]))) - 64;   // (as a float it is off by less than a tile)
+        }
+    }
+
     auto is_there = [&](int id) __attribute__((always_inline)) { return (unsigned)id < (unsigned)p.c.n_pages; };
     // bit b: the page of the tile's block b is there
     auto there_of = [&](const Pages& pg) __attribute__((always_inline)) {
-        return (is_there(pg.id[0]) ? 1 : 0) | (is_there(pg.id[1]) ? 2 : 0) | (is_there(pg.id[2]) ? 4 : 0) | (is_there(pg.id[3]) ? 8 : 0);
+        int r = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) r |= is_there(pg.id[b]) ? 1 << b : 0;
+        return r;
     };
-    // whether all 64 rows of a tile exist and hold what was written to them
-    auto whole = [&](int kt, int there) __attribute__((always_inline)) { return kt * 64 + 64 <= ctx && there == 15; };
+    // whether all rows of a tile exist and hold what was written to them
+    auto whole = [&](int kt, int there) __attribute__((always_inline)) { return kt * KEYS + KEYS <= ctx && there == (1 << NB) - 1; };
     const int page_mask = (1 << p.c.page_log2) - 1;
     // rows first .. of tile kt, which lie in page `id`: their offset in a pool, in elements (a page that is not there: page 0, whose
     // rows are there to be read)
@@ -164,15 +190,15 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         k_off = (uint32_t)(row_in * (int)p.c.row_stride + 8 * (gr ^ GEO::swz_k(row))) * 2u;
         v_off = (uint32_t)(row_in * (int)p.c.row_stride + 8 * (gr ^ GEO::swz_v(row))) * 2u;
     }
-    auto copy_tile = [&](int kt, const Pages& pg, auto stage_tag) __attribute__((always_inline)) {
+    auto copy_tile = [&](int kt, const Pages& pg, auto stage_tag, uint32_t dst) __attribute__((always_inline)) {
         for_range<0, NLD>([&](auto j_tag) __attribute__((always_inline)) {
             constexpr int j = decltype(j_tag)::value, b0 = j * NW * RPI / 16;
             constexpr int AT = decltype(stage_tag)::value * STAGE_BYTES + j * NW * 1024;
-            const int id = NW * RPI == 16 ? pg.id[b0] : (w * RPI < 16 ? pg.id[b0] : pg.id[(b0 + 1) & 3]);
+            const int id = NW * RPI == 16 ? pg.id[b0] : (w * RPI < 16 ? pg.id[b0] : pg.id[(b0 + 1) % NB]);
             static_assert(NW * RPI == 16 || NW * RPI == 32, "a round of copies covers one or two blocks of 16 rows");
-            const int64_t at = rows_at(id, kt * 64 + (j * NW + w) * RPI);
-            copy16_global_to_lds_at<AT, true>((const short*)p.c.k + at, k_off, dst0);
-            copy16_global_to_lds_at<AT + GEO::TILE_BYTES, true>((const short*)p.c.v + at, v_off, dst0);
+            const int64_t at = rows_at(id, kt * KEYS + (j * NW + w) * RPI);
+            copy16_global_to_lds_at<AT, true>((const short*)p.c.k + at, k_off, dst);
+            copy16_global_to_lds_at<AT + GEO::TILE_BYTES, true>((const short*)p.c.v + at, v_off, dst);
         });
     };
     // V rows of a tile that nothing may be multiplied with: the wave clears those that it copied itself
@@ -180,38 +206,71 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         for_range<0, NLD>([&](auto j_tag) __attribute__((always_inline)) {
             constexpr int j = decltype(j_tag)::value;
             const int row = (j * NW + w) * RPI + lane / G;
-            if (kt * 64 + row >= ctx || !(there >> (row >> 4) & 1))
+            if (kt * KEYS + row >= ctx || !(there >> (row >> 4) & 1))
                 *reinterpret_cast<u32x4*>(lds + stage * STAGE_BYTES + GEO::TILE_BYTES + (j * NW + w) * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
         });
     };
     // ---- 8-bit rows: global -> the wave's own LDS area as they are, and from there through registers into a stage.  Load j of the wave covers
     // rows (j * NW + w) * RPI8 .., 8 or 16 of one block, 16 codes a lane, which the lane itself reads back.
     constexpr int NR = LDS::NR, RPI8 = GEO::RPI8;
-    const uint32_t raw0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(lds + (FP8 ? LDS::RAW_AT + w * LDS::RAW_BYTES : 0)));
+    const uint32_t raw0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(lds + (FP8 ? LDS::RAW_AT + w * LDS::RAW_BYTES * (SHARED ? LDS::RING : 1) : 0)));
     struct Scales { uint32_t k[NR], v[NR]; } scales{};   // of the tile in the raw area, as their bytes
     const uint32_t c_off = (uint32_t)((lane / (D / 16)) * (int)p.c.row_stride + 16 * (lane % (D / 16)));
     auto block_of = [&](int j) __attribute__((always_inline)) { return ((j * NW + w) * RPI8) >> 4; };
-    auto request_codes = [&](int kt, const Pages& pg) __attribute__((always_inline)) {
+    auto page_of = [&](const Pages& pg, int b) __attribute__((always_inline)) {
+        return NB == 2 ? (b == 0 ? pg.id[0] : pg.id[1]) : b == 0 ? pg.id[0] : b == 1 ? pg.id[1] : b == 2 ? pg.id[NB / 2] : pg.id[NB - 1];
+    };
+    auto request_codes = [&](int kt, const Pages& pg, uint32_t raw) __attribute__((always_inline)) {
         for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
             constexpr int j = decltype(j_tag)::value;
-            const int b = block_of(j), id = b == 0 ? pg.id[0] : b == 1 ? pg.id[1] : b == 2 ? pg.id[2] : pg.id[3];
-            const int64_t at = rows_at(id, kt * 64 + (j * NW + w) * RPI8);
-            copy16_global_to_lds_at<2 * j * 1024, true>((const char*)p.c.k + at, c_off, raw0);
-            copy16_global_to_lds_at<(2 * j + 1) * 1024, true>((const char*)p.c.v + at, c_off, raw0);
+            const int id = page_of(pg, block_of(j));
+            const int64_t at = rows_at(id, kt * KEYS + (j * NW + w) * RPI8);
+            copy16_global_to_lds_at<2 * j * 1024, true>((const char*)p.c.k + at, c_off, raw);
+            copy16_global_to_lds_at<(2 * j + 1) * 1024, true>((const char*)p.c.v + at, c_off, raw);
         });
     };
     auto scales_of = [&](const Pages& pg) __attribute__((always_inline)) {
         Scales r;
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
-            const int b = block_of(j), id = b == 0 ? pg.id[0] : b == 1 ? pg.id[1] : b == 2 ? pg.id[2] : pg.id[3];
+            const int id = page_of(pg, block_of(j));
             const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
             r.k[j] = const_byte(p.c.k_scales + sc);
             r.v[j] = const_byte(p.c.v_scales + sc);
         }
         return r;
     };
-    auto widen_tile = [&](int kt, int there, int stage) __attribute__((always_inline)) {
+    // The same in two halves (SHARED): the codes of the wave's own area widened into registers in front of a barrier, and behind it stored.
+    struct Wide { s16x8 k[2 * NR], v[2 * NR]; };
+    auto widen = [&](int kt, int there, uint32_t raw) __attribute__((always_inline)) {
+        Wide r;
+        for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
+            constexpr int j = decltype(j_tag)::value;
+            const bool on = (there >> block_of(j) & 1) && kt * KEYS + (j * NW + w) * RPI8 + lane / (D / 16) < ctx;
+            s16x8 x[2];
+            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw + 16 * lane, 2 * j * 1024)), scale_value(scales.k[j]), x);
+            r.k[2 * j] = x[0]; r.k[2 * j + 1] = x[1];
+            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw + 16 * lane, (2 * j + 1) * 1024)), scale_value(scales.v[j]), x);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) r.v[2 * j + h] = on ? x[h] : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        });
+        return r;
+    };
+    auto store_wide = [&](const Wide& x, int stage) __attribute__((always_inline)) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));   // (as below)
+        const int row_in = ln / (D / 16), gr = 2 * (ln % (D / 16)), row_w = w * RPI8 + row_in;
+        const uint32_t base = lds_addr(lds) + stage * STAGE_BYTES + row_w * RB;
+        const uint32_t k_to = base + 16 * (gr ^ GEO::swz_k(row_w)), v_to = base + GEO::TILE_BYTES + 16 * (gr ^ GEO::swz_v(row_w));
+        for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
+            constexpr int j = decltype(j_tag)::value, AT = j * NW * RPI8 * RB;
+            lds_write_b128(k_to, AT, x.k[2 * j]);
+            lds_write_b128(k_to ^ 16u, AT, x.k[2 * j + 1]);
+            lds_write_b128(v_to, AT, x.v[2 * j]);
+            lds_write_b128(v_to ^ 16u, AT, x.v[2 * j + 1]);
+        });
+    };
+    auto widen_tile = [&](int kt, int there, int stage, uint32_t raw) __attribute__((always_inline)) {
         // (the lane's places are worked out for every tile: ten instructions; kept across tiles they do not fit the registers at D = 128)
         int ln = lane;
         asm volatile("" : "+v"(ln));
@@ -221,12 +280,12 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         static_assert((NW * RPI8) % 16 == 0 && GEO::TILE_BYTES % 32 == 0, "granule gr + 1 is at the address of gr with bit 4 turned");
         for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
             constexpr int j = decltype(j_tag)::value, AT = j * NW * RPI8 * RB;
-            const bool on = (there >> block_of(j) & 1) && kt * 64 + j * NW * RPI8 + row_w < ctx;
+            const bool on = (there >> block_of(j) & 1) && kt * KEYS + j * NW * RPI8 + row_w < ctx;
             s16x8 x[2];
-            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw0 + 16 * ln, 2 * j * 1024)), scale_value(scales.k[j]), x);
+            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw + 16 * ln, 2 * j * 1024)), scale_value(scales.k[j]), x);
             lds_write_b128(k_to, AT, x[0]);
             lds_write_b128(k_to ^ 16u, AT, x[1]);
-            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw0 + 16 * ln, (2 * j + 1) * 1024)), scale_value(scales.v[j]), x);
+            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw + 16 * ln, (2 * j + 1) * 1024)), scale_value(scales.v[j]), x);
             lds_write_b128(v_to, AT, on ? x[0] : s16x8{0, 0, 0, 0, 0, 0, 0, 0});
             lds_write_b128(v_to ^ 16u, AT, on ? x[1] : s16x8{0, 0, 0, 0, 0, 0, 0, 0});
         });
@@ -264,7 +323,7 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
 
     auto process_tile = [&](auto stage_tag, int kt, int there) __attribute__((always_inline)) {
         constexpr int SOFF = decltype(stage_tag)::value * STAGE_BYTES;
-        const int key0 = kt * 64;
+        const int key0 = kt * KEYS;
         auto pin = [&]() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
         auto read_v = [&](int ck, int db) __attribute__((always_inline)) -> s16x8 {
             const s16x4 t0 = lds_read_tr16(v_rd[db], SOFF + (32 * ck) * RB), t1 = lds_read_tr16(v_rd[db], SOFF + (32 * ck + 16) * RB);
@@ -272,16 +331,16 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         };
         s16x8 va[DB];
         // S^T = K Q^T: register e of block [kb][qb] is key 16kb + 4 quad + e of row 16qb + l16
-        f32x4 e_acc[4][2];
+        f32x4 e_acc[NB][2];
         {
-            s16x8 kf[2][4];
+            s16x8 kf[2][NB];
 #pragma unroll
             for (int c = 0; c < 2 && c < KC; ++c)
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb) kf[c][kb] = lds_read_b128(k_rd[c], SOFF + 16 * kb * RB);
+                for (int kb = 0; kb < NB; ++kb) kf[c][kb] = lds_read_b128(k_rd[c], SOFF + 16 * kb * RB);
             pin();
-            for_range<0, KC * 4>([&](auto i_tag) __attribute__((always_inline)) {
-                constexpr int i = decltype(i_tag)::value, c = i / 4, kb = i % 4;
+            for_range<0, KC * NB>([&](auto i_tag) __attribute__((always_inline)) {
+                constexpr int i = decltype(i_tag)::value, c = i / NB, kb = i % NB;
 #pragma unroll
                 for (int qb = 0; qb < 2; ++qb) e_acc[kb][qb] = T::mfma16(kf[c & 1][kb], qf[qb][c], c == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : e_acc[kb][qb]);
                 pin();
@@ -289,25 +348,28 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
                     kf[c & 1][kb] = lds_read_b128(k_rd[c + 2], SOFF + 16 * kb * RB);
                 } else if (c + 1 == KC) {
 #pragma unroll
-                    for (int db = kb * (DB / 4); db < (kb + 1) * (DB / 4); ++db) va[db] = read_v(0, db);
+                    for (int db = kb * (DB / NB); db < (kb + 1) * (DB / NB); ++db) va[db] = read_v(0, db);
                 }
                 pin();
             });
         }
-        if (key0 + 63 > wave_first) {
+        if (key0 + KEYS - 1 > wave_first) {
             // V rows that some of the wave's tokens attend and others do not: whether all are finite is what products with zero say
             f32x4 probe = {0.f, 0.f, 0.f, 0.f};
             const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-            for (int db = 0; db < DB; ++db) probe = T::mfma16(read_v(1, db), zero, T::mfma16(va[db], zero, probe));
+            for (int db = 0; db < DB; ++db) {
+                probe = T::mfma16(va[db], zero, probe);
+                if (NB == 4) probe = T::mfma16(read_v(1, db), zero, probe);
+            }
             if (__any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.f))) { by_key = kt; return; }
         }
-        if (key0 + 63 > wave_first || !whole(kt, there)) {
+        if (key0 + KEYS - 1 > wave_first || !whole(kt, there)) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
                 const int lim = pos[qb] - key0 - 4 * quad;   // largest kept 16kb + e
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb) {
+                for (int kb = 0; kb < NB; ++kb) {
                     const int lim_kb = there >> kb & 1 ? lim : -1;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) e_acc[kb][qb][e] = 16 * kb + e <= lim_kb ? e_acc[kb][qb][e] : -INFINITY;
@@ -321,9 +383,9 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
                 float m = max3(e_acc[0][qb][0], e_acc[0][qb][1], e_acc[0][qb][2]);
                 m = max3(m, e_acc[0][qb][3], e_acc[1][qb][0]);
 #pragma unroll
-                for (int kb = 1; kb < 4; ++kb) {
+                for (int kb = 1; kb < NB; ++kb) {
                     m = max3(m, e_acc[kb][qb][1], e_acc[kb][qb][2]);
-                    m = kb < 3 ? max3(m, e_acc[kb][qb][3], e_acc[kb + 1][qb][0]) : max2(m, e_acc[kb][qb][3]);
+                    m = kb < NB - 1 ? max3(m, e_acc[kb][qb][3], e_acc[(kb + 1) % NB][qb][0]) : max2(m, e_acc[kb][qb][3]);
                 }
                 mx[qb] = m;
             }
@@ -361,15 +423,15 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         for (int i = 0; i < 4; ++i) pw[0][i] = weights_quarter(0, 0, i);
         pin();
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int s = 0; s < NB; ++s) {
             const int ck = s >> 1, qb = s & 1;
             const s16x8 pcur = __builtin_bit_cast(s16x8, u32x4{pw[s & 1][0], pw[s & 1][1], pw[s & 1][2], pw[s & 1][3]});
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
                 o_acc[db][qb] = T::mfma16(va[db], pcur, o_acc[db][qb]);
                 pin();
-                if (qb == 1 && ck == 0) va[db] = read_v(1, db);
-                if (s + 1 < 4 && db < 4) pw[(s + 1) & 1][db] = weights_quarter((s + 1) >> 1, (s + 1) & 1, db);
+                if (qb == 1 && ck + 1 < NB / 2) va[db] = read_v(1, db);
+                if (s + 1 < NB && db < 4) pw[(s + 1) & 1][db] = weights_quarter((s + 1) >> 1, (s + 1) & 1, db);
                 pin();
             }
         }
@@ -377,71 +439,162 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         l_sum[1] += ls[1];
     };
 
-    // ---- main loop: one barrier per tile, the next tile's rows on their way under it ----
-    Pages pg{};                   // of the next tile to be requested
-    int there = 0, there_1 = 0;   // pages of the tile at work and of the one behind it
-    if (n_own > 0) {
-        pg = pages_of(t_lo);
-        there = there_of(pg);
-        if (FP8) { request_codes(t_lo, pg); scales = scales_of(pg); }
-        else copy_tile(t_lo, pg, std::integral_constant<int, 0>{});
-        pg = pages_of(t_lo + 1);
-    }
-    // the query rows were requested first
-    if (!FP8 && n_own > 0) wait_vmcnt<2 * NLD>(); else wait_vmcnt<0>();
-    {
+    // ---- main loop: one barrier per tile, the rows of the next ones on their way under it ----
+    auto read_queries = [&]() __attribute__((always_inline)) {
         const uint32_t qa = lds_addr(q_stage) + l16 * RB;
         const int sw = GEO::swz_k(l16);
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
             for (int c = 0; c < KC; ++c) qf[qb][c] = lds_read_b128(qa + 16 * ((4 * c + quad) ^ sw), 16 * qb * RB);
-    }
-    if (FP8 && n_own > 0) {
-        widen_tile(t_lo, there, 0);
-        if (n_own > 1) { request_codes(t_lo + 1, pg); scales = scales_of(pg); }
-        there_1 = there_of(pg);
-        pg = pages_of(t_lo + 2);
-    }
-    auto iteration = [&](auto stage_tag, int it) {
-        constexpr int STAGE = decltype(stage_tag)::value;
-        const int kt = t_lo + it;
-        int there_2 = 0;
-        // The table's entries, and the scales of codes about to be sent for, are asked for here and waited for in front of the barrier, where the wave
-        // waits anyway: scalar loads return in no order, so that with one on its way every wait for an LDS read is one for all of them.
-        Pages after = pages_of(FP8 ? kt + 3 : kt + 2);
-        Scales scales_2{};
-        if (FP8) scales_2 = scales_of(pg);
-        if (!FP8) {
-            wait_vmcnt<0>();       // this wave's share of the tile has landed
-            if (!whole(kt, there)) clear_rows(kt, there, STAGE);
-        }
-        asm volatile("" : "+s"(after.id[0]), "+s"(after.id[1]), "+s"(after.id[2]), "+s"(after.id[3]));
-        if (FP8) {
-#pragma unroll
-            for (int j = 0; j < NR; ++j) asm volatile("" : "+s"(scales_2.k[j]), "+s"(scales_2.v[j]));
-        }
-        __syncthreads();           // everyone's has; the other stage is no longer being read
-        if (it + 1 < n_own) {
-            if (FP8) {
-                wait_vmcnt<0>();   // the wave's codes of the next tile have
-                widen_tile(kt + 1, there_1, STAGE ^ 1);
-                if (it + 2 < n_own) request_codes(kt + 2, pg);
-                there_2 = there_of(pg);
-                scales = scales_2;
-            } else {
-                copy_tile(kt + 1, pg, std::integral_constant<int, STAGE ^ 1>{});
-                there_1 = there_of(pg);
-            }
-            pg = after;
-        }
-        if (wave_on && there && kt * 64 <= wave_last && kt < by_key) process_tile(stage_tag, kt, there);
-        there = there_1;
-        there_1 = there_2;
     };
-    for (int it = 0; it < n_own; it += 2) {
-        iteration(std::integral_constant<int, 0>{}, it);
-        if (it + 1 < n_own) iteration(std::integral_constant<int, 1>{}, it + 1);
+    auto pin_pages = [&](Pages& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) asm volatile("" : "+s"(x.id[b]));
+    };
+    if constexpr (!SHARED) {
+        Pages pg{};                   // of the next tile to be requested
+        int there = 0, there_1 = 0;   // pages of the tile at work and of the one behind it
+        if (n_own > 0) {
+            pg = pages_of(t_lo);
+            there = there_of(pg);
+            if (FP8) { request_codes(t_lo, pg, raw0); scales = scales_of(pg); }
+            else copy_tile(t_lo, pg, std::integral_constant<int, 0>{}, dst0);
+            pg = pages_of(t_lo + 1);
+        }
+        // the query rows were requested first
+        if (!FP8 && n_own > 0) wait_vmcnt<2 * NLD>(); else wait_vmcnt<0>();
+        read_queries();
+        if (FP8 && n_own > 0) {
+            widen_tile(t_lo, there, 0, raw0);
+            if (n_own > 1) { request_codes(t_lo + 1, pg, raw0); scales = scales_of(pg); }
+            there_1 = there_of(pg);
+            pg = pages_of(t_lo + 2);
+        }
+        auto iteration = [&](auto stage_tag, int it) {
+            constexpr int STAGE = decltype(stage_tag)::value;
+            const int kt = t_lo + it;
+            int there_2 = 0;
+            // The table's entries, and the scales of codes about to be sent for, are asked for here and waited for in front of the barrier, where the wave
+            // waits anyway: scalar loads return in no order, so that with one on its way every wait for an LDS read is one for all of them.
+            Pages after = pages_of(FP8 ? kt + 3 : kt + 2);
+            Scales scales_2{};
+            if (FP8) scales_2 = scales_of(pg);
+            if (!FP8) {
+                wait_vmcnt<0>();       // this wave's share of the tile has landed
+                if (!whole(kt, there)) clear_rows(kt, there, STAGE);
+            }
+            pin_pages(after);
+            if (FP8) {
+    #pragma unroll
+                for (int j = 0; j < NR; ++j) asm volatile("" : "+s"(scales_2.k[j]), "+s"(scales_2.v[j]));
+            }
+            __syncthreads();           // everyone's has; the other stage is no longer being read
+            if (it + 1 < n_own) {
+                if (FP8) {
+                    wait_vmcnt<0>();   // the wave's codes of the next tile have
+                    widen_tile(kt + 1, there_1, STAGE ^ 1, raw0);
+                    if (it + 2 < n_own) request_codes(kt + 2, pg, raw0);
+                    there_2 = there_of(pg);
+                    scales = scales_2;
+                } else {
+                    copy_tile(kt + 1, pg, std::integral_constant<int, STAGE ^ 1>{}, dst0);
+                    there_1 = there_of(pg);
+                }
+                pg = after;
+            }
+            if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(stage_tag, kt, there);
+            there = there_1;
+            there_1 = there_2;
+        };
+        for (int it = 0; it < n_own; it += 2) {
+            iteration(std::integral_constant<int, 0>{}, it);
+            if (it + 1 < n_own) iteration(std::integral_constant<int, 1>{}, it + 1);
+        }
+    } else {
+        constexpr int RING = LDS::RING, STAGES = LDS::STAGES, LOADS = FP8 ? 2 * NR : 2 * NLD;   // a wave's copies of a tile
+        // until all but the last `tiles` tiles of those that the wave asked for are there
+        auto wait_but = [&](int tiles) __attribute__((always_inline)) {
+            static_assert(3 * LOADS < 64, "counted by six bits");
+            if (tiles >= 3) wait_vmcnt<3 * LOADS>(); else if (tiles == 2) wait_vmcnt<2 * LOADS>(); else if (tiles == 1) wait_vmcnt<LOADS>(); else wait_vmcnt<0>();
+        };
+        // (on to the next stage: the addresses, not the code, go round the ring)
+        auto next_stage = [&](int it) __attribute__((always_inline)) {
+            const uint32_t step = (it & (STAGES - 1)) == STAGES - 1 ? (uint32_t)(-(STAGES - 1) * STAGE_BYTES) : (uint32_t)STAGE_BYTES;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) k_rd[c] += step;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) v_rd[db] += step;
+        };
+        const std::integral_constant<int, 0> zero{};
+        Pages pg = next3[0], pg1 = next3[1];
+        const Pages pg2 = next3[2];
+        int theres = there_of(pg) | there_of(pg1) << NB;   // pages that are there, NB bits a tile: of the tile at work and those behind it
+        if constexpr (!FP8) {
+            if (n_own > 0) copy_tile(t_lo, pg, zero, dst0);
+            if (n_own > 1) copy_tile(t_lo + 1, pg1, zero, dst0 + STAGE_BYTES);
+            wait_but(min(n_own, 2));   // the query rows were requested first
+            read_queries();
+            __syncthreads();           // everyone's are read, out of the stages of the next tiles
+            if (n_own > 2) copy_tile(t_lo + 2, pg2, zero, dst0 + 2 * STAGE_BYTES);
+            theres |= there_of(pg2) << 2 * NB;
+            pg = pages_of(t_lo + 3);
+            for (int it = 0; it < n_own; ++it) {
+                const int kt = t_lo + it, there = theres & ((1 << NB) - 1);
+                Pages after = pages_of(kt + 4);
+                wait_but(min(n_own - 1 - it, 2));   // this wave's share of the tile has landed
+                if (!whole(kt, there)) clear_rows(kt, there, it & (STAGES - 1));
+                pin_pages(after);
+                __syncthreads();                    // everyone's has; the stage of the tile in front is no longer being read
+                if (it + 3 < n_own) copy_tile(kt + 3, pg, zero, dst0 + ((it + 3) & (STAGES - 1)) * STAGE_BYTES);
+                theres = theres >> NB | there_of(pg) << 2 * NB;
+                pg = after;
+                if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(zero, kt, there);
+                next_stage(it);
+            }
+        } else {
+            constexpr int AREA = LDS::RAW_BYTES;
+            if (n_own > 0) request_codes(t_lo, pg, raw0);
+            if (n_own > 1) request_codes(t_lo + 1, pg1, raw0 + AREA);
+            if (n_own > 2) request_codes(t_lo + 2, pg2, raw0 + 2 * AREA);
+            scales = scales_of(pg);
+            Scales scales_1 = scales_of(pg1);
+            pg = pages_of(t_lo + 3);
+            pg1 = pg2;                 // of the tile whose scales are asked for next
+            wait_but(min(n_own, 3));
+            read_queries();
+            __syncthreads();
+            if (n_own > 3) request_codes(t_lo + 3, pg, raw0 + 3 * AREA);
+            if (n_own > 0) {
+                wait_but(min(n_own - 1, 3));
+                store_wide(widen(t_lo, theres & ((1 << NB) - 1), raw0), 0);
+            }
+            scales = scales_1;
+            pg = pages_of(t_lo + 4);
+            for (int it = 0; it < n_own; ++it) {
+                const int kt = t_lo + it, there = theres & ((1 << NB) - 1);
+                Pages after = pages_of(kt + 5), after_1 = pages_of(kt + 3);
+                scales_1 = scales_of(pg1);
+                pin_pages(after);
+                pin_pages(after_1);
+#pragma unroll
+                for (int j = 0; j < NR; ++j) asm volatile("" : "+s"(scales_1.k[j]), "+s"(scales_1.v[j]));
+                Wide wide{};
+                if (it + 1 < n_own) {
+                    wait_but(min(n_own - 2 - it, 2));   // the wave's codes of the next tile have landed
+                    wide = widen(kt + 1, theres >> NB & ((1 << NB) - 1), raw0 + ((it + 1) & (RING - 1)) * AREA);
+                }
+                __syncthreads();       // everyone's share of the tile is widened; the other stage is no longer being read
+                theres = theres >> NB | there_of(pg1) << NB;
+                if (it + 4 < n_own) request_codes(kt + 4, pg, raw0 + (it & (RING - 1)) * AREA);
+                if (it + 1 < n_own) store_wide(wide, (it + 1) & 1);
+                scales = scales_1;
+                pg = after;
+                pg1 = after_1;
+                if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(zero, kt, there);
+                next_stage(it);
+            }
+        }
     }
 
     if (!wave_on) return;
@@ -453,7 +606,7 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
             const int r = min(row0 + 16 * qb + l16, last_row), t = r / p.n_rep;
             q[qb] = (const short*)p.q + (int64_t)(job.lo + t) * p.q2 + (int64_t)(g * p.n_rep + r - t * p.n_rep) * p.q1;
         }
-        attend_key_by_key<T, D, FP8, 2>(p.c, p.Hkv, seq, g, by_key * 64, min(wave_last + 1, (t_lo + n_own) * 64), q, limit, c2,
+        attend_key_by_key<T, D, FP8, 2>(p.c, p.Hkv, seq, g, by_key * KEYS, min(wave_last + 1, (t_lo + n_own) * KEYS), q, limit, c2,
                                         [&](int db, int qb) __attribute__((always_inline)) -> f32x4& { return o_acc[db][qb]; }, m_ref, l_sum);
     }
     float l_all[2];

@@ -18,18 +18,23 @@ namespace minfer_attn {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSharedWaves = 4, kBlockRows = kSharedWaves * 32;
-constexpr int kSharedUnits = 256, kSharedWgs = 2 * kSharedUnits;   // workgroups of the launch: what the chip holds at once
+// Waves of a workgroup, up to 32 rows of a block each, and workgroups of the launch, as many as the chip holds at once: four tiles of 32 KiB leave room for one on a
+// compute unit, of 16 KiB (head_dim 64) for two.
+constexpr int shared_waves(int64_t D) { return D == 128 ? 8 : 4; }
+constexpr int shared_wgs(int64_t D) { return 256 * 8 / shared_waves(D); }
+template <int D> constexpr int kSharedWaves = shared_waves(D);
+template <int D> constexpr int kBlockRows = shared_waves(D) * 32;
+constexpr int64_t kSharedBytes = 220000000, kSharedBytesCodes = 150000000;   // of all rows that the tables may name (shared_takes)
 constexpr int kMaxSharedHeads = 128;                               // KV heads: each has workgroups of its own for the prefix
 
 struct SharedWork {
     DecodeWork d;                    // of the own rows; part_o / part_ml of d.p are theirs
     const int32_t* cu_groups; const int32_t* prefix;
     int n_groups;
-    float* tile_o; float* tile_ml;   // partial results of the prefixes: [piece][KV head][128][D] and their references and sums
+    float* tile_o; float* tile_ml;   // partial results of the tiles: [piece][KV head][row of the block][D] and their references and sums
     int max_pieces;                  // that there is room for
-    int32_t* seq_tab;                // [n_seqs][2]: a sequence's place on the line, its group (-1: none); then the quota
-    i32x4* group_tab;                 // [n_groups]: first token, (token, head) rows, first piece, pieces of a block of rows
+    i32x4* seq_tab;                  // [n_seqs]: a sequence's place on its line, its group (-1: none); then the quotas of both lines
+    i32x4* group_tab;                // [n_groups]: first token, (token, head) rows, place of its first block on the line of tiles, that block's number
 };
 
 // Rows of group i's prefix that are computed for all its tokens together: whole tiles.
@@ -45,15 +50,15 @@ MA_DEV int group_of(const SharedWork& w, int s) {
     return lo < w.n_groups && w.cu_groups[lo] <= s ? lo : -1;
 }
 
-struct OwnSeq { SeqInfo info; int group, g0, groups; };   // g0: the first group of rows behind the prefix; groups: how many there are
+// What a sequence has behind the prefix: the first group of rows and how many there are.
+struct OwnSeq { SeqInfo info; int group, g0, groups; };
 template <int GR> MA_DEV OwnSeq own_seq(const SharedWork& w, int s) {   // (per lane)
     OwnSeq r{{0, 0, 0}, -1, 0, 0};
     if (s < w.d.p.n_seqs) {
-        const LineSeq q = line_seq<GR>(w.d, s);
-        r.info = q.info;
+        r.info = line_seq<16>(w.d, s).info;
         r.group = group_of(w, s);
         r.g0 = r.group >= 0 ? shared_rows(w, r.group) / GR : 0;
-        r.groups = max(q.groups - r.g0, 0);
+        r.groups = r.info.len > 0 ? max((r.info.ctx + GR - 1) / GR - r.g0, 0) : 0;
     }
     return r;
 }
@@ -87,89 +92,118 @@ MA_DEV Group group_at(const SharedWork& w, int i) {
     return r;
 }
 
-// How the launch is laid out, worked out by every wave.
-struct SharedPlan {
-    int n_tile;         // workgroups for the prefixes, the launch's first ones
-    int size;           // tiles of a piece
-    int pieces;         // per KV head
-    int total, quota;   // of the line
-    OwnSeq kept;        // per lane: the first 64 sequences
-    Group group;        // per lane: the first 64 groups
-};
-MA_DEV int blocks_of(const Group& g) { return g.tiles > 0 ? (g.rows + kBlockRows - 1) / kBlockRows : 0; }
-MA_DEV int parts_of(const Group& g, int size) { return (g.tiles + size - 1) / size; }
+// Blocks of a group's rows, equal to within a wave's: every row of a block attends all tiles of the prefix.
+template <int D> MA_DEV int blocks_of(const Group& g) { return g.tiles > 0 ? (g.rows + kBlockRows<D> - 1) / kBlockRows<D> : 0; }
+MA_DEV int rows_of_block(int rows, int blocks) { return ((rows + blocks - 1) / blocks + 31) & ~31; }
 
-template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes) {
+// What it costs to begin with a block, or with a (sequence, KV head, group of columns), inside a share (looking it up, requesting its first rows and waiting for
+// them), in tiles and in groups of rows: that many places of the line in front of it are its, where nothing is.
+// (Groups of rows, us without / with: 90 sequences in 7 groups 97.4 / 93.2, 64 of one token over head_dim 64 36.2 / 34.3, over codes 35.2 / 33.5.)
+constexpr int kTileLead = 2, kPairLead = 2;
+
+// How the launch is laid out, worked out by every wave.  Both kinds of work are lines, cut into equal shares: the tiles of all blocks of the
+// groups' rows, for every KV head; and the groups of the sequences' own rows, for every KV head and group of columns.
+struct SharedPlan {
+    int n_tile;                   // workgroups for tiles, the launch's first ones
+    int tiles, tile_quota;        // of the line of tiles, per KV head
+    int total, quota;             // of the other
+    bool inside;                  // a token stands inside its group's prefix
+};
+
+// What a workgroup takes for a tile, in units of what its share of a group of own rows takes: 2 us to 0.2 at head_dim 128 (over codes 2.5, 0.24), where both were
+// measured in one launch, and the ratio that was best at head_dim 64.  us with 5 / 7 / 9 / 10: 64 sequences behind 6000 rows 68.5 / 59.9 / 54.5 / 53.6, 192 behind 16000 to
+// 24000 of codes 254 / 220 / 201 / 197; 64 over head_dim 64 33.3 / 34.0 / 35 / 36.
+template <int D, int GR> constexpr float kTileCost = D == 128 ? 10.f : 6.f;
+MA_DEV int own_length(int groups) { return groups > 0 ? groups + kPairLead : 0; }
+
+template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes, Group* kept) {
     const PagedParams& p = w.d.p;
     const int lane = threadIdx.x & 63, pairs = p.Hkv * w.d.n_hg;
-    SharedPlan r;
-    // ---- the groups: blocks of rows and tiles ----
-    int blocks = 0;
-    float units = 0.f;   // tiles of all blocks
+    SharedPlan r{};
+    int blocks = 0, longest = 0, longest_own = 0;
     for (int base = 0; base < w.n_groups; base += 64) {
         const Group q = group_at(w, base + lane);
-        if (base == 0) r.group = q;
-        blocks += lane_value(wave_inclusive_scan(blocks_of(q)), 63);
-        units += lane_sum<64>((float)blocks_of(q) * (float)q.tiles);
+        if (base == 0) kept[lane] = q;   // (all waves write the same, and each reads what it wrote)
+        const int n = blocks_of<D>(q), length = n * (q.tiles + kTileLead), incl = wave_inclusive_scan(length), count = wave_inclusive_scan(n);
+        if (writes && base + lane < w.n_groups) w.group_tab[base + lane] = i32x4{q.lo, q.rows, r.tiles + incl - length, blocks + count - n};
+        r.tiles += lane_value(incl, 63);
+        blocks += lane_value(count, 63);
+        longest = max(longest, q.tiles);
     }
-    // ---- the line ----
-    int total = 0, longest = 0;
     for (int base = 0; base < p.n_seqs; base += 64) {
         const OwnSeq q = own_seq<GR>(w, base + lane);
-        if (base == 0) r.kept = q;
-        const int incl = wave_inclusive_scan(q.groups * pairs);
-        if (writes && base + lane < p.n_seqs) {
-            w.seq_tab[2 * (base + lane)] = total + incl - q.groups * pairs;
-            w.seq_tab[2 * (base + lane) + 1] = q.group;
-        }
-        total += lane_value(incl, 63);
-        longest = max(longest, q.groups);
+        const int length = own_length(q.groups) * pairs, incl = wave_inclusive_scan(length);
+        if (writes && base + lane < p.n_seqs) w.seq_tab[base + lane] = i32x4{r.total + incl - length, q.group, 0, 0};
+        r.total += lane_value(incl, 63);
+        longest_own = max(longest_own, q.groups);
+        r.inside = r.inside || __any(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
     }
-    longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));
-    r.total = total;
-    // ---- who does what: a tile of a block takes a workgroup about twice as long as 64 rows of the line (16-bit rows; four groups of them) ----
-    constexpr float kTileCost = 2.f;
-    const float tile_work = units * (float)p.Hkv * kTileCost, line_work = (float)total / (float)(64 / GR) ;
+    // ---- who does what ----
+    const float tile_work = (float)r.tiles * (float)p.Hkv * kTileCost<D, GR>, line_work = (float)r.total;
     const int G = (int)gridDim.x;
     int ranks = 0;
-    if (__any(tile_work > 0.f)) {
-        const int least_line = total > 0 ? G / 8 : 0;
+    if (r.tiles > 0) {
+        const int least_line = r.total > 0 ? G / 8 : 0;
         ranks = (int)((float)G * tile_work / (tile_work + line_work) / (float)p.Hkv + 0.5f);
         ranks = __builtin_amdgcn_readfirstlane(min(max(ranks, 1), (G - least_line) / p.Hkv));
     }
     r.n_tile = ranks * p.Hkv;
-    // ---- pieces: equal to within a tile, no more of them than workgroups where blocks may be cut; more than 64 groups are not cut ----
-    r.size = 0x3fffffff;
-    r.pieces = blocks;
-    if (ranks > 0 && w.n_groups <= 64) {
-        constexpr int kLeastTiles = 2;
-        const int most = max(ranks, blocks), tiles = (int)wave_max((float)r.group.tiles);
-        int size = __builtin_amdgcn_readfirstlane(max(max((int)(units / (float)most), kLeastTiles), tiles / kMaxParts + 1));
-        for (;; size += 1 + size / 8) {   // (ends: with the most tiles of a group as the size there is a piece for every block)
-            r.pieces = lane_value(wave_inclusive_scan(blocks_of(r.group) * parts_of(r.group, size)), 63);
-            if (r.pieces <= most) break;
-        }
-        r.size = size;
-    }
-    r.pieces = min(r.pieces, w.max_pieces);   // (of groups that overlap, which no valid call has, there may be more than there is room for)
-    const int n_waves = (G - r.n_tile) * kLineWaves;
-    r.quota = max(max((total + n_waves - 1) / max(n_waves, 1), kLeastShare / GR), longest / (kMaxParts - 3) + 1);
-    if (writes) {
-        if (lane == 0) w.seq_tab[2 * p.n_seqs] = r.quota;
-        int first = 0;
-        for (int base = 0; base < w.n_groups; base += 64) {
-            const Group q = base == 0 ? r.group : group_at(w, base + lane);
-            const int parts = parts_of(q, r.size), incl = wave_inclusive_scan(blocks_of(q) * parts);
-            if (base + lane < w.n_groups) w.group_tab[base + lane] = i32x4{q.lo, q.rows, first + incl - blocks_of(q) * parts, parts};
-            first += lane_value(incl, 63);
-        }
-    }
+    longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));
+    longest_own = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest_own));
+    constexpr int kLeastTiles = 2;
+    r.tile_quota = max(max((r.tiles + ranks - 1) / max(ranks, 1), kLeastTiles), longest / (kMaxParts - 3) + 1);
+    const int n_waves = (G - r.n_tile) * kSharedWaves<D>;
+    r.quota = max(max((r.total + n_waves - 1) / max(n_waves, 1), kLeastShare / GR), longest_own / (kMaxParts - 3) + 1);
+    if (writes && lane == 0) w.seq_tab[p.n_seqs] = i32x4{r.quota, r.tile_quota, 0, 0};
     return r;
 }
 
-// Pieces rank, rank + ranks, .. of KV head g.
-template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w, const SharedPlan& plan, PagedParams p, char* lds) {
-    const int lane = threadIdx.x & 63, ranks = plan.n_tile / p.Hkv;
+// The block that holds place x of the line of tiles: its job (n_own: its tiles from there on; 0: there is no such block).
+template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look_inside, const Group* kept) {
+    const PagedParams& p = w.d.p;
+    const int lane = threadIdx.x & 63;
+    TileJob job{};
+    int before = 0;
+    for (int base = 0; base < w.n_groups; base += 64) {
+        const Group q = base == 0 ? kept[lane] : group_at(w, base + lane);
+        const int blocks = blocks_of<D>(q), n = blocks * (q.tiles + kTileLead), incl = wave_inclusive_scan(n), sum = lane_value(incl, 63), count = wave_inclusive_scan(blocks);
+        if (x >= sum) {
+            x -= sum;
+            before += lane_value(count, 63);
+            continue;
+        }
+        const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
+        const int tiles = lane_value(q.tiles, src), n_blocks = lane_value(blocks, src);
+        job.seq = job.first = lane_value(q.first, src);
+        job.last = lane_value(q.last, src);
+        job.lo = lane_value(q.lo, src);
+        job.rows = lane_value(q.rows, src);
+        job.ctx = tiles * 64;
+        x -= lane_value(incl - n, src);
+        if (x < 0 || tiles <= 0 || x >= lane_value(n, src)) return job;   // (groups that overlap: sums past 31 bits)
+        const int length = tiles + kTileLead, block = x / length, per = rows_of_block(job.rows, n_blocks);
+        job.row0 = block * per;
+        job.row_end = min(job.row0 + per, job.rows);
+        job.t_lo = x - block * length - kTileLead;   // (below zero: places in front of the first tile)
+        job.n_own = tiles - job.t_lo;
+        job.slot = before + lane_value(count - blocks, src) + block;
+        job.prefix = true;
+        bool inside = false;
+        for (int from = job.first; look_inside && from < job.last; from += 64) {
+            const int s = from + lane;
+            if (s < job.last) {
+                const TokenRange t = token_range(p.cu[s], p.cu[s + 1], p.T);
+                inside = inside || (t.len > 0 && context_of(p.c, p.ctx[s], t) - t.len < job.ctx - 1);
+            }
+        }
+        job.inside = __any(inside) != 0;
+        return job;
+    }
+    return job;
+}
+
+// A share of the tiles of a KV head.
+template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w, const SharedPlan& plan, PagedParams p, char* lds, const Group* kept) {
     int g, rank;
     if ((p.Hkv & 7) == 0) {   // a KV head's workgroups on one XCD (ids go round-robin)
         const int per = p.Hkv >> 3, m = (int)blockIdx.x >> 3;
@@ -181,45 +215,25 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
     }
     p.part_o = w.tile_o;
     p.part_ml = w.tile_ml;
-    for (int x = rank; x < plan.pieces; x += ranks) {
-        TileJob job{};
+    if (rank > (plan.tiles - 1) / plan.tile_quota) return;   // (fewer shares than workgroups)
+    const int x0 = rank * plan.tile_quota, x1 = x0 + min(plan.tile_quota, plan.tiles - x0);
+    bool busy = false;
+    for (int x = x0; x < x1;) {
+        TileJob job = shared_job<D>(w, x, plan.inside, kept);
+        job.n_own = min(job.n_own, x1 - x);
+        job.slot += rank;
+        if (job.n_own <= 0 || job.slot < 0 || job.slot >= w.max_pieces) break;
+        x += job.n_own;
+        job.n_own += min(job.t_lo, 0);
+        job.t_lo = max(job.t_lo, 0);
+        if (job.n_own <= 0) continue;   // (groups that overlap, which no valid call has: more of them than there is room for)
         job.g = g;
-        job.slot = x;
-        int left = x;
-        for (int base = 0; base < w.n_groups; base += 64) {
-            const Group q = base == 0 ? plan.group : group_at(w, base + lane);
-            const int parts = parts_of(q, plan.size), n = blocks_of(q) * parts, incl = wave_inclusive_scan(n), sum = lane_value(incl, 63);
-            if (left < sum) {
-                const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(left < incl)) - 1);
-                job.first = lane_value(q.first, src);
-                job.last = lane_value(q.last, src);
-                job.lo = lane_value(q.lo, src);
-                job.rows = lane_value(q.rows, src);
-                job.ctx = lane_value(q.tiles, src) * 64;
-                job.parts = lane_value(parts, src);
-                left -= lane_value(incl - n, src);
-                break;
-            }
-            left -= sum;
-        }
-        if (job.parts <= 0) break;   // (groups that overlap, and sums of them past 31 bits: there is no such piece)
-        job.seq = job.first;
-        job.block = left / job.parts;
-        job.part = left - job.block * job.parts;
-        bool inside = false;   // sequences whose first new token stands inside the prefix
-        for (int base = job.first; base < job.last; base += 64) {
-            const int s = base + lane;
-            if (s < job.last) {
-                const TokenRange t = token_range(p.cu[s], p.cu[s + 1], p.T);
-                inside = inside || (t.len > 0 && context_of(p.c, p.ctx[s], t) - t.len < job.ctx - 1);
-            }
-        }
-        job.inside = __any(inside) != 0;
-        if (x != rank) {   // every wave is done with the stages, and its results are on their way no more
+        if (busy) {   // every wave is done with the stages, and its results are on their way no more
             wait_vmcnt<0>();
             __syncthreads();
         }
-        attend_tiles<T, D, FP8, kSharedWaves, true>(p, job, lds);
+        busy = true;
+        attend_tiles<T, D, FP8, kSharedWaves<D>, true>(p, job, lds);
     }
 }
 
@@ -231,28 +245,28 @@ template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w,
     const int lane = threadIdx.x & 63, wid = wave_id(), pairs = p.Hkv * d.n_hg;
     const int n_wg = (int)gridDim.x - plan.n_tile, wg = (int)blockIdx.x - plan.n_tile, quota = plan.quota, total = plan.total;
     const int n_shares = total > 0 ? (total - 1) / quota + 1 : 0;
-    const int wave = n_shares <= n_wg ? wid * n_wg + wg : wg * kLineWaves + wid;
+    const int wave = n_shares <= n_wg ? wid * n_wg + wg : wg * kSharedWaves<D> + wid;
     if (wave >= n_shares) return;
     int x = wave * quota;
     const int x_end = x + min(quota, total - x);
     int s = 0, off = 0, groups = 0, first = 0;
     for (int base = 0, start = 0; base < p.n_seqs; base += 64) {
-        const OwnSeq q = base == 0 ? plan.kept : own_seq<GR>(w, base + lane);
-        const int incl = wave_inclusive_scan(q.groups * pairs), sum = lane_value(incl, 63);
+        const OwnSeq q = own_seq<GR>(w, base + lane);
+        const int incl = wave_inclusive_scan(own_length(q.groups) * pairs), sum = lane_value(incl, 63);
         if (x < start + sum) {
             const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < start + incl)) - 1);
             s = base + src;
             groups = lane_value(q.groups, src);
             first = lane_value(q.g0, src);
-            off = start + lane_value(incl, src) - groups * pairs;
+            off = start + lane_value(incl, src) - own_length(groups) * pairs;
             break;
         }
         start += sum;
     }
     SeqInfo info = seq_info(p, s);
     while (x < x_end) {
-        if (x >= off + pairs * groups) {   // the sequence is done: on to the next that has rows
-            off += pairs * groups;
+        if (x >= off + pairs * own_length(groups)) {   // the sequence is done: on to the next that has rows
+            off += pairs * own_length(groups);
             do {
                 info = seq_info(p, ++s);
                 const int i = __builtin_amdgcn_readfirstlane(group_of(w, s));
@@ -260,21 +274,25 @@ template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w,
                 groups = info.len > 0 ? max((info.ctx + GR - 1) / GR - first, 0) : 0;
             } while (groups == 0);
         }
-        const int y = x - off, pair = y / groups, g0 = y - pair * groups, g1 = min(groups, g0 + (x_end - x));
-        const int hg = d.n_hg == 1 ? 0 : pair / p.Hkv, g = pair - hg * p.Hkv;
+        const int length = own_length(groups), pair = (x - off) / length, y = x - off - pair * length;   // y: the first pair_lead places are empty
+        const int n = min(length - y, x_end - x), g1 = y + n - kPairLead, g0 = max(y - kPairLead, 0);
+        x += n;
+        if (g1 <= g0) continue;
+        const int g = d.n_hg == 1 ? pair : pair / d.n_hg, hg = pair - g * d.n_hg;   // (a KV head's groups of columns read the same rows one after the other)
         ColumnAcc<D> acc;
         stream_pages<T, D, FP8>(d, s, info, g, hg, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
         store_part<D>(d, hg, (int64_t)s * pairs + pair + wave, acc);
-        x += g1 - g0;
     }
 }
 
 template <class T, int D, bool FP8>
-__global__ __launch_bounds__(kSharedWaves * 64, 2) void shared_kernel(const SharedWork w) {
-    static_assert(kSharedWaves == kLineWaves && kLineWaves * kWaveLds<D, FP8> <= TileLds<D, FP8, kSharedWaves>::BYTES, "one size of workgroup, one area");
-    __shared__ __attribute__((aligned(1024))) char lds[TileLds<D, FP8, kSharedWaves>::BYTES];
-    const SharedPlan plan = plan_shared<D, kRows<FP8>>(w, blockIdx.x == 0 && wave_id() == 0);
-    if ((int)blockIdx.x < plan.n_tile) shared_tiles<T, D, FP8>(w, plan, w.d.p, lds);
+__global__ __launch_bounds__(kSharedWaves<D> * 64, 2) void shared_kernel(const SharedWork w) {
+    using LDS = TileLds<D, FP8, kSharedWaves<D>, true>;
+    static_assert(kSharedWaves<D> * kWaveLds<D, FP8> <= LDS::BYTES, "one area for both");
+    __shared__ __attribute__((aligned(1024))) char lds[LDS::BYTES];
+    __shared__ Group kept[64];
+    const SharedPlan plan = plan_shared<D, kRows<FP8>>(w, blockIdx.x == 0 && wave_id() == 0, kept);
+    if ((int)blockIdx.x < plan.n_tile) shared_tiles<T, D, FP8>(w, plan, w.d.p, lds, kept);
     else shared_line<T, D, FP8>(w, plan, lds);
 }
 
@@ -293,46 +311,71 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
     const SeqInfo info = seq_info(p, s);
     const int tok = col / p.n_rep, head = col - tok * p.n_rep;
     if (tok >= info.len) return;
-    const int group = const_load(w.seq_tab + 2 * s + 1), quota = const_load(w.seq_tab + 2 * p.n_seqs), pair = (col / 16) * p.Hkv + g;
+    const i32x4 own = const_load(w.seq_tab + s);   // as written by plan_shared
+    const int group = own[1];
+    const i32x4 quotas = const_load(w.seq_tab + p.n_seqs);
+    constexpr int BR = kBlockRows<D>;
+    const int64_t tile_step = (int64_t)p.Hkv * BR;
+    // partial results of an item's tiles, which are n from place x of the line on: their number, and the first one's
+    struct Span { int n; int64_t first; };
+    auto span_of = [&](int x, int n, int quota) {
+        const int share = x / quota;
+        return Span{n > 0 ? min((x + n - 1) / quota - share + 1, kMaxParts) : 0, share};
+    };
+    auto tiles_from = [&](int x, int n, int item) {
+        Span r = span_of(x, n, quotas[1]);
+        r.first += item;
+        r.n = x >= 0 && item >= 0 && r.first + r.n <= w.max_pieces ? r.n : 0;
+        return r;
+    };
     // the parts of the group's prefix
     int n_pre = 0, skip = 0;
     int64_t pre0 = 0;
-    const int64_t pre_step = (int64_t)p.Hkv * kBlockRows;
     if (group >= 0) {
         skip = shared_rows(w, group);
-        const i32x4 t = const_load(w.group_tab + group);   // as written by plan_shared
+        const i32x4 t = const_load(w.group_tab + group);
         const int r = (info.lo + tok - t[0]) * p.n_rep + head;
         if (skip > 0 && r >= 0 && r < t[1]) {
-            const int64_t piece = t[2] + (int64_t)(r / kBlockRows) * t[3];
-            if (piece >= 0 && piece < w.max_pieces) {
-                n_pre = min(min(t[3], kMaxParts), (int)(w.max_pieces - piece));
-                pre0 = (piece * p.Hkv + g) * kBlockRows + r % kBlockRows;
-            }
+            const int blocks = (t[1] + BR - 1) / BR, per = rows_of_block(t[1], blocks), block = r / per;
+            const Span a = tiles_from(t[2] + block * ((skip >> 6) + kTileLead) + kTileLead, skip >> 6, t[3] + block);
+            n_pre = a.n;
+            pre0 = n_pre > 0 ? (a.first * p.Hkv + g) * BR + r - block * per : 0;
         }
     }
-    // those of the line
-    const int groups = max((info.ctx + GR - 1) / GR - skip / GR, 0);
-    const int start = const_load(w.seq_tab + 2 * s) + pair * groups, first = start / quota;
-    const int ns = groups > 0 ? min((start + groups - 1) / quota - first + 1, kMaxParts) : 0;
-    const int64_t at0 = part_row(work, (int64_t)s * p.Hkv * work.n_hg + pair + first, col % 16);
-    f32x2 ml = {-INFINITY, 0.f}, pre = {-INFINITY, 0.f};
-    if (lane < ns) ml = *reinterpret_cast<const f32x2*>(p.part_ml + (at0 + (int64_t)lane * work.per_part) * 2);
-    if (lane < n_pre) pre = *reinterpret_cast<const f32x2*>(w.tile_ml + (pre0 + lane * pre_step) * 2);
+    // those of the sequence's own rows
+    const int groups = max((info.ctx + GR - 1) / GR - skip / GR, 0), pair = g * work.n_hg + col / 16;
+    const Span own_span = span_of(own[0] + pair * own_length(groups) + kPairLead, groups, quotas[0]);
+    const int ns = own_span.n;
+    const int64_t at0 = part_row(work, (int64_t)s * p.Hkv * work.n_hg + pair + own_span.first, col % 16);
+    const float* const pre_o = w.tile_o + pre0 * D + EPL * lane;
+    const float* const own_o = p.part_o + at0 * D + EPL * lane;
+    const int64_t pre_step = tile_step * D, own_step = (int64_t)work.per_part * D;
     auto load_o = [&](const float* at, float (&x)[EPL]) __attribute__((always_inline)) {
         if (EPL == 2) { const f32x2 v = *reinterpret_cast<const f32x2*>(at); x[0] = v[0]; x[EPL - 1] = v[1]; }
         else x[0] = at[0];
     };
+    // the first parts' rows beside their references and sums (of none: a row that is there, unused)
+    f32x2 ml = {-INFINITY, 0.f}, pre = {-INFINITY, 0.f};
+    if (lane < ns) ml = *reinterpret_cast<const f32x2*>(p.part_ml + (at0 + (int64_t)lane * work.per_part) * 2);
+    if (lane < n_pre) pre = *reinterpret_cast<const f32x2*>(w.tile_ml + (pre0 + lane * tile_step) * 2);
+    constexpr int kEarly = 4;
+    float x_pre[8][EPL], x_own[8][EPL];
+#pragma unroll
+    for (int u = 0; u < kEarly; ++u) {
+        if (n_pre > 0) load_o(pre_o + min(u, n_pre - 1) * pre_step, x_pre[u]);
+        if (ns > 0) load_o(own_o + min(u, ns - 1) * own_step, x_own[u]);
+    }
     const float top = wave_max(max2(ml[0], pre[0]));
     const float w_own = ml[0] > -INFINITY ? fast_exp2(ml[0] - top) : 0.f, w_pre = pre[0] > -INFINITY ? fast_exp2(pre[0] - top) : 0.f;
     const float all = lane_sum<64>(ml[1] * w_own + pre[1] * w_pre);
     float acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-    auto add = [&](const float* src, int64_t step, int n, float weight) __attribute__((always_inline)) {
+    auto add = [&](const float* src, int64_t step, int n, float weight, float (&x)[8][EPL]) __attribute__((always_inline)) {
         for (int i0 = 0; i0 < n; i0 += 8) {
-            float x[8][EPL];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) load_o(src + min(i0 + u, n - 1) * step, x[u]);
+            for (int u = 0; u < 8; ++u)
+                if (i0 > 0 || u >= kEarly) load_o(src + min(i0 + u, n - 1) * step, x[u]);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float wi = lane_value(weight, min(i0 + u, 63));
@@ -341,18 +384,24 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
             }
         }
     };
-    add(w.tile_o + pre0 * D + EPL * lane, pre_step * D, n_pre, w_pre);
-    add(p.part_o + at0 * D + EPL * lane, (int64_t)work.per_part * D, ns, w_own);
+    add(pre_o, pre_step, n_pre, w_pre, x_pre);
+    add(own_o, own_step, ns, w_own, x_own);
     const float inv = all > 0.f ? 1.f / all : 0.f;
     uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(info.lo + tok) * p.o2 + (int64_t)(g * p.n_rep + head) * p.o1 + EPL * lane;
     if (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = T::pack2(acc[0] * inv, acc[EPL - 1] * inv);
     else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
 }
 
-// Whether a call is one for these kernels; others go to flash_attn_paged, whose blocks of rows fill up with a single sequence's tokens.
-static bool shared_takes(int64_t n_groups, int64_t Hq, int64_t Hkv, int64_t max_q) {
-    const int64_t n_rep = Hq / Hkv;
-    return n_groups > 0 && Hkv <= kMaxSharedHeads && (max_q == 1 || (n_rep <= 16 && max_q * n_rep <= 64));
+// Whether a call is one for these kernels; others go to flash_attn_paged.  Longer chunks fill its blocks of rows with a single sequence's tokens.  And where all
+// sequences' rows together are no more than the memory-side cache holds, a prefix that is read once for each of them comes from there, and one launch or two
+// that know nothing of groups end sooner.  (us, shared / not, 400 own rows at most; 32 heads on 8 of 128: 8 sequences behind 4000 rows, 144 MB, 20.8 / 17.7, 4 behind
+// 16000, 269 MB, 29.4 / 33.2, 16 behind 4000, 288 MB, 23.1 / 27.3, 64 behind 256, 172 MB, 24.9 / 23.1; 8 on 2 of 64: 64 behind 4000, 144 MB, 20.3 / 17.4, 32 behind 16000,
+// 269 MB, 22.8 / 26.5; of codes: 8 behind 4000, 72 MB, 24.3 / 17.7, 16 behind 4000, 144 MB, 25.3 / 24.4, 64 behind 1000, 183 MB, 27.6 / 36.6.)  The host knows the table's
+// width, not the contexts: a table far wider than they are costs a short call 8 us.
+static bool shared_takes(bool eight, int64_t n_seqs, int64_t n_groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
+    const int64_t n_rep = Hq / Hkv, bytes = 2 * Hkv * D * (eight ? 1 : 2);   // of a row of all heads, k and v
+    if (n_groups == 0 || Hkv > kMaxSharedHeads || (max_q > 1 && (n_rep > 16 || max_q * n_rep > 64))) return false;
+    return n_seqs * max_context >= (eight ? kSharedBytesCodes : kSharedBytes) / bytes;
 }
 
 // How a call is laid out, from its sizes alone.
@@ -364,19 +413,21 @@ static SharedSizes shared_sizes(int64_t n_seqs, int64_t n_groups, int64_t T, int
     r.n_col = max_q * n_rep;
     r.n_hg = (r.n_col + 15) / 16;
     r.per_part = std::min<int64_t>(r.n_col, 16);
-    r.parts = (int64_t)kSharedWgs * kLineWaves + n_seqs * Hkv * r.n_hg;
-    r.pieces = std::max<int64_t>(kSharedWgs / Hkv, T * n_rep / kBlockRows + n_groups);
+    const int64_t wgs = shared_wgs(D), block_rows = shared_waves(D) * 32;
+    // shares and pairs; shares and blocks, those of groups that do not overlap
+    r.parts = wgs * shared_waves(D) + n_seqs * Hkv * r.n_hg;
+    r.pieces = wgs / Hkv + T * n_rep / block_rows + n_groups;
     r.o_bytes = lines(r.parts * r.per_part * D * 4);
     r.ml_bytes = lines(r.parts * r.per_part * 2 * 4);
-    r.tile_o_bytes = lines(r.pieces * Hkv * kBlockRows * D * 4);
-    r.tile_ml_bytes = lines(r.pieces * Hkv * kBlockRows * 2 * 4);
-    r.seq_bytes = lines((2 * n_seqs + 1) * 4);
+    r.tile_o_bytes = lines(r.pieces * Hkv * block_rows * D * 4);
+    r.tile_ml_bytes = lines(r.pieces * Hkv * block_rows * 2 * 4);
+    r.seq_bytes = lines((n_seqs + 1) * 16);
     r.bytes = r.o_bytes + r.ml_bytes + r.tile_o_bytes + r.tile_ml_bytes + r.seq_bytes + lines(n_groups * 16);
     return r;
 }
 
 template <class T, int D, bool FP8> static int launch_shared(const SharedWork& w, hipStream_t stream) {
-    hipLaunchKernelGGL((shared_kernel<T, D, FP8>), dim3(kSharedWgs), dim3(kSharedWaves * 64), 0, stream, w);
+    hipLaunchKernelGGL((shared_kernel<T, D, FP8>), dim3(shared_wgs(D)), dim3(kSharedWaves<D> * 64), 0, stream, w);
     if (int rc = check_launch("shared_kernel")) return rc;
     const int64_t rows = (int64_t)w.d.p.n_seqs * w.d.p.Hkv * w.d.n_col;
     hipLaunchKernelGGL((shared_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
@@ -397,8 +448,11 @@ MINFER_ATTN_EXPORT size_t minfer_flash_attn_paged_shared_workspace_bytes(int64_t
                                                                          int64_t max_context, int64_t max_q_len) {
     if (n_seqs <= 0 || n_groups < 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_context < 0 || Hq % Hkv != 0) return 0;
     const int64_t max_q = bounded_tokens(T, max_q_len);
-    if (!shared_takes(n_groups, Hq, Hkv, max_q)) return minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, max_context, max_q_len);
-    return shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q).bytes;
+    const size_t plain = minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, max_context, max_q_len);
+    size_t most = 0;   // of both kinds of pages
+    for (const bool eight : {false, true})
+        most = std::max(most, shared_takes(eight, n_seqs, n_groups, Hq, Hkv, D, max_context, max_q) ? shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q).bytes : plain);
+    return most;
 }
 
 MINFER_ATTN_EXPORT int minfer_flash_attn_paged_shared(int dtype, int page_type, const void* q, const minfer_kv_pages* pages, const int32_t* cu_seqlens,
@@ -418,17 +472,17 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged_shared(int dtype, int page_type, 
     if (n_seqs == 0 || T == 0) return MINFER_ATTN_OK;
     if (!q || !out || !cu_seqlens || !ctx_lens) return bad("flash_attn_paged_shared: q, out, cu_seqlens and ctx_lens must be non-null");
     if (n_groups > 0 && (!cu_groups || !prefix_lens)) return bad("flash_attn_paged_shared: cu_groups and prefix_lens must be non-null");
-    const int64_t max_q = bounded_tokens(T, max_q_len);
-    if (!shared_takes(n_groups, Hq, Hkv, max_q))
+    const int64_t max_q = bounded_tokens(T, max_q_len), max_context = (int64_t)p.c.width << p.c.page_log2;
+    const bool eight = page_type == MINFER_FP8_E4M3;
+    if (!shared_takes(eight, n_seqs, n_groups, Hq, Hkv, D, max_context, max_q))
         return minfer_flash_attn_paged(dtype, page_type, q, pages, cu_seqlens, ctx_lens, out, n_seqs, T, Hq, Hkv, D, max_q_len, st, workspace, workspace_bytes, stream_v);
     if (!aligned16(q) || !aligned16(out)) return bad("flash_attn_paged_shared: q and out must be 16-byte aligned");
     const int64_t s[4] = {st->q1, st->q2, st->o1, st->o2};
     for (int i = 0; i < 4; ++i)
         if (s[i] < 0 || s[i] % 8 != 0) return bad("flash_attn_paged_shared: strides of q and out must be non-negative multiples of 8 elements");
-    const int64_t max_context = (int64_t)p.c.width << p.c.page_log2;
     if (T > (1 << 30) || T * Hq > 0x7fffffffLL - 4096 || n_seqs > (1 << 24)) return bad("flash_attn_paged_shared: problem too large for one launch");
     const SharedSizes z = shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q);
-    if (n_seqs * Hkv * z.n_col > 0x7fffffffLL || n_seqs * Hkv * z.n_hg * ((max_context + 15) / 16 + 1) > 0x7fffffffLL - 65536)
+    if (z.pieces * (max_context / 64 + 4) > 0x7fffffffLL - 65536 || n_seqs * Hkv * z.n_col > 0x7fffffffLL || n_seqs * Hkv * z.n_hg * ((max_context + 15) / 16 + 4) > 0x7fffffffLL - 65536)
         return bad("flash_attn_paged_shared: problem too large for one launch");
     if (!workspace || !aligned16(workspace) || workspace_bytes < z.bytes)
         return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged_shared: workspace too small or misaligned (see minfer_flash_attn_paged_shared_workspace_bytes)");
@@ -443,11 +497,10 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged_shared(int dtype, int page_type, 
     p.part_ml = (float*)at; at += z.ml_bytes;
     w.tile_o = (float*)at; at += z.tile_o_bytes;
     w.tile_ml = (float*)at; at += z.tile_ml_bytes;
-    w.seq_tab = (int32_t*)at; at += z.seq_bytes;
+    w.seq_tab = (i32x4*)at; at += z.seq_bytes;
     w.group_tab = (i32x4*)at;
     w.d.n_col = (int)z.n_col; w.d.n_hg = (int)z.n_hg; w.d.per_part = (int)z.per_part;
     w.cu_groups = cu_groups; w.prefix = prefix_lens; w.n_groups = (int)n_groups;
     w.max_pieces = (int)z.pieces;
-    const bool eight = page_type == MINFER_FP8_E4M3;
     return dtype == MINFER_ATTN_F16 ? launch_shared_as<F16>(w, D, eight, (hipStream_t)stream_v) : launch_shared_as<BF16>(w, D, eight, (hipStream_t)stream_v);
 }
