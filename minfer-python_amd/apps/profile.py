@@ -142,6 +142,69 @@ def rope_kv_append_paged_fp8(backend: str, which: str, workload: str, repeat: in
     rope_kv_append_paged(backend, which, workload, repeat, True)
 
 
+def flash_attn_paged_shared(backend: str, which: str, workload: str, repeat: int, eight: bool = False):
+    """The decode workload in pages of 16 rows, its 64 sequences behind one prefix: the first half of every context, 2048 rows at least, in the first
+    sequence's pages; `ref` is flash_attn_paged, which reads it for each of them."""
+    kerns = KernelBackend(backend)
+    q, kc, vc, ctx = workloads.decode_cache(device="cuda")
+    q = q.squeeze(2).transpose(0, 1)[None]
+    kp, vp, table = workloads.in_pages(kc, vc)
+    del kc, vc
+    n, prefix = ctx.numel(), 2048
+    table[:, :prefix // 16] = table[0, :prefix // 16]
+    ctx = ctx.clamp(min=prefix + 1)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    groups, lens = torch.tensor([0, n], dtype=torch.int32, device="cuda"), torch.tensor([prefix], dtype=torch.int32, device="cuda")
+    out, scales = torch.zeros_like(q), ()
+    if eight:
+        (kp, ks), (vp, vs) = workloads.e4m3_pages(kp), workloads.e4m3_pages(vp)
+        scales = (ks, vs)
+    if which == "minfer":
+        call = kerns.flash_attn_paged_shared_fp8 if eight else kerns.flash_attn_paged_shared
+        fn = lambda: call(QT, QB, QS, q, kp, vp, *scales, table, cu, ctx, groups, lens, 1, out)
+    else:
+        call = kerns.flash_attn_paged_fp8 if eight else kerns.flash_attn_paged
+        fn = lambda: call(QT, QB, QS, q, kp, vp, *scales, table, cu, ctx, 1, out)
+    for _ in range(repeat):
+        fn()
+    torch.cuda.synchronize()
+
+
+def flash_attn_paged_shared_fp8(backend: str, which: str, workload: str, repeat: int):
+    """flash_attn_paged_shared over e4m3 pages."""
+    flash_attn_paged_shared(backend, which, workload, repeat, True)
+
+
+def paged_tables(backend: str, which: str, workload: str, repeat: int):
+    """Tables and slots of a decode step of 256 sequences (--workload long: of 16 prompts of 4096 tokens) in pages of 16 rows."""
+    assert which == "minfer", "no counterpart"
+    kerns = KernelBackend(backend)
+    n, new, past = (16, 4096, 0) if workload == "long" else (256, 1, 1000)
+    i32 = lambda x: torch.full((n,), x, dtype=torch.int32, device="cuda")
+    held, width, pool = past // 16, (past + new) // 16 + 1, n * ((past + new) // 16 + 1)
+    ring, state = torch.randperm(pool, device="cuda").to(torch.int32), torch.tensor([0, pool, 0], dtype=torch.int32, device="cuda")
+    table, cu = torch.zeros(n, width, dtype=torch.int32, device="cuda"), torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    outs = i32(0), torch.empty(n * new, dtype=torch.int64, device="cuda"), i32(0), torch.zeros_like(state)
+    args = 16, i32(past), i32(new), i32(held), ring, state, table, cu, *outs
+    for _ in range(repeat):
+        kerns.paged_tables(*args)
+    torch.cuda.synchronize()
+
+
+def verify_drafts(backend: str, which: str, workload: str, repeat: int):
+    """Four drafts of each of 64 sequences over 128256 tokens, fp32 probabilities."""
+    assert which == "minfer", "no counterpart"
+    kerns = KernelBackend(backend)
+    n, T, V = 64, 320, 128256
+    p, q = (torch.softmax(3.0 * torch.randn(T, V, device="cuda"), -1) for _ in range(2))
+    tokens = torch.multinomial(q, 1)[:, 0].roll(1)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda") * 5
+    au, su, out, kept = torch.rand(T, device="cuda"), torch.rand(n, device="cuda"), torch.empty_like(tokens), torch.empty(n, dtype=torch.int32, device="cuda")
+    for _ in range(repeat):
+        kerns.verify_drafts(tokens, cu, p, q, au, su, out, kept)
+    torch.cuda.synchronize()
+
+
 def flash_attn_varlen(backend: str, which: str, workload: str, repeat: int):
     kerns = KernelBackend(backend)
     q, k, v, cu = workloads.ragged_prefill(device="cuda")
@@ -347,7 +410,8 @@ if __name__ == "__main__":
     KERNELS = {"mfma_rate": mfma_rate, "gemm_q8_0": gemm_q8_0, "flash_attn": flash_attn, "flash_attn_decode": flash_attn_decode, "flash_attn_varlen": flash_attn_varlen,
                "flash_attn_decode_q8_0": flash_attn_decode_q8_0, "il_rope": il_rope, "rope_kv_append": rope_kv_append,
                "rope_kv_append_q8_0": rope_kv_append_q8_0, "rope_kv_append_norm": rope_kv_append_norm,
-               "flash_attn_paged": flash_attn_paged, "flash_attn_paged_fp8": flash_attn_paged_fp8, "rope_kv_append_paged": rope_kv_append_paged,
+               "flash_attn_paged_shared": flash_attn_paged_shared, "flash_attn_paged_shared_fp8": flash_attn_paged_shared_fp8, "paged_tables": paged_tables,
+               "verify_drafts": verify_drafts, "flash_attn_paged": flash_attn_paged, "flash_attn_paged_fp8": flash_attn_paged_fp8, "rope_kv_append_paged": rope_kv_append_paged,
                "rope_kv_append_paged_fp8": rope_kv_append_paged_fp8, "qkv": qkv, "quant": quant, "rmsnorm": rmsnorm, "gemm": gemm, "gemm_decode": gemm_decode, "copy": copy}
     parser = argparse.ArgumentParser()
     parser.add_argument("--backend", choices=["torch_ext"], default="torch_ext")

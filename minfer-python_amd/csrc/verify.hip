@@ -20,6 +20,11 @@ namespace minfer_attn {
 constexpr int kVerifyThreads = 256, kVerifyWaves = kVerifyThreads / 64;
 constexpr int kMaxChunks = kVerifyThreads;   // of a row: a thread each where they are put together
 constexpr int kLeastChunk = 2048;            // elements: what the threads of a workgroup request at once
+constexpr int64_t kVerifyWgs = 2048;         // that the chip holds at once
+// Workgroups up to which the last one of a sequence goes on (a counter per sequence); more of them wait for one another at the counters, which lie in a few lines of
+// memory, longer than a second launch takes (us, one launch / two: 16 workgroups 8.1 / 9.9, 100 9.0 / 10.0, 252 11.0 / 10.4, 2048 25.2 / 20.3).
+constexpr int64_t kCountedWgs = 128;
+static_assert(kCountedWgs <= kStreamCounters, "a counter for every sequence");
 constexpr int kMostChunk = 8192;             // what is read again by one workgroup (longer only where a row would have more than kMaxChunks)
 
 struct VerifyParams {
@@ -27,7 +32,7 @@ struct VerifyParams {
     const void* target; const void* draft;   // [T, V]; draft null: every draft has the probability one
     const float* accept_u; const float* sample_u;
     void* out; int32_t* n_accepted;
-    double* sums;        // [n_seqs][chunks][2]: of p - q where it is positive, and of p
+    double* sums;        // [n_seqs][chunks]
     int32_t* kept;       // [n_seqs] for the second launch
     uint32_t* done;      // zeroed counters, one per sequence, left zero; or null: a second launch
     int64_t target_stride, draft_stride;
@@ -85,26 +90,23 @@ template <class E> MA_DEV Row row_of(const VerifyParams& p, int s) {
     return out;
 }
 
-// Weights of an element: what p has more than q, and p; what is negative or no number weighs nothing.
-struct Weights { double more, p; };
-MA_DEV Weights weights_of(float pt, float qd) {
-    const double d = (double)pt - (double)qd;
-    return Weights{d > 0.0 ? d : 0.0, pt > 0.f ? (double)pt : 0.0};
-}
+// Weight of an element: what p has more than q; what is negative or no number weighs nothing.
+MA_DEV double weight_of(float pt, float qd) { return fmax((double)pt - (double)qd, 0.0); }   // (fmax of NaN and 0 is 0)
 
-// Elements lo .. lo + N - 1 of the row (those below hi), f(index, weights); rows start anywhere, loads of 16 bytes do not mind.
+// The row and what is taken from it: the draft's probabilities where a draft was not kept (of drafts without: one at the draft), nothing where all were, or where
+// p has nothing more than q (whole).  Rows start anywhere; loads of 16 bytes do not mind.
 template <class E> struct RowReader {
     typedef typename E::elem elem;
     static constexpr int N = 16 / (int)sizeof(elem);
     struct Piece { elem x[N]; };
     const elem* p; const elem* q;
     int64_t draft; bool refused;
-    MA_DEV RowReader(const VerifyParams& v, const Row& r) {
+    MA_DEV RowReader(const VerifyParams& v, const Row& r, bool whole = false) {
         const int64_t at = r.lo + r.kept;
         p = (const elem*)v.target + at * v.target_stride;
-        q = v.draft && r.refused ? (const elem*)v.draft + at * v.draft_stride : nullptr;
+        refused = r.refused && !whole;
+        q = v.draft && refused ? (const elem*)v.draft + at * v.draft_stride : nullptr;
         draft = r.draft;
-        refused = r.refused;
     }
     static MA_DEV Piece load(const elem* at) {
         Piece r;
@@ -112,7 +114,35 @@ template <class E> struct RowReader {
         return r;
     }
     MA_DEV float other(int i, float qd) const { return q ? qd : (refused && i == draft ? 1.f : 0.f); }
-    MA_DEV Weights one(int i) const { return weights_of(E::value(p[i]), other(i, q ? E::value(q[i]) : 0.f)); }
+    MA_DEV double one(int i) const { return weight_of(E::value(p[i]), other(i, q ? E::value(q[i]) : 0.f)); }
+    MA_DEV double of(const Piece& a, const Piece& b, int at) const {
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += weight_of(E::value(a.x[e]), other(at + e, E::value(b.x[e])));
+        return sum;
+    }
+    // elements lo .. hi - 1 of the row, this thread's share of them
+    MA_DEV double share(int lo, int hi) const {
+        double sum = 0.0;
+        constexpr int UN = 4, STEP = kVerifyThreads * N;
+        int i = lo + (int)threadIdx.x * N;
+        for (; i + (UN - 1) * STEP + N <= hi; i += UN * STEP) {
+            Piece a[UN], b[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                a[u] = load(p + i + u * STEP);
+                b[u] = q ? load(q + i + u * STEP) : a[u];
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) sum += of(a[u], b[u], i + u * STEP);
+        }
+        for (; i + N <= hi; i += STEP) {
+            const Piece a = load(p + i), b = q ? load(q + i) : a;
+            sum += of(a, b, i);
+        }
+        for (; i < hi; ++i) sum += one(i);   // the one thread whose piece the end cuts
+        return sum;
+    }
 };
 
 // x over the workgroup: the sum of the threads in front, and of all.  `part` holds one entry a wave; a barrier stands in front of its next use.
@@ -165,38 +195,40 @@ MA_DEV void store_sum(double* p, double x) {
 }
 
 // The token, from the chunks' sums (one to a thread), and what the sequence gets; the whole workgroup.
-template <class E> MA_DEV void finish_row(const VerifyParams& p, int s, const Row& r, double more, double whole, double* part, int* ipart) {
+template <class E> MA_DEV void finish_row(const VerifyParams& p, int s, const Row& r, double mine, double* part, int* ipart) {
+    __shared__ double front_s;
+    typedef RowReader<E> Reader;
     const int tid = threadIdx.x;
-    Scan of = block_scan(more, part);
-    const bool rest = r.refused && of.all > 0.0;   // (else p itself: all are kept, or p has nothing more than q)
-    double mine = more;
-    if (!rest) {
-        of = block_scan(whole, part);
-        mine = whole;
+    Scan of = block_scan(mine, part);
+    bool whole = false;
+    if (r.refused && !(of.all > 0.0)) {   // p has nothing more than q: p itself (one workgroup for all of the row; sums of probabilities that are off by their roundings)
+        whole = true;
+        const Reader row(p, r, true);
+        for (int c = 0; c < p.chunks; ++c) {
+            const double sum = block_scan(row.share(c * p.chunk_len, min((c + 1) * p.chunk_len, p.V)), part).all;
+            if (tid == c) mine = sum;
+        }
+        of = block_scan(mine, part);
     }
     const double mark = (double)p.sample_u[s] * of.all;
     const int chunk = first_thread(of.front + mine > mark, mine > 0.0, ipart);
     int64_t token = -1;   // a row that holds no probability
     if (chunk >= 0) {
         // the sum in front of the chunk, from the thread that has it
-        __shared__ double front_s;
         if (tid == chunk) front_s = of.front;
         __syncthreads();
         const double front = front_s;
-        typedef RowReader<E> Reader;
-        const Reader row(p, r);
+        const Reader row(p, r, whole);
         const int lo = chunk * p.chunk_len, hi = min(lo + p.chunk_len, p.V), per = p.chunk_len / kVerifyThreads;
-        auto weight = [&](const Weights& w) __attribute__((always_inline)) { return rest ? w.more : w.p; };
         const int i0 = min(lo + tid * per, hi), i1 = min(i0 + per, hi);
         double sum = 0.0;
         int i = i0;
 #pragma unroll 4
         for (; i + Reader::N <= i1; i += Reader::N) {
             const typename Reader::Piece a = Reader::load(row.p + i), b = row.q ? Reader::load(row.q + i) : a;
-#pragma unroll
-            for (int e = 0; e < Reader::N; ++e) sum += weight(weights_of(E::value(a.x[e]), row.other(i + e, E::value(b.x[e]))));
+            sum += row.of(a, b, i);
         }
-        for (; i < i1; ++i) sum += weight(row.one(i));
+        for (; i < i1; ++i) sum += row.one(i);
         const Scan in = block_scan(sum, part);
         const int owner = first_thread(front + in.front + sum > mark, sum > 0.0, ipart);
         if (tid == owner) front_s = front + in.front;
@@ -205,7 +237,7 @@ template <class E> MA_DEV void finish_row(const VerifyParams& p, int s, const Ro
             double before = front_s;
             const int lane = tid & 63, o0 = lo + owner * per, o1 = min(o0 + per, hi);
             for (int at = o0; at < o1; at += 64) {
-                const double w = at + lane < o1 ? weight(row.one(at + lane)) : 0.0;
+                const double w = at + lane < o1 ? row.one(at + lane) : 0.0;
                 double incl = w;
 #pragma unroll
                 for (int m = 1; m < 64; m <<= 1) {
@@ -231,7 +263,6 @@ template <class E> __global__ __launch_bounds__(kVerifyThreads) void verify_kern
     __shared__ int ipart[2 * kVerifyWaves];
     __shared__ int last_s;
     typedef RowReader<E> Reader;
-    constexpr int N = Reader::N;
     const int tid = threadIdx.x, c = blockIdx.x, s = blockIdx.y;
     const Row r = row_of<E>(p, s);
     if (r.len == 0) {
@@ -239,48 +270,13 @@ template <class E> __global__ __launch_bounds__(kVerifyThreads) void verify_kern
         return;
     }
     const Reader row(p, r);
-    const int lo = c * p.chunk_len, hi = min(lo + p.chunk_len, p.V);
-    double more = 0.0, whole = 0.0;
-    constexpr int UN = 4;
-    int i = lo + tid * N;
-    auto add = [&](const typename Reader::Piece& a, const typename Reader::Piece& b, int at) __attribute__((always_inline)) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const Weights w = weights_of(E::value(a.x[e]), row.other(at + e, E::value(b.x[e])));
-            more += w.more;
-            whole += w.p;
-        }
-    };
-    for (; i + (UN - 1) * kVerifyThreads * N + N <= hi; i += UN * kVerifyThreads * N) {
-        typename Reader::Piece a[UN], b[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            a[u] = Reader::load(row.p + i + u * kVerifyThreads * N);
-            b[u] = row.q ? Reader::load(row.q + i + u * kVerifyThreads * N) : a[u];
-        }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) add(a[u], b[u], i + u * kVerifyThreads * N);
-    }
-    for (; i + N <= hi; i += kVerifyThreads * N) {
-        const typename Reader::Piece a = Reader::load(row.p + i), b = row.q ? Reader::load(row.q + i) : a;
-        add(a, b, i);
-    }
-    for (; i < hi; ++i) {   // the one thread whose piece the row's end cuts
-        const Weights w = row.one(i);
-        more += w.more;
-        whole += w.p;
-    }
-    more = block_scan(more, part).all;
-    whole = block_scan(whole, part).all;
+    const double sum = block_scan(row.share(c * p.chunk_len, min((c + 1) * p.chunk_len, p.V)), part).all;
     if (p.chunks == 1) {
-        finish_row<E>(p, s, r, tid == 0 ? more : 0.0, tid == 0 ? whole : 0.0, part, ipart);
+        finish_row<E>(p, s, r, tid == 0 ? sum : 0.0, part, ipart);
         return;
     }
-    double* const sums = p.sums + (int64_t)s * p.chunks * 2;
-    if (tid == 0) {
-        store_sum(sums + 2 * c, more);
-        store_sum(sums + 2 * c + 1, whole);
-    }
+    double* const sums = p.sums + (int64_t)s * p.chunks;
+    if (tid == 0) store_sum(sums + c, sum);
     if (!p.done) {
         if (c == 0 && tid == 0) p.kept[s] = r.kept;
         return;
@@ -295,8 +291,7 @@ template <class E> __global__ __launch_bounds__(kVerifyThreads) void verify_kern
     }
     __syncthreads();
     if (!last_s) return;
-    const bool on = tid < p.chunks;
-    finish_row<E>(p, s, r, on ? load_sum(sums + 2 * tid) : 0.0, on ? load_sum(sums + 2 * tid + 1) : 0.0, part, ipart);
+    finish_row<E>(p, s, r, tid < p.chunks ? load_sum(sums + tid) : 0.0, part, ipart);
 }
 
 // (where there are no counters) a workgroup per sequence
@@ -309,19 +304,17 @@ template <class E> __global__ __launch_bounds__(kVerifyThreads) void verify_fini
     Row r{t.lo, t.len, const_load(p.kept + s), false, 0};
     r.refused = r.kept < r.len - 1;
     if (r.refused) r.draft = token_at(p, (int64_t)r.lo + r.kept + 1);
-    const double* const sums = p.sums + (int64_t)s * p.chunks * 2;
-    const bool on = tid < p.chunks;
-    finish_row<E>(p, s, r, on ? sums[2 * tid] : 0.0, on ? sums[2 * tid + 1] : 0.0, part, ipart);
+    finish_row<E>(p, s, r, tid < p.chunks ? p.sums[(int64_t)s * p.chunks + tid] : 0.0, part, ipart);
 }
 
-// Chunks of a row: as many as make 1024 workgroups, of whole rounds of loads, 2048 to 8192 elements; from the sizes alone.
+// Chunks of a row: as many as make kVerifyWgs workgroups, of whole rounds of loads, 2048 to 8192 elements; from the sizes alone.
 struct VerifyPlan { int64_t chunks, chunk_len; size_t bytes; };
 static VerifyPlan plan_verify(int64_t n_seqs, int64_t V) {
     VerifyPlan r{};
-    const int64_t want = std::min<int64_t>(std::max<int64_t>((1024 + n_seqs - 1) / n_seqs, (V + kMostChunk - 1) / kMostChunk), kMaxChunks);
+    const int64_t want = std::min<int64_t>(std::max<int64_t>((kVerifyWgs + n_seqs - 1) / n_seqs, (V + kMostChunk - 1) / kMostChunk), kMaxChunks);
     r.chunk_len = std::max<int64_t>(((V + want - 1) / want + kLeastChunk - 1) / kLeastChunk * kLeastChunk, kLeastChunk);
     r.chunks = std::max<int64_t>((V + r.chunk_len - 1) / r.chunk_len, 1);
-    if (r.chunks > 1) r.bytes = (size_t)(n_seqs * r.chunks * 16 + (n_seqs * 4 + 255) / 256 * 256);
+    if (r.chunks > 1) r.bytes = (size_t)(n_seqs * r.chunks * 8 + (n_seqs * 4 + 255) / 256 * 256);
     return r;
 }
 
@@ -367,9 +360,9 @@ MINFER_ATTN_EXPORT int minfer_verify_drafts(int prob_dtype, int token_bits, cons
     p.n_seqs = (int)n_seqs; p.T = (int)T; p.V = (int)V; p.chunks = (int)plan.chunks; p.chunk_len = (int)plan.chunk_len;
     p.wide = token_bits == 64;
     p.sums = (double*)workspace;
-    p.kept = (int32_t*)((char*)workspace + n_seqs * plan.chunks * 16);
+    p.kept = (int32_t*)((char*)workspace + n_seqs * plan.chunks * 8);
     hipStream_t stream = (hipStream_t)stream_v;
-    if (plan.chunks > 1 && n_seqs <= kStreamCounters) p.done = stream_counters(stream);
+    if (plan.chunks > 1 && n_seqs * plan.chunks <= kCountedWgs) p.done = stream_counters(stream);
     if (prob_dtype == MINFER_ATTN_F32) return launch_verify<F32>(p, stream);
     return prob_dtype == MINFER_ATTN_F16 ? launch_verify<H16>(p, stream) : launch_verify<B16>(p, stream);
 }

@@ -125,8 +125,13 @@ def test_cu_seqlens_that_nobody_checked(kerns):
     c = Case(6, 0, 700, lens=[3] * 6)
     c.cu = [0, 3, 3, 9, 40, 0, 0]
     c.check(kerns)
+    # tokens 0 and 1, none, 1 to 4, ..: token 1 is in two sequences, and gets what either of them says
     c.cu = [-4, 2, 1, 5, 18, 19, 30]
-    c.check(kerns)
+    want, kept = ref.verify(c.tokens, c.cu, c.target, c.draft, c.accept_u, c.sample_u)
+    first, _ = ref.verify(c.tokens, c.cu[:2], c.target, c.draft, c.accept_u, c.sample_u[:1])
+    got = c.call(kerns)
+    assert got[1] == kept and got[0][1] in (first[1], want[1])
+    assert [x for i, x in enumerate(got[0]) if i != 1] == [LEFT if x is None else x for i, x in enumerate(want) if i != 1]
 
 
 def test_another_stream_and_a_graph(kerns):
