@@ -418,12 +418,13 @@ int minfer_rope_kv_append_q8_0(int dtype, int style, void* q, const void* k, con
  * minfer_flash_attn_paged for sequences of which groups share their first rows, in pages that all their tables name: the result is that of
  * minfer_flash_attn_paged up to the order of the sums, and a prefix is read once for a group instead of once for each sequence.  Group i are the sequences
  * cu_groups[i] .. cu_groups[i+1]-1, the first prefix_lens[i] rows of which lie in the same pages (read through the table of the group's first sequence, in
- * whole pieces of 64 rows; what is left of a prefix is read through each sequence's own table); sequences in front of the first group and behind the
- * last have none.  A prefix may reach beyond a sequence's context or into its new tokens: each token attends the rows up to its own.
+ * whole pieces of 64 rows, so that table has to name all of them; what is left of a prefix is read through each sequence's own table); sequences in front
+ * of the first group and behind the last have none.  A prefix may reach beyond another sequence's context or into new tokens: each token attends the rows up to its own.
  * cu_groups int32 [n_groups + 1] and prefix_lens int32 [n_groups] are on the device and not trusted: what they hold is cut to the sequences and to the table, and no
  * address is made from more; but the result is that above only where cu_groups does not fall, and cu_seqlens does not either, except for
- * entries behind the last sequence with tokens.  max_q_len, where it is small, makes the call one for single tokens and drafts (max_q_len * Hq / Hkv <= 64); longer
- * chunks of prompts are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
+ * entries behind the last sequence with tokens.  Meant for single tokens and drafts (max_q_len * Hq / Hkv <= 64, and max_q_len 1 where Hq / Hkv > 16) whose tables name
+ * more rows than the memory-side cache holds (n_seqs * pages_per_seq * page_size rows of 220 MB or more, of 150 MB of 8-bit pages); all other calls, which gain
+ * nothing by groups, are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
  */
 size_t minfer_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                                       int64_t max_context, int64_t max_q_len);

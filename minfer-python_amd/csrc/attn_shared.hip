@@ -110,10 +110,33 @@ struct SharedPlan {
     bool inside;                  // a token stands inside its group's prefix
 };
 
-// What a workgroup takes for a tile, in units of what its share of a group of own rows takes: 2 us to 0.2 at head_dim 128 (over codes 2.5, 0.24), where both were
-// measured in one launch, and the ratio that was best at head_dim 64.  us with 5 / 7 / 9 / 10: 64 sequences behind 6000 rows 68.5 / 59.9 / 54.5 / 53.6, 192 behind 16000 to
-// 24000 of codes 254 / 220 / 201 / 197; 64 over head_dim 64 33.3 / 34.0 / 35 / 36.
-template <int D, int GR> constexpr float kTileCost = D == 128 ? 10.f : 6.f;
+// Time of the own rows in tiles (what a workgroup takes for one whose waves all have rows: 2.05 us at head_dim 128, 2.5 over codes, 1.2 and 1.6 at head_dim 64, and 3 us before its first): `own`
+// of them a group for one workgroup, less with more of them, but never less than `chip` / workgroups of the launch a group, the memory's share.  Fitted to the times of seven
+// calls at every division of the workgroups; us at the division that comes of it / at the best: 64 sequences behind 6000 rows 51.9 / 51.9, over codes 43.3 / 43.0, 90 in seven
+// groups 90.7 / 90.2, 24 with drafts 54.9 / 54.3, 192 behind 16000 to 24000 rows 217 / 213, of codes 193 / 190, at head_dim 64 119 / 118.
+struct OwnCost { float own, chip; };
+template <int D, int GR> constexpr OwnCost kOwnCost = D == 128 ? (GR == 16 ? OwnCost{0.0545f, 0.112f} : OwnCost{0.0845f, 0.051f}) : (GR == 16 ? OwnCost{0.102f, 0.107f} : OwnCost{0.17f, 0.224f});
+
+// A tile's time where some waves have no rows: 1.6 us with two of eight.
+template <int D> MA_DEV float tile_time(int rows) { return 0.73f + 0.27f * (float)((rows + 31) >> 5) / (float)kSharedWaves<D>; }
+
+// Workgroups per KV head for the tiles, of G in all: those with which both kinds of work take the same time, tiles W / n and own rows A / (G - n) + B / G, or one or
+// two more where whole tiles to a share make that the shorter.  `each`: a tile's time on average.
+template <int D, int GR> MA_DEV int tile_ranks(int tiles, float each, int total, int Hkv, int G) {
+    const float W = (float)tiles * each * (float)Hkv, A = kOwnCost<D, GR>.own * (float)total, B = kOwnCost<D, GR>.chip * (float)total, S = W + A + B;
+    const int most = (G - (total > 0 ? G / 8 : 0)) / Hkv;
+    const int first = min(max((int)(2.f * W * (float)G / (S + sqrtf(fmaxf(S * S - 4.f * B * W, 0.f))) / (float)Hkv), 1), most);
+    int best = first;
+    float least = 3.0e38f;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const int r = min(first + i, most);
+        const float t = fmaxf((float)((tiles + r - 1) / r) * each + 1.5f, A / (float)max(G - r * Hkv, 1) + B / (float)G);
+        if (t < least) { least = t; best = r; }
+    }
+    return __builtin_amdgcn_readfirstlane(best);
+}
+
 MA_DEV int own_length(int groups) { return groups > 0 ? groups + kPairLead : 0; }
 
 template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes, Group* kept) {
@@ -121,11 +144,13 @@ template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool
     const int lane = threadIdx.x & 63, pairs = p.Hkv * w.d.n_hg;
     SharedPlan r{};
     int blocks = 0, longest = 0, longest_own = 0;
+    float work = 0.f;
     for (int base = 0; base < w.n_groups; base += 64) {
         const Group q = group_at(w, base + lane);
         if (base == 0) kept[lane] = q;   // (all waves write the same, and each reads what it wrote)
         const int n = blocks_of<D>(q), length = n * (q.tiles + kTileLead), incl = wave_inclusive_scan(length), count = wave_inclusive_scan(n);
         if (writes && base + lane < w.n_groups) w.group_tab[base + lane] = i32x4{q.lo, q.rows, r.tiles + incl - length, blocks + count - n};
+        work += lane_sum<64>(n > 0 ? (float)length * tile_time<D>(rows_of_block(q.rows, n)) : 0.f);
         r.tiles += lane_value(incl, 63);
         blocks += lane_value(count, 63);
         longest = max(longest, q.tiles);
@@ -138,15 +163,7 @@ template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool
         longest_own = max(longest_own, q.groups);
         r.inside = r.inside || __any(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
     }
-    // ---- who does what ----
-    const float tile_work = (float)r.tiles * (float)p.Hkv * kTileCost<D, GR>, line_work = (float)r.total;
-    const int G = (int)gridDim.x;
-    int ranks = 0;
-    if (r.tiles > 0) {
-        const int least_line = r.total > 0 ? G / 8 : 0;
-        ranks = (int)((float)G * tile_work / (tile_work + line_work) / (float)p.Hkv + 0.5f);
-        ranks = __builtin_amdgcn_readfirstlane(min(max(ranks, 1), (G - least_line) / p.Hkv));
-    }
+    const int G = (int)gridDim.x, ranks = r.tiles > 0 ? tile_ranks<D, GR>(r.tiles, work / (float)r.tiles, r.total, p.Hkv, G) : 0;
     r.n_tile = ranks * p.Hkv;
     longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));
     longest_own = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest_own));

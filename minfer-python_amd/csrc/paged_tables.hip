@@ -36,16 +36,30 @@ struct TableParams {
 MA_DEV int cut(int x, int most) { return min(max(x, 0), most); }
 // The ring's state, whatever the memory holds: indexes made from it stay inside.
 MA_DEV Ring ring_of(const TableParams& p) {
-    const int head = p.state[0];
-    return Ring{p.n_pages > 0 && head >= 0 ? head % p.n_pages : 0, cut(p.state[1], p.n_pages)};
+    int head = p.state[0];
+    if ((unsigned)head >= (unsigned)p.n_pages) head = p.n_pages > 0 && head >= 0 ? head % p.n_pages : 0;
+    return Ring{head, cut(p.state[1], p.n_pages)};
 }
-MA_DEV int ring_at(const TableParams& p, const Ring& r, int64_t i) { return (int)((r.head + i) % p.n_pages); }
+// Entry i from the head on, i at most n_pages.
+MA_DEV int ring_at(const TableParams& p, const Ring& r, int64_t i) {
+    const uint32_t at = (uint32_t)r.head + (uint32_t)i;
+    return (int)(at >= (uint32_t)p.n_pages ? at - (uint32_t)p.n_pages : at);
+}
 MA_DEV int saturated(int64_t x) { return (int)min(x, (int64_t)0x7fffffff); }
 
+// x of another lane, as row_exchange; the sum over a wave is lane 63's of a prefix sum.
+template <int CTRL, int ROW_MASK = 0xf> MA_DEV int64_t row_exchange64(int64_t x) {
+    const uint32_t lo = row_exchange<CTRL, ROW_MASK>((uint32_t)x), hi = row_exchange<CTRL, ROW_MASK>((uint32_t)(x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
 MA_DEV int64_t wave_sum(int64_t x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-    return x;
+    x += row_exchange64<0x111>(x);
+    x += row_exchange64<0x112>(x);
+    x += row_exchange64<0x114>(x);
+    x += row_exchange64<0x118>(x);
+    x += row_exchange64<0x142, 0xa>(x);
+    x += row_exchange64<0x143, 0xc>(x);
+    return (int64_t)((uint64_t)(uint32_t)lane_value((int)(x >> 32), 63) << 32 | (uint32_t)lane_value((int)x, 63));
 }
 // x summed over the workgroup, in every thread; `part` is the caller's, one entry a wave.
 MA_DEV int64_t block_sum(int64_t x, int64_t* part) {
@@ -67,7 +81,7 @@ MA_DEV Grown grown(const TableParams& p, int s) {
     return r;
 }
 
-// grid (workgroups of per_wg sequences, parts of their tokens).  256 sequences of a token each 4 us.
+// grid (workgroups of per_wg sequences, parts of their tokens).  256 sequences of a token each 3.3 us, 23 prompts of 300 to 4095 3.4; a call 6.0, which is what issuing it takes.
 __global__ __launch_bounds__(kTableThreads) void paged_tables_kernel(const TableParams p) {
     __shared__ int64_t parts[2][kTableThreads / 64];
     const int tid = threadIdx.x, s0 = (int)blockIdx.x * p.per_wg, s1 = min(s0 + p.per_wg, p.n_seqs);
@@ -119,49 +133,87 @@ MA_DEV Shrunk shrunk(const TableParams& p, int s) {
     return Shrunk{min((keep + (1 << p.page_log2) - 1) >> p.page_log2, held), held};
 }
 
-// A wave per sequence: its entries that name a page.
+// f(entries, lane's is a page, the pages in front of it), 64 entries of a sequence's surplus at a time, eight times 64 requested together; the number of pages.  The whole wave.
+template <class F> MA_DEV int each_page(const TableParams& p, int s, int stay, int held, F f) {
+    const int lane = threadIdx.x & 63;
+    const int32_t* const row = p.table + (int64_t)s * p.table_stride;
+    constexpr int UN = 8;
+    int n = 0;
+    for (int base = stay; base < held; base += 64 * UN) {
+        int page[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) page[u] = base + 64 * u + lane < held ? row[base + 64 * u + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const bool on = (unsigned)page[u] < (unsigned)p.n_pages;
+            const uint64_t all = __ballot(on);
+            f(page[u], on, n + __popcll(all & (((uint64_t)1 << lane) - 1)));
+            n += __popcll(all);
+        }
+    }
+    return n;
+}
+// A sequence's pages to the ring, behind `front` pages of the sequences in front of it.
+MA_DEV int give_back(const TableParams& p, const Ring& ring, int s, const Shrunk& q, int64_t front) {
+    const int64_t room = p.n_pages - ring.count;   // (more pages than the ring has room for are there only if some were named twice)
+    return each_page(p, s, q.stay, q.held, [&](int page, bool on, int before) __attribute__((always_inline)) {
+        if (on && front + before < room) p.ring[ring_at(p, ring, ring.count + front + before)] = page;
+    });
+}
+MA_DEV void leave_state(const TableParams& p, const Ring& ring, int64_t given) {
+    const int took = (int)min(given, (int64_t)(p.n_pages - ring.count));
+    p.state_after[0] = ring.head;
+    p.state_after[1] = ring.count + took;
+    p.state_after[2] = saturated(given - took);
+}
+
+// Up to 64 sequences: one workgroup counts and moves, a wave every sixteenth sequence.  64 sequences, a tenth of them ended, 5.4 us where two launches take 9.1.
+constexpr int kFewSeqs = 64, kFewWaves = 16;
+__global__ __launch_bounds__(kFewWaves * 64) void paged_release_few_kernel(const TableParams p) {
+    __shared__ int counts[kFewSeqs];
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const Ring ring = ring_of(p);
+    const Shrunk mine = lane < p.n_seqs ? shrunk(p, lane) : Shrunk{0, 0};   // a sequence to a lane
+    for (int s = w; s < p.n_seqs; s += kFewWaves) {
+        const int n = each_page(p, s, lane_value(mine.stay, s), lane_value(mine.held, s), [](int, bool, int) {});
+        if (lane == 0) { counts[s] = n; p.held_after[s] = lane_value(mine.stay, s); }
+    }
+    __syncthreads();
+    const int n = lane < p.n_seqs ? counts[lane] : 0, incl = wave_inclusive_scan(n);   // (64 times 2^26 pages at most: as many as a table names)
+    for (int s = w; s < p.n_seqs; s += kFewWaves) {
+        const Shrunk q{lane_value(mine.stay, s), lane_value(mine.held, s)};
+        if (lane_value(n, s) > 0) give_back(p, ring, s, q, lane_value(incl - n, s));
+    }
+    if (threadIdx.x == 0) leave_state(p, ring, lane_value(incl, 63));
+}
+
+// More of them.  A wave per sequence: its entries that name a page.
 __global__ __launch_bounds__(kTableThreads) void paged_release_count_kernel(const TableParams p) {
     const int s = (int)blockIdx.x * (kTableThreads / 64) + wave_id(), lane = threadIdx.x & 63;
     if (s >= p.n_seqs) return;
     const Shrunk q = shrunk(p, s);
-    const int32_t* const row = p.table + (int64_t)s * p.table_stride;
-    int n = 0;
-#pragma unroll 4
-    for (int i = q.stay + lane; i < q.held; i += 64) n += (unsigned)row[i] < (unsigned)p.n_pages;
-    n = (int)wave_sum(n);
+    const int n = each_page(p, s, q.stay, q.held, [](int, bool, int) {});
     if (lane == 0) { p.counts[s] = n; p.held_after[s] = q.stay; }
 }
 
 // A wave per sequence again: its pages behind those of the sequences in front.
 __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const TableParams p) {
     __shared__ int64_t parts[kTableThreads / 64];
+    constexpr int NW = kTableThreads / 64;
     const int tid = threadIdx.x, lane = tid & 63, w = wave_id();
-    const int s0 = (int)blockIdx.x * (kTableThreads / 64), s1 = min(s0 + kTableThreads / 64, p.n_seqs);
+    const int s0 = (int)blockIdx.x * NW, s = s0 + w;
     const Ring ring = ring_of(p);
-    const int64_t room = p.n_pages - ring.count;   // (more pages than the ring has room for are there only if some were named twice)
     int64_t front = 0;
-    for (int s = tid; s < s0; s += kTableThreads) front += p.counts[s];
+    for (int i = tid; i < s0; i += kTableThreads) front += p.counts[i];
     front = block_sum(front, parts);
-    for (int s = s0; s < min(s0 + w, s1); ++s) front += p.counts[s];
-    const int s = s0 + w;
-    if (s < s1) {
-        const Shrunk q = shrunk(p, s);
-        const int32_t* const row = p.table + (int64_t)s * p.table_stride;
-        for (int base = q.stay; base < q.held; base += 64) {
-            const int page = base + lane < q.held ? row[base + lane] : -1;
-            const bool on = (unsigned)page < (unsigned)p.n_pages;
-            const uint64_t all = __ballot(on);
-            const int64_t at = front + __popcll(all & (((uint64_t)1 << lane) - 1));
-            if (on && at < room) p.ring[ring_at(p, ring, ring.count + at)] = page;
-            front += __popcll(all);
-        }
-    }
-    if (lane == 0 && (s == p.n_seqs - 1 || (p.n_seqs == 0 && w == 0))) {   // front: the pages of all sequences
-        const int given = (int)min(front, room);
-        p.state_after[0] = ring.head;
-        p.state_after[1] = ring.count + given;
-        p.state_after[2] = saturated(front - given);
-    }
+    int mine[NW - 1];   // of the workgroup's other sequences in front, requested together
+#pragma unroll
+    for (int i = 0; i < NW - 1; ++i) mine[i] = s0 + i < p.n_seqs ? p.counts[s0 + i] : 0;
+#pragma unroll
+    for (int i = 0; i < NW - 1; ++i) front += i < w ? mine[i] : 0;
+    if (s >= p.n_seqs) return;
+    front += give_back(p, ring, s, shrunk(p, s), front);
+    if (lane == 0 && s == p.n_seqs - 1) leave_state(p, ring, front);
 }
 
 static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -222,7 +274,7 @@ MINFER_ATTN_EXPORT int minfer_paged_tables(int64_t page_size, const int32_t* pas
     return check_launch("paged_tables_kernel");
 }
 
-MINFER_ATTN_EXPORT size_t minfer_paged_release_workspace_bytes(int64_t n_seqs) { return n_seqs > 0 ? ((size_t)n_seqs * 4 + 255) / 256 * 256 : 0; }
+MINFER_ATTN_EXPORT size_t minfer_paged_release_workspace_bytes(int64_t n_seqs) { return n_seqs > kFewSeqs ? ((size_t)n_seqs * 4 + 255) / 256 * 256 : 0; }
 
 MINFER_ATTN_EXPORT int minfer_paged_release(int64_t page_size, const int32_t* keep_lens, const int32_t* pages_held, const minfer_page_ring* ring,
                                             const int32_t* block_table, int64_t table_stride, int64_t pages_per_seq, int32_t* held_after, int64_t n_seqs,
@@ -235,18 +287,20 @@ MINFER_ATTN_EXPORT int minfer_paged_release(int64_t page_size, const int32_t* ke
         return bad("paged_release: keep_lens, pages_held, block_table and held_after must be non-null");
     if (overlap(keep_lens, 4 * n_seqs, held_after, 4 * n_seqs) || overlap(pages_held, 4 * n_seqs, held_after, 4 * n_seqs))
         return bad("paged_release: outputs must not be inputs: the second launch reads them again");
-    if (n_seqs > 0 && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < minfer_paged_release_workspace_bytes(n_seqs)))
+    if (n_seqs > kFewSeqs && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < minfer_paged_release_workspace_bytes(n_seqs)))
         return fail(MINFER_ATTN_EWORKSPACE, "paged_release: workspace too small or misaligned (see minfer_paged_release_workspace_bytes)");
     p.past = keep_lens; p.held = pages_held;
     p.table = const_cast<int32_t*>(block_table);
     p.held_after = held_after;
     p.counts = (int32_t*)workspace;
     hipStream_t stream = (hipStream_t)stream_v;
-    const unsigned wgs = (unsigned)std::max<int64_t>((n_seqs + kTableThreads / 64 - 1) / (kTableThreads / 64), 1);
-    if (n_seqs > 0) {
-        hipLaunchKernelGGL(paged_release_count_kernel, dim3(wgs), dim3(kTableThreads), 0, stream, p);
-        if (int rc = check_launch("paged_release_count_kernel")) return rc;
+    if (n_seqs <= kFewSeqs) {
+        hipLaunchKernelGGL(paged_release_few_kernel, dim3(1), dim3(kFewWaves * 64), 0, stream, p);
+        return check_launch("paged_release_few_kernel");
     }
+    const unsigned wgs = (unsigned)((n_seqs + kTableThreads / 64 - 1) / (kTableThreads / 64));
+    hipLaunchKernelGGL(paged_release_count_kernel, dim3(wgs), dim3(kTableThreads), 0, stream, p);
+    if (int rc = check_launch("paged_release_count_kernel")) return rc;
     hipLaunchKernelGGL(paged_release_kernel, dim3(wgs), dim3(kTableThreads), 0, stream, p);
     return check_launch("paged_release_kernel");
 }

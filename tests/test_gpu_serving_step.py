@@ -154,3 +154,21 @@ def test_a_captured_step(kerns):
             assert torch.equal(got[k], e[k]), k
         # (rows that nothing was written to hold NaN)
         assert torch.equal(live["k"].view(torch.int16), again["k"].view(torch.int16)) and torch.equal(live["table"], again["table"])
+
+
+def test_opcheck(kerns):
+    from test_gpu_shared import QT, Shared, queries
+    ops = torch.ops.minfer
+    utils = ("test_schema", "test_faketensor")
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=DEV)
+    long = lambda n: torch.zeros(n, dtype=torch.int64, device=DEV)
+    torch.library.opcheck(ops.paged_tables.default, (16, i32([3, 0]), i32([2, 1]), i32([1, 0]), i32([3, 2, 0, 1]), i32([0, 3, 0]), z(2, 3), z(3), z(2), long(3), z(2), z(3)), test_utils=utils)
+    torch.library.opcheck(ops.paged_release.default, (16, i32([0, 9]), i32([1, 1]), i32([[2, 0], [1, 0]]), z(4), i32([0, 2, 0]), z(2), z(3)), test_utils=utils)
+    p = torch.softmax(torch.randn(4, 9, device=DEV), -1)
+    for draft in (None, p.flip(0).contiguous()):
+        torch.library.opcheck(ops.verify_drafts.default, (torch.arange(4, device=DEV), i32([0, 3, 4]), p, draft, torch.rand(4, device=DEV), torch.rand(2, device=DEV), long(4), z(2)), test_utils=utils)
+    for eight in (False, True):
+        c = Shared([(1, 70), (2, 90)], [(0, 2, 64)], 16, 2, 64, torch.float16, eight=eight)
+        q = queries(c, 4, torch.float16)
+        op = ops.flash_attn_paged_shared_fp8 if eight else ops.flash_attn_paged_shared
+        torch.library.opcheck(op.default, (*QT[q.dtype], q, c.k_pages, c.v_pages, *c.scales(), c.table, c.cu, c.ctx, i32([0, 2]), i32([64]), 2, torch.zeros_like(q)), test_utils=("test_faketensor",))

@@ -133,7 +133,7 @@ def check_release(kerns, c, keep, gap=0):
     assert torch.equal(table, before)
 
 
-@pytest.mark.parametrize("n,page,past_hi,free,ends,gone", [(1, 16, 500, 3, 1.0, 0.0), (9, 16, 4000, 50, 0.5, 0.2), (64, 16, 900, 10, 0.1, 0.0), (300, 32, 3000, 0, 0.4, 0.3),
+@pytest.mark.parametrize("n,page,past_hi,free,ends,gone", [(1, 16, 500, 3, 1.0, 0.0), (9, 16, 4000, 50, 0.5, 0.2), (64, 16, 900, 10, 0.1, 0.0), (300, 32, 3000, 0, 0.4, 0.3), (63, 16, 20000, 40, 1.0, 0.1), (65, 16, 20000, 40, 1.0, 0.1),
                                                            (1030, 64, 700, 9, 1.0, 0.05), (5, 16, 100, 7, 0.0, 0.0)])
 def test_release(kerns, n, page, past_hi, free, ends, gone):
     c = Pool(n, page, past_hi, 0, -(-past_hi // page) + 1, free, n + 1, gone=gone)

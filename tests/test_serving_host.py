@@ -58,10 +58,10 @@ def test_release_refuses():
     for change in (dict(after=A[5]), dict(after=A[3] + 4)):
         assert release(**change) == capi.EINVAL and "must not be inputs" in capi.last_error()
     assert release(keep=None) == capi.EINVAL
-    need = cs.lib().minfer_paged_release_workspace_bytes(4)
-    assert need >= 16 and cs.lib().minfer_paged_release_workspace_bytes(0) == 0
+    need = cs.lib().minfer_paged_release_workspace_bytes(65)
+    assert need >= 260 and cs.lib().minfer_paged_release_workspace_bytes(64) == 0   # (one launch does without)
     for ws, n in ((None, need), (A[11], need - 1), (A[11] + 2, need)):
-        assert release(ws=ws, ws_bytes=n) == capi.EWORKSPACE and "workspace" in capi.last_error()
+        assert release(n=65, ws=ws, ws_bytes=n) == capi.EWORKSPACE and "workspace" in capi.last_error()
     null = cs.lib()
     assert null.minfer_paged_release(16, A[3], A[5], None, A[6], 8, 8, A[10], 4, A[11], 1 << 20, None) == capi.EINVAL and "ring is null" in capi.last_error()
 
