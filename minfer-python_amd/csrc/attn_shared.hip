@@ -40,29 +40,6 @@ struct SharedWork {
 // Rows of group i's prefix that are computed for all its tokens together: whole tiles.
 MA_DEV int shared_rows(const SharedWork& w, int i) { return min(max(w.prefix[i], 0), w.d.p.c.width << w.d.p.c.page_log2) & ~63; }
 
-// The group of sequence s (-1: none): cu_groups is a list of increasing starts.
-MA_DEV int group_of(const SharedWork& w, int s) {
-    int lo = 0, hi = w.n_groups;   // the last entry that is <= s, of n_groups + 1
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (w.cu_groups[mid] <= s) lo = mid; else hi = mid - 1;
-    }
-    return lo < w.n_groups && w.cu_groups[lo] <= s ? lo : -1;
-}
-
-// What a sequence has behind the prefix: the first group of rows and how many there are.
-struct OwnSeq { SeqInfo info; int group, g0, groups; };
-template <int GR> MA_DEV OwnSeq own_seq(const SharedWork& w, int s) {   // (per lane)
-    OwnSeq r{{0, 0, 0}, -1, 0, 0};
-    if (s < w.d.p.n_seqs) {
-        r.info = line_seq<16>(w.d, s).info;
-        r.group = group_of(w, s);
-        r.g0 = r.group >= 0 ? shared_rows(w, r.group) / GR : 0;
-        r.groups = r.info.len > 0 ? max((r.info.ctx + GR - 1) / GR - r.g0, 0) : 0;
-    }
-    return r;
-}
-
 struct Group { int first, last, lo, rows, tiles; };   // sequences, first token, (token, head) rows, tiles of the prefix
 // The whole wave, a group to a lane.
 MA_DEV Group group_at(const SharedWork& w, int i) {
@@ -92,6 +69,38 @@ MA_DEV Group group_at(const SharedWork& w, int i) {
     return r;
 }
 
+// What the waves of a workgroup have looked up (all of them the same, each for itself): the first 64 groups, and of the first 64 times 64 what lies on the line of tiles
+// in front of them.
+struct SharedLds { Group groups[64]; int tiles_before[64], blocks_before[64]; };
+
+// The group of sequence s (-1: none): cu_groups is a list of increasing starts.
+MA_DEV int group_of(const SharedWork& w, const SharedLds& l, int s) {
+    if (w.n_groups <= 64) {
+        int lo = 0, hi = w.n_groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (l.groups[mid].first <= s) lo = mid; else hi = mid - 1;
+        }
+        return l.groups[lo].first <= s && s < l.groups[lo].last ? lo : -1;
+    }
+    int lo = 0, hi = w.n_groups;   // the last entry that is <= s, of n_groups + 1
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (w.cu_groups[mid] <= s) lo = mid; else hi = mid - 1;
+    }
+    return lo < w.n_groups && w.cu_groups[lo] <= s ? lo : -1;
+}
+
+// What a sequence has behind the prefix: the first group of rows and how many there are.
+struct OwnSeq { SeqInfo info; int group, g0, groups; };
+template <int GR> MA_DEV OwnSeq own_of(const SharedWork& w, const SharedLds& l, int s, const SeqInfo& info) {   // (per lane)
+    OwnSeq r{info, s < w.d.p.n_seqs ? group_of(w, l, s) : -1, 0, 0};
+    if (r.group >= 0) r.g0 = (w.n_groups <= 64 ? l.groups[r.group].tiles * 64 : shared_rows(w, r.group)) / GR;
+    r.groups = info.len > 0 ? max((info.ctx + GR - 1) / GR - r.g0, 0) : 0;
+    return r;
+}
+template <int GR> MA_DEV OwnSeq own_seq(const SharedWork& w, const SharedLds& l, int s) { return own_of<GR>(w, l, s, line_seq<GR>(w.d, s).info); }
+
 // Blocks of a group's rows, equal to within a wave's: every row of a block attends all tiles of the prefix.
 template <int D> MA_DEV int blocks_of(const Group& g) { return g.tiles > 0 ? (g.rows + kBlockRows<D> - 1) / kBlockRows<D> : 0; }
 MA_DEV int rows_of_block(int rows, int blocks) { return ((rows + blocks - 1) / blocks + 31) & ~31; }
@@ -108,6 +117,7 @@ struct SharedPlan {
     int tiles, tile_quota;        // of the line of tiles, per KV head
     int total, quota;             // of the other
     bool inside;                  // a token stands inside its group's prefix
+    int starts;                   // lane i: what lies on that line in front of sequence 64 i
 };
 
 // Time of the own rows in tiles (what a workgroup takes for one whose waves all have rows: 2.05 us at head_dim 128, 2.5 over codes, 1.2 and 1.6 at head_dim 64, and 3 us before its first): `own`
@@ -139,7 +149,7 @@ template <int D, int GR> MA_DEV int tile_ranks(int tiles, float each, int total,
 
 MA_DEV int own_length(int groups) { return groups > 0 ? groups + kPairLead : 0; }
 
-template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes, Group* kept) {
+template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes, SharedLds& l) {
     const PagedParams& p = w.d.p;
     const int lane = threadIdx.x & 63, pairs = p.Hkv * w.d.n_hg;
     SharedPlan r{};
@@ -147,7 +157,11 @@ template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool
     float work = 0.f;
     for (int base = 0; base < w.n_groups; base += 64) {
         const Group q = group_at(w, base + lane);
-        if (base == 0) kept[lane] = q;   // (all waves write the same, and each reads what it wrote)
+        if (base == 0) l.groups[lane] = q;   // (all waves write the same, and each reads what it wrote)
+        if (base < 64 * 64 && lane == 0) {
+            l.tiles_before[base >> 6] = r.tiles;
+            l.blocks_before[base >> 6] = blocks;
+        }
         const int n = blocks_of<D>(q), length = n * (q.tiles + kTileLead), incl = wave_inclusive_scan(length), count = wave_inclusive_scan(n);
         if (writes && base + lane < w.n_groups) w.group_tab[base + lane] = i32x4{q.lo, q.rows, r.tiles + incl - length, blocks + count - n};
         work += lane_sum<64>(n > 0 ? (float)length * tile_time<D>(rows_of_block(q.rows, n)) : 0.f);
@@ -155,13 +169,24 @@ template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool
         blocks += lane_value(count, 63);
         longest = max(longest, q.tiles);
     }
-    for (int base = 0; base < p.n_seqs; base += 64) {
-        const OwnSeq q = own_seq<GR>(w, base + lane);
-        const int length = own_length(q.groups) * pairs, incl = wave_inclusive_scan(length);
-        if (writes && base + lane < p.n_seqs) w.seq_tab[base + lane] = i32x4{r.total + incl - length, q.group, 0, 0};
-        r.total += lane_value(incl, 63);
-        longest_own = max(longest_own, q.groups);
-        r.inside = r.inside || __any(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
+    wave_lds_order();
+    constexpr int UN = 4;   // times 64 sequences requested together
+    for (int base = 0; base < p.n_seqs; base += 64 * UN) {
+        SeqInfo info[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) info[u] = line_seq<GR>(w.d, base + 64 * u + lane).info;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int from = base + 64 * u;
+            if (from >= p.n_seqs) break;
+            const OwnSeq q = own_of<GR>(w, l, from + lane, info[u]);
+            const int length = own_length(q.groups) * pairs, incl = wave_inclusive_scan(length);
+            if (writes && from + lane < p.n_seqs) w.seq_tab[from + lane] = i32x4{r.total + incl - length, q.group, 0, 0};
+            if (lane == from >> 6) r.starts = r.total;
+            r.total += lane_value(incl, 63);
+            longest_own = max(longest_own, q.groups);
+            r.inside = r.inside || __any(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
+        }
     }
     const int G = (int)gridDim.x, ranks = r.tiles > 0 ? tile_ranks<D, GR>(r.tiles, work / (float)r.tiles, r.total, p.Hkv, G) : 0;
     r.n_tile = ranks * p.Hkv;
@@ -176,13 +201,17 @@ template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool
 }
 
 // The block that holds place x of the line of tiles: its job (n_own: its tiles from there on; 0: there is no such block).
-template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look_inside, const Group* kept) {
+template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look_inside, const SharedLds& l) {
     const PagedParams& p = w.d.p;
     const int lane = threadIdx.x & 63;
     TileJob job{};
-    int before = 0;
-    for (int base = 0; base < w.n_groups; base += 64) {
-        const Group q = base == 0 ? kept[lane] : group_at(w, base + lane);
+    // the 64 groups that it lies in
+    const uint64_t in_front = __ballot(lane == 0 || (lane * 64 < w.n_groups && l.tiles_before[lane] <= x));
+    const int strip = 63 - __builtin_amdgcn_readfirstlane(__clzll((long long)in_front));
+    int before = strip > 0 ? __builtin_amdgcn_readfirstlane(l.blocks_before[strip]) : 0;
+    x -= strip > 0 ? __builtin_amdgcn_readfirstlane(l.tiles_before[strip]) : 0;
+    for (int base = strip * 64; base < w.n_groups; base += 64) {
+        const Group q = base == 0 ? l.groups[lane] : group_at(w, base + lane);
         const int blocks = blocks_of<D>(q), n = blocks * (q.tiles + kTileLead), incl = wave_inclusive_scan(n), sum = lane_value(incl, 63), count = wave_inclusive_scan(blocks);
         if (x >= sum) {
             x -= sum;
@@ -220,7 +249,7 @@ template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look
 }
 
 // A share of the tiles of a KV head.
-template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w, const SharedPlan& plan, PagedParams p, char* lds, const Group* kept) {
+template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w, const SharedPlan& plan, PagedParams p, char* lds, const SharedLds& l) {
     int g, rank;
     if ((p.Hkv & 7) == 0) {   // a KV head's workgroups on one XCD (ids go round-robin)
         const int per = p.Hkv >> 3, m = (int)blockIdx.x >> 3;
@@ -236,7 +265,7 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
     const int x0 = rank * plan.tile_quota, x1 = x0 + min(plan.tile_quota, plan.tiles - x0);
     bool busy = false;
     for (int x = x0; x < x1;) {
-        TileJob job = shared_job<D>(w, x, plan.inside, kept);
+        TileJob job = shared_job<D>(w, x, plan.inside, l);
         job.n_own = min(job.n_own, x1 - x);
         job.slot += rank;
         if (job.n_own <= 0 || job.slot < 0 || job.slot >= w.max_pieces) break;
@@ -255,7 +284,7 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
 }
 
 // The line, as in paged_line_kernel, of the rows behind the prefixes.
-template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w, const SharedPlan& plan, char* lds) {
+template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w, const SharedPlan& plan, char* lds, const SharedLds& l) {
     constexpr int GR = kRows<FP8>;
     const DecodeWork& d = w.d;
     const PagedParams& p = d.p;
@@ -267,8 +296,9 @@ template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w,
     int x = wave * quota;
     const int x_end = x + min(quota, total - x);
     int s = 0, off = 0, groups = 0, first = 0;
-    for (int base = 0, start = 0; base < p.n_seqs; base += 64) {
-        const OwnSeq q = own_seq<GR>(w, base + lane);
+    const int strip = 63 - __builtin_amdgcn_readfirstlane(__clzll((long long)__ballot(lane == 0 || (lane * 64 < p.n_seqs && plan.starts <= x))));
+    for (int base = strip * 64, start = lane_value(plan.starts, strip); base < p.n_seqs; base += 64) {
+        const OwnSeq q = own_seq<GR>(w, l, base + lane);
         const int incl = wave_inclusive_scan(own_length(q.groups) * pairs), sum = lane_value(incl, 63);
         if (x < start + sum) {
             const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < start + incl)) - 1);
@@ -286,9 +316,9 @@ template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w,
             off += pairs * own_length(groups);
             do {
                 info = seq_info(p, ++s);
-                const int i = __builtin_amdgcn_readfirstlane(group_of(w, s));
-                first = i >= 0 ? __builtin_amdgcn_readfirstlane(shared_rows(w, i)) / GR : 0;
-                groups = info.len > 0 ? max((info.ctx + GR - 1) / GR - first, 0) : 0;
+                const OwnSeq q = own_of<GR>(w, l, s, info);
+                first = __builtin_amdgcn_readfirstlane(q.g0);
+                groups = __builtin_amdgcn_readfirstlane(q.groups);
             } while (groups == 0);
         }
         const int length = own_length(groups), pair = (x - off) / length, y = x - off - pair * length;   // y: the first pair_lead places are empty
@@ -307,10 +337,10 @@ __global__ __launch_bounds__(kSharedWaves<D> * 64, 2) void shared_kernel(const S
     using LDS = TileLds<D, FP8, kSharedWaves<D>, true>;
     static_assert(kSharedWaves<D> * kWaveLds<D, FP8> <= LDS::BYTES, "one area for both");
     __shared__ __attribute__((aligned(1024))) char lds[LDS::BYTES];
-    __shared__ Group kept[64];
-    const SharedPlan plan = plan_shared<D, kRows<FP8>>(w, blockIdx.x == 0 && wave_id() == 0, kept);
-    if ((int)blockIdx.x < plan.n_tile) shared_tiles<T, D, FP8>(w, plan, w.d.p, lds, kept);
-    else shared_line<T, D, FP8>(w, plan, lds);
+    __shared__ SharedLds looked_up;
+    const SharedPlan plan = plan_shared<D, kRows<FP8>>(w, blockIdx.x == 0 && wave_id() == 0, looked_up);
+    if ((int)blockIdx.x < plan.n_tile) shared_tiles<T, D, FP8>(w, plan, w.d.p, lds, looked_up);
+    else shared_line<T, D, FP8>(w, plan, lds, looked_up);
 }
 
 // out = sum_i O_i w_i / sum_i l_i w_i, w_i = 2^(m_i - max m), over the parts of a row, those of the line and those of its group's prefix; a wave per row (sequence,

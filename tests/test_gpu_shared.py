@@ -130,6 +130,18 @@ def test_many_sequences_and_groups(kerns, n, groups):
     check(kerns, Shared(lens, [(i * per, (i + 1) * per, 128) for i in range(groups)], 16, 2, 64, torch.float16), 8, torch.float16)
 
 
+def test_more_sequences_than_are_looked_up_at_once(kerns):
+    """More than 64 times 64 sequences, and as many groups of one and two behind each other."""
+    lens = [(1, 64 + s % 3) for s in range(4300)]
+    check(kerns, Shared(lens, [(10, 4290, 64)], 16, 1, 64, torch.float16, extra=1), 2, torch.float16)
+    groups, at = [], 0
+    while at < 4250:
+        n = 1 + (at // 7) % 2
+        groups.append((at, at + n, 64))
+        at += n
+    check(kerns, Shared(lens, groups[:4200], 16, 1, 64, torch.float16, extra=1), 2, torch.float16)
+
+
 def test_long_prefix_of_a_few(kerns):
     """More pieces than a merge takes of one row, were they as short as they may be."""
     lens = [(1, 20000 + 100 * i) for i in range(3)]
