@@ -2,11 +2,13 @@
 // document, whose pages every table names.  The prefix's rows are read once for all of a group's tokens instead of once for each sequence.
 //
 // out = softmax over [prefix, own rows] is made of two softmaxes with references and sums of their own:
-// * the prefix: the tokens of a group times the query heads of a KV head are a list of rows, 128 of which walk the prefix's 64-key tiles together (attend_tiles),
-//   cut into pieces that fill the chip: matrix work, a group's K and V read once for every 128 rows and from the L2 where several blocks of rows meet;
-// * the own rows: streamed by single waves over a line of equal shares (stream_pages): bound by memory.
-// Both are one launch, which the workgroups divide between them by what each part is estimated to take, so that matrix units and memory work side by side
-// and both end together.  Everything is a partial result, and shared_merge_kernel puts a row's together.
+// * the prefix: the tokens of a group times the query heads of a KV head are a list of rows, up to 256 of which (128 at head_dim 64) walk the prefix's 64-key tiles
+//   together (attend_tiles): matrix work, 2.05 us a tile of 256 rows, 1.07 PFLOP/s (codes 2.5), the rate of the prompts' kernel;
+// * the own rows: streamed by single waves (stream_pages): bound by memory.
+// Both are lines of places, cut into equal shares, and one launch, whose workgroups are divided between them so that both end together (tile_ranks).  Everything
+// is a partial result, and shared_merge_kernel puts a row's together.  32 heads on 8 of 128: 64 tokens behind 6000 rows and 50 to 1500 of their own 52 us, 4.5 TB/s of
+// what has to be read once (flash_attn_paged 233); 192 behind 16000 to 24000 rows of codes 192, bound by products and widening (1316); 24 sequences of 3 to 6 tokens behind
+// 12000 rows 55 (145).  Of that the start is 7 us (lengths and groups looked up 2.2, the first rows 4), the merge 5 to 9.
 //
 // How the work is cut follows from device data (lengths, contexts, groups) that every wave looks up for itself, a sequence or a group to a lane.
 #include <algorithm>
@@ -46,23 +48,30 @@ MA_DEV Group group_at(const SharedWork& w, int i) {
     const PagedParams& p = w.d.p;
     Group r{0, 0, 0, 0, 0};
     int hi = 0;
+    bool ends_empty = false;
     if (i < w.n_groups) {
         r.first = min(max(w.cu_groups[i], 0), p.n_seqs);
         r.last = min(max(w.cu_groups[i + 1], r.first), p.n_seqs);
         r.tiles = shared_rows(w, i) >> 6;
+        const int begin = p.cu[max(r.last - 1, 0)], end = p.cu[r.last];
         r.lo = min(max(p.cu[r.first], 0), p.T);
-        hi = min(max(p.cu[r.last], 0), p.T);
+        hi = min(max(end, 0), p.T);
+        ends_empty = r.last > r.first && r.tiles > 0 && token_range(begin, end, p.T).len == 0;
     }
-    // (a group with sequences and no tokens, or one whose last sequences have none and entries of zero: looked at one by one)
-    uint64_t odd = __ballot(r.last > r.first && r.tiles > 0 && hi <= r.lo);
+    // (a group whose last sequence has no tokens: where its entries fall, as behind the last sequence of a padded batch, they say nothing of the group's end, which is that of
+    // its last sequence with tokens, looked for 64 at a time)
+    uint64_t odd = __ballot(ends_empty);
     while (odd) {
-        const int lane = threadIdx.x & 63, at = __ffsll((unsigned long long)odd) - 1, last = lane_value(r.last, at);
-        int top = 0, low = p.T;
-        for (int s = lane_value(r.first, at); s < last; ++s) {
-            const TokenRange t = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
-            if (t.len > 0) { top = max(top, t.lo + t.len); low = min(low, t.lo); }
+        const int lane = threadIdx.x & 63, at = __ffsll((unsigned long long)odd) - 1, first = lane_value(r.first, at);
+        int found = lane_value(r.lo, at);
+        for (int end = lane_value(r.last, at); end > first; end -= 64) {
+            const int s = end - 1 - lane;
+            TokenRange t{0, 0, 0};
+            if (s >= first) t = token_range(p.cu[s], p.cu[s + 1], p.T);
+            const uint64_t some = __ballot(t.len > 0);
+            if (some) { found = lane_value(t.lo + t.len, __ffsll((unsigned long long)some) - 1); break; }
         }
-        if (lane == at) { r.lo = min(low, top); hi = top; }
+        if (lane == at) hi = found;
         odd &= odd - 1;
     }
     r.rows = r.last > r.first ? max(hi - r.lo, 0) * p.n_rep : 0;
@@ -268,11 +277,11 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
         TileJob job = shared_job<D>(w, x, plan.inside, l);
         job.n_own = min(job.n_own, x1 - x);
         job.slot += rank;
-        if (job.n_own <= 0 || job.slot < 0 || job.slot >= w.max_pieces) break;
+        if (job.n_own <= 0 || job.slot < 0 || job.slot >= w.max_pieces) break;   // (groups that overlap, which no valid call has: more of them than there is room for)
         x += job.n_own;
         job.n_own += min(job.t_lo, 0);
         job.t_lo = max(job.t_lo, 0);
-        if (job.n_own <= 0) continue;   // (groups that overlap, which no valid call has: more of them than there is room for)
+        if (job.n_own <= 0) continue;   // (the share ends in front of the block's first tile)
         job.g = g;
         if (busy) {   // every wave is done with the stages, and its results are on their way no more
             wait_vmcnt<0>();

@@ -159,7 +159,7 @@ def test_empty_sequences_and_padding(kerns):
     cut = c.call(kerns, q, max_q=2, cu=c.cu_list[:6] + [0, 0, 0])
     assert torch.equal(cut[:, :, :3], want[:, :, :3]) and torch.isnan(cut[:, :, 3]).all()
     # the group reaches over the sequences without tokens behind the last one
-    for cu in (c.cu_list[:6] + [4, 0, 0], c.cu_list[:6] + [4, 4, 4]):
+    for cu in (c.cu_list[:6] + [4, 0, 0], c.cu_list[:6] + [4, 4, 4], c.cu_list[:6] + [4, 2, 0], c.cu_list[:6] + [4, 3, 1], c.cu_list[:6] + [4, 9, 2]):
         assert torch.equal(c.call(kerns, q, max_q=2, cu=cu, groups=[0, 8]), want)
     # rows behind the last sequence stay as they were
     out = torch.full((1, 8, c.T + 3, 64), 7.0, dtype=torch.float16, device=DEV)
@@ -244,6 +244,21 @@ def test_the_same_bits_again_on_another_stream_and_in_a_graph(kerns):
         assert torch.equal(got, out)
         if k != 1:
             assert torch.equal(got, want)
+
+
+def test_calls_in_flight_on_two_streams(kerns):
+    cases = [Shared([(1 + i % 2, 500 + 40 * i) for i in range(10)], [(0, 10, 448)], 16, 2, D, torch.float16, seed=D) for D in (64, 128)]
+    qs = [queries(c, 8, torch.float16) for c in cases]
+    wants = [c.call(kerns, q) for c, q in zip(cases, qs)]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(cases[i].call(kerns, qs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, wants[i]) for o in outs[i])
 
 
 def test_strides_and_large_offsets(kerns):
