@@ -21,10 +21,12 @@ constexpr int kVerifyThreads = 256, kVerifyWaves = kVerifyThreads / 64;
 constexpr int kMaxChunks = kVerifyThreads;   // of a row: a thread each where they are put together
 constexpr int kLeastChunk = 2048;            // elements: what the threads of a workgroup request at once
 constexpr int64_t kVerifyWgs = 2048;         // that the chip holds at once
-// Workgroups up to which the last one of a sequence goes on (a counter per sequence); more of them wait for one another at the counters, which lie in a few lines of
-// memory, longer than a second launch takes (us, one launch / two: 16 workgroups 8.1 / 9.9, 100 9.0 / 10.0, 252 11.0 / 10.4, 2048 25.2 / 20.3).
-constexpr int64_t kCountedWgs = 128;
-static_assert(kCountedWgs <= kStreamCounters, "a counter for every sequence");
+// Workgroups, and bytes that each of them reads, up to which the last one of a sequence goes on (a counter per sequence, each in 64 bytes of its own: side by side, 2048 arrivals
+// wait 3 us longer for one another).  Beyond, where workgroups hold their places on the chip for an answer that comes behind all those loads, a second launch is shorter
+// (us, one launch / two: 16 workgroups of 16 KiB 6.9 / 8.1, 1008 9.7 / 10.8, 1512 10.7 / 11.8, 1600 11.0 / 11.9, 2048 20.6 / 18.3; 1300 of 8 KiB 11.4 / 12.5, 1560 13.1 / 13.2,
+// 1950 14.2 / 13.9; 1536 of 32 KiB 16.7 / 15.8).
+constexpr int64_t kCountedWgs = 1600, kCountedBytes = 16384;
+constexpr int kCounterStep = 16;
 constexpr int kMostChunk = 8192;             // what is read again by one workgroup (longer only where a row would have more than kMaxChunks)
 
 struct VerifyParams {
@@ -34,7 +36,7 @@ struct VerifyParams {
     void* out; int32_t* n_accepted;
     double* sums;        // [n_seqs][chunks]
     int32_t* kept;       // [n_seqs] for the second launch
-    uint32_t* done;      // zeroed counters, one per sequence, left zero; or null: a second launch
+    uint32_t* done;      // zeroed counters, one per sequence, kCounterStep apart, left zero; or null: a second launch
     int64_t target_stride, draft_stride;
     int n_seqs, T, V, chunks, chunk_len;
     bool wide;           // tokens and out are 64-bit numbers
@@ -295,9 +297,9 @@ template <class E> __global__ __launch_bounds__(kVerifyThreads) void verify_kern
     // counts itself when its sums have arrived)
     if (tid == 0) {
         wait_vmcnt<0>();
-        const uint32_t before = __hip_atomic_fetch_add(p.done + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t before = __hip_atomic_fetch_add(p.done + s * kCounterStep, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         last_s = before == (uint32_t)(p.chunks - 1);
-        if (last_s) __hip_atomic_store(p.done + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (last_s) __hip_atomic_store(p.done + s * kCounterStep, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!last_s) return;
@@ -373,7 +375,8 @@ MINFER_ATTN_EXPORT int minfer_verify_drafts(int prob_dtype, int token_bits, cons
     p.sums = (double*)workspace;
     p.kept = (int32_t*)((char*)workspace + n_seqs * plan.chunks * 8);
     hipStream_t stream = (hipStream_t)stream_v;
-    if (plan.chunks > 1 && n_seqs * plan.chunks <= kCountedWgs) p.done = stream_counters(stream);
+    const int64_t chunk_bytes = plan.chunk_len * (prob_dtype == MINFER_ATTN_F32 ? 4 : 2) * (draft_probs ? 2 : 1);
+    if (plan.chunks > 1 && n_seqs * plan.chunks <= kCountedWgs && n_seqs * kCounterStep <= kStreamCounters && chunk_bytes <= kCountedBytes) p.done = stream_counters(stream);
     if (prob_dtype == MINFER_ATTN_F32) return launch_verify<F32>(p, stream);
     return prob_dtype == MINFER_ATTN_F16 ? launch_verify<H16>(p, stream) : launch_verify<B16>(p, stream);
 }

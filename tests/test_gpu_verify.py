@@ -81,6 +81,16 @@ def test_many_sequences(kerns):
     Case(2500, 1, 4100, torch.float16, seed=4).check(kerns)
 
 
+@pytest.mark.parametrize("n,V", [(20, 16001), (100, 4100), (128, 4097), (129, 4097)])
+def test_calls_one_after_the_other(kerns, n, V):
+    """Several chunks to a row, whether or not the last workgroup of a sequence ends it, sequences without tokens among them; what one call counted is not the next one's."""
+    lens = [(0, 1, 3, 2)[(s * 7 + s // 4) % 4] for s in range(n)]
+    c = Case(n, 0, V, seed=n, lens=lens)
+    want = (lambda r: ([LEFT if x is None else x for x in r[0]], r[1]))(ref.verify(c.tokens, c.cu, c.target, c.draft, c.accept_u, c.sample_u))
+    for _ in range(3):
+        assert c.call(kerns) == want
+
+
 def test_marks_on_borders(kerns):
     """Equal weights of a power of two: every sum is exact, and a mark on a border belongs to the token behind it."""
     V = 4096
