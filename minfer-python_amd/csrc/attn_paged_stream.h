@@ -67,9 +67,9 @@ MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg,
     return c;
 }
 
-// Streams groups g0 .. g1 - 1 (at least one) of (sequence s, KV head g) for the columns of group hg; `area` is the wave's own LDS.
-template <class T, int D, bool FP8>
-MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D>& acc) {
+// Streams groups g0 .. g1 - 1 (at least one) of (sequence s, KV head g) for the columns of NC groups from hg on; `area` is the wave's own LDS.
+template <class T, int D, bool FP8, int NC>
+MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D> (&acc)[NC]) {
     const PagedParams& p = work.p;
     using GEO = DecodeGeom<D>;
     constexpr int RB = GEO::RB, G = GEO::G, RPI = GEO::RPI, NI = GEO::NI, RPI8 = GEO::RPI8, NI8 = GEO::NI8;
@@ -78,19 +78,23 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
     const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
     const int ctx = info.ctx, page_mask = (1 << p.c.page_log2) - 1;
     const int32_t* const table = p.c.table + (int64_t)s * p.c.table_stride;
-    const Column col = column_of(work, info, g, hg, l16);
+    Column col[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) col[n] = column_of(work, info, g, hg + n, l16);
     const int edge = ctx - info.len + 1;   // from this row on some columns attend what others do not
     int by_key = 0x7fffffff;               // the group from which on keys are taken one by one
 
     // Q^T fragments (B operand): column l16; contraction step c takes d = 32c + 8 quad + 0..7, or for codes, whose 16-byte pieces hold
     // two steps, d = 64 (c / 2) + 16 quad + 8 (c % 2) + 0..7
-    s16x8 qf[KC];
+    s16x8 qf[NC][KC];
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-        const int d = FP8 ? 64 * (c / 2) + 16 * quad + 8 * (c % 2) : 32 * c + 8 * quad;
-        qf[c] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (col.q) qf[c] = *reinterpret_cast<const s16x8*>(col.q + d);
-    }
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int d = FP8 ? 64 * (c / 2) + 16 * quad + 8 * (c % 2) : 32 * c + 8 * quad;
+            qf[n][c] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (col[n].q) qf[n][c] = *reinterpret_cast<const s16x8*>(col[n].q + d);
+        }
 
     // ---- pages ----
     struct Ids { int id[NH]; };
@@ -147,10 +151,14 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
         }
     };
 
-    f32x4 (&o_acc)[DB] = acc.o;
+    float m_ref[NC], l_sum[NC];
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o_acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_ref = -INFINITY, l_sum = 0.f;
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[n].o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m_ref[n] = -INFINITY;
+        l_sum[n] = 0.f;
+    }
     const float c2 = p.scale_log2;
     constexpr float kLazyLog2 = 6.f;
     char* const my_v = area;
@@ -158,9 +166,9 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
 
     auto consume = [&](int t, Stage& st) __attribute__((always_inline)) {
         int ln = threadIdx.x & 63;
-        if (FP8 && D == 128) asm volatile("" : "+v"(ln));   // (places in LDS are worked out for every group: kept, they do not fit the registers of codes)
+        if ((FP8 || NC > 1) && D == 128) asm volatile("" : "+v"(ln));   // (places in LDS are worked out for every group: kept, they do not fit the registers of codes or of two columns a lane)
         const int lane = ln, l16 = ln & 15, quad = ln >> 4;
-        f32x4 sc[NH];
+        f32x4 sc[NC][NH];
         // V rows behind the context may hold anything, NaN too, and their weight of zero would not take it out of the sums (of K only the
         // row's own scores are made, which are replaced)
         const int past = ctx - t * GR;
@@ -171,14 +179,16 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
         if constexpr (FP8) {
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
-                sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = 0; n < NC; ++n) sc[n][h] = f32x4{0.f, 0.f, 0.f, 0.f};
                 const float ks = scale_value(st.ks[h] >> 8 * (st.there >> (8 + 4 * h) & 3) & 255u);
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
                     const u32x4 x = st.k[h * (D / 64) + c / 2];
                     const uint32_t lo = x[2 * (c % 2)], hi = x[2 * (c % 2) + 1];
                     const u32x4 a = {widen2<T, false>(lo, ks), widen2<T, true>(lo, ks), widen2<T, false>(hi, ks), widen2<T, true>(hi, ks)};
-                    sc[h] = T::mfma16(__builtin_bit_cast(s16x8, a), qf[c], sc[h]);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) sc[n][h] = T::mfma16(__builtin_bit_cast(s16x8, a), qf[n][c], sc[n][h]);
                 }
             }
 #pragma unroll
@@ -205,9 +215,14 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
             }
             const char* rowp = my_k + l16 * RB;
             const int sw = GEO::swz_k(l16);
-            sc[0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < KC; ++c) sc[0] = T::mfma16(*reinterpret_cast<const s16x8*>(rowp + 16 * ((4 * c + quad) ^ sw)), qf[c], sc[0]);
+            for (int n = 0; n < NC; ++n) sc[n][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const s16x8 a = *reinterpret_cast<const s16x8*>(rowp + 16 * ((4 * c + quad) ^ sw));
+#pragma unroll
+                for (int n = 0; n < NC; ++n) sc[n][0] = T::mfma16(a, qf[n][c], sc[n][0]);
+            }
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const int row = j * RPI + lane / G;
@@ -228,32 +243,36 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
             }
             if (__any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.f))) { by_key = t; return; }
         }
-        // rows that the column does not attend
+        uint32_t pk[NC][2 * NH];
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            const int left = (NH == 1 || (st.there >> h & 1)) ? col.limit - (t * GR + 16 * h + 4 * quad) : 0;
+        for (int n = 0; n < NC; ++n) {
+            f32x4 (&x)[NH] = sc[n];
+            // rows that the column does not attend
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[h][r] = r < left ? sc[h][r] : -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
-        if (NH == 2) mx = fmaxf(mx, fmaxf(fmaxf(sc[NH - 1][0], sc[NH - 1][1]), fmaxf(sc[NH - 1][2], sc[NH - 1][3])));
-        auto grows = [&](float x) { return (x * c2 - m_ref) > kLazyLog2 || (m_ref == -INFINITY && x > -INFINITY); };
-        if (__any(grows(mx))) {   // (one of the column's four lanes holds its largest score)
-            mx = max_across_quads(mx);
-            const float m_new = grows(mx) ? mx * c2 : m_ref;
-            const float alpha = (m_ref == -INFINITY) ? 0.f : fast_exp2(m_ref - m_new);
-            m_ref = m_new;
-            l_sum *= alpha;
+            for (int h = 0; h < NH; ++h) {
+                const int left = (NH == 1 || (st.there >> h & 1)) ? col[n].limit - (t * GR + 16 * h + 4 * quad) : 0;
 #pragma unroll
-            for (int db = 0; db < DB; ++db) o_acc[db] *= alpha;
-        }
-        const float mc = (m_ref == -INFINITY) ? 0.f : m_ref;
-        uint32_t pk[2 * NH];
+                for (int r = 0; r < 4; ++r) x[h][r] = r < left ? x[h][r] : -INFINITY;
+            }
+            float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+            if (NH == 2) mx = fmaxf(mx, fmaxf(fmaxf(x[NH - 1][0], x[NH - 1][1]), fmaxf(x[NH - 1][2], x[NH - 1][3])));
+            auto grows = [&](float y) { return (y * c2 - m_ref[n]) > kLazyLog2 || (m_ref[n] == -INFINITY && y > -INFINITY); };
+            if (__any(grows(mx))) {   // (one of the column's four lanes holds its largest score)
+                mx = max_across_quads(mx);
+                const float m_new = grows(mx) ? mx * c2 : m_ref[n];
+                const float alpha = (m_ref[n] == -INFINITY) ? 0.f : fast_exp2(m_ref[n] - m_new);
+                m_ref[n] = m_new;
+                l_sum[n] *= alpha;
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            pk[2 * h] = T::pack2(fast_exp2(fmaf(sc[h][0], c2, -mc)), fast_exp2(fmaf(sc[h][1], c2, -mc)));
-            pk[2 * h + 1] = T::pack2(fast_exp2(fmaf(sc[h][2], c2, -mc)), fast_exp2(fmaf(sc[h][3], c2, -mc)));
-            l_sum = T::add_pair(pk[2 * h + 1], T::add_pair(pk[2 * h], l_sum));   // sums the rounded weights that are multiplied (as in paged_tile_kernel)
+                for (int db = 0; db < DB; ++db) acc[n].o[db] *= alpha;
+            }
+            const float mc = (m_ref[n] == -INFINITY) ? 0.f : m_ref[n];
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                pk[n][2 * h] = T::pack2(fast_exp2(fmaf(x[h][0], c2, -mc)), fast_exp2(fmaf(x[h][1], c2, -mc)));
+                pk[n][2 * h + 1] = T::pack2(fast_exp2(fmaf(x[h][2], c2, -mc)), fast_exp2(fmaf(x[h][3], c2, -mc)));
+                l_sum[n] = T::add_pair(pk[n][2 * h + 1], T::add_pair(pk[n][2 * h], l_sum[n]));   // sums the rounded weights that are multiplied (as in paged_tile_kernel)
+            }
         }
         // O^T += V^T P^T: row d = 16db + l16, keys 4 quad + 0..3 (and 16 + 4 quad + 0..3)
 #pragma unroll
@@ -262,17 +281,25 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
             const s16x4 a0 = lds_read_tr16(rowp_v + at);
             if constexpr (NH == 2) {
                 const s16x4 a1 = lds_read_tr16(rowp_v + 16 * RB + at);
-                o_acc[db] = T::mfma16(s16x8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
-                                      __builtin_bit_cast(s16x8, u32x4{pk[0], pk[1], pk[2 * NH - 2], pk[2 * NH - 1]}), o_acc[db]);
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+                    acc[n].o[db] = T::mfma16(s16x8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
+                                             __builtin_bit_cast(s16x8, u32x4{pk[n][0], pk[n][1], pk[n][2 * NH - 2], pk[n][2 * NH - 1]}), acc[n].o[db]);
             } else {
-                uint2 pu; pu.x = pk[0]; pu.y = pk[1];
-                o_acc[db] = T::mfma16k16(a0, __builtin_bit_cast(s16x4, pu), o_acc[db]);
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    uint2 pu; pu.x = pk[n][0]; pu.y = pk[n][1];
+                    acc[n].o[db] = T::mfma16k16(a0, __builtin_bit_cast(s16x4, pu), acc[n].o[db]);
+                }
             }
         }
     };
 
-    acc.m = -INFINITY;
-    acc.l = 0.f;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        acc[n].m = -INFINITY;
+        acc[n].l = 0.f;
+    }
     Ids first[NS + 1];   // requested together: one wait
 #pragma unroll
     for (int i = 0; i <= NS; ++i) first[i] = ids_of(g0 + i);
@@ -315,17 +342,27 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
     if (by_key < g1) {
         int l = l16;   // (worked out again: kept over the loop, the column's query row does not fit the registers of codes at D = 128)
         asm volatile("" : "+v"(l));
-        const Column again = column_of(work, info, g, hg, l);
-        const short* const q[1] = {again.q};
-        const int limit[1] = {again.limit};
-        float m[1] = {m_ref}, sum[1] = {l_sum};
-        attend_key_by_key<T, D, FP8, 1>(p.c, p.Hkv, s, g, by_key * GR, min(g1 * GR, ctx), q, limit, c2,
-                                        [&](int db, int) __attribute__((always_inline)) -> f32x4& { return o_acc[db]; }, m, sum);
-        m_ref = m[0];
-        l_sum = sum[0];
+        const short* q[NC];
+        int limit[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const Column again = column_of(work, info, g, hg + n, l);
+            q[n] = again.q;
+            limit[n] = again.limit;
+        }
+        attend_key_by_key<T, D, FP8, NC>(p.c, p.Hkv, s, g, by_key * GR, min(g1 * GR, ctx), q, limit, c2,
+                                         [&](int db, int n) __attribute__((always_inline)) -> f32x4& { return acc[n].o[db]; }, m_ref, l_sum);
     }
-    acc.m = m_ref;
-    acc.l = sum_across_quads(l_sum);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        acc[n].m = m_ref[n];
+        acc[n].l = sum_across_quads(l_sum[n]);
+    }
+}
+// One group of columns.
+template <class T, int D, bool FP8>
+MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D>& acc) {
+    stream_columns<T, D, FP8, 1>(work, s, info, g, hg, g0, g1, area, reinterpret_cast<ColumnAcc<D> (&)[1]>(acc));
 }
 
 // Where column c of a column group's partial result `part` lies.  Partial results are numbered through the launch, those of a (sequence, KV head,
@@ -333,11 +370,11 @@ MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int
 // (which for 256 sequences of 64 heads was 0.5 GiB, now 16 MiB; 4096 of 32 4 GiB, now 69 MiB).
 MA_DEV int64_t part_row(const DecodeWork& w, int64_t part, int c) { return part * w.per_part + c; }
 
-// A wave's partial result of every column, into the workspace.
-template <int D> MA_DEV void store_part(const DecodeWork& w, int hg, int64_t part, const ColumnAcc<D>& acc) {
+// A wave's partial result of every column of group hg, into the workspace, `first` columns behind the partial result's first.
+template <int D> MA_DEV void store_part(const DecodeWork& w, int hg, int64_t part, const ColumnAcc<D>& acc, int first = 0) {
     const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
     if (hg * 16 + l16 >= w.n_col) return;
-    const int64_t at = part_row(w, part, l16);
+    const int64_t at = part_row(w, part, first + l16);
     float* dst = w.p.part_o + at * D + 4 * quad;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc.o[db];

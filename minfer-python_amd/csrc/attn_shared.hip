@@ -4,11 +4,11 @@
 // out = softmax over [prefix, own rows] is made of two softmaxes with references and sums of their own:
 // * the prefix: the tokens of a group times the query heads of a KV head are a list of rows, up to 256 of which (128 at head_dim 64) walk the prefix's 64-key tiles
 //   together (attend_tiles): matrix work, 2.05 us a tile of 256 rows, 1.07 PFLOP/s (codes 2.5), the rate of the prompts' kernel;
-// * the own rows: streamed by single waves (stream_pages): bound by memory.
+// * the own rows: streamed by single waves (stream_columns), for up to 32 (token, head) columns together: bound by memory.
 // Both are lines of places, cut into equal shares, and one launch, whose workgroups are divided between them so that both end together (tile_ranks).  Everything
 // is a partial result, and shared_merge_kernel puts a row's together.  32 heads on 8 of 128: 64 tokens behind 6000 rows and 50 to 1500 of their own 52 us, 4.5 TB/s of
 // what has to be read once (flash_attn_paged 233); 192 behind 16000 to 24000 rows of codes 192, bound by products and widening (1316); 24 sequences of 3 to 6 tokens behind
-// 12000 rows 55 (145).  Of that the start is 7 us (lengths and groups looked up 2.2, the first rows 4), the merge 5 to 9.
+// 12000 rows 54 (145).  Of that the start is 7 us (lengths and groups looked up 2.2, the first rows 4), the merge 5 to 9.
 //
 // How the work is cut follows from device data (lengths, contexts, groups) that every wave looks up for itself, a sequence or a group to a lane.
 #include <algorithm>
@@ -133,16 +133,19 @@ struct SharedPlan {
 // of them a group for one workgroup, less with more of them, but never less than `chip` / workgroups of the launch a group, the memory's share.  Fitted to the times of seven
 // calls at every division of the workgroups; us at the division that comes of it / at the best: 64 sequences behind 6000 rows 51.9 / 51.9, over codes 43.3 / 43.0, 90 in seven
 // groups 90.7 / 90.2, 24 with drafts 54.9 / 54.3, 192 behind 16000 to 24000 rows 217 / 213, of codes 193 / 190, at head_dim 64 119 / 118.
+// Two groups of columns together, fitted to 24 calls with drafts: at most 3 % from the best division, in 20 of them at it.
 struct OwnCost { float own, chip; };
-template <int D, int GR> constexpr OwnCost kOwnCost = D == 128 ? (GR == 16 ? OwnCost{0.0545f, 0.112f} : OwnCost{0.0845f, 0.051f}) : (GR == 16 ? OwnCost{0.102f, 0.107f} : OwnCost{0.17f, 0.224f});
+template <int D, int GR, int NC> constexpr OwnCost kOwnCost =
+    NC == 1 ? (D == 128 ? (GR == 16 ? OwnCost{0.0545f, 0.112f} : OwnCost{0.0845f, 0.051f}) : (GR == 16 ? OwnCost{0.102f, 0.107f} : OwnCost{0.17f, 0.224f}))
+            : (D == 128 ? (GR == 16 ? OwnCost{0.104f, 0.035f} : OwnCost{0.1f, 0.04f}) : (GR == 16 ? OwnCost{0.21f, 0.045f} : OwnCost{0.09f, 0.39f}));
 
 // A tile's time where some waves have no rows: 1.6 us with two of eight.
 template <int D> MA_DEV float tile_time(int rows) { return 0.73f + 0.27f * (float)((rows + 31) >> 5) / (float)kSharedWaves<D>; }
 
 // Workgroups per KV head for the tiles, of G in all: those with which both kinds of work take the same time, tiles W / n and own rows A / (G - n) + B / G, or one or
 // two more where whole tiles to a share make that the shorter.  `each`: a tile's time on average.
-template <int D, int GR> MA_DEV int tile_ranks(int tiles, float each, int total, int Hkv, int G) {
-    const float W = (float)tiles * each * (float)Hkv, A = kOwnCost<D, GR>.own * (float)total, B = kOwnCost<D, GR>.chip * (float)total, S = W + A + B;
+template <int D, int GR, int NC> MA_DEV int tile_ranks(int tiles, float each, int total, int Hkv, int G) {
+    const float W = (float)tiles * each * (float)Hkv, A = kOwnCost<D, GR, NC>.own * (float)total, B = kOwnCost<D, GR, NC>.chip * (float)total, S = W + A + B;
     const int most = (G - (total > 0 ? G / 8 : 0)) / Hkv;
     const int first = min(max((int)(2.f * W * (float)G / (S + sqrtf(fmaxf(S * S - 4.f * B * W, 0.f))) / (float)Hkv), 1), most);
     int best = first;
@@ -158,7 +161,7 @@ template <int D, int GR> MA_DEV int tile_ranks(int tiles, float each, int total,
 
 MA_DEV int own_length(int groups) { return groups > 0 ? groups + kPairLead : 0; }
 
-template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes, SharedLds& l) {
+template <int D, int GR, int NC> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool writes, SharedLds& l) {
     const PagedParams& p = w.d.p;
     const int lane = threadIdx.x & 63, pairs = p.Hkv * w.d.n_hg;
     SharedPlan r{};
@@ -197,7 +200,7 @@ template <int D, int GR> MA_DEV SharedPlan plan_shared(const SharedWork& w, bool
             r.inside = r.inside || __any(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
         }
     }
-    const int G = (int)gridDim.x, ranks = r.tiles > 0 ? tile_ranks<D, GR>(r.tiles, work / (float)r.tiles, r.total, p.Hkv, G) : 0;
+    const int G = (int)gridDim.x, ranks = r.tiles > 0 ? tile_ranks<D, GR, NC>(r.tiles, work / (float)r.tiles, r.total, p.Hkv, G) : 0;
     r.n_tile = ranks * p.Hkv;
     longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));
     longest_own = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest_own));
@@ -293,7 +296,7 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
 }
 
 // The line, as in paged_line_kernel, of the rows behind the prefixes.
-template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w, const SharedPlan& plan, char* lds, const SharedLds& l) {
+template <class T, int D, bool FP8, int NC> MA_DEV void shared_line(const SharedWork& w, const SharedPlan& plan, char* lds, const SharedLds& l) {
     constexpr int GR = kRows<FP8>;
     const DecodeWork& d = w.d;
     const PagedParams& p = d.p;
@@ -335,26 +338,27 @@ template <class T, int D, bool FP8> MA_DEV void shared_line(const SharedWork& w,
         x += n;
         if (g1 <= g0) continue;
         const int g = d.n_hg == 1 ? pair : pair / d.n_hg, hg = pair - g * d.n_hg;   // (a KV head's groups of columns read the same rows one after the other)
-        ColumnAcc<D> acc;
-        stream_pages<T, D, FP8>(d, s, info, g, hg, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
-        store_part<D>(d, hg, (int64_t)s * pairs + pair + wave, acc);
+        ColumnAcc<D> acc[NC];
+        stream_columns<T, D, FP8, NC>(d, s, info, g, hg * NC, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) store_part<D>(d, hg * NC + n, (int64_t)s * pairs + pair + wave, acc[n], 16 * n);
     }
 }
 
-template <class T, int D, bool FP8>
+template <class T, int D, bool FP8, int NC>
 __global__ __launch_bounds__(kSharedWaves<D> * 64, 2) void shared_kernel(const SharedWork w) {
     using LDS = TileLds<D, FP8, kSharedWaves<D>, true>;
     static_assert(kSharedWaves<D> * kWaveLds<D, FP8> <= LDS::BYTES, "one area for both");
     __shared__ __attribute__((aligned(1024))) char lds[LDS::BYTES];
     __shared__ SharedLds looked_up;
-    const SharedPlan plan = plan_shared<D, kRows<FP8>>(w, blockIdx.x == 0 && wave_id() == 0, looked_up);
+    const SharedPlan plan = plan_shared<D, kRows<FP8>, NC>(w, blockIdx.x == 0 && wave_id() == 0, looked_up);
     if ((int)blockIdx.x < plan.n_tile) shared_tiles<T, D, FP8>(w, plan, w.d.p, lds, looked_up);
-    else shared_line<T, D, FP8>(w, plan, lds, looked_up);
+    else shared_line<T, D, FP8, NC>(w, plan, lds, looked_up);
 }
 
 // out = sum_i O_i w_i / sum_i l_i w_i, w_i = 2^(m_i - max m), over the parts of a row, those of the line and those of its group's prefix; a wave per row (sequence,
 // token, head), lane i holding the references and sums of both parts i.
-template <class T, int D, int GR>
+template <class T, int D, int GR, int NC>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
     const DecodeWork& work = w.d;
     const PagedParams& p = work.p;
@@ -399,10 +403,10 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
         }
     }
     // those of the sequence's own rows
-    const int groups = max((info.ctx + GR - 1) / GR - skip / GR, 0), pair = g * work.n_hg + col / 16;
+    const int groups = max((info.ctx + GR - 1) / GR - skip / GR, 0), pair = g * work.n_hg + col / (16 * NC);
     const Span own_span = span_of(own[0] + pair * own_length(groups) + kPairLead, groups, quotas[0]);
     const int ns = own_span.n;
-    const int64_t at0 = part_row(work, (int64_t)s * p.Hkv * work.n_hg + pair + own_span.first, col % 16);
+    const int64_t at0 = part_row(work, (int64_t)s * p.Hkv * work.n_hg + pair + own_span.first, col % (16 * NC));
     const float* const pre_o = w.tile_o + pre0 * D + EPL * lane;
     const float* const own_o = p.part_o + at0 * D + EPL * lane;
     const int64_t pre_step = tile_step * D, own_step = (int64_t)work.per_part * D;
@@ -460,6 +464,11 @@ static bool shared_takes(bool eight, int64_t n_seqs, int64_t n_groups, int64_t H
     return n_seqs * max_context >= (eight ? kSharedBytesCodes : kSharedBytes) / bytes;
 }
 
+// Groups of 16 columns that a wave streams a sequence's own rows for together: two where there are more than one.  (us, one at a time / two, each at the best division of the workgroups;
+// 32 heads on 8 of 128, sequences of 3 to 6 tokens behind 12000 rows: 24 with 10 to 900 own rows 54.7 / 53.7, of codes 60.1 / 58.9; 40 with 1000 to 6000 225 / 141, of codes 165 / 116;
+// 64 heads, 24 with 10 to 3000 125 / 107; at head_dim 64, 60 with 1000 to 6000 175 / 114, of codes 146 / 112.)
+static int64_t column_groups(int64_t n_col) { return n_col > 16 ? 2 : 1; }
+
 // How a call is laid out, from its sizes alone.
 struct SharedSizes { int64_t n_col, n_hg, per_part, parts, pieces; size_t o_bytes, ml_bytes, tile_o_bytes, tile_ml_bytes, seq_bytes, bytes; };
 static size_t lines(int64_t bytes) { return ((size_t)bytes + 255) / 256 * 256; }
@@ -467,8 +476,9 @@ static SharedSizes shared_sizes(int64_t n_seqs, int64_t n_groups, int64_t T, int
     SharedSizes r{};
     const int64_t n_rep = Hq / Hkv;
     r.n_col = max_q * n_rep;
-    r.n_hg = (r.n_col + 15) / 16;
-    r.per_part = std::min<int64_t>(r.n_col, 16);
+    const int64_t cols = 16 * column_groups(r.n_col);
+    r.n_hg = (r.n_col + cols - 1) / cols;
+    r.per_part = std::min<int64_t>(r.n_col, cols);
     const int64_t wgs = shared_wgs(D), block_rows = shared_waves(D) * 32;
     // shares and pairs; shares and blocks, those of groups that do not overlap
     r.parts = wgs * shared_waves(D) + n_seqs * Hkv * r.n_hg;
@@ -482,16 +492,19 @@ static SharedSizes shared_sizes(int64_t n_seqs, int64_t n_groups, int64_t T, int
     return r;
 }
 
-template <class T, int D, bool FP8> static int launch_shared(const SharedWork& w, hipStream_t stream) {
-    hipLaunchKernelGGL((shared_kernel<T, D, FP8>), dim3(shared_wgs(D)), dim3(kSharedWaves<D> * 64), 0, stream, w);
+template <class T, int D, bool FP8, int NC> static int launch_shared(const SharedWork& w, hipStream_t stream) {
+    hipLaunchKernelGGL((shared_kernel<T, D, FP8, NC>), dim3(shared_wgs(D)), dim3(kSharedWaves<D> * 64), 0, stream, w);
     if (int rc = check_launch("shared_kernel")) return rc;
     const int64_t rows = (int64_t)w.d.p.n_seqs * w.d.p.Hkv * w.d.n_col;
-    hipLaunchKernelGGL((shared_merge_kernel<T, D, kRows<FP8>>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
+    hipLaunchKernelGGL((shared_merge_kernel<T, D, kRows<FP8>, NC>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, w);
     return check_launch("shared_merge_kernel");
 }
+template <class T, int D, bool FP8> static int launch_columns(const SharedWork& w, hipStream_t stream) {
+    return column_groups(w.d.n_col) == 1 ? launch_shared<T, D, FP8, 1>(w, stream) : launch_shared<T, D, FP8, 2>(w, stream);
+}
 template <class T> static int launch_shared_as(const SharedWork& w, int64_t D, bool eight, hipStream_t stream) {
-    if (eight) return D == 128 ? launch_shared<T, 128, true>(w, stream) : launch_shared<T, 64, true>(w, stream);
-    return D == 128 ? launch_shared<T, 128, false>(w, stream) : launch_shared<T, 64, false>(w, stream);
+    if (eight) return D == 128 ? launch_columns<T, 128, true>(w, stream) : launch_columns<T, 64, true>(w, stream);
+    return D == 128 ? launch_columns<T, 128, false>(w, stream) : launch_columns<T, 64, false>(w, stream);
 }
 
 static int64_t bounded_tokens(int64_t T, int64_t max_q_len) { return max_q_len > 0 && max_q_len < T ? max_q_len : T; }

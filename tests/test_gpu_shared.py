@@ -105,6 +105,33 @@ def test_drafts(kerns, dtype, eight, Hq, Hkv, D, most):
     check(kerns, Shared(lens, [(0, 9, 320)], 64, Hkv, D, dtype, eight=eight, seed=most), Hq, dtype)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D,most", [(24, 4, 128, 3), (8, 2, 128, 6), (16, 1, 64, 2), (8, 2, 64, 11), (48, 4, 128, 3), (40, 2, 64, 1), (13, 1, 128, 4)])
+def test_more_than_16_columns(kerns, eight, Hq, Hkv, D, most):
+    """17 to 52 (token, head) rows per KV head, in whole and partly filled pairs of 16; sequences that fill the first 16 alone; shares that end inside a sequence."""
+    lens = [(1 + (5 * i) % most, 192 + (37 * i) % 900) for i in range(14)] + [(most, 3), (1, 200)]
+    check(kerns, Shared(lens, [(0, 14, 192)], 32, Hkv, D, torch.bfloat16 if most == 3 else torch.float16, eight=eight, seed=Hq), Hq, torch.bfloat16 if most == 3 else torch.float16)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_row_that_some_of_a_pair_of_columns_attend(kerns, eight, D):
+    """A NaN that the last drafts of a sequence attend and the first ones do not, at a border of 16 columns and on either side of it."""
+    lens = [(7, 256 + 20 * i) for i in range(3)]
+    clean = Shared(lens, [(0, 3, 256)], 16, 2, D, torch.float16, eight=eight)
+    q = queries(clean, 8, torch.float16)
+    want, bound = ref.attend(clean, q[0].cpu())
+    for tok in (3, 4, 5):
+        c = Shared(lens, [(0, 3, 256)], 16, 2, D, torch.float16, eight=eight)
+        raw, row = c.v_pages.view(torch.uint8) if eight else c.v_pages, 276 + tok
+        raw[c.table_list[1][row // 16], 1, row % 16, 9] = 0x7F if eight else float("nan")
+        out = c.call(kerns, q)
+        seen = torch.isnan(out[0]).any(-1)
+        assert seen[4:].any(0).nonzero().flatten().tolist() == list(range(7 + tok, 14)) and not seen[:4].any()
+        rest = [t for t in range(21) if not 7 + tok <= t < 14]
+        assert ((out[0].cpu().double() - want).abs() <= bound)[:, rest].all()
+
+
 def test_longer_chunks_are_flash_attn_paged(kerns):
     c = Shared([(40, 128), (3, 140), (70, 200)], [(0, 3, 128)], 16, 2, 128, torch.float16)
     q = queries(c, 8, torch.float16)
