@@ -130,14 +130,13 @@ struct SharedPlan {
 };
 
 // Time of the own rows in tiles (what a workgroup takes for one whose waves all have rows: 2.05 us at head_dim 128, 2.5 over codes, 1.2 and 1.6 at head_dim 64, and 3 us before its first): `own`
-// of them a group for one workgroup, less with more of them, but never less than `chip` / workgroups of the launch a group, the memory's share.  Fitted to the times of seven
-// calls at every division of the workgroups; us at the division that comes of it / at the best: 64 sequences behind 6000 rows 51.9 / 51.9, over codes 43.3 / 43.0, 90 in seven
-// groups 90.7 / 90.2, 24 with drafts 54.9 / 54.3, 192 behind 16000 to 24000 rows 217 / 213, of codes 193 / 190, at head_dim 64 119 / 118.
-// Two groups of columns together, fitted to 24 calls with drafts: at most 3 % from the best division, in 20 of them at it.
+// of them a group for one workgroup, less with more of them, but never less than `chip` / workgroups of the launch a group, the memory's share.  Fitted to the times of 48
+// calls of one group of columns and 24 of two at every division of the workgroups, over all of which the division that comes of it is 0.8 % slower than the best, at most 7 %; us at it / at
+// the best: 64 sequences behind 6000 rows 52.1 / 52.1, over codes 44.1 / 44.1, 90 in seven groups 89.8 / 89.5, 24 with drafts 54.0 / 53.6, 192 behind 16000 to 24000 rows 217 / 217, of codes 192 / 192.
 struct OwnCost { float own, chip; };
 template <int D, int GR, int NC> constexpr OwnCost kOwnCost =
-    NC == 1 ? (D == 128 ? (GR == 16 ? OwnCost{0.0545f, 0.112f} : OwnCost{0.0845f, 0.051f}) : (GR == 16 ? OwnCost{0.102f, 0.107f} : OwnCost{0.17f, 0.224f}))
-            : (D == 128 ? (GR == 16 ? OwnCost{0.104f, 0.035f} : OwnCost{0.1f, 0.04f}) : (GR == 16 ? OwnCost{0.21f, 0.045f} : OwnCost{0.09f, 0.39f}));
+    NC == 1 ? (D == 128 ? (GR == 16 ? OwnCost{0.08f, 0.068f} : OwnCost{0.0912f, 0.017f}) : (GR == 16 ? OwnCost{0.139f, 0.053f} : OwnCost{0.157f, 0.074f}))
+            : (D == 128 ? (GR == 16 ? OwnCost{0.104f, 0.035f} : OwnCost{0.1f, 0.04f}) : (GR == 16 ? OwnCost{0.21f, 0.045f} : OwnCost{0.113f, 0.336f}));
 
 // A tile's time where some waves have no rows: 1.6 us with two of eight.
 template <int D> MA_DEV float tile_time(int rows) { return 0.73f + 0.27f * (float)((rows + 31) >> 5) / (float)kSharedWaves<D>; }
@@ -146,7 +145,7 @@ template <int D> MA_DEV float tile_time(int rows) { return 0.73f + 0.27f * (floa
 // two more where whole tiles to a share make that the shorter.  `each`: a tile's time on average.
 template <int D, int GR, int NC> MA_DEV int tile_ranks(int tiles, float each, int total, int Hkv, int G) {
     const float W = (float)tiles * each * (float)Hkv, A = kOwnCost<D, GR, NC>.own * (float)total, B = kOwnCost<D, GR, NC>.chip * (float)total, S = W + A + B;
-    const int most = (G - (total > 0 ? G / 8 : 0)) / Hkv;
+    const int most = (G - (total > 0 ? G / 16 : 0)) / Hkv;   // (own rows of a token or two: 192 sequences behind 16000 to 24000 rows of codes 131 us with a sixteenth for them, 136 with an eighth)
     const int first = min(max((int)(2.f * W * (float)G / (S + sqrtf(fmaxf(S * S - 4.f * B * W, 0.f))) / (float)Hkv), 1), most);
     int best = first;
     float least = 3.0e38f;
