@@ -3,7 +3,7 @@
 //
 // A wave streams rows of one (sequence, KV head) on its own, with a ring of groups of rows in registers: 16 rows of 16-bit values,
 // loaded as whole rows and turned into matrix operands in the wave's LDS; or 32 rows of e4m3 codes, K loaded straight in the
-// operand's layout (the order of the contraction is free as long as q is loaded in the same), V as whole rows, both widened on the way.
+// operand's layout (the order of the contraction is free as long as q is loaded in the same) or as whole rows, V as whole rows, both widened on the way.
 // A page holds at least 16 rows, so a group (or half of one) lies in one page, whose table entry is read as a scalar a group ahead.
 // S^T[keys x 16 columns] = K Q^T, softmax per column with a lazy reference, O^T += V^T P^T.
 #pragma once
@@ -50,6 +50,7 @@ template <int D> struct DecodeGeom {
     static constexpr int RPI8 = 1024 / D;              // the same for rows of codes
     static constexpr int NI8 = 16 / RPI8;
     static MA_DEV int swz_v(int row) { return D == 128 ? ((row & 7) << 1) : (((row >> 1) & 3) << 1); }
+    static MA_DEV int swz_c(int row) { return D == 128 ? (row & 7) : ((row >> 1) & 3); }   // of codes
     static MA_DEV int swz_k(int row) { return D == 128 ? (row & 15) : ((row >> 1) & 7); }
 };
 template <int D, bool FP8> constexpr int kWaveLds = FP8 ? 32 * D * 2 : 2 * 16 * D * 2;   // V of 32 rows; or K and V of 16
@@ -68,7 +69,10 @@ MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg,
 }
 
 // Streams groups g0 .. g1 - 1 (at least one) of (sequence s, KV head g) for the columns of NC groups from hg on; `area` is the wave's own LDS.
-template <class T, int D, bool FP8, int NC>
+// WHOLE_K: K's codes are loaded as whole rows as well and turned in the LDS.  Straight in the operand's layout a load's neighbouring lanes read 16 bytes of different rows, which the
+// unit's address path takes in pieces: no matter where the memory bounds all units together (64 sequences to 8192 rows 100.8 us straight, 101.4 whole), but with a few
+// units streaming beside others' products it does (attn_shared.hip, 192 sequences behind 16000 to 24000 rows 196 / 178; at head_dim 64, whose rows are 64 bytes, 129 / 132).
+template <class T, int D, bool FP8, int NC, bool WHOLE_K>
 MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D> (&acc)[NC]) {
     const PagedParams& p = work.p;
     using GEO = DecodeGeom<D>;
@@ -132,7 +136,8 @@ MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, i
                 const char* kb = (const char*)p.c.k + at;
                 const char* vb = (const char*)p.c.v + at;
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) st.k[h * (D / 64) + j] = stream_load(reinterpret_cast<const u32x4*>(kb + (uint32_t)(l16 * step + k_piece + 64 * j)));
+                for (int j = 0; j < NI8; ++j)
+                    st.k[h * NI8 + j] = stream_load(reinterpret_cast<const u32x4*>(kb + (uint32_t)(WHOLE_K ? (j * RPI8 + v_row) * step + v_piece : l16 * step + k_piece + 64 * j)));
 #pragma unroll
                 for (int j = 0; j < NI8; ++j) st.v[h * NI8 + j] = stream_load(reinterpret_cast<const u32x4*>(vb + (uint32_t)((j * RPI8 + v_row) * step + v_piece)));
                 const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
@@ -177,6 +182,18 @@ MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, i
             for (int j = 0; j < NV; ++j) st.v[j] = j * VPI + v_row < past ? st.v[j] : u32x4{0u, 0u, 0u, 0u};
         }
         if constexpr (FP8) {
+            static_assert(D / 64 == NI8, "as many loads either way");
+            if (WHOLE_K) {   // (through the place where V's values go behind them)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    const int row = i * RPI8 + lane / (D / 16);
+                    *reinterpret_cast<u32x4*>(my_v + row * D + 16 * ((lane % (D / 16)) ^ GEO::swz_c(row))) = st.k[i];
+                }
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int j = 0; j < NI8; ++j) st.k[h * NI8 + j] = *reinterpret_cast<const u32x4*>(my_v + (16 * h + l16) * D + 16 * ((4 * j + quad) ^ GEO::swz_c(l16)));
+            }
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
 #pragma unroll
@@ -184,7 +201,7 @@ MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, i
                 const float ks = scale_value(st.ks[h] >> 8 * (st.there >> (8 + 4 * h) & 3) & 255u);
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
-                    const u32x4 x = st.k[h * (D / 64) + c / 2];
+                    const u32x4 x = st.k[h * NI8 + c / 2];
                     const uint32_t lo = x[2 * (c % 2)], hi = x[2 * (c % 2) + 1];
                     const u32x4 a = {widen2<T, false>(lo, ks), widen2<T, true>(lo, ks), widen2<T, false>(hi, ks), widen2<T, true>(hi, ks)};
 #pragma unroll
@@ -362,7 +379,7 @@ MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, i
 // One group of columns.
 template <class T, int D, bool FP8>
 MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D>& acc) {
-    stream_columns<T, D, FP8, 1>(work, s, info, g, hg, g0, g1, area, reinterpret_cast<ColumnAcc<D> (&)[1]>(acc));
+    stream_columns<T, D, FP8, 1, false>(work, s, info, g, hg, g0, g1, area, reinterpret_cast<ColumnAcc<D> (&)[1]>(acc));
 }
 
 // Where column c of a column group's partial result `part` lies.  Partial results are numbered through the launch, those of a (sequence, KV head,

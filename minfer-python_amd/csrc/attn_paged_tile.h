@@ -240,34 +240,57 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
         }
         return r;
     };
-    // The same in two halves (SHARED): the codes of the wave's own area widened into registers in front of a barrier, and behind it stored.
-    struct Wide { s16x8 k[2 * NR], v[2 * NR]; };
-    auto widen = [&](int kt, int there, uint32_t raw) __attribute__((always_inline)) {
-        Wide r;
-        for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
-            constexpr int j = decltype(j_tag)::value;
-            const bool on = (there >> block_of(j) & 1) && kt * KEYS + (j * NW + w) * RPI8 + lane / (D / 16) < ctx;
-            s16x8 x[2];
-            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw + 16 * lane, 2 * j * 1024)), scale_value(scales.k[j]), x);
-            r.k[2 * j] = x[0]; r.k[2 * j + 1] = x[1];
-            widen16<T>(__builtin_bit_cast(u32x4, lds_read_b128(raw + 16 * lane, (2 * j + 1) * 1024)), scale_value(scales.v[j]), x);
+    // The words that hold a tile's scales and, two bits each, which byte of them: to take the bytes out is to wait for the words.
+    struct ScaleWords { uint32_t k[NR], v[NR]; int bytes; };
+    auto words_of = [&](const Pages& pg) __attribute__((always_inline)) {
+        ScaleWords r{};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) r.v[2 * j + h] = on ? x[h] : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        });
+        for (int j = 0; j < NR; ++j) {
+            const int id = page_of(pg, block_of(j));
+            const int64_t sc = (int64_t)(is_there(id) ? id : 0) * p.Hkv + g;
+            const uintptr_t ka = (uintptr_t)(p.c.k_scales + sc), va = (uintptr_t)(p.c.v_scales + sc);
+            r.k[j] = const_load((const uint32_t*)(ka & ~(uintptr_t)3));
+            r.v[j] = const_load((const uint32_t*)(va & ~(uintptr_t)3));
+            r.bytes |= ((int)(ka & 3) | (int)(va & 3) << 2) << 4 * j;
+        }
         return r;
     };
-    auto store_wide = [&](const Wide& x, int stage) __attribute__((always_inline)) {
+    auto bytes_of = [&](const ScaleWords& x) __attribute__((always_inline)) {
+        Scales r;
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            r.k[j] = x.k[j] >> 8 * (x.bytes >> 4 * j & 3) & 255u;
+            r.v[j] = x.v[j] >> 8 * (x.bytes >> (4 * j + 2) & 3) & 255u;
+        }
+        return r;
+    };
+    // The same (SHARED) of K (kv 0) or V (1) alone, read and stored at different places.
+    struct Half { u32x4 x[NR]; };
+    auto read_half = [&](uint32_t raw, int kv, Half& r) __attribute__((always_inline)) {
+        for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
+            constexpr int j = decltype(j_tag)::value;
+            r.x[j] = __builtin_bit_cast(u32x4, kv == 0 ? lds_read_b128(raw + 16 * lane, 2 * j * 1024) : lds_read_b128(raw + 16 * lane, (2 * j + 1) * 1024));
+        });
+    };
+    auto store_half = [&](int kt, int there, int stage, int kv, Half& from) __attribute__((always_inline)) {
         int ln = lane;
         asm volatile("" : "+v"(ln));   // (as below)
         const int row_in = ln / (D / 16), gr = 2 * (ln % (D / 16)), row_w = w * RPI8 + row_in;
         const uint32_t base = lds_addr(lds) + stage * STAGE_BYTES + row_w * RB;
-        const uint32_t k_to = base + 16 * (gr ^ GEO::swz_k(row_w)), v_to = base + GEO::TILE_BYTES + 16 * (gr ^ GEO::swz_v(row_w));
+        const uint32_t to = kv == 0 ? base + 16 * (gr ^ GEO::swz_k(row_w)) : base + GEO::TILE_BYTES + 16 * (gr ^ GEO::swz_v(row_w));
         for_range<0, NR>([&](auto j_tag) __attribute__((always_inline)) {
             constexpr int j = decltype(j_tag)::value, AT = j * NW * RPI8 * RB;
-            lds_write_b128(k_to, AT, x.k[2 * j]);
-            lds_write_b128(k_to ^ 16u, AT, x.k[2 * j + 1]);
-            lds_write_b128(v_to, AT, x.v[2 * j]);
-            lds_write_b128(v_to ^ 16u, AT, x.v[2 * j + 1]);
+            s16x8 x[2];
+            float scale = scale_value(kv == 0 ? scales.k[j] : scales.v[j]);
+            if (kv == 1) {   // (V of no row, and the scale of no page, are not multiplied)
+                const bool on = (there >> block_of(j) & 1) && kt * KEYS + j * NW * RPI8 + row_w < ctx;
+                scale = on ? scale : 1.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) from.x[j][e] = on ? from.x[j][e] : 0u;
+            }
+            widen16<T>(from.x[j], scale, x);
+            lds_write_b128(to, AT, x[0]);
+            lds_write_b128(to ^ 16u, AT, x[1]);
         });
     };
     auto widen_tile = [&](int kt, int there, int stage, uint32_t raw) __attribute__((always_inline)) {
@@ -321,7 +344,8 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
     s16x8 qf[2][KC];
     int by_key = 0x7fffffff;   // the tile from which on the wave's keys are taken one by one
 
-    auto process_tile = [&](auto stage_tag, int kt, int there) __attribute__((always_inline)) {
+    // `beside(i)`, i = 0, 1, 2: what is done between the products with V
+    auto process_tile = [&](auto stage_tag, int kt, int there, auto beside) __attribute__((always_inline)) {
         constexpr int SOFF = decltype(stage_tag)::value * STAGE_BYTES;
         const int key0 = kt * KEYS;
         auto pin = [&]() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
@@ -362,7 +386,12 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
                 probe = T::mfma16(va[db], zero, probe);
                 if (NB == 4) probe = T::mfma16(read_v(1, db), zero, probe);
             }
-            if (__any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.f))) { by_key = kt; return; }
+            if (__any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.f))) {
+                by_key = kt;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) beside(i);
+                return;
+            }
         }
         if (key0 + KEYS - 1 > wave_first || !whole(kt, there)) {
 #pragma unroll
@@ -434,6 +463,7 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
                 if (s + 1 < NB && db < 4) pw[(s + 1) & 1][db] = weights_quarter((s + 1) >> 1, (s + 1) & 1, db);
                 pin();
             }
+            if (s < 3) beside(s);
         }
         l_sum[0] += ls[0];
         l_sum[1] += ls[1];
@@ -503,7 +533,7 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
                 }
                 pg = after;
             }
-            if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(stage_tag, kt, there);
+            if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(stage_tag, kt, there, [](int) {});
             there = there_1;
             there_1 = there_2;
         };
@@ -549,7 +579,7 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
                 if (it + 3 < n_own) copy_tile(kt + 3, pg, zero, dst0 + ((it + 3) & (STAGES - 1)) * STAGE_BYTES);
                 theres = theres >> NB | there_of(pg) << 2 * NB;
                 pg = after;
-                if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(zero, kt, there);
+                if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(zero, kt, there, [](int) {});
                 next_stage(it);
             }
         } else {
@@ -567,31 +597,47 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
             if (n_own > 3) request_codes(t_lo + 3, pg, raw0 + 3 * AREA);
             if (n_own > 0) {
                 wait_but(min(n_own - 1, 3));
-                store_wide(widen(t_lo, theres & ((1 << NB) - 1), raw0), 0);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    Half half;
+                    read_half(raw0, kv, half);
+                    store_half(t_lo, theres & ((1 << NB) - 1), 0, kv, half);
+                }
             }
             scales = scales_1;
             pg = pages_of(t_lo + 4);
             for (int it = 0; it < n_own; ++it) {
                 const int kt = t_lo + it, there = theres & ((1 << NB) - 1);
+                // the table's entries, the scales and the codes are asked for together: one wait
                 Pages after = pages_of(kt + 5), after_1 = pages_of(kt + 3);
-                scales_1 = scales_of(pg1);
+                ScaleWords words = words_of(pg1);
+                __builtin_amdgcn_sched_barrier(0);
                 pin_pages(after);
                 pin_pages(after_1);
 #pragma unroll
-                for (int j = 0; j < NR; ++j) asm volatile("" : "+s"(scales_1.k[j]), "+s"(scales_1.v[j]));
-                Wide wide{};
-                if (it + 1 < n_own) {
-                    wait_but(min(n_own - 2 - it, 2));   // the wave's codes of the next tile have landed
-                    wide = widen(kt + 1, theres >> NB & ((1 << NB) - 1), raw0 + ((it + 1) & (RING - 1)) * AREA);
-                }
+                for (int j = 0; j < NR; ++j) asm volatile("" : "+s"(words.k[j]), "+s"(words.v[j]));
+                scales_1 = bytes_of(words);
                 __syncthreads();       // everyone's share of the tile is widened; the other stage is no longer being read
                 theres = theres >> NB | there_of(pg1) << NB;
                 if (it + 4 < n_own) request_codes(kt + 4, pg, raw0 + (it & (RING - 1)) * AREA);
-                if (it + 1 < n_own) store_wide(wide, (it + 1) & 1);
+                // the next tile's codes, K's and V's one after the other (behind the last tile: what the area holds, into a stage that nobody reads)
+                const uint32_t area = raw0 + ((it + 1) & (RING - 1)) * AREA;
+                Half half;
+                auto next_tile = [&](int i) __attribute__((always_inline)) {
+                    if (i == 0) {
+                        wait_but(min(n_own - 2 - it, 3));   // the wave's codes of the next tile have landed
+                        read_half(area, 0, half);
+                    } else {
+                        store_half(kt + 1, theres & ((1 << NB) - 1), (it + 1) & 1, i - 1, half);
+                        if (i == 1) read_half(area, 1, half);
+                    }
+                };
+                if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(zero, kt, there, next_tile);
+                else
+                    for (int i = 0; i < 3; ++i) next_tile(i);
                 scales = scales_1;
                 pg = after;
                 pg1 = after_1;
-                if (wave_on && there && kt * KEYS <= wave_last && kt < by_key) process_tile(zero, kt, there);
                 next_stage(it);
             }
         }

@@ -7,7 +7,7 @@
 // * the own rows: streamed by single waves (stream_columns), for up to 32 (token, head) columns together: bound by memory.
 // Both are lines of places, cut into equal shares, and one launch, whose workgroups are divided between them so that both end together (tile_ranks).  Everything
 // is a partial result, and shared_merge_kernel puts a row's together.  32 heads on 8 of 128: 64 tokens behind 6000 rows and 50 to 1500 of their own 52 us, 4.5 TB/s of
-// what has to be read once (flash_attn_paged 233); 192 behind 16000 to 24000 rows of codes 192, bound by products and widening (1316); 24 sequences of 3 to 6 tokens behind
+// what has to be read once (flash_attn_paged 233); 192 behind 16000 to 24000 rows of codes 176, bound by products and widening (1316); 24 sequences of 3 to 6 tokens behind
 // 12000 rows 54 (145).  Of that the start is 7 us (lengths and groups looked up 2.2, the first rows 4), the merge 5 to 9.
 //
 // How the work is cut follows from device data (lengths, contexts, groups) that every wave looks up for itself, a sequence or a group to a lane.
@@ -132,7 +132,7 @@ struct SharedPlan {
 // Time of the own rows in tiles (what a workgroup takes for one whose waves all have rows: 2.05 us at head_dim 128, 2.5 over codes, 1.2 and 1.6 at head_dim 64, and 3 us before its first): `own`
 // of them a group for one workgroup, less with more of them, but never less than `chip` / workgroups of the launch a group, the memory's share.  Fitted to the times of 48
 // calls of one group of columns and 24 of two at every division of the workgroups, over all of which the division that comes of it is 0.8 % slower than the best, at most 7 %; us at it / at
-// the best: 64 sequences behind 6000 rows 52.1 / 52.1, over codes 44.1 / 44.1, 90 in seven groups 89.8 / 89.5, 24 with drafts 54.0 / 53.6, 192 behind 16000 to 24000 rows 217 / 217, of codes 192 / 192.
+// the best: 64 sequences behind 6000 rows 52.1 / 52.1, over codes 41.1 / 41.1, 90 in seven groups 89.8 / 89.5, 24 with drafts 54.0 / 53.6, 192 behind 16000 to 24000 rows 217 / 217, of codes 175 / 175.
 struct OwnCost { float own, chip; };
 template <int D, int GR, int NC> constexpr OwnCost kOwnCost =
     NC == 1 ? (D == 128 ? (GR == 16 ? OwnCost{0.08f, 0.068f} : OwnCost{0.0912f, 0.017f}) : (GR == 16 ? OwnCost{0.139f, 0.053f} : OwnCost{0.157f, 0.074f}))
@@ -145,7 +145,7 @@ template <int D> MA_DEV float tile_time(int rows) { return 0.73f + 0.27f * (floa
 // two more where whole tiles to a share make that the shorter.  `each`: a tile's time on average.
 template <int D, int GR, int NC> MA_DEV int tile_ranks(int tiles, float each, int total, int Hkv, int G) {
     const float W = (float)tiles * each * (float)Hkv, A = kOwnCost<D, GR, NC>.own * (float)total, B = kOwnCost<D, GR, NC>.chip * (float)total, S = W + A + B;
-    const int most = (G - (total > 0 ? G / 16 : 0)) / Hkv;   // (own rows of a token or two: 192 sequences behind 16000 to 24000 rows of codes 131 us with a sixteenth for them, 136 with an eighth)
+    const int most = (G - (total > 0 ? G / 16 : 0)) / Hkv;   // (own rows of a token or two: 192 sequences behind 16000 to 24000 rows of codes 127 us with a sixteenth for them, 133 with an eighth)
     const int first = min(max((int)(2.f * W * (float)G / (S + sqrtf(fmaxf(S * S - 4.f * B * W, 0.f))) / (float)Hkv), 1), most);
     int best = first;
     float least = 3.0e38f;
@@ -338,7 +338,7 @@ template <class T, int D, bool FP8, int NC> MA_DEV void shared_line(const Shared
         if (g1 <= g0) continue;
         const int g = d.n_hg == 1 ? pair : pair / d.n_hg, hg = pair - g * d.n_hg;   // (a KV head's groups of columns read the same rows one after the other)
         ColumnAcc<D> acc[NC];
-        stream_columns<T, D, FP8, NC>(d, s, info, g, hg * NC, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
+        stream_columns<T, D, FP8, NC, FP8 && D == 128>(d, s, info, g, hg * NC, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
 #pragma unroll
         for (int n = 0; n < NC; ++n) store_part<D>(d, hg * NC + n, (int64_t)s * pairs + pair + wave, acc[n], 16 * n);
     }

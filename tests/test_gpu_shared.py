@@ -169,6 +169,23 @@ def test_more_sequences_than_are_looked_up_at_once(kerns):
     check(kerns, Shared(lens, groups[:4200], 16, 1, 64, torch.float16, extra=1), 2, torch.float16)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_missing_pages_beside_a_page_of_no_numbers(kerns, D):
+    """Codes: pages that are missing in the prefix and among own rows, where nothing of the pool's first page, which is nobody's and holds codes and scales that are no numbers, is taken in their place."""
+    lens = [(1 + i % 2, 300 + 30 * i) for i in range(5)]
+    gone = {(s, i) for s in range(5) for i in (3, 8)} | {(1, 19), (3, 22)}
+    c = Shared(lens, [(0, 5, 256)], 16, 2, D, torch.float16, gone=gone, eight=True)
+    used = {x for row in c.table_list for x in row}
+    free = next(i for i in range(1, c.n_pages) if i not in used)
+    for pool in (c.k_pages, c.v_pages, c.k_scales, c.v_scales):
+        x = pool.view(torch.uint8)
+        x[free] = x[0]
+        x[0] = 0x7F if pool.dim() == 4 else 0xFF
+    c.table[c.table == 0] = free
+    c.table_list = [[free if x == 0 else x for x in row] for row in c.table_list]
+    check(kerns, c, 8, torch.float16)
+
+
 def test_long_prefix_of_a_few(kerns):
     """More pieces than a merge takes of one row, were they as short as they may be."""
     lens = [(1, 20000 + 100 * i) for i in range(3)]
