@@ -106,9 +106,9 @@ def test_drafts(kerns, dtype, eight, Hq, Hkv, D, most):
 
 
 @pytest.mark.parametrize("eight", [False, True])
-@pytest.mark.parametrize("Hq,Hkv,D,most", [(24, 4, 128, 3), (8, 2, 128, 6), (16, 1, 64, 2), (8, 2, 64, 11), (48, 4, 128, 3), (40, 2, 64, 1), (13, 1, 128, 4)])
+@pytest.mark.parametrize("Hq,Hkv,D,most", [(24, 4, 128, 3), (8, 2, 128, 6), (16, 1, 64, 2), (8, 2, 64, 11), (48, 4, 128, 3), (40, 2, 64, 1), (13, 1, 128, 4), (96, 1, 64, 1), (101, 1, 128, 1)])
 def test_more_than_16_columns(kerns, eight, Hq, Hkv, D, most):
-    """17 to 52 (token, head) rows per KV head, in whole and partly filled pairs of 16; sequences that fill the first 16 alone; shares that end inside a sequence."""
+    """17 to 101 (token, head) rows per KV head, in whole and partly filled pairs of 16; sequences that fill the first 16 alone; shares that end inside a sequence."""
     lens = [(1 + (5 * i) % most, 192 + (37 * i) % 900) for i in range(14)] + [(most, 3), (1, 200)]
     check(kerns, Shared(lens, [(0, 14, 192)], 32, Hkv, D, torch.bfloat16 if most == 3 else torch.float16, eight=eight, seed=Hq), Hq, torch.bfloat16 if most == 3 else torch.float16)
 
