@@ -132,6 +132,18 @@ def test_a_row_that_some_of_a_pair_of_columns_attend(kerns, eight, D):
         assert ((out[0].cpu().double() - want).abs() <= bound)[:, rest].all()
 
 
+def test_drafts_over_codes_in_a_table_just_wide_enough(kerns):
+    """From 25 MB on the kernels for groups take what goes to flash_attn_paged below: both sides right, and 16 columns still the latter's."""
+    lens = [(1 + 5 * (i % 2), 1100 + 10 * i) for i in range(8)]
+    for Hkv, most in ((4, 6), (8, 6), (8, 4)):
+        c = Shared([(min(n, most), past) for n, past in lens], [(0, 8, 512)], 512, Hkv, 128, torch.float16, wide=False, eight=True)
+        q = queries(c, 4 * Hkv, torch.float16)
+        out = check(kerns, c, 4 * Hkv, torch.float16)
+        takes = most == 6 and 8 * c.width * 512 * 2 * Hkv * 128 >= 25000000
+        assert takes == ((Hkv, most) == (8, 6))
+        assert takes or torch.equal(out, c.unshared(kerns, q))
+
+
 def test_longer_chunks_are_flash_attn_paged(kerns):
     c = Shared([(40, 128), (3, 140), (70, 200)], [(0, 3, 128)], 16, 2, 128, torch.float16)
     q = queries(c, 8, torch.float16)

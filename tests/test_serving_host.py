@@ -120,6 +120,18 @@ def test_shared_refuses(text, change):
     assert text in capi.last_error()
 
 
+@pytest.mark.parametrize("D,max_q,rows", [(64, 4, (220000000 // 512, 150000000 // 256)), (64, 6, (70000000 // 512, 25000000 // 256)), (128, 4, (220000000 // 1024, 150000000 // 512)),
+                                          (128, 6, (220000000 // 1024, 25000000 // 512))])
+def test_shared_is_for_tables_of_many_rows(D, max_q, rows):
+    """The workspace is that of flash_attn_paged below the first of the two kinds of pages' bounds, and larger from there on."""
+    n, first = 16, -(-min(rows) // 16)
+    f, plain = cs.lib().minfer_flash_attn_paged_shared_workspace_bytes, cs.lib().minfer_flash_attn_paged_workspace_bytes
+    for context in (first - 1, first):
+        args = (n * max_q, 8, 2, D, context, max_q)
+        assert (f(n, 1, *args) > plain(n, *args)) == (context >= first)
+        assert f(n, 0, *args) == plain(n, *args)
+
+
 def test_shared_workspace_and_empty_calls():
     w = cs.lib().minfer_flash_attn_paged_shared_workspace_bytes
     for bad in ((0, 1, 1, 8, 2, 128, 1024, 1), (1, -1, 1, 8, 2, 128, 1024, 1), (1, 1, 0, 8, 2, 128, 1024, 1), (1, 1, 1, 7, 2, 128, 1024, 1)):
