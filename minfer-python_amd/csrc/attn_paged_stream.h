@@ -69,16 +69,17 @@ MA_DEV Column column_of(const DecodeWork& w, const SeqInfo& info, int g, int hg,
 }
 
 // Streams groups g0 .. g1 - 1 (at least one) of (sequence s, KV head g) for the columns of NC groups from hg on; `area` is the wave's own LDS.
+// NS: groups on their way.  Three where nothing else runs; beside others' products two end sooner by up to 5 % (seven groups of sequences, 16-bit / codes, at head_dim 128 98 / 73 us with three,
+// 97 / 71 with two, 99 / 76 with four; at 64 54 / 46, 51 / 44, 54 / 48).
 // WHOLE_K: K's codes are loaded as whole rows as well and turned in the LDS.  Straight in the operand's layout a load's neighbouring lanes read 16 bytes of different rows, which the
 // unit's address path takes in pieces: no matter where the memory bounds all units together (64 sequences to 8192 rows 100.8 us straight, 101.4 whole), but with a few
 // units streaming beside others' products it does (attn_shared.hip, 192 sequences behind 16000 to 24000 rows 196 / 178; at head_dim 64, whose rows are 64 bytes, 129 / 132).
-template <class T, int D, bool FP8, int NC, bool WHOLE_K>
+template <class T, int D, bool FP8, int NC, int NS, bool WHOLE_K>
 MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D> (&acc)[NC]) {
     const PagedParams& p = work.p;
     using GEO = DecodeGeom<D>;
     constexpr int RB = GEO::RB, G = GEO::G, RPI = GEO::RPI, NI = GEO::NI, RPI8 = GEO::RPI8, NI8 = GEO::NI8;
     constexpr int KC = D / 32, DB = D / 16, GR = kRows<FP8>, NH = GR / 16;   // halves of 16 rows in a group
-    constexpr int NS = 3;
     const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
     const int ctx = info.ctx, page_mask = (1 << p.c.page_log2) - 1;
     const int32_t* const table = p.c.table + (int64_t)s * p.c.table_stride;
@@ -379,7 +380,7 @@ MA_DEV void stream_columns(const DecodeWork& work, int s, const SeqInfo& info, i
 // One group of columns.
 template <class T, int D, bool FP8>
 MA_DEV void stream_pages(const DecodeWork& work, int s, const SeqInfo& info, int g, int hg, int g0, const int g1, char* area, ColumnAcc<D>& acc) {
-    stream_columns<T, D, FP8, 1, false>(work, s, info, g, hg, g0, g1, area, reinterpret_cast<ColumnAcc<D> (&)[1]>(acc));
+    stream_columns<T, D, FP8, 1, 3, false>(work, s, info, g, hg, g0, g1, area, reinterpret_cast<ColumnAcc<D> (&)[1]>(acc));
 }
 
 // Where column c of a column group's partial result `part` lies.  Partial results are numbered through the launch, those of a (sequence, KV head,

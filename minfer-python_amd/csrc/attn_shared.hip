@@ -339,7 +339,7 @@ template <class T, int D, bool FP8, int NC> MA_DEV void shared_line(const Shared
         if (g1 <= g0) continue;
         const int g = d.n_hg == 1 ? pair : pair / d.n_hg, hg = pair - g * d.n_hg;   // (a KV head's groups of columns read the same rows one after the other)
         ColumnAcc<D> acc[NC];
-        stream_columns<T, D, FP8, NC, FP8 && D == 128>(d, s, info, g, hg * NC, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
+        stream_columns<T, D, FP8, NC, 2, FP8 && D == 128>(d, s, info, g, hg * NC, first + g0, first + g1, lds + wid * kWaveLds<D, FP8>, acc);
 #pragma unroll
         for (int n = 0; n < NC; ++n) store_part<D>(d, hg * NC + n, (int64_t)s * pairs + pair + wave, acc[n], 16 * n);
     }
