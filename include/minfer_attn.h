@@ -424,7 +424,7 @@ int minfer_rope_kv_append_q8_0(int dtype, int style, void* q, const void* k, con
  * address is made from more; but the result is that above only where cu_groups does not fall, and cu_seqlens does not either, except for
  * entries behind the last sequence with tokens.  Meant for single tokens and drafts (max_q_len * Hq / Hkv <= 64, and max_q_len 1 where Hq / Hkv > 16) whose tables name
  * more rows than the memory-side cache holds (n_seqs * pages_per_seq * page_size rows of 220 MB or more, of 150 MB of 8-bit pages; where max_q_len * Hq / Hkv > 16, of 70 MB at
- * head_dim 64 and of 25 MB of 8-bit pages); all other calls, which gain nothing by groups, are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
+ * head_dim 64 and of 25 MB of 8-bit pages), in tables not too short (where max_q_len * Hq / Hkv > 16) and groups not too small (two to four sequences on average); all other calls, which gain nothing by groups, are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
  */
 size_t minfer_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                                       int64_t max_context, int64_t max_q_len);

@@ -27,7 +27,7 @@ constexpr int shared_wgs(int64_t D) { return 256 * 8 / shared_waves(D); }
 template <int D> constexpr int kSharedWaves = shared_waves(D);
 template <int D> constexpr int kBlockRows = shared_waves(D) * 32;
 // Of all rows that the tables may name (shared_takes): from here on; where there are more than 16 columns, at head_dim 64 and over codes.
-constexpr int64_t kSharedBytes = 220000000, kSharedBytesCodes = 150000000, kSharedBytesPairs = 70000000, kSharedBytesPairsCodes = 25000000;
+constexpr int64_t kSharedBytes = 220000000, kSharedBytesCodes = 150000000, kSharedBytesPairs = 70000000, kSharedBytesPairsCodes = 25000000, kSharedBytesLong = 600000000;
 constexpr int kMaxSharedHeads = 128;                               // KV heads: each has workgroups of its own for the prefix
 
 struct SharedWork {
@@ -459,14 +459,20 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
 // 269 MB, 22.8 / 26.5; of codes: 8 behind 4000, 72 MB, 24.3 / 17.7, 16 behind 4000, 144 MB, 25.3 / 24.4, 64 behind 1000, 183 MB, 27.6 / 36.6.)  More than 16 columns
 // are read once here and twice or more often there, which matters over codes and at head_dim 64 (3 to 6 tokens, 32 heads on 8 of 128, codes: 8 sequences behind 1000, 22 MB, 24.0 / 23.8, 8 behind
 // 2000, 38 MB, 27.1 / 28.3, 8 behind 8000, 139 MB, 36.8 / 54.6; 16-bit 16 behind 2000, 154 MB, 30.4 / 29.3; 8 on 2 of 64: 32 behind 4000, 72 MB, 24.3 / 23.7, 32 behind 8000, 139 MB, 27.0 / 31.7;
-// of codes 32 behind 2000, 19 MB, 20.2 / 22.5, 64 behind 8000, 139 MB, 34.1 / 59.4).  The host knows the table's width, not the contexts: a table far wider than they are costs a short
+// of codes 32 behind 2000, 19 MB, 20.2 / 22.5, 64 behind 8000, 139 MB, 34.1 / 59.4).  But every row of theirs makes partial results, whose way through memory short contexts do not pay for (64
+// sequences of 3 to 6 tokens, 32 heads on 8 of 128, codes: behind 384 36.6 / 24.2, 768 38.9 / 36.6, 1536 45.3 / 60.9; 160 behind 768, 294 MB, 67.6 / 96.4; 16-bit 64 behind 768 38.5 / 26.8, behind 1536 42.3 / 44.1,
+// 64 heads 59.0 / 48.7; 160 behind 1536, 1.1 GB, 118 / 131), nor does a prefix of two (60 sequences in groups of 2 / 3 / 4 behind 2000 with 1000 of their own, codes 84.5, 65.8, 56.8 / 65; with
+// drafts 104, 84, 80 / 105; 16-bit 92, 75, 63 / 111; with drafts 114, 91, 81 / 86).  The host knows the table's width, not the contexts: a table far wider than they are costs a short
 // call 8 us.
 static bool shared_takes(bool eight, int64_t n_seqs, int64_t n_groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
     const int64_t n_rep = Hq / Hkv, bytes = 2 * Hkv * D * (eight ? 1 : 2);   // of a row of all heads, k and v
     if (n_groups == 0 || Hkv > kMaxSharedHeads || (max_q > 1 && (n_rep > 16 || max_q * n_rep > 64))) return false;
     const bool pairs = max_q * n_rep > 16;
-    const int64_t from = eight ? (pairs ? kSharedBytesPairsCodes : kSharedBytesCodes) : (pairs && D == 64 ? kSharedBytesPairs : kSharedBytes);
-    return n_seqs * max_context >= from / bytes;
+    const int64_t rows = n_seqs * max_context;
+    auto most = [&](int64_t total) { return rows >= total / bytes; };
+    if (!pairs) return most(eight ? kSharedBytesCodes : kSharedBytes) && (!eight || n_seqs >= 3 * n_groups);
+    if (eight) return most(kSharedBytesCodes) ? max_context >= 600 && n_seqs >= 2 * n_groups : most(kSharedBytesPairsCodes) && max_context >= 1000 && n_seqs >= 3 * n_groups;
+    return most(D == 64 ? kSharedBytesPairs : kSharedBytes) && max_context >= (most(kSharedBytesLong) ? 1200 : 2000) && n_seqs >= 4 * n_groups;
 }
 
 // Groups of 16 columns that a wave streams a sequence's own rows for together: two where there are more than one.  (us, one at a time / two, each at the best division of the workgroups;

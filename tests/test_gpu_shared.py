@@ -117,18 +117,18 @@ def test_more_than_16_columns(kerns, eight, Hq, Hkv, D, most):
 @pytest.mark.parametrize("D", [64, 128])
 def test_a_row_that_some_of_a_pair_of_columns_attend(kerns, eight, D):
     """A NaN that the last drafts of a sequence attend and the first ones do not, at a border of 16 columns and on either side of it."""
-    lens = [(7, 256 + 20 * i) for i in range(3)]
-    clean = Shared(lens, [(0, 3, 256)], 16, 2, D, torch.float16, eight=eight)
+    lens = [(7, 256 + 20 * i) for i in range(5)]
+    clean = Shared(lens, [(0, 5, 256)], 16, 2, D, torch.float16, eight=eight)
     q = queries(clean, 8, torch.float16)
     want, bound = ref.attend(clean, q[0].cpu())
     for tok in (3, 4, 5):
-        c = Shared(lens, [(0, 3, 256)], 16, 2, D, torch.float16, eight=eight)
+        c = Shared(lens, [(0, 5, 256)], 16, 2, D, torch.float16, eight=eight)
         raw, row = c.v_pages.view(torch.uint8) if eight else c.v_pages, 276 + tok
         raw[c.table_list[1][row // 16], 1, row % 16, 9] = 0x7F if eight else float("nan")
         out = c.call(kerns, q)
         seen = torch.isnan(out[0]).any(-1)
         assert seen[4:].any(0).nonzero().flatten().tolist() == list(range(7 + tok, 14)) and not seen[:4].any()
-        rest = [t for t in range(21) if not 7 + tok <= t < 14]
+        rest = [t for t in range(35) if not 7 + tok <= t < 14]
         assert ((out[0].cpu().double() - want).abs() <= bound)[:, rest].all()
 
 

@@ -132,6 +132,17 @@ def test_shared_is_for_tables_of_many_rows(D, max_q, rows):
         assert f(n, 0, *args) == plain(n, *args)
 
 
+def test_shared_is_not_for_drafts_of_short_tables_or_small_groups():
+    """More than 16 columns: 600 rows at least, 1000 and groups of three below 150 MB of codes; 16-bit rows, of which there are more bytes, 1200 or 2000 and groups of four."""
+    f, plain = cs.lib().minfer_flash_attn_paged_shared_workspace_bytes, cs.lib().minfer_flash_attn_paged_workspace_bytes
+    takes = lambda n, groups, context, max_q=6: f(n, groups, n * max_q, 32, 8, 128, context, max_q) > plain(n, n * max_q, 32, 8, 128, context, max_q)
+    assert [takes(160, 1, c) for c in (592, 608)] == [False, True]
+    assert [takes(40, 1, c) for c in (992, 1008)] == [False, True]
+    assert [takes(40, g, 1500) for g in (14, 13)] == [False, True]
+    assert [takes(160, g, 1500) for g in (81, 80)] == [False, True]
+    assert takes(160, 160, 1500, max_q=1)
+
+
 def test_shared_workspace_and_empty_calls():
     w = cs.lib().minfer_flash_attn_paged_shared_workspace_bytes
     for bad in ((0, 1, 1, 8, 2, 128, 1024, 1), (1, -1, 1, 8, 2, 128, 1024, 1), (1, 1, 0, 8, 2, 128, 1024, 1), (1, 1, 1, 7, 2, 128, 1024, 1)):
