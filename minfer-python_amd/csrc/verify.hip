@@ -228,7 +228,8 @@ template <class E> MA_DEV void finish_row(const VerifyParams& p, int s, const Ro
         of = block_scan(mine, part);
     }
     const double mark = (double)p.sample_u[s] * of.all;
-    const int chunk = first_thread(of.front + mine > mark, mine > 0.0, ipart);
+    // (a thread that weighs nothing is not a hit: sums to its front and to the end of the one before are added in different orders, and a mark may lie between them)
+    const int chunk = first_thread(mine > 0.0 && of.front + mine > mark, mine > 0.0, ipart);
     int64_t token = -1;   // a row that holds no probability
     if (chunk >= 0) {
         // the sum in front of the chunk, from the thread that has it
@@ -247,7 +248,7 @@ template <class E> MA_DEV void finish_row(const VerifyParams& p, int s, const Ro
         }
         for (; i < i1; ++i) sum += row.one(i);
         const Scan in = block_scan(sum, part);
-        const int owner = first_thread(front + in.front + sum > mark, sum > 0.0, ipart);
+        const int owner = first_thread(sum > 0.0 && front + in.front + sum > mark, sum > 0.0, ipart);
         if (tid == owner) front_s = front + in.front;
         __syncthreads();
         if (wave_id() == 0 && owner >= 0) {   // the owner's elements, one to a lane
