@@ -52,15 +52,19 @@ template <int CTRL, int ROW_MASK = 0xf> MA_DEV int64_t row_exchange64(int64_t x)
     const uint32_t lo = row_exchange<CTRL, ROW_MASK>((uint32_t)x), hi = row_exchange<CTRL, ROW_MASK>((uint32_t)(x >> 32));
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
-MA_DEV int64_t wave_sum(int64_t x) {
+MA_DEV int64_t wave_scan(int64_t x) {
     x += row_exchange64<0x111>(x);
     x += row_exchange64<0x112>(x);
     x += row_exchange64<0x114>(x);
     x += row_exchange64<0x118>(x);
     x += row_exchange64<0x142, 0xa>(x);
     x += row_exchange64<0x143, 0xc>(x);
-    return (int64_t)((uint64_t)(uint32_t)lane_value((int)(x >> 32), 63) << 32 | (uint32_t)lane_value((int)x, 63));
+    return x;
 }
+MA_DEV int64_t lane_value(int64_t x, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)lane_value((int)(x >> 32), lane) << 32 | (uint32_t)lane_value((int)x, lane));
+}
+MA_DEV int64_t wave_sum(int64_t x) { return lane_value(wave_scan(x), 63); }
 // x summed over the workgroup, in every thread; `part` is the caller's, one entry a wave.
 MA_DEV int64_t block_sum(int64_t x, int64_t* part) {
     x = wave_sum(x);
@@ -179,7 +183,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void paged_release_few_kernel(const
         if (lane == 0) { counts[s] = n; p.held_after[s] = lane_value(mine.stay, s); }
     }
     __syncthreads();
-    const int n = lane < p.n_seqs ? counts[lane] : 0, incl = wave_inclusive_scan(n);   // (64 times 2^26 pages at most: as many as a table names)
+    const int n = lane < p.n_seqs ? counts[lane] : 0;
+    const int64_t incl = wave_scan((int64_t)n);   // (64 times 2^26 pages, which a table may name, are 2^32)
     for (int s = w; s < p.n_seqs; s += kFewWaves) {
         const Shrunk q{lane_value(mine.stay, s), lane_value(mine.held, s)};
         if (lane_value(n, s) > 0) give_back(p, ring, s, q, lane_value(incl - n, s));
