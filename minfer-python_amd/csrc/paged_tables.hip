@@ -201,24 +201,33 @@ __global__ __launch_bounds__(kTableThreads) void paged_release_count_kernel(cons
     if (lane == 0) { p.counts[s] = n; p.held_after[s] = q.stay; }
 }
 
-// A wave per sequence again: its pages behind those of the sequences in front.
+// A wave per sequence again: its pages behind those of the sequences in front.  Up to kReleaseWgs workgroups of per_wg consecutive sequences, four at a time: every workgroup sums all counts in front of
+// its first sequence, so that more of them would cost sequences times sequences (2^18 that end 2.0 ms with a workgroup for every four of them, 0.36 so; 2^24 27 ms).
+constexpr int64_t kReleaseWgs = 1024;
 __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const TableParams p) {
     __shared__ int64_t parts[kTableThreads / 64];
     constexpr int NW = kTableThreads / 64;
     const int tid = threadIdx.x, lane = tid & 63, w = wave_id();
-    const int s0 = (int)blockIdx.x * NW, s = s0 + w;
+    const int first = (int)blockIdx.x * p.per_wg, last = min(first + p.per_wg, p.n_seqs);
     const Ring ring = ring_of(p);
     int64_t front = 0;
-    for (int i = tid; i < s0; i += kTableThreads) front += p.counts[i];
+    for (int i = tid; i < first; i += kTableThreads) front += p.counts[i];
     front = block_sum(front, parts);
-    int mine[NW - 1];   // of the workgroup's other sequences in front, requested together
+    for (int s0 = first; s0 < last; s0 += NW) {
+        int count[NW];   // of the four, requested together
 #pragma unroll
-    for (int i = 0; i < NW - 1; ++i) mine[i] = s0 + i < p.n_seqs ? p.counts[s0 + i] : 0;
+        for (int i = 0; i < NW; ++i) count[i] = s0 + i < last ? p.counts[s0 + i] : 0;
+        int64_t mine = front;
 #pragma unroll
-    for (int i = 0; i < NW - 1; ++i) front += i < w ? mine[i] : 0;
-    if (s >= p.n_seqs) return;
-    front += give_back(p, ring, s, shrunk(p, s), front);
-    if (lane == 0 && s == p.n_seqs - 1) leave_state(p, ring, front);
+        for (int i = 0; i < NW; ++i) {
+            mine += i < w ? count[i] : 0;
+            front += count[i];
+        }
+        const int s = s0 + w;
+        if (s >= last) continue;
+        give_back(p, ring, s, shrunk(p, s), mine);
+        if (lane == 0 && s == p.n_seqs - 1) leave_state(p, ring, front);
+    }
 }
 
 static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -303,9 +312,11 @@ MINFER_ATTN_EXPORT int minfer_paged_release(int64_t page_size, const int32_t* ke
         hipLaunchKernelGGL(paged_release_few_kernel, dim3(1), dim3(kFewWaves * 64), 0, stream, p);
         return check_launch("paged_release_few_kernel");
     }
-    const unsigned wgs = (unsigned)((n_seqs + kTableThreads / 64 - 1) / (kTableThreads / 64));
-    hipLaunchKernelGGL(paged_release_count_kernel, dim3(wgs), dim3(kTableThreads), 0, stream, p);
+    constexpr int64_t NW = kTableThreads / 64;
+    const int64_t wgs = (n_seqs + NW - 1) / NW;
+    p.per_wg = (int)((wgs + kReleaseWgs - 1) / kReleaseWgs * NW);
+    hipLaunchKernelGGL(paged_release_count_kernel, dim3((unsigned)wgs), dim3(kTableThreads), 0, stream, p);
     if (int rc = check_launch("paged_release_count_kernel")) return rc;
-    hipLaunchKernelGGL(paged_release_kernel, dim3(wgs), dim3(kTableThreads), 0, stream, p);
+    hipLaunchKernelGGL(paged_release_kernel, dim3((unsigned)((n_seqs + p.per_wg - 1) / p.per_wg)), dim3(kTableThreads), 0, stream, p);
     return check_launch("paged_release_kernel");
 }
