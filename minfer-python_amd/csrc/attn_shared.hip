@@ -452,29 +452,6 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
     else dst[0] = (uint16_t)(T::pack2(acc[0] * inv, 0.f) & 0xffffu);
 }
 
-// Whether a call is one for these kernels; others go to flash_attn_paged.  Longer chunks fill its blocks of rows with a single sequence's tokens.  And where all
-// sequences' rows together are no more than the memory-side cache holds, a prefix that is read once for each of them comes from there, and one launch or two
-// that know nothing of groups end sooner.  (us, shared / not, 400 own rows at most; 32 heads on 8 of 128: 8 sequences behind 4000 rows, 144 MB, 20.8 / 17.7, 4 behind
-// 16000, 269 MB, 29.4 / 33.2, 16 behind 4000, 288 MB, 23.1 / 27.3, 64 behind 256, 172 MB, 24.9 / 23.1; 8 on 2 of 64: 64 behind 4000, 144 MB, 20.3 / 17.4, 32 behind 16000,
-// 269 MB, 22.8 / 26.5; of codes: 8 behind 4000, 72 MB, 24.3 / 17.7, 16 behind 4000, 144 MB, 25.3 / 24.4, 64 behind 1000, 183 MB, 27.6 / 36.6.)  More than 16 columns
-// are read once here and twice or more often there, which matters over codes and at head_dim 64 (3 to 6 tokens, 32 heads on 8 of 128, codes: 8 sequences behind 1000, 22 MB, 24.0 / 23.8, 8 behind
-// 2000, 38 MB, 27.1 / 28.3, 8 behind 8000, 139 MB, 36.8 / 54.6; 16-bit 16 behind 2000, 154 MB, 30.4 / 29.3; 8 on 2 of 64: 32 behind 4000, 72 MB, 24.3 / 23.7, 32 behind 8000, 139 MB, 27.0 / 31.7;
-// of codes 32 behind 2000, 19 MB, 20.2 / 22.5, 64 behind 8000, 139 MB, 34.1 / 59.4).  But every row of theirs makes partial results, whose way through memory short contexts do not pay for (64
-// sequences of 3 to 6 tokens, 32 heads on 8 of 128, codes: behind 384 36.6 / 24.2, 768 38.9 / 36.6, 1536 45.3 / 60.9; 160 behind 768, 294 MB, 67.6 / 96.4; 16-bit 64 behind 768 38.5 / 26.8, behind 1536 42.3 / 44.1,
-// 64 heads 59.0 / 48.7; 160 behind 1536, 1.1 GB, 118 / 131), nor does a prefix of two (60 sequences in groups of 2 / 3 / 4 behind 2000 with 1000 of their own, codes 84.5, 65.8, 56.8 / 65; with
-// drafts 104, 84, 80 / 105; 16-bit 92, 75, 63 / 111; with drafts 114, 91, 81 / 86).  The host knows the table's width, not the contexts: a table far wider than they are costs a short
-// call 8 us.
-static bool shared_takes(bool eight, int64_t n_seqs, int64_t n_groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
-    const int64_t n_rep = Hq / Hkv, bytes = 2 * Hkv * D * (eight ? 1 : 2);   // of a row of all heads, k and v
-    if (n_groups == 0 || Hkv > kMaxSharedHeads || (max_q > 1 && (n_rep > 16 || max_q * n_rep > 64))) return false;
-    const bool pairs = max_q * n_rep > 16;
-    const int64_t rows = n_seqs * max_context;
-    auto most = [&](int64_t total) { return rows >= total / bytes; };
-    if (!pairs) return most(eight ? kSharedBytesCodes : kSharedBytes) && (!eight || n_seqs >= 3 * n_groups);
-    if (eight) return most(kSharedBytesCodes) ? max_context >= 600 && n_seqs >= 2 * n_groups : most(kSharedBytesPairsCodes) && max_context >= 1000 && n_seqs >= 3 * n_groups;
-    return most(D == 64 ? kSharedBytesPairs : kSharedBytes) && max_context >= (most(kSharedBytesLong) ? 1200 : 2000) && n_seqs >= 4 * n_groups;
-}
-
 // Groups of 16 columns that a wave streams a sequence's own rows for together: two where there are more than one.  (us, one at a time / two, each at the best division of the workgroups;
 // 32 heads on 8 of 128, sequences of 3 to 6 tokens behind 12000 rows: 24 with 10 to 900 own rows 54.7 / 53.7, of codes 60.1 / 58.9; 40 with 1000 to 6000 225 / 141, of codes 165 / 116;
 // 64 heads, 24 with 10 to 3000 125 / 107; at head_dim 64, 60 with 1000 to 6000 175 / 114, of codes 146 / 112.)
@@ -501,6 +478,38 @@ static SharedSizes shared_sizes(int64_t n_seqs, int64_t n_groups, int64_t T, int
     r.seq_bytes = lines((n_seqs + 1) * 16);
     r.bytes = r.o_bytes + r.ml_bytes + r.tile_o_bytes + r.tile_ml_bytes + r.seq_bytes + lines(n_groups * 16);
     return r;
+}
+
+// Whether the lines and the merge's rows are 32-bit numbers, were all contexts as long as the tables: of several thousand sequences with tables of a million rows they are not.
+static bool fits_a_launch(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
+    constexpr int64_t kMost = 0x7fffffffLL;
+    if (T > (1 << 30) || T * Hq > kMost - 4096 || n_seqs > (1 << 24) || max_context > (1 << 30)) return false;
+    const SharedSizes z = shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q);
+    return z.pieces * (max_context / 64 + 4) <= kMost - 65536 && n_seqs * Hkv * z.n_col <= kMost && n_seqs * Hkv * z.n_hg * ((max_context + 15) / 16 + 4) <= kMost - 65536;
+}
+
+// Whether a call is one for these kernels; others go to flash_attn_paged.  Longer chunks fill its blocks of rows with a single sequence's tokens.  And where all
+// sequences' rows together are no more than the memory-side cache holds, a prefix that is read once for each of them comes from there, and one launch or two
+// that know nothing of groups end sooner.  (us, shared / not, 400 own rows at most; 32 heads on 8 of 128: 8 sequences behind 4000 rows, 144 MB, 20.8 / 17.7, 4 behind
+// 16000, 269 MB, 29.4 / 33.2, 16 behind 4000, 288 MB, 23.1 / 27.3, 64 behind 256, 172 MB, 24.9 / 23.1; 8 on 2 of 64: 64 behind 4000, 144 MB, 20.3 / 17.4, 32 behind 16000,
+// 269 MB, 22.8 / 26.5; of codes: 8 behind 4000, 72 MB, 24.3 / 17.7, 16 behind 4000, 144 MB, 25.3 / 24.4, 64 behind 1000, 183 MB, 27.6 / 36.6.)  More than 16 columns
+// are read once here and twice or more often there, which matters over codes and at head_dim 64 (3 to 6 tokens, 32 heads on 8 of 128, codes: 8 sequences behind 1000, 22 MB, 24.0 / 23.8, 8 behind
+// 2000, 38 MB, 27.1 / 28.3, 8 behind 8000, 139 MB, 36.8 / 54.6; 16-bit 16 behind 2000, 154 MB, 30.4 / 29.3; 8 on 2 of 64: 32 behind 4000, 72 MB, 24.3 / 23.7, 32 behind 8000, 139 MB, 27.0 / 31.7;
+// of codes 32 behind 2000, 19 MB, 20.2 / 22.5, 64 behind 8000, 139 MB, 34.1 / 59.4).  But every row of theirs makes partial results, whose way through memory short contexts do not pay for (64
+// sequences of 3 to 6 tokens, 32 heads on 8 of 128, codes: behind 384 36.6 / 24.2, 768 38.9 / 36.6, 1536 45.3 / 60.9; 160 behind 768, 294 MB, 67.6 / 96.4; 16-bit 64 behind 768 38.5 / 26.8, behind 1536 42.3 / 44.1,
+// 64 heads 59.0 / 48.7; 160 behind 1536, 1.1 GB, 118 / 131), nor does a prefix of two (60 sequences in groups of 2 / 3 / 4 behind 2000 with 1000 of their own, codes 84.5, 65.8, 56.8 / 65; with
+// drafts 104, 84, 80 / 105; 16-bit 92, 75, 63 / 111; with drafts 114, 91, 81 / 86).  The host knows the table's width, not the contexts: a table far wider than they are costs a short
+// call 8 us.
+static bool shared_takes(bool eight, int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
+    const int64_t n_rep = Hq / Hkv, bytes = 2 * Hkv * D * (eight ? 1 : 2);   // of a row of all heads, k and v
+    if (n_groups == 0 || Hkv > kMaxSharedHeads || (max_q > 1 && (n_rep > 16 || max_q * n_rep > 64))) return false;
+    if (!fits_a_launch(n_seqs, n_groups, T, Hq, Hkv, D, max_context, max_q)) return false;
+    const bool pairs = max_q * n_rep > 16;
+    const int64_t rows = n_seqs * max_context;
+    auto most = [&](int64_t total) { return rows >= total / bytes; };
+    if (!pairs) return most(eight ? kSharedBytesCodes : kSharedBytes) && (!eight || n_seqs >= 3 * n_groups);
+    if (eight) return most(kSharedBytesCodes) ? max_context >= 600 && n_seqs >= 2 * n_groups : most(kSharedBytesPairsCodes) && max_context >= 1000 && n_seqs >= 3 * n_groups;
+    return most(D == 64 ? kSharedBytesPairs : kSharedBytes) && max_context >= (most(kSharedBytesLong) ? 1200 : 2000) && n_seqs >= 4 * n_groups;
 }
 
 template <class T, int D, bool FP8, int NC> static int launch_shared(const SharedWork& w, hipStream_t stream) {
@@ -531,7 +540,7 @@ MINFER_ATTN_EXPORT size_t minfer_flash_attn_paged_shared_workspace_bytes(int64_t
     const size_t plain = minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, max_context, max_q_len);
     size_t most = 0;   // of both kinds of pages
     for (const bool eight : {false, true})
-        most = std::max(most, shared_takes(eight, n_seqs, n_groups, Hq, Hkv, D, max_context, max_q) ? shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q).bytes : plain);
+        most = std::max(most, shared_takes(eight, n_seqs, n_groups, T, Hq, Hkv, D, max_context, max_q) ? shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q).bytes : plain);
     return most;
 }
 
@@ -554,16 +563,13 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged_shared(int dtype, int page_type, 
     if (n_groups > 0 && (!cu_groups || !prefix_lens)) return bad("flash_attn_paged_shared: cu_groups and prefix_lens must be non-null");
     const int64_t max_q = bounded_tokens(T, max_q_len), max_context = (int64_t)p.c.width << p.c.page_log2;
     const bool eight = page_type == MINFER_FP8_E4M3;
-    if (!shared_takes(eight, n_seqs, n_groups, Hq, Hkv, D, max_context, max_q))
+    if (!shared_takes(eight, n_seqs, n_groups, T, Hq, Hkv, D, max_context, max_q))
         return minfer_flash_attn_paged(dtype, page_type, q, pages, cu_seqlens, ctx_lens, out, n_seqs, T, Hq, Hkv, D, max_q_len, st, workspace, workspace_bytes, stream_v);
     if (!aligned16(q) || !aligned16(out)) return bad("flash_attn_paged_shared: q and out must be 16-byte aligned");
     const int64_t s[4] = {st->q1, st->q2, st->o1, st->o2};
     for (int i = 0; i < 4; ++i)
         if (s[i] < 0 || s[i] % 8 != 0) return bad("flash_attn_paged_shared: strides of q and out must be non-negative multiples of 8 elements");
-    if (T > (1 << 30) || T * Hq > 0x7fffffffLL - 4096 || n_seqs > (1 << 24)) return bad("flash_attn_paged_shared: problem too large for one launch");
     const SharedSizes z = shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q);
-    if (z.pieces * (max_context / 64 + 4) > 0x7fffffffLL - 65536 || n_seqs * Hkv * z.n_col > 0x7fffffffLL || n_seqs * Hkv * z.n_hg * ((max_context + 15) / 16 + 4) > 0x7fffffffLL - 65536)
-        return bad("flash_attn_paged_shared: problem too large for one launch");
     if (!workspace || !aligned16(workspace) || workspace_bytes < z.bytes)
         return fail(MINFER_ATTN_EWORKSPACE, "flash_attn_paged_shared: workspace too small or misaligned (see minfer_flash_attn_paged_shared_workspace_bytes)");
     p.q = q; p.out = out; p.cu = cu_seqlens; p.ctx = ctx_lens;

@@ -1,0 +1,34 @@
+"""Host side of the operators of a serving step, without a GPU: calls whose worst case is past what the kernels for groups count, which are flash_attn_paged's."""
+import pytest
+
+import capi
+import capi_serving as cs
+from test_serving_host import P, shared, wide
+
+
+def sizes(n_seqs, n_groups, T, Hq, Hkv, D, rows, max_q):
+    """Workspaces of the call with groups, of the call without."""
+    lib = cs.lib()
+    return (lib.minfer_flash_attn_paged_shared_workspace_bytes(n_seqs, n_groups, T, Hq, Hkv, D, rows, max_q),
+            lib.minfer_flash_attn_paged_workspace_bytes(n_seqs, T, Hq, Hkv, D, rows, max_q))
+
+
+@pytest.mark.parametrize("n_seqs,n_groups,T,Hq,Hkv,D,rows,max_q", [
+    (4096, 8, 4096 * 6, 32, 8, 128, 1 << 20, 6),         # drafts in tables of a million rows: a line of 2^31 places for their own rows
+    (4096, 1024, 4096 * 4, 24, 8, 64, 1 << 20, 8),
+    (2048, 2, 2048, 32, 8, 128, (1 << 21) - 16, 1),      # single tokens, in the few places between the two operators' bounds
+])
+def test_lines_past_31_bits_are_flash_attn_pageds(n_seqs, n_groups, T, Hq, Hkv, D, rows, max_q):
+    with_groups, without = sizes(n_seqs, n_groups, T, Hq, Hkv, D, rows, max_q)
+    assert with_groups == without
+    # (half as many sequences are the kernels for groups' own)
+    with_groups, without = sizes(n_seqs // 2, n_groups // 2, T // 2, Hq, Hkv, D, rows, max_q)
+    assert with_groups > without
+
+
+def test_what_flash_attn_paged_takes_is_not_refused():
+    """The call between the bounds gets as far as its workspace; beyond both of them it is too large."""
+    pages = lambda rows: wide(page_size=16, pages_per_seq=rows // 16, table_stride=rows // 16)
+    big = dict(n_seqs=2048, n_groups=2, T=2048, Hq=32, Hkv=8, max_q=1, st=capi.Strides(0, 128, 4096, 0, 0, 0, 0, 128, 4096))
+    assert shared(**big, pg=pages((1 << 21) - 16), ws=None) == capi.EWORKSPACE and "workspace" in capi.last_error()
+    assert shared(**big, pg=pages(1 << 22), ws=P, ws_bytes=1 << 50) == capi.EINVAL and "too large" in capi.last_error()
