@@ -419,12 +419,13 @@ int minfer_rope_kv_append_q8_0(int dtype, int style, void* q, const void* k, con
  * minfer_flash_attn_paged up to the order of the sums, and a prefix is read once for a group instead of once for each sequence.  Group i are the sequences
  * cu_groups[i] .. cu_groups[i+1]-1, the first prefix_lens[i] rows of which lie in the same pages (read through the table of the group's first sequence, in
  * whole pieces of 64 rows, so that table has to name all of them; what is left of a prefix is read through each sequence's own table); sequences in front
- * of the first group and behind the last have none.  A prefix may reach beyond another sequence's context or into new tokens: each token attends the rows up to its own.
+ * of the first group and behind the last have none, and one between two groups that shares nothing is a group of its own with a prefix of zero.  A prefix may reach beyond another sequence's context or into new tokens: each token attends the rows up to its own.
  * cu_groups int32 [n_groups + 1] and prefix_lens int32 [n_groups] are on the device and not trusted: what they hold is cut to the sequences and to the table, and no
  * address is made from more; but the result is that above only where cu_groups does not fall, and cu_seqlens does not either, except for
  * entries behind the last sequence with tokens.  Meant for single tokens and drafts (max_q_len * Hq / Hkv <= 64, and max_q_len 1 where Hq / Hkv > 16) whose tables name
  * more rows than the memory-side cache holds (n_seqs * pages_per_seq * page_size rows of 220 MB or more, of 150 MB of 8-bit pages; where max_q_len * Hq / Hkv > 16, of 70 MB at
- * head_dim 64 and of 25 MB of 8-bit pages), in tables not too short (where max_q_len * Hq / Hkv > 16) and groups not too small (two to four sequences on average); all other calls, which gain nothing by groups, are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
+ * head_dim 64 and of 25 MB of 8-bit pages), in tables not too short (where max_q_len * Hq / Hkv > 16) and groups not too small (two to four sequences on average); all other calls, which gain nothing by groups or
+ * whose rows, were all contexts as long as the tables, are more than 31 bits count, are what minfer_flash_attn_paged makes of them.  At most n_seqs groups.
  */
 size_t minfer_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                                       int64_t max_context, int64_t max_q_len);
@@ -449,11 +450,12 @@ typedef struct minfer_page_ring {
 /*
  * Block tables and slot maps for a step of a paged cache, from lengths: sequence s holds past_lens[s] rows in its table's first
  * pages_held[s] pages and gets new_lens[s] new rows.  Where these need more pages they are taken from the ring, sequence by sequence, page by
- * page, and written to the table behind those that are there; where the ring has no more, -1 is.  Written besides:
+ * page, and written to the table behind those that are there; where the ring has no more, -1 is.  Rows without a page are held nowhere: past_lens of the next call must not count
+ * them, or the page that it maps there is taken to hold them.  Written besides:
  *   cu_seqlens [n_seqs + 1]  sums of new_lens, as the operators over packed tokens take them
  *   ctx_lens [n_seqs]        past_lens + new_lens, as the attention takes them (the append's positions are past_lens)
  *   slots [n_slots]          of token cu_seqlens[s] + i its row past_lens[s] + i in the pool, page * page_size + row of the page, -1 where it has no
- *                            page; entries behind the last token are left alone, tokens behind the last entry have none
+ *                            page; entries behind the last token are left alone, tokens behind the last entry have none (n_slots 0: nobody needs them)
  *   held_after [n_seqs]      pages_held with the pages that were had
  * int32 but for slots, int64; all contiguous, the table's rows table_stride apart.  Nothing of it is trusted: negative lengths are zero, lengths past 2^30
  * are cut to it, sums saturate; pages_held is cut to 0 .. pages_per_seq, and rows behind the table get no page; a page outside the pool is no slot.
@@ -484,7 +486,8 @@ int minfer_paged_release(int64_t page_size, const int32_t* keep_lens, const int3
  *   n_accepted[s]  the drafts that are kept
  * The next token is the least j with w_0 + .. + w_j > sample_u[s] * (w_0 + .. + w_{V-1}), w = max(target - draft, 0) of the row where a draft was not
  * kept, and the target's row where all were or where the former is zero everywhere; the last j with w_j > 0 where no sum is larger (sample_u of
- * one or more), -1 where all are zero.  Sums are held in 64 bits.  Probabilities need not add up to one; negative ones and NaN count as zero there, and a draft
+ * one or more), -1 only where all are zero.  Sums are held in 64 bits.  Probabilities need not add up to one; w is zero where the difference (or the target's probability, where
+ * that is the weight) is negative or NaN, so a token whose draft probability is NaN is not drawn from a difference and a negative draft probability adds to one.  A draft
  * whose comparison is with NaN, or that is no token (outside 0..V-1), is not kept; infinite ones are not meant.  Sequences without tokens get n_accepted 0.
  * prob_dtype MINFER_ATTN_F32, F16 or BF16, for both; rows contiguous, *_stride elements apart, at any address of the type's alignment; tokens and
  * out_tokens of token_bits 32 or 64; accept_u [T] and sample_u [n_seqs] fp32 in [0, 1); cu_seqlens and n_accepted int32, cu_seqlens not trusted, as

@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
         if (EPL == 2) { const f32x2 v = *reinterpret_cast<const f32x2*>(at); x[0] = v[0]; x[EPL - 1] = v[1]; }
         else x[0] = at[0];
     };
-    // the first parts' rows beside their references and sums (of none: a row that is there, unused)
+    // the first parts' rows behind the requests of their references and sums (each behind a branch, of which the built code waits in front of some for what is on its way)
     f32x2 ml = {-INFINITY, 0.f}, pre = {-INFINITY, 0.f};
     if (lane < ns) ml = *reinterpret_cast<const f32x2*>(p.part_ml + (at0 + (int64_t)lane * work.per_part) * 2);
     if (lane < n_pre) pre = *reinterpret_cast<const f32x2*>(w.tile_ml + (pre0 + lane * tile_step) * 2);

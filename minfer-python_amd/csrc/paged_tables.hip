@@ -9,7 +9,7 @@
 // waiting for one another.  Only pages that are given back have to be looked at (a window that moved on may have left no page), so paged_release
 // counts in one launch and moves in a second.
 //
-// Bound by latency: a launch and two or three loads that depend on one another.
+// Bound by latency: a launch and, for tables, two or three loads that depend on one another; for pages given back up to eight loads a sequence one after the other, twice.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -137,7 +137,8 @@ MA_DEV Shrunk shrunk(const TableParams& p, int s) {
     return Shrunk{min((keep + (1 << p.page_log2) - 1) >> p.page_log2, held), held};
 }
 
-// f(entries, lane's is a page, the pages in front of it), 64 entries of a sequence's surplus at a time, eight times 64 requested together; the number of pages.  The whole wave.
+// f(entries, lane's is a page, the pages in front of it), 64 entries of a sequence's surplus at a time, eight times 64 a round; the number of pages.  The whole wave.  (Each of a round's loads
+// stands behind the condition that its entry is the sequence's, and the built code waits for it in front of the next one.)
 template <class F> MA_DEV int each_page(const TableParams& p, int s, int stay, int held, F f) {
     const int lane = threadIdx.x & 63;
     const int32_t* const row = p.table + (int64_t)s * p.table_stride;
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(kTableThreads) void paged_release_kernel(const Tabl
     for (int i = tid; i < first; i += kTableThreads) front += p.counts[i];
     front = block_sum(front, parts);
     for (int s0 = first; s0 < last; s0 += NW) {
-        int count[NW];   // of the four, requested together
+        int count[NW];   // of the four
 #pragma unroll
         for (int i = 0; i < NW; ++i) count[i] = s0 + i < last ? p.counts[s0 + i] : 0;
         int64_t mine = front;

@@ -354,7 +354,7 @@ def flash_attn_paged_shared(
 ):
     """flash_attn_paged where groups of sequences share their first rows, a prompt that a whole batch stands behind: sequences
     cu_groups[i] .. cu_groups[i+1]-1 name the same pages for their first prefix_lens[i] rows, which are then read once for the group
-    instead of once for each of them; sequences in front of the first group and behind the last share nothing.  The result is
+    instead of once for each of them; sequences in front of the first group and behind the last share nothing, one between two groups is a group with a prefix of 0.  The result is
     flash_attn_paged's up to the order of the sums.  cu_groups int32 [n_groups+1] and prefix_lens int32 [n_groups] on the device.  Meant for single
     tokens and drafts: max_q_len, the bound of a sequence's tokens, times the query heads of a KV head up to 64; above that it is flash_attn_paged."""
     return torch.ops.minfer.flash_attn_paged_shared.default(qtype_int, qblock_size, qtype_size, q, k_pages, v_pages,
@@ -422,7 +422,8 @@ def paged_tables(
     pages, unused}.  Written: cu_seqlens [n_seqs+1] and ctx_lens [n_seqs] as the paged operators take them (their `positions`
     are past_lens), slots [T] int64 (the row of the pool of every new token, page * page_size + row, or -1), held_after [n_seqs]
     and state_after [3] = {first entry, free pages, pages that were lacking}; these two go into the next call, in place of
-    pages_held and ring_state, which must be other tensors.  All other tensors int32."""
+    pages_held and ring_state, which must be other tensors.  Rows that got no page are held nowhere, and the next past_lens must not count them.  slots may be
+    empty.  All other tensors int32."""
     return torch.ops.minfer.paged_tables.default(page_size, past_lens, new_lens, pages_held, free_ring, ring_state, block_table, cu_seqlens,
                                                  ctx_lens, slots, held_after, state_after)
 
