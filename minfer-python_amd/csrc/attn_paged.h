@@ -167,7 +167,7 @@ struct PagedParams {
     PagedCache c;
     const void* q; void* out;
     const int32_t* cu; const int32_t* ctx;
-    float* part_o;     // partial results, un-normalised: decode [part][column][D], tiles [piece][KV head][row of the block][D] ...
+    float* part_o;     // partial results, un-normalised: decode [part][column][D], tiles [piece][KV head][row of the block][D], of shared prefixes [row][D] ...
     float* part_ml;    // ... with their reference (log2 units) and sum
     int64_t q1, q2, o1, o2;
     int n_seqs, T, Hq, Hkv, n_rep;

@@ -77,6 +77,7 @@ template <int D, bool FP8, int NW, bool SHARED> struct TileLds {
 // The rows are (token, head) pairs from token `lo` on, `rows` in all, of which the workgroup's are row0 .. row_end - 1: those of a sequence, whose table row and
 // context these are and whose token 0 stands at pos0; or (`prefix`) those of the sequences first .. last - 1 that share one, ctx being its rows, whole tiles, all
 // of which every row attends, but for tokens that stand inside them (`inside`: there are some).
+// Its partial results: the `slot`-th of all pieces, or (SHARED) from row `slot` of them on.
 struct TileJob { int g, seq, lo, ctx, pos0, rows, row0, row_end, part, parts, slot, t_lo, n_own, first, last; bool prefix, inside; };
 
 MA_DEV int tiles_of(int pos0, int rows, int n_rep, int block, int BR) { return (max(pos0 + min(block * BR + BR - 1, rows - 1) / n_rep + 1, 0) + 63) >> 6; }
@@ -659,7 +660,7 @@ template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tile
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) l_all[qb] = sum_across_quads(l_sum[qb]);
     if (SHARED || job.parts > 1) {
-        const int64_t part = ((int64_t)job.slot * p.Hkv + g) * BR;
+        const int64_t part = SHARED ? (int64_t)job.slot : ((int64_t)job.slot * p.Hkv + g) * BR;
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
             if (row0 + 16 * qb + l16 > last_row) continue;

@@ -34,10 +34,10 @@ struct SharedWork {
     DecodeWork d;                    // of the own rows; part_o / part_ml of d.p are theirs
     const int32_t* cu_groups; const int32_t* prefix;
     int n_groups;
-    float* tile_o; float* tile_ml;   // partial results of the tiles: [piece][KV head][row of the block][D] and their references and sums
-    int max_pieces;                  // that there is room for
+    float* tile_o; float* tile_ml;   // partial results of the tiles: [KV head][part_rows][D] and their references and sums (tile_row)
+    int part_rows;                   // that there is room for, per KV head
     i32x4* seq_tab;                  // [n_seqs]: a sequence's place on its line, its group (-1: none); then the quotas of both lines
-    i32x4* group_tab;                // [n_groups]: first token, (token, head) rows, place of its first block on the line of tiles, that block's number
+    i32x4* group_tab;                // [n_groups]: first token, (token, head) rows, place of its first block on the line of tiles, rows of the groups in front
 };
 
 // Rows of group i's prefix that are computed for all its tokens together: whole tiles.
@@ -81,7 +81,7 @@ MA_DEV Group group_at(const SharedWork& w, int i) {
 
 // What the waves of a workgroup have looked up (all of them the same, each for itself): the first 64 groups, and of the first 64 times 64 what lies on the line of tiles
 // in front of them.
-struct SharedLds { Group groups[64]; int tiles_before[64], blocks_before[64]; };
+struct SharedLds { Group groups[64]; int tiles_before[64], rows_before[64]; };
 
 // The group of sequence s (-1: none): cu_groups is a list of increasing starts.
 MA_DEV int group_of(const SharedWork& w, const SharedLds& l, int s) {
@@ -114,6 +114,12 @@ template <int GR> MA_DEV OwnSeq own_seq(const SharedWork& w, const SharedLds& l,
 // Blocks of a group's rows, equal to within a wave's: every row of a block attends all tiles of the prefix.
 template <int D> MA_DEV int blocks_of(const Group& g) { return g.tiles > 0 ? (g.rows + kBlockRows<D> - 1) / kBlockRows<D> : 0; }
 MA_DEV int rows_of_block(int rows, int blocks) { return ((rows + blocks - 1) / blocks + 31) & ~31; }
+MA_DEV int prefix_rows(const Group& g) { return g.tiles > 0 ? g.rows : 0; }   // that have partial results of tiles
+
+// Where the partial results of a share's part of a block lie, `row` rows of all groups in front of the block's first.  From one to the next along the line either the share's
+// number goes up by one, and with it a whole block's rows, or the rows in front by the block's, or both: they do not meet, and all rows and a block for
+// every share are room enough, however many groups there are.  (With room for a whole block of each group 4096 of them, 32 heads on 8 of 128, were 4.2 GiB, now 0.1.)
+template <int D> MA_DEV uint32_t tile_row(int row, int share) { return (uint32_t)row + (uint32_t)(share * kBlockRows<D>); }
 
 // What it costs to begin with a block, or with a (sequence, KV head, group of columns), inside a share (looking it up, requesting its first rows and waiting for
 // them), in tiles and in groups of rows: that many places of the line in front of it are its, where nothing is.
@@ -165,20 +171,20 @@ template <int D, int GR, int NC> MA_DEV SharedPlan plan_shared(const SharedWork&
     const PagedParams& p = w.d.p;
     const int lane = threadIdx.x & 63, pairs = p.Hkv * w.d.n_hg;
     SharedPlan r{};
-    int blocks = 0, longest = 0, longest_own = 0;
+    int rows = 0, longest = 0, longest_own = 0;
     float work = 0.f;
     for (int base = 0; base < w.n_groups; base += 64) {
         const Group q = group_at(w, base + lane);
         if (base == 0) l.groups[lane] = q;   // (all waves write the same, and each reads what it wrote)
         if (base < 64 * 64 && lane == 0) {
             l.tiles_before[base >> 6] = r.tiles;
-            l.blocks_before[base >> 6] = blocks;
+            l.rows_before[base >> 6] = rows;
         }
-        const int n = blocks_of<D>(q), length = n * (q.tiles + kTileLead), incl = wave_inclusive_scan(length), count = wave_inclusive_scan(n);
-        if (writes && base + lane < w.n_groups) w.group_tab[base + lane] = i32x4{q.lo, q.rows, r.tiles + incl - length, blocks + count - n};
+        const int n = blocks_of<D>(q), length = n * (q.tiles + kTileLead), incl = wave_inclusive_scan(length), in_front = wave_inclusive_scan(prefix_rows(q));
+        if (writes && base + lane < w.n_groups) w.group_tab[base + lane] = i32x4{q.lo, q.rows, r.tiles + incl - length, rows + in_front - prefix_rows(q)};
         work += lane_sum<64>(n > 0 ? (float)length * tile_time<D>(rows_of_block(q.rows, n)) : 0.f);
         r.tiles += lane_value(incl, 63);
-        blocks += lane_value(count, 63);
+        rows += lane_value(in_front, 63);
         longest = max(longest, q.tiles);
     }
     wave_lds_order();
@@ -220,14 +226,14 @@ template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look
     // the 64 groups that it lies in
     const uint64_t in_front = __ballot(lane == 0 || (lane * 64 < w.n_groups && l.tiles_before[lane] <= x));
     const int strip = 63 - __builtin_amdgcn_readfirstlane(__clzll((long long)in_front));
-    int before = strip > 0 ? __builtin_amdgcn_readfirstlane(l.blocks_before[strip]) : 0;
+    int before = strip > 0 ? __builtin_amdgcn_readfirstlane(l.rows_before[strip]) : 0;   // rows
     x -= strip > 0 ? __builtin_amdgcn_readfirstlane(l.tiles_before[strip]) : 0;
     for (int base = strip * 64; base < w.n_groups; base += 64) {
         const Group q = base == 0 ? l.groups[lane] : group_at(w, base + lane);
-        const int blocks = blocks_of<D>(q), n = blocks * (q.tiles + kTileLead), incl = wave_inclusive_scan(n), sum = lane_value(incl, 63), count = wave_inclusive_scan(blocks);
+        const int blocks = blocks_of<D>(q), n = blocks * (q.tiles + kTileLead), incl = wave_inclusive_scan(n), sum = lane_value(incl, 63), rows = wave_inclusive_scan(prefix_rows(q));
         if (x >= sum) {
             x -= sum;
-            before += lane_value(count, 63);
+            before += lane_value(rows, 63);
             continue;
         }
         const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(x < incl)) - 1);
@@ -244,7 +250,7 @@ template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look
         job.row_end = min(job.row0 + per, job.rows);
         job.t_lo = x - block * length - kTileLead;   // (below zero: places in front of the first tile)
         job.n_own = tiles - job.t_lo;
-        job.slot = before + lane_value(count - blocks, src) + block;
+        job.slot = before + lane_value(rows - prefix_rows(q), src) + job.row0;
         job.prefix = true;
         bool inside = false;
         for (int from = job.first; look_inside && from < job.last; from += 64) {
@@ -279,8 +285,9 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
     for (int x = x0; x < x1;) {
         TileJob job = shared_job<D>(w, x, plan.inside, l);
         job.n_own = min(job.n_own, x1 - x);
-        job.slot += rank;
-        if (job.n_own <= 0 || job.slot < 0 || job.slot >= w.max_pieces) break;   // (groups that overlap, which no valid call has: more of them than there is room for)
+        const uint32_t slot = tile_row<D>(job.slot, rank);
+        if (job.n_own <= 0 || slot > (uint32_t)(w.part_rows - kBlockRows<D>)) break;   // (groups that overlap, which no valid call has: more rows than there is room for)
+        job.slot = g * w.part_rows + (int)slot;
         x += job.n_own;
         job.n_own += min(job.t_lo, 0);
         job.t_lo = max(job.t_lo, 0);
@@ -375,18 +382,11 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
     const int group = own[1];
     const i32x4 quotas = const_load(w.seq_tab + p.n_seqs);
     constexpr int BR = kBlockRows<D>;
-    const int64_t tile_step = (int64_t)p.Hkv * BR;
     // partial results of an item's tiles, which are n from place x of the line on: their number, and the first one's
     struct Span { int n; int64_t first; };
     auto span_of = [&](int x, int n, int quota) {
         const int share = x / quota;
         return Span{n > 0 ? min((x + n - 1) / quota - share + 1, kMaxParts) : 0, share};
-    };
-    auto tiles_from = [&](int x, int n, int item) {
-        Span r = span_of(x, n, quotas[1]);
-        r.first += item;
-        r.n = x >= 0 && item >= 0 && r.first + r.n <= w.max_pieces ? r.n : 0;
-        return r;
     };
     // the parts of the group's prefix
     int n_pre = 0, skip = 0;
@@ -397,9 +397,11 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
         const int r = (info.lo + tok - t[0]) * p.n_rep + head;
         if (skip > 0 && r >= 0 && r < t[1]) {
             const int blocks = (t[1] + BR - 1) / BR, per = rows_of_block(t[1], blocks), block = r / per;
-            const Span a = tiles_from(t[2] + block * ((skip >> 6) + kTileLead) + kTileLead, skip >> 6, t[3] + block);
-            n_pre = a.n;
-            pre0 = n_pre > 0 ? (a.first * p.Hkv + g) * BR + r - block * per : 0;
+            const int x = t[2] + block * ((skip >> 6) + kTileLead) + kTileLead, at = t[3] + r;
+            const Span a = span_of(x, skip >> 6, quotas[1]);
+            const int64_t end = (int64_t)at + (a.first + a.n - 1) * BR;
+            n_pre = x >= 0 && at >= 0 && end < w.part_rows ? a.n : 0;   // (what groups that overlap have no room for)
+            pre0 = n_pre > 0 ? (int64_t)g * w.part_rows + at + a.first * BR : 0;
         }
     }
     // those of the sequence's own rows
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
     const int64_t at0 = part_row(work, (int64_t)s * p.Hkv * work.n_hg + pair + own_span.first, col % (16 * NC));
     const float* const pre_o = w.tile_o + pre0 * D + EPL * lane;
     const float* const own_o = p.part_o + at0 * D + EPL * lane;
-    const int64_t pre_step = tile_step * D, own_step = (int64_t)work.per_part * D;
+    const int64_t pre_step = (int64_t)BR * D, own_step = (int64_t)work.per_part * D;
     auto load_o = [&](const float* at, float (&x)[EPL]) __attribute__((always_inline)) {
         if (EPL == 2) { const f32x2 v = *reinterpret_cast<const f32x2*>(at); x[0] = v[0]; x[EPL - 1] = v[1]; }
         else x[0] = at[0];
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
     // the first parts' rows behind the requests of their references and sums (each behind a branch, of which the built code waits in front of some for what is on its way)
     f32x2 ml = {-INFINITY, 0.f}, pre = {-INFINITY, 0.f};
     if (lane < ns) ml = *reinterpret_cast<const f32x2*>(p.part_ml + (at0 + (int64_t)lane * work.per_part) * 2);
-    if (lane < n_pre) pre = *reinterpret_cast<const f32x2*>(w.tile_ml + (pre0 + lane * tile_step) * 2);
+    if (lane < n_pre) pre = *reinterpret_cast<const f32x2*>(w.tile_ml + (pre0 + (int64_t)lane * BR) * 2);
     constexpr int kEarly = 4;
     float x_pre[8][EPL], x_own[8][EPL];
 #pragma unroll
@@ -458,7 +460,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedWork w) {
 static int64_t column_groups(int64_t n_col) { return n_col > 16 ? 2 : 1; }
 
 // How a call is laid out, from its sizes alone.
-struct SharedSizes { int64_t n_col, n_hg, per_part, parts, pieces; size_t o_bytes, ml_bytes, tile_o_bytes, tile_ml_bytes, seq_bytes, bytes; };
+struct SharedSizes { int64_t n_col, n_hg, per_part, parts, blocks, part_rows; size_t o_bytes, ml_bytes, tile_o_bytes, tile_ml_bytes, seq_bytes, bytes; };
 static size_t lines(int64_t bytes) { return ((size_t)bytes + 255) / 256 * 256; }
 static SharedSizes shared_sizes(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q) {
     SharedSizes r{};
@@ -468,13 +470,14 @@ static SharedSizes shared_sizes(int64_t n_seqs, int64_t n_groups, int64_t T, int
     r.n_hg = (r.n_col + cols - 1) / cols;
     r.per_part = std::min<int64_t>(r.n_col, cols);
     const int64_t wgs = shared_wgs(D), block_rows = shared_waves(D) * 32;
-    // shares and pairs; shares and blocks, those of groups that do not overlap
+    // shares and pairs; rows and shares (tile_row), those of groups that do not overlap
     r.parts = wgs * shared_waves(D) + n_seqs * Hkv * r.n_hg;
-    r.pieces = wgs / Hkv + T * n_rep / block_rows + n_groups;
+    r.blocks = T * n_rep / block_rows + n_groups;
+    r.part_rows = T * n_rep + wgs / Hkv * block_rows;
     r.o_bytes = lines(r.parts * r.per_part * D * 4);
     r.ml_bytes = lines(r.parts * r.per_part * 2 * 4);
-    r.tile_o_bytes = lines(r.pieces * Hkv * block_rows * D * 4);
-    r.tile_ml_bytes = lines(r.pieces * Hkv * block_rows * 2 * 4);
+    r.tile_o_bytes = lines(r.part_rows * Hkv * D * 4);
+    r.tile_ml_bytes = lines(r.part_rows * Hkv * 2 * 4);
     r.seq_bytes = lines((n_seqs + 1) * 16);
     r.bytes = r.o_bytes + r.ml_bytes + r.tile_o_bytes + r.tile_ml_bytes + r.seq_bytes + lines(n_groups * 16);
     return r;
@@ -485,7 +488,7 @@ static bool fits_a_launch(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t H
     constexpr int64_t kMost = 0x7fffffffLL;
     if (T > (1 << 30) || T * Hq > kMost - 4096 || n_seqs > (1 << 24) || max_context > (1 << 30)) return false;
     const SharedSizes z = shared_sizes(n_seqs, n_groups, T, Hq, Hkv, D, max_q);
-    return z.pieces * (max_context / 64 + 4) <= kMost - 65536 && n_seqs * Hkv * z.n_col <= kMost && n_seqs * Hkv * z.n_hg * ((max_context + 15) / 16 + 4) <= kMost - 65536;
+    return z.blocks * (max_context / 64 + kTileLead) <= kMost - 65536 && z.part_rows * Hkv <= kMost && n_seqs * Hkv * z.n_col <= kMost && n_seqs * Hkv * z.n_hg * ((max_context + 15) / 16 + 4) <= kMost - 65536;
 }
 
 // Whether a call is one for these kernels; others go to flash_attn_paged.  Longer chunks fill its blocks of rows with a single sequence's tokens.  And where all
@@ -587,6 +590,6 @@ MINFER_ATTN_EXPORT int minfer_flash_attn_paged_shared(int dtype, int page_type, 
     w.group_tab = (i32x4*)at;
     w.d.n_col = (int)z.n_col; w.d.n_hg = (int)z.n_hg; w.d.per_part = (int)z.per_part;
     w.cu_groups = cu_groups; w.prefix = prefix_lens; w.n_groups = (int)n_groups;
-    w.max_pieces = (int)z.pieces;
+    w.part_rows = (int)z.part_rows;
     return dtype == MINFER_ATTN_F16 ? launch_shared_as<F16>(w, D, eight, (hipStream_t)stream_v) : launch_shared_as<BF16>(w, D, eight, (hipStream_t)stream_v);
 }

@@ -122,3 +122,16 @@ def test_a_captured_call_over_codes(kerns, D, most):
         assert torch.equal(got, out)
         if k % 2 == 0:
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("most", [1, 3])
+def test_several_blocks_of_several_groups(kerns, eight, D, most):
+    """Groups of more rows than a block has, one that fills its last block to the row, one without a prefix between them: partial results of blocks, shares and groups lie side by side."""
+    n = [75, 3, 64, 50] if most == 1 else [40, 3, 32, 26]
+    lens = [(1 + s % most, 1000 + 3 * s) for s in range(sum(n))]
+    at = [sum(n[:i]) for i in range(5)]
+    c = Shared(lens, [(at[0], at[1], 960), (at[1], at[2], 0), (at[2], at[3], 512), (at[3], at[4], 768)], 64, 2, D, torch.bfloat16, eight=eight)
+    for_groups(c, 16, most)
+    check(kerns, c, 16, torch.bfloat16)

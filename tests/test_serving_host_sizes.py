@@ -32,3 +32,14 @@ def test_what_flash_attn_paged_takes_is_not_refused():
     big = dict(n_seqs=2048, n_groups=2, T=2048, Hq=32, Hkv=8, max_q=1, st=capi.Strides(0, 128, 4096, 0, 0, 0, 0, 128, 4096))
     assert shared(**big, pg=pages((1 << 21) - 16), ws=None) == capi.EWORKSPACE and "workspace" in capi.last_error()
     assert shared(**big, pg=pages(1 << 22), ws=P, ws_bytes=1 << 50) == capi.EINVAL and "too large" in capi.last_error()
+
+
+@pytest.mark.parametrize("n_seqs,T,Hq,Hkv,D,max_q", [(4096, 4096, 32, 8, 128, 1), (4096, 4096, 8, 2, 64, 1), (1000, 4000, 32, 8, 128, 6), (600, 2400, 24, 4, 64, 4)])
+def test_the_workspace_does_not_grow_with_the_groups(n_seqs, T, Hq, Hkv, D, max_q):
+    """Partial results of prefixes: a row for every (token, head) and a block for each of 256 or 512 shares, whatever the number of groups; the rest is a few words a group."""
+    most = n_seqs // 4
+    one, many = (sizes(n_seqs, n, T, Hq, Hkv, D, 1 << 13, max_q)[0] for n in (1, most))
+    assert one > sizes(n_seqs, 0, T, Hq, Hkv, D, 1 << 13, max_q)[0]
+    assert many - one <= 16 * most + 256
+    own = n_seqs * max_q * Hq + (2048 + 16) * min(max_q * Hq // Hkv, 32) + T * Hq + (512 // Hkv) * 128 * Hkv * (D // 64)
+    assert many <= own * (D + 2) * 4 + 16 * (n_seqs + most) + 4096
