@@ -82,14 +82,17 @@ struct TileJob { int g, seq, lo, ctx, pos0, rows, row0, row_end, part, parts, sl
 
 MA_DEV int tiles_of(int pos0, int rows, int n_rep, int block, int BR) { return (max(pos0 + min(block * BR + BR - 1, rows - 1) / n_rep + 1, 0) + 63) >> 6; }
 
-// Position of packed token t, which is one of the sequences first .. last - 1 (cu_seqlens' entries do not fall there, but for those behind the last sequence
-// with tokens); -1 if it is not.
+// Position of packed token t, which is one of the sequences first .. last - 1 (cu_seqlens' entries do not fall up to the last one's end); -1 if it is not.  A search by halves: 4000 sequences behind 1024 rows,
+// one of them inside, 138 us (131 with none; 2034 along the sequences), 192 behind 6400 74 (67; 134).
 MA_DEV int position_of(const PagedParams& p, int first, int last, int t) {
-    for (int s = first; s < last; ++s) {
-        const TokenRange r = token_range(const_load(p.cu + s), const_load(p.cu + s + 1), p.T);
-        if (t >= r.lo && t < r.lo + r.len) return context_of(p.c, const_load(p.ctx + s), r) - r.len + t - r.lo;
+    int s = first, end = last - 1;   // the last sequence that does not begin behind t
+    while (s < end) {
+        const int mid = (s + end + 1) >> 1;
+        if (p.cu[mid] <= t) s = mid; else end = mid - 1;
     }
-    return -1;
+    if (s >= last) return -1;
+    const TokenRange r = token_range(p.cu[s], p.cu[s + 1], p.T);
+    return t >= r.lo && t < r.lo + r.len ? context_of(p.c, p.ctx[s], r) - r.len + t - r.lo : -1;
 }
 
 template <class T, int D, bool FP8, int NW, bool SHARED> MA_DEV void attend_tiles(const PagedParams& p, const TileJob& job, char* const lds) {

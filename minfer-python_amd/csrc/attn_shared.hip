@@ -43,7 +43,7 @@ struct SharedWork {
 // Rows of group i's prefix that are computed for all its tokens together: whole tiles.
 MA_DEV int shared_rows(const SharedWork& w, int i) { return min(max(w.prefix[i], 0), w.d.p.c.width << w.d.p.c.page_log2) & ~63; }
 
-struct Group { int first, last, lo, rows, tiles; };   // sequences, first token, (token, head) rows, tiles of the prefix
+struct Group { int first, last, lo, rows, tiles; };   // sequences (up to the last one with tokens), first token, (token, head) rows, tiles of the prefix
 // The whole wave, a group to a lane.
 MA_DEV Group group_at(const SharedWork& w, int i) {
     const PagedParams& p = w.d.p;
@@ -64,15 +64,20 @@ MA_DEV Group group_at(const SharedWork& w, int i) {
     uint64_t odd = __ballot(ends_empty);
     while (odd) {
         const int lane = threadIdx.x & 63, at = __ffsll((unsigned long long)odd) - 1, first = lane_value(r.first, at);
-        int found = lane_value(r.lo, at);
+        int found = lane_value(r.lo, at), found_last = first;
         for (int end = lane_value(r.last, at); end > first; end -= 64) {
             const int s = end - 1 - lane;
             TokenRange t{0, 0, 0};
             if (s >= first) t = token_range(p.cu[s], p.cu[s + 1], p.T);
             const uint64_t some = __ballot(t.len > 0);
-            if (some) { found = lane_value(t.lo + t.len, __ffsll((unsigned long long)some) - 1); break; }
+            if (some) {
+                const int src = __ffsll((unsigned long long)some) - 1;
+                found = lane_value(t.lo + t.len, src);
+                found_last = end - src;
+                break;
+            }
         }
-        if (lane == at) hi = found;
+        if (lane == at) { hi = found; r.last = found_last; }
         odd &= odd - 1;
     }
     r.rows = r.last > r.first ? max(hi - r.lo, 0) * p.n_rep : 0;
@@ -132,7 +137,7 @@ struct SharedPlan {
     int n_tile;                   // workgroups for tiles, the launch's first ones
     int tiles, tile_quota;        // of the line of tiles, per KV head
     int total, quota;             // of the other
-    bool inside;                  // a token stands inside its group's prefix
+    int inside_first, inside_last;   // sequences, the first and the last one with a token inside its group's prefix (none: the first is behind the last)
     int starts;                   // lane i: what lies on that line in front of sequence 64 i
 };
 
@@ -171,6 +176,8 @@ template <int D, int GR, int NC> MA_DEV SharedPlan plan_shared(const SharedWork&
     const PagedParams& p = w.d.p;
     const int lane = threadIdx.x & 63, pairs = p.Hkv * w.d.n_hg;
     SharedPlan r{};
+    r.inside_first = 0x7fffffff;
+    r.inside_last = -1;
     int rows = 0, longest = 0, longest_own = 0;
     float work = 0.f;
     for (int base = 0; base < w.n_groups; base += 64) {
@@ -203,7 +210,11 @@ template <int D, int GR, int NC> MA_DEV SharedPlan plan_shared(const SharedWork&
             if (lane == from >> 6) r.starts = r.total;
             r.total += lane_value(incl, 63);
             longest_own = max(longest_own, q.groups);
-            r.inside = r.inside || __any(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
+            const uint64_t in = __ballot(q.info.len > 0 && q.info.ctx - q.info.len < q.g0 * GR - 1);
+            if (in) {
+                r.inside_first = min(r.inside_first, from + __ffsll((unsigned long long)in) - 1);
+                r.inside_last = from + 63 - __clzll((long long)in);
+            }
         }
     }
     const int G = (int)gridDim.x, ranks = r.tiles > 0 ? tile_ranks<D, GR, NC>(r.tiles, work / (float)r.tiles, r.total, p.Hkv, G) : 0;
@@ -219,8 +230,7 @@ template <int D, int GR, int NC> MA_DEV SharedPlan plan_shared(const SharedWork&
 }
 
 // The block that holds place x of the line of tiles: its job (n_own: its tiles from there on; 0: there is no such block).
-template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look_inside, const SharedLds& l) {
-    const PagedParams& p = w.d.p;
+template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, const SharedPlan& plan, const SharedLds& l) {
     const int lane = threadIdx.x & 63;
     TileJob job{};
     // the 64 groups that it lies in
@@ -252,15 +262,7 @@ template <int D> MA_DEV TileJob shared_job(const SharedWork& w, int x, bool look
         job.n_own = tiles - job.t_lo;
         job.slot = before + lane_value(rows - prefix_rows(q), src) + job.row0;
         job.prefix = true;
-        bool inside = false;
-        for (int from = job.first; look_inside && from < job.last; from += 64) {
-            const int s = from + lane;
-            if (s < job.last) {
-                const TokenRange t = token_range(p.cu[s], p.cu[s + 1], p.T);
-                inside = inside || (t.len > 0 && context_of(p.c, p.ctx[s], t) - t.len < job.ctx - 1);
-            }
-        }
-        job.inside = __any(inside) != 0;
+        job.inside = plan.inside_first < job.last && plan.inside_last >= job.first;   // (of a group between two that have such tokens: looked for in vain)
         return job;
     }
     return job;
@@ -283,7 +285,7 @@ template <class T, int D, bool FP8> MA_DEV void shared_tiles(const SharedWork& w
     const int x0 = rank * plan.tile_quota, x1 = x0 + min(plan.tile_quota, plan.tiles - x0);
     bool busy = false;
     for (int x = x0; x < x1;) {
-        TileJob job = shared_job<D>(w, x, plan.inside, l);
+        TileJob job = shared_job<D>(w, x, plan, l);
         job.n_own = min(job.n_own, x1 - x);
         const uint32_t slot = tile_row<D>(job.slot, rank);
         if (job.n_own <= 0 || slot > (uint32_t)(w.part_rows - kBlockRows<D>)) break;   // (groups that overlap, which no valid call has: more rows than there is room for)
