@@ -503,13 +503,17 @@ static bool fits_a_launch(int64_t n_seqs, int64_t n_groups, int64_t T, int64_t H
 // of codes 32 behind 2000, 19 MB, 20.2 / 22.5, 64 behind 8000, 139 MB, 34.1 / 59.4).  But every row of theirs makes partial results, whose way through memory short contexts do not pay for (64
 // sequences of 3 to 6 tokens, 32 heads on 8 of 128, codes: behind 384 36.6 / 24.2, 768 38.9 / 36.6, 1536 45.3 / 60.9; 160 behind 768, 294 MB, 67.6 / 96.4; 16-bit 64 behind 768 38.5 / 26.8, behind 1536 42.3 / 44.1,
 // 64 heads 59.0 / 48.7; 160 behind 1536, 1.1 GB, 118 / 131), nor does a prefix of two (60 sequences in groups of 2 / 3 / 4 behind 2000 with 1000 of their own, codes 84.5, 65.8, 56.8 / 65; with
-// drafts 104, 84, 80 / 105; 16-bit 92, 75, 63 / 111; with drafts 114, 91, 81 / 86).  The host knows the table's width, not the contexts: a table far wider than they are costs a short
+// drafts 104, 84, 80 / 105; 16-bit 92, 75, 63 / 111; with drafts 114, 91, 81 / 86).  Of more columns there are more partial results, and past 32 of them own rows are read twice, so that what pays for them goes by
+// their number (kSharedRowsPerColumn; 8 to 2000 sequences of 17 to 64 columns in tables no wider than contexts, 1208 calls: against the better one a call loses 14, 4.5, 16 and 11 % on average without this line, 3, 2, 4 and 5 with it (codes at
+// head_dim 64 and 128, 16 bits at 64 and 128); 555 of 48 columns of codes behind 256 with 441 of their own at head_dim 64 343 / 139, 342 at 128 behind 320 with 248 225 / 144, 16-bit 508 of 64 behind 512 with 2627 221 / 114; 305 of 24 behind 5312 259 / 476).  The host knows the table's width, not the contexts: a table far wider than they are costs a short
 // call 8 us.
+constexpr int64_t kSharedRowsPerColumn[2][2] = {{100, 70}, {70, 25}};   // [codes][head_dim 128]
 static bool shared_takes(bool eight, int64_t n_seqs, int64_t n_groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context, int64_t max_q) {
     const int64_t n_rep = Hq / Hkv, bytes = 2 * Hkv * D * (eight ? 1 : 2);   // of a row of all heads, k and v
     if (n_groups == 0 || Hkv > kMaxSharedHeads || (max_q > 1 && (n_rep > 16 || max_q * n_rep > 64))) return false;
     if (!fits_a_launch(n_seqs, n_groups, T, Hq, Hkv, D, max_context, max_q)) return false;
     const bool pairs = max_q * n_rep > 16;
+    if (pairs && max_context < max_q * n_rep * kSharedRowsPerColumn[eight][D == 128]) return false;
     const int64_t rows = n_seqs * max_context;
     auto most = [&](int64_t total) { return rows >= total / bytes; };
     if (!pairs) return most(eight ? kSharedBytesCodes : kSharedBytes) && (!eight || n_seqs >= 3 * n_groups);

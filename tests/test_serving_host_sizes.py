@@ -43,3 +43,24 @@ def test_the_workspace_does_not_grow_with_the_groups(n_seqs, T, Hq, Hkv, D, max_
     assert many - one <= 16 * most + 256
     own = n_seqs * max_q * Hq + (2048 + 16) * min(max_q * Hq // Hkv, 32) + T * Hq + (512 // Hkv) * 128 * Hkv * (D // 64)
     assert many <= own * (D + 2) * 4 + 16 * (n_seqs + most) + 4096
+
+
+@pytest.mark.parametrize("D,codes", [(64, 70), (128, 25)])
+@pytest.mark.parametrize("Hq,max_q", [(32, 6), (48, 8), (64, 8)])
+def test_more_columns_ask_for_longer_tables(D, codes, Hq, max_q):
+    """24 to 64 columns of a KV head: partial results of each, and own rows read twice past 32, are paid for by so many rows a column of a table; below that the call is flash_attn_paged's.
+    (Codes, of which fewer rows are enough: the workspace is that of either kind.)"""
+    n, columns = 1500, Hq // 8 * max_q
+    takes = lambda rows: (lambda x: x[0] > x[1])(sizes(n, 1, n * max_q, Hq, 8, D, rows, max_q))
+    least = max(codes * columns, 600)
+    assert [takes(rows) for rows in (least - 16, least)] == [False, True]
+
+
+@pytest.mark.parametrize("D,rows_per_column", [(64, 100), (128, 70)])
+def test_more_columns_ask_for_longer_tables_of_16_bit_rows(D, rows_per_column):
+    """Which of the two operators asks for its workspace (20 sequences, whose blocks flash_attn_paged cuts, so that it asks, too)."""
+    least = 48 * rows_per_column
+    for rows, op in ((least - 16, "flash_attn_paged:"), (least, "flash_attn_paged_shared:")):
+        pg = wide(page_size=16, pages_per_seq=rows // 16, table_stride=rows // 16)
+        assert shared(pg=pg, n_seqs=20, n_groups=1, T=160, Hq=48, Hkv=8, D=D, max_q=8, st=capi.Strides(0, D, 48 * D, 0, 0, 0, 0, D, 48 * D), ws=None) == capi.EWORKSPACE
+        assert capi.last_error().startswith(op)
